@@ -308,6 +308,63 @@ int mpl_mrf_energy(const mpl_shape* shape, int n_labelings, const float* unary,
 int mpl_transpose(const float* src, float* dst, int batch, int64_t rows, int64_t cols,
                   void* stream);
 
+/* Element types of mpl_dropout_*. */
+#define MPL_F32 0
+#define MPL_F16 1
+#define MPL_BF16 2
+/* What shares one random word: an entry of its own, all labels of a pixel, all pixels of a label's plane. */
+#define MPL_DROPOUT_ELEMENT 0
+#define MPL_DROPOUT_PIXEL 1
+#define MPL_DROPOUT_LABEL 2
+
+/* Dropout of the unary costs within the layout change to the layers' layout; no counterpart in the reference, which
+ * leaves dropout to the network in front of the layer.  mpl_dropout_labels_last: src (batch, n_disp, pixels) of
+ * `dtype` -> dst (batch, pixels, n_disp) fp32, src / (1 - rate) where a label stays and 0 where it does not.
+ * mpl_dropout_labels_first is its gradient: src (batch, pixels, n_disp) fp32 -> dst (batch, n_disp, pixels) of
+ * `dtype`, the same labels of the same pixels times the same factor.  Products are formed in fp32.  Which labels stay is
+ * nowhere stored; it follows from state, two 64-bit DEVICE words (seed, offset) that both calls are given: the generator
+ * of Salmon, Moraes, Dror and Shaw ("Parallel random numbers: as easy as 1, 2, 3", SC 2011; 4x32, ten rounds) with the
+ * seed as its key and (group, offset) as its counter.  With quads = ceil(n_disp / 4) the group and the word are
+ *   MPL_DROPOUT_ELEMENT  (item * pixels + pixel) * quads + label / 4, word label % 4
+ *   MPL_DROPOUT_PIXEL    item * pixels + pixel, word 0
+ *   MPL_DROPOUT_LABEL    item * quads + label / 4, word label % 4
+ * and an entry stays where its word >= floor(rate * 2^32).  rate in [0, 1]; with 1 nothing stays.  A captured call
+ * reads state when it is replayed.  At most MPL_MAX_LABELS labels. */
+int mpl_dropout_labels_last(int dtype, int share, double rate, const int64_t* state, const void* src, float* dst,
+                            int batch, int n_disp, int64_t pixels, void* stream);
+int mpl_dropout_labels_first(int dtype, int share, double rate, const int64_t* state, const float* src, void* dst,
+                             int batch, int n_disp, int64_t pixels, void* stream);
+
+/* Pairwise tables whose entries go by buckets of the label distance k = |a - b|, for the layers' `context`; no
+ * counterpart in the reference.  Bucket b is the distances starts[b] <= k < starts[b + 1]; starts is a HOST array of
+ * n_buckets + 1 numbers in order, from 0 to n_disp, read during the call (a bucket may be empty).  table
+ * (n_tables, n_buckets) -> context (n_tables, n_disp) with square = 0, (n_tables, n_disp, n_disp) otherwise: with
+ * square = 1 the entries b >= a, zeros below the diagonal, with square = 2 both triangles.  mpl_bucket_sums is the
+ * gradient: dtable[t][b] = the sum of dcontext over the entries that table[t][b] went to, in fp64 and in a fixed
+ * order, rounded once. */
+int mpl_bucket_context(const float* table, const int32_t* starts, int n_tables, int n_buckets, int n_disp, int square,
+                       float* context, void* stream);
+int mpl_bucket_sums(const float* dcontext, const int32_t* starts, int n_tables, int n_buckets, int n_disp, int square,
+                    float* dtable, void* stream);
+
+/* Labels drawn from the layers' costs, their downstream beside the labels of least cost; no counterpart in the
+ * reference.  cost (batch, n_cv, n_disp, pixels) fp32 with labels_first, else (batch, n_cv, pixels, n_disp); uniforms
+ * (n_draws, batch, n_cv, pixels) fp32 in [0, 1) -> labels of that shape, uint8.  Label l of a pixel has weight
+ * exp((best - cost[l]) / temperature), best the pixel's least cost; +inf and NaN are no candidates (weight 0), beside a
+ * cost of -inf only others of -inf are.  Filters, in this order, equal costs ordered by label:
+ *   top_k  the k best stay (off: k <= 0 or k >= n_disp)
+ *   top_p  of these the shortest run of best ones that weighs at least top_p of their sum, one at least (off: >= 1)
+ *   min_p  of these the ones of at least min_p of the best one's weight (off: <= 0)
+ * The label drawn is the first, in label order, whose running sum of what stays exceeds uniform * (sum of what stays),
+ * or the last that stays where none does (a uniform of 1 or more); a uniform below 0 or NaN counts as 0.  A
+ * temperature that is not above 0 takes the label of least cost, the lowest of equals; a pixel without candidates
+ * gets label 0.  Weights and sums are formed in fp64.  temperatures, top_ks, top_ps, min_ps: batch numbers each in
+ * DEVICE memory, one per image, or NULL for the number beside. */
+int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms, int batch, int n_cv, int n_disp,
+                      int64_t pixels, int n_draws, const float* temperatures, float temperature, const int32_t* top_ks,
+                      int top_k, const float* top_ps, float top_p, const float* min_ps, float min_p, uint8_t* labels,
+                      void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* mpl_last_error(void);
 

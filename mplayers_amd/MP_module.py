@@ -15,8 +15,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib, lib_seg, lib_stereo
-from .label_context import create_label_context
-from .layout import gradient_labels_last, labels_first, labels_last
+from .label_context import bucket_context, create_bucket_table, create_label_context
+from .layout import gradient_labels_last, labels_first, labels_last, labels_last_dropout
 
 
 def _ops_for(n_disp):
@@ -218,6 +218,12 @@ class MPModule(torch.nn.Module):
   n_classes, mpnet_term_weight, mpnet_smoothness_train, mpnet_diag_value, enable_symmetric (and the
   fields create_label_context needs); writes rho (0.5 for TRWP, else 1), enable_saving_label,
   enable_min_a_dir, enable_sgm, enable_seg and, per call, training -- as the reference does.
+
+  Not in the reference, and off unless the field is there: mpnet_unary_dropout (a rate; in training mode the
+  unary costs are dropped out by it, the masks seeded from torch's generator of the device) with
+  mpnet_unary_dropout_share ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has
+  that many entries, which go by buckets of the label distance) with mpnet_smoothness_bucket_far (the distance
+  from which on they share the last one).
   """
 
   def __init__(self, args, enable_create_label_context=False, enable_saving_label=False,
@@ -250,12 +256,21 @@ class MPModule(torch.nn.Module):
   def get_label_context(self):
     return self.label_context, self.label_context_loc, self.label_context_diag_loc
 
-  def set_label_context(self, label_context, label_context_loc, label_context_diag_loc):
+  def set_label_context(self, label_context, label_context_loc, label_context_diag_loc, label_buckets=None):
+    """label_buckets (not in the reference): label_context has one entry per bucket of label distances, as
+    label_context.label_buckets lists them; the locations are then those of its entries."""
+    self.label_buckets = label_buckets
     self.label_context = label_context
     self.label_context_loc = label_context_loc
     self.label_context_diag_loc = label_context_diag_loc
 
   def create_label_context(self):
+    buckets = getattr(self.args, "mpnet_smoothness_buckets", 0)
+    if buckets:
+      self.set_label_context(*create_bucket_table(self.args, int(buckets),
+                                                  getattr(self.args, "mpnet_smoothness_bucket_far", None)))
+      return
+    self.label_buckets = None
     self.label_context, self.label_context_loc, self.label_context_diag_loc = \
         create_label_context(self.args, enable_seg=self.args.enable_seg,
                              enable_symmetric=self.args.enable_symmetric)
@@ -304,6 +319,16 @@ class MPModule(torch.nn.Module):
     return kept[2]
 
   def _effective_label_context(self, weight_first=False):
+    """The table that the operators read: the learned context re-parameterised and, where its entries go by
+    buckets, laid out by label distance."""
+    label_context = self._reparameterised_label_context(weight_first)
+    buckets = getattr(self, "label_buckets", None)
+    if buckets is None:
+      return label_context
+    return bucket_context(label_context, buckets, square=self.args.enable_seg,
+                          symmetric=bool(self.args.enable_symmetric))
+
+  def _reparameterised_label_context(self, weight_first):
     """Re-parameterisation of the learned context (MP_module.py:207-220).  weight_first: the term
     weight scales the stored parameter before the re-parameterisation instead of the sigmoid's
     output (the hard/soft module, MP_module_hard_soft.py:148-163)."""
@@ -331,9 +356,18 @@ class MPModule(torch.nn.Module):
       label_context[tuple(diag) if isinstance(diag, list) else diag] = self.args.mpnet_diag_value
     return label_context
 
+  def _labels_last(self, unary):
+    """The unary costs in the kernels' layout, in training mode with the dropout that args asks for."""
+    rate = getattr(self.args, "mpnet_unary_dropout", None)
+    if not rate or not self.training:
+      return labels_last(unary)
+    # (from torch's generator: it follows manual_seed, and a captured call has a new mask at every replay)
+    state = torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), device=unary.device)
+    return labels_last_dropout(unary, rate, state, getattr(self.args, "mpnet_unary_dropout_share", "element"))
+
   def forward(self, unary, edge_weights=None):
     # label axis innermost for the kernels; direction axis outermost for the edge weights
-    unary = labels_last(unary)
+    unary = self._labels_last(unary)
     if edge_weights is not None:
       edge_weights = edge_weights.unsqueeze(1).permute(2, 0, 1, 3, 4).contiguous()
       assert unary.size()[-3:-1] == edge_weights.size()[-2:]

@@ -14,7 +14,7 @@ the HIP library of this package.
 import torch
 
 from . import _lib, lib_seg, lib_stereo
-from .layout import gradient_labels_last, labels_first, labels_last
+from .layout import gradient_labels_last, labels_first
 from .MP_module import MPModule as _HardModule, _context_gradient, _sums_labels_first
 
 _U8 = dict(dtype=torch.uint8)
@@ -134,7 +134,7 @@ class MPModule(_HardModule):
 
   def forward(self, unary, edge_weights=None, msg_norm_index=None, pairwise_terms=None):
     assert self.args.mpnet_mrf_mode == 'TRWP'
-    unary = labels_last(unary)
+    unary = self._labels_last(unary)
     if edge_weights is not None:
       edge_weights = edge_weights.unsqueeze(1).permute(2, 0, 1, 3, 4).contiguous()
       assert unary.size()[-3:-1] == edge_weights.size()[-2:]

@@ -11,7 +11,9 @@ SYMBOLS = ("mpl_trwp_forward", "mpl_trwp_backward", "mpl_isgmr_forward", "mpl_is
            "mpl_last_error", "mpl_version", "mpl_edge_shift", "mpl_edge_shift_static",
            "mpl_trwp_soft_forward",
            "mpl_trwp_soft_backward", "mpl_soft_weighted_message", "mpl_soft_weighted_message_back", "mpl_set_option",
-           "mpl_stereo_data_cost", "mpl_gradient_cues", "mpl_mrf_energy", "mpl_transpose")
+           "mpl_stereo_data_cost", "mpl_gradient_cues", "mpl_mrf_energy", "mpl_transpose",
+           "mpl_dropout_labels_last", "mpl_dropout_labels_first", "mpl_bucket_context", "mpl_bucket_sums",
+           "mpl_sample_labels")
 
 KERNEL_KINDS = ("fwd_sweep", "bwd_sweep", "belief", "aggregate", "label", "combine", "other",
                 "fwd_sweep_all", "bwd_sweep_all", "unary_all")
@@ -73,6 +75,12 @@ def load():
   lib.mpl_gradient_cues.argtypes = [vp, ci, ci, ci, ci, cf, vp, vp, vp]
   lib.mpl_mrf_energy.argtypes = [sp, ci, vp, vp, vp, vp, vp, vp]
   lib.mpl_transpose.argtypes = [vp, vp, ci, ctypes.c_int64, ctypes.c_int64, vp]
+  i64, cd = ctypes.c_int64, ctypes.c_double
+  lib.mpl_dropout_labels_last.argtypes = [ci, ci, cd, vp, vp, vp, ci, ci, i64, vp]
+  lib.mpl_dropout_labels_first.argtypes = [ci, ci, cd, vp, vp, vp, ci, ci, i64, vp]
+  lib.mpl_bucket_context.argtypes = [vp, vp, ci, ci, ci, ci, vp, vp]
+  lib.mpl_bucket_sums.argtypes = [vp, vp, ci, ci, ci, ci, vp, vp]
+  lib.mpl_sample_labels.argtypes = [ci, vp, vp, ci, ci, ci, i64, ci, vp, cf, vp, ci, vp, cf, vp, cf, vp, vp]
   lib.mpl_n_chains.argtypes = [ci, ci, ci]
   lib.mpl_dcontext_copies.argtypes = [sp, ci]
   lib.mpl_table_is_dense.argtypes = [vp, ci]

@@ -1265,7 +1265,7 @@ extern "C" {
 
 const char* mpl_last_error(void) { return g_err; }
 
-int mpl_version(void) { return 210; }  // (2.10: the probes left the library; MPL_OPT_BELIEF_REBUILD; CPU forward)
+int mpl_version(void) { return 211; }  // (2.11: dropout in the layout change, bucketed tables, sampled labels)
 
 int mpl_set_option(int option, int value) {
   if (option == MPL_OPT_PACKED_SCANS) {

@@ -1,0 +1,134 @@
+// Pairwise tables whose entries go by buckets of the label distance, and their gradient, for gfx950.
+//
+// A layer of n labels with a learned 1-D table has n - 1 entries to learn, of which the far ones see few pairs.
+// With buckets it learns n_buckets: context[k] = table[bucket(k)], k = |a - b|, as a vector or as the (n, n) table
+// of all pairs of labels.  Bucket b is the distances starts[b] <= k < starts[b + 1], so its gradient is the sum of the
+// context's over these distances.
+//
+// At most 256 labels: a vector is 1 KiB, a square table 256 KiB, so the launches are what these calls cost.  Hence
+// one launch each, and the borders travel as kernel arguments (no copy to the device, nothing a capture could not
+// hold).
+
+#include "mp_common.h"
+
+using namespace mpl;
+
+namespace {
+
+struct BucketOf {
+  uint8_t of[kMaxL];
+};
+struct BucketStarts {
+  int16_t at[kMaxL + 1];
+};
+
+// One thread per entry of a row; a workgroup of 64 x 4 threads takes kRows rows of a square table, or one vector.
+constexpr int kRows = 16;
+template <bool SQUARE>
+__global__ void __launch_bounds__(256) bucket_context_kernel(BucketOf map, const float* __restrict__ table,
+                                                             float* __restrict__ context, int n_buckets, int n,
+                                                             int lower) {
+  const int tid = (int)(threadIdx.y * 64 + threadIdx.x);
+  const float* t = table + (int64_t)blockIdx.y * n_buckets;
+  if (!SQUARE) {
+    if (tid < n) context[(int64_t)blockIdx.y * n + tid] = t[map.of[tid]];
+    return;
+  }
+  __shared__ float value[kMaxL];
+  if (tid < n) value[tid] = t[map.of[tid]];
+  __syncthreads();
+  float* c = context + (int64_t)blockIdx.y * n * n;
+  const int end = min(n, ((int)blockIdx.x + 1) * kRows);
+  for (int a = (int)blockIdx.x * kRows + (int)threadIdx.y; a < end; a += 4)
+    for (int b = (int)threadIdx.x; b < n; b += 64) c[a * n + b] = b >= a || lower ? value[abs(a - b)] : 0.f;
+}
+
+// One workgroup per bucket and table.  The pairs (row, distance in the bucket) are dealt to the threads with the
+// distance innermost, so that a wide bucket reads runs of a row.  Sums in 64 bits and in a fixed order: a bucket of
+// a square table adds up to 65 536 entries.
+template <bool SQUARE>
+__global__ void __launch_bounds__(256) bucket_sums_kernel(BucketStarts starts, const float* __restrict__ dcontext,
+                                                          float* __restrict__ dtable, int n_buckets, int n, int lower) {
+  const int b = (int)blockIdx.x, t = (int)threadIdx.x;
+  const int first = starts.at[b], width = starts.at[b + 1] - first;
+  double sum = 0;
+  if (SQUARE) {
+    const float* d = dcontext + (int64_t)blockIdx.y * n * n;
+    const unsigned pairs = (unsigned)(n * width);
+#pragma unroll 4
+    for (unsigned i = (unsigned)t; i < pairs; i += 256) {
+      const int a = (int)(i / (unsigned)width);
+      const int k = first + (int)(i - (unsigned)(a * width));
+      if (a + k < n) sum += (double)d[a * n + a + k];
+      if (lower && k > 0 && a >= k) sum += (double)d[a * n + a - k];
+    }
+  } else {
+    const float* d = dcontext + (int64_t)blockIdx.y * n;
+    for (int k = t; k < width; k += 64) sum += (double)d[first + k];
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
+  if (SQUARE) {
+    __shared__ double part[4];
+    if ((t & 63) == 0) part[t >> 6] = sum;
+    __syncthreads();
+    sum = (part[0] + part[1]) + (part[2] + part[3]);
+  }
+  if (t == 0) dtable[(int64_t)blockIdx.y * n_buckets + b] = (float)sum;
+}
+
+int check_buckets(const char* what, const void* a, const void* b, const int32_t* starts, int n_tables, int n_buckets,
+                  int n_disp) {
+  if (a == nullptr || b == nullptr || starts == nullptr) return fail(MPL_EINVAL, "%s: null pointer", what);
+  if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
+  if (n_buckets < 1 || n_buckets > kMaxL)
+    return fail(MPL_EINVAL, "%s: n_buckets must be in [1, %d], got %d", what, kMaxL, n_buckets);
+  if (n_tables < 0 || n_tables > 65535) return fail(MPL_EINVAL, "%s: n_tables must be in [0, 65535]", what);
+  if (starts[0] != 0 || starts[n_buckets] != n_disp)
+    return fail(MPL_EINVAL, "%s: the buckets must run from distance 0 to n_disp", what);
+  for (int i = 0; i < n_buckets; ++i)
+    if (starts[i] > starts[i + 1]) return fail(MPL_EINVAL, "%s: the buckets must be in order", what);
+  return MPL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mpl_bucket_context(const float* table, const int32_t* starts, int n_tables, int n_buckets, int n_disp, int square,
+                       float* context, void* stream) {
+  if (int rc = check_buckets("bucket_context", table, context, starts, n_tables, n_buckets, n_disp)) return rc;
+  if (square < 0 || square > 2) return fail(MPL_EINVAL, "bucket_context: square must be 0, 1 or 2, got %d", square);
+  if (n_tables == 0) return MPL_OK;
+  BucketOf map = {};
+  for (int b = 0; b < n_buckets; ++b)
+    for (int k = starts[b]; k < starts[b + 1]; ++k) map.of[k] = (uint8_t)b;
+  const hipStream_t st = (hipStream_t)stream;
+  if (square)
+    bucket_context_kernel<true><<<dim3((unsigned)((n_disp + kRows - 1) / kRows), (unsigned)n_tables), dim3(64, 4), 0, st>>>(
+        map, table, context, n_buckets, n_disp, square == 2);
+  else
+    bucket_context_kernel<false><<<dim3(1, (unsigned)n_tables), dim3(64, 4), 0, st>>>(map, table, context, n_buckets,
+                                                                                     n_disp, 0);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "bucket_context: %s", hipGetErrorString(e));
+}
+
+int mpl_bucket_sums(const float* dcontext, const int32_t* starts, int n_tables, int n_buckets, int n_disp, int square,
+                    float* dtable, void* stream) {
+  if (int rc = check_buckets("bucket_sums", dcontext, dtable, starts, n_tables, n_buckets, n_disp)) return rc;
+  if (square < 0 || square > 2) return fail(MPL_EINVAL, "bucket_sums: square must be 0, 1 or 2, got %d", square);
+  if (n_tables == 0) return MPL_OK;
+  BucketStarts at = {};
+  for (int b = 0; b <= n_buckets; ++b) at.at[b] = (int16_t)starts[b];
+  const dim3 grid((unsigned)n_buckets, (unsigned)n_tables);
+  const hipStream_t st = (hipStream_t)stream;
+  if (square)
+    bucket_sums_kernel<true><<<grid, 256, 0, st>>>(at, dcontext, dtable, n_buckets, n_disp, square == 2);
+  else
+    bucket_sums_kernel<false><<<grid, 64, 0, st>>>(at, dcontext, dtable, n_buckets, n_disp, 0);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "bucket_sums: %s", hipGetErrorString(e));
+}
+
+}  // extern "C"

@@ -24,6 +24,7 @@ import torch
 from . import compute_terms
 from .label_context import create_label_context
 from .MP_module import MPModule
+from .sampling import sample_labels
 
 
 def parse_unary_cost(file_path):
@@ -72,6 +73,13 @@ def build_parser():
   parser.add_argument('--save_dir', type=str, default='../experiments')
   parser.add_argument('--synthetic', type=int, nargs=2, metavar=('H', 'W'), default=None,
                       help='use a random-dot stereo pair of this size instead of image files')
+  # (not in the reference: labellings drawn from the final costs beside the ones of least cost)
+  parser.add_argument('--n_draws', type=int, default=0)
+  parser.add_argument('--temperature', type=float, default=1.0)
+  parser.add_argument('--top_k', type=int, default=0)
+  parser.add_argument('--top_p', type=float, default=1.0)
+  parser.add_argument('--min_p', type=float, default=0.0)
+  parser.add_argument('--draw_seed', type=int, default=2019)
   return parser
 
 
@@ -147,6 +155,19 @@ def minimise(args, unary, table, n_disp):
   return labels.view(n_iter, height, width), energy, cost_final.view(n_disp, height, width), seconds
 
 
+def draw_labels(args, unary, table, cost_final):
+  """args.n_draws labellings drawn from the final costs (n_disp, H, W); -> labels (n, H, W) uint8, energy (n, 2)
+  fp64 as minimise returns it."""
+  n_disp, height, width = cost_final.shape
+  generator = torch.Generator(device=cost_final.device).manual_seed(args.draw_seed)
+  uniforms = torch.rand((args.n_draws, 1, 1, height, width), device=cost_final.device, generator=generator)
+  labels = sample_labels(cost_final.view(1, 1, n_disp, height, width), uniforms, temperature=args.temperature,
+                         top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
+  energy = compute_terms.mrf_energy(unary.view(1, height, width, n_disp).contiguous(), table.contiguous(),
+                                    labels.view(args.n_draws, 1, height, width), None, args.n_dir)
+  return labels.view(args.n_draws, height, width), energy
+
+
 def result_path(args, rho):
   """File name of the reference's result (main.py:163-168)."""
   name = '%s_%s_iter_%d_%s_trunc_%d_dir_%d_rho_%s' % (args.img_name, args.mode, args.n_iter,
@@ -184,6 +205,13 @@ def main(argv=None):
   for it in sorted(set([0, args.n_iter // 2, args.n_iter - 1])):
     print('iteration %3d: energy %.6g (unary %.6g, pairwise %.6g)' %
           (it + 1, total[it], energy_host[it, 0], energy_host[it, 1]))
+  draws = {}
+  if args.n_draws > 0:
+    drawn, drawn_energy = draw_labels(args, unary, table, cost_final)
+    total = drawn_energy.sum(1)
+    print('%d draws at temperature %g: energy %.6g on average, %.6g at least' %
+          (args.n_draws, args.temperature, total.mean().item(), total.min().item()))
+    draws = {'draws': drawn, 'draws_energy': drawn_energy}
   if file_path is not None:
     import scipy.io as scio
     os.makedirs(os.path.dirname(file_path), exist_ok=True)
@@ -195,10 +223,11 @@ def main(argv=None):
         'label_context': table.view(1, n_disp, n_disp).repeat(args.n_dir, 1, 1)
                               .permute(1, 2, 0).cpu().numpy(),
         'seg_all': labels.permute(1, 2, 0).cpu().numpy().astype(np.uint8),
-        'energy': energy_host})
+        'energy': energy_host,
+        **{key: value.cpu().numpy() for key, value in draws.items()}})
     print('saved %s' % file_path)
   return {'labels': labels, 'energy': energy, 'cost_final': cost_final, 'seconds': seconds,
-          'file_path': file_path}
+          'file_path': file_path, **draws}
 
 
 if __name__ == '__main__':

@@ -8,10 +8,18 @@ entries (upper triangle / k >= 1), `diag_loc` the pinned ones (diagonal / k == 0
 args fields read: n_classes, mpnet_smoothness_mode ('Potts' | 'potts' | 'TL' | 'TQ' | 'NPotts'),
 mpnet_smoothness_train, mpnet_smoothness_trunct_value, mpnet_smoothness_trunct_loc,
 mpnet_term_weight, enable_cuda.
+
+Tables whose entries go by buckets of the label distance (no counterpart in the reference): label_buckets
+says which distances share an entry, bucket_context makes the table of a layer of such entries, on the GPU
+through mpl_bucket_context with mpl_bucket_sums as its gradient, and create_bucket_table the parameter.
 """
+import argparse
+
 import numpy as np
 import torch
 import torch.nn as nn
+
+from . import _lib
 
 
 def _gap_cost(mode, gap):
@@ -80,3 +88,107 @@ def create_label_context(args, enable_seg=None, enable_symmetric=False):
     loc = range(1, n)
     diag_loc = range(1)
   return label_context, loc, diag_loc
+
+
+def label_buckets(n_classes, n_buckets, max_distance=None):
+  """int32 CPU tensor `starts` of n_buckets + 1: bucket b is the label distances starts[b] <= k < starts[b + 1].
+  The first half of the buckets hold one distance each, the others widen in equal ratios up to max_distance
+  (default n_classes); the last one goes on to n_classes.  The borders are found in whole numbers."""
+  if not (1 <= n_classes <= 256 and 1 <= n_buckets <= 256):
+    raise ValueError('label_buckets: 1 to 256 labels and buckets, got %r and %r' % (n_classes, n_buckets))
+  half = n_buckets // 2
+  far = n_classes if max_distance is None else int(max_distance)
+  if far < 1:
+    raise ValueError('label_buckets: max_distance must be positive, got %r' % (max_distance,))
+  far = max(far, half)
+  logs = n_buckets - half
+  starts = list(range(half)) + [half if half else 0]
+  for j in range(1, logs):
+    k = max(starts[-1], 1)
+    # k >= half * (far / half) ** (j / logs)
+    while k < n_classes and k ** logs * half ** j < half ** logs * far ** j:
+      k += 1
+    starts.append(k)
+  return torch.tensor([min(k, n_classes) for k in starts] + [n_classes], dtype=torch.int32)
+
+
+def _bucket_call(name, src, starts, square, shape):
+  src = src.contiguous()
+  out = torch.empty(shape, dtype=torch.float32, device=src.device)
+  n_buckets, n = starts.numel() - 1, int(starts[-1])
+  lead = out.numel() // (n_buckets if name == 'mpl_bucket_sums' else n * n if square else n)
+  if lead == 0:
+    return out
+  with torch.cuda.device(src.device):
+    rc = getattr(_lib.load(), name)(src.data_ptr(), starts.data_ptr(), lead, n_buckets, n, square, out.data_ptr(),
+                                    torch.cuda.current_stream().cuda_stream)
+  _lib.check(rc, name[4:])
+  return out
+
+
+class _BucketContext(torch.autograd.Function):
+  """(..., n_buckets) -> (..., n) or (..., n, n)."""
+
+  @staticmethod
+  def forward(ctx, table, starts, square):
+    ctx.rest = (starts, square)
+    n = int(starts[-1])
+    return _bucket_call('mpl_bucket_context', table, starts, square,
+                        tuple(table.shape[:-1]) + ((n, n) if square else (n,)))
+
+  @staticmethod
+  def backward(ctx, grad):
+    return _BucketSums.apply(grad, *ctx.rest), None, None
+
+
+class _BucketSums(torch.autograd.Function):
+  """The gradient of _BucketContext; linear, so its gradient is _BucketContext."""
+
+  @staticmethod
+  def forward(ctx, grad, starts, square):
+    ctx.rest = (starts, square)
+    return _bucket_call('mpl_bucket_sums', grad, starts, square,
+                        tuple(grad.shape[:-2 if square else -1]) + (starts.numel() - 1,))
+
+  @staticmethod
+  def backward(ctx, grad):
+    return _BucketContext.apply(grad, *ctx.rest), None, None
+
+
+def bucket_context(table, starts, square=False, symmetric=True):
+  """The pairwise table of a layer from one entry per bucket of label distances.
+
+  table   (..., n_buckets) fp32; leading axes are tables of their own (one per direction, say)
+  starts  as label_buckets returns it
+  square  False: (..., n) indexed by |a - b|; True: (..., n, n), with symmetric=False zeros below the diagonal
+  -> the table, with autograd; the gradient of an entry is the sum over the distances of its bucket."""
+  if not isinstance(table, torch.Tensor) or not isinstance(starts, torch.Tensor):
+    raise TypeError('bucket_context: table and starts must be tensors')
+  if starts.is_cuda or starts.dtype != torch.int32 or starts.dim() != 1 or not starts.is_contiguous():
+    raise RuntimeError('bucket_context: starts must be an int32 CPU tensor, as label_buckets returns it')
+  if table.dtype != torch.float32:
+    raise RuntimeError('bucket_context: table must be float32, got %s' % table.dtype)
+  if table.dim() < 1 or starts.numel() < 2 or table.size(-1) != starts.numel() - 1:
+    raise RuntimeError('bucket_context: table has %s entries for %d buckets' %
+                       (table.size(-1) if table.dim() else 'no', starts.numel() - 1))
+  if table.is_cuda:
+    return _BucketContext.apply(table, starts, 0 if not square else 2 if symmetric else 1)
+  if int(starts[0]) != 0 or bool((starts[1:] < starts[:-1]).any()):
+    raise RuntimeError('bucket_context: the buckets must be in order, from distance 0')
+  bucket = torch.repeat_interleave(torch.arange(starts.numel() - 1), (starts[1:] - starts[:-1]).long())
+  if not square:
+    return table[..., bucket]
+  label = torch.arange(bucket.numel())
+  context = table[..., bucket[(label[:, None] - label).abs()]]
+  return context if symmetric else context.triu()
+
+
+def create_bucket_table(args, n_buckets, max_distance=None):
+  """(nn.Parameter (n_buckets,), loc, diag_loc, starts): create_label_context's vector at the first distance of
+  each bucket; the reads of args are its own."""
+  starts = label_buckets(args.n_classes, n_buckets, max_distance)
+  plain = argparse.Namespace(**vars(args))
+  vector, _, _ = create_label_context(plain, enable_seg=False)
+  first = starts[:-1].long().clamp(max=args.n_classes - 1).to(vector.device)
+  return (nn.Parameter(vector.detach()[first].clone(), requires_grad=vector.requires_grad), range(1, n_buckets),
+          range(1), starts)

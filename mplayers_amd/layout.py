@@ -4,6 +4,10 @@ The reference's modules move the label axis with permute().contiguous()
 (pytorch/MP_module.py:199,203,233, pytorch/MP_module_hard_soft.py); these functions return the same
 contiguous tensors through mpl_transpose (a batched 2-D transpose bound by HBM), and their backward
 passes are the opposite transposes.
+
+`labels_last_dropout` is dropout of the unary costs within that change (no counterpart in the
+reference, whose networks have their dropout in front of the layer): mpl_dropout_labels_last and
+mpl_dropout_labels_first, which form the mask anew from a seed instead of storing it.
 """
 import ctypes
 
@@ -73,3 +77,78 @@ def labels_first(x):
   if _usable(x):
     return _LabelsFirst.apply(x)
   return x.permute(0, 1, 4, 2, 3).contiguous()
+
+
+_DROPOUT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # MPL_F32, MPL_F16, MPL_BF16
+_DROPOUT_SHARES = {"element": 0, "pixel": 1, "label": 2}  # MPL_DROPOUT_*
+
+
+def _dropout(call, dtype, share, p, state, src, dst, batch, n, pixels):
+  if src.numel() == 0:
+    return dst
+  with torch.cuda.device(src.device):
+    rc = getattr(_lib.load(), call)(_DROPOUT_TYPES[dtype], _DROPOUT_SHARES[share], p, state.data_ptr(), src.data_ptr(),
+                                    dst.data_ptr(), batch, n, pixels, torch.cuda.current_stream().cuda_stream)
+  _lib.check(rc, call[4:])
+  return dst
+
+
+class _DropoutLast(torch.autograd.Function):
+  """(batch, cv, labels, H, W) -> (batch, cv, H, W, labels) fp32 with dropout."""
+
+  @staticmethod
+  def forward(ctx, x, state, p, share):
+    ctx.save_for_backward(state)
+    ctx.rest = (p, share, x.dtype)
+    b, cv, n, h, w = x.shape
+    return _dropout("mpl_dropout_labels_last", x.dtype, share, p, state, x.contiguous(),
+                    torch.empty((b, cv, h, w, n), dtype=torch.float32, device=x.device), b * cv, n, h * w)
+
+  @staticmethod
+  def backward(ctx, grad):
+    p, share, dtype = ctx.rest
+    return _DropoutFirst.apply(grad, ctx.saved_tensors[0], p, share, dtype), None, None, None
+
+
+class _DropoutFirst(torch.autograd.Function):
+  """The gradient of _DropoutLast, back in the type of its input; linear, so its gradient is _DropoutLast."""
+
+  @staticmethod
+  def forward(ctx, grad, state, p, share, dtype):
+    ctx.save_for_backward(state)
+    ctx.rest = (p, share)
+    b, cv, h, w, n = grad.shape
+    return _dropout("mpl_dropout_labels_first", dtype, share, p, state, grad.contiguous(),
+                    torch.empty((b, cv, n, h, w), dtype=dtype, device=grad.device), b * cv, n, h * w)
+
+  @staticmethod
+  def backward(ctx, grad):
+    p, share = ctx.rest
+    return _DropoutLast.apply(grad, ctx.saved_tensors[0], p, share), None, None, None, None
+
+
+def labels_last_dropout(x, p, state, share="element"):
+  """labels_last(dropout(x)) in one pass over the costs, in fp32.
+
+  x      (batch, cv, labels, H, W) fp32, fp16 or bf16 on the GPU, at most 256 labels
+  p      rate in [0, 1]; what stays is multiplied by 1 / (1 - p)
+  state  int64 tensor of two on the device of x, (seed, offset): the mask follows from it and is formed
+         again in the backward pass, so it must not be written to before that.  A captured call reads it
+         at every replay.
+  share  'element': every entry by itself; 'pixel': all labels of a pixel (its neighbours' messages then
+         decide); 'label': all pixels of a label's plane"""
+  if not isinstance(x, torch.Tensor) or not isinstance(state, torch.Tensor):
+    raise TypeError("labels_last_dropout: x and state must be tensors")
+  if not x.is_cuda or x.dim() != 5:
+    raise RuntimeError("labels_last_dropout: x must be a (batch, cv, labels, H, W) GPU tensor")
+  if x.dtype not in _DROPOUT_TYPES:
+    raise RuntimeError("labels_last_dropout: x must be float32, float16 or bfloat16, got %s" % x.dtype)
+  if not 1 <= x.size(2) <= 256:
+    raise RuntimeError("labels_last_dropout: 1 to 256 labels, got %d" % x.size(2))
+  if state.device != x.device or state.dtype != torch.int64 or state.shape != (2,) or not state.is_contiguous():
+    raise RuntimeError("labels_last_dropout: state must be two int64 numbers (seed, offset) on the device of x")
+  if not 0 <= p <= 1:
+    raise RuntimeError("labels_last_dropout: p must be in [0, 1], got %r" % (p,))
+  if share not in _DROPOUT_SHARES:
+    raise RuntimeError("labels_last_dropout: share must be 'element', 'pixel' or 'label', got %r" % (share,))
+  return _DropoutLast.apply(x, state, float(p), share)
