@@ -2,6 +2,8 @@
 import ctypes
 import os
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MPLAYERS_HIP_LIB", os.path.join(HERE, "libmplayers_hip.so"))
 
@@ -149,3 +151,18 @@ def dcontext_copies(shape, n_iter):
 def check(rc, what):
   if rc != 0:
     raise RuntimeError("%s failed (%d): %s" % (what, rc, load().mpl_last_error().decode()))
+
+
+def launch(name, like, *args):
+  """Calls an entry point whose last argument is the stream, on the device and the current stream of the tensor
+  `like`.  (Where that is the current device, as nearly always, without the context manager's two microseconds.)"""
+  call = getattr(_lib or load(), name)
+  index = like.device.index
+  stream = torch._C._cuda_getCurrentRawStream(index)
+  if torch.cuda.current_device() == index:
+    rc = call(*args, stream)
+  else:
+    with torch.cuda.device(index):
+      rc = call(*args, stream)
+  if rc != 0:
+    check(rc, name[4:])

@@ -33,40 +33,56 @@ struct Sample {
   int top_k_all;
   int64_t pixels, tiles, items_pixels;
   int n, n_cv, n_draws;
+  uint32_t reciprocal;  // 2^32 / n, rounded up
+  int quads;            // labels last: whole and aligned quads
 };
 
 constexpr float kInf = __builtin_huge_valf();
 
-// +inf for what is no candidate, and one zero: comparisons of the results are those of numbers.  By bits: the library
-// is compiled for code without NaNs.
+// +inf for what is no candidate.  By bits: the library is compiled for code without NaNs.
 __device__ __forceinline__ float candidate(float c) {
-  const int bits = __builtin_bit_cast(int, c);
-  const float clean = (bits & 0x7fffffff) > 0x7f800000 ? kInf : c;
-  return clean == 0.f ? 0.f : clean;
+  return (__builtin_bit_cast(int, c) & 0x7fffffff) > 0x7f800000 ? kInf : c;
 }
-// x > 0 and a number, x >= 1 or no number
+
+// 2^y, y <= 0, to about 2^-51: the exponential series of the fraction, whose 14th term is below 2^-52 of the first.
+__device__ __forceinline__ double exp2_64(double y) {
+  y = y > -2000.0 ? y : -2000.0;
+  const double whole = rint(y), x = (y - whole) * 0.69314718055994530942;
+  double e = 1.0 / 6227020800;
+  e = fma(e, x, 1.0 / 479001600);
+  e = fma(e, x, 1.0 / 39916800);
+  e = fma(e, x, 1.0 / 3628800);
+  e = fma(e, x, 1.0 / 362880);
+  e = fma(e, x, 1.0 / 40320);
+  e = fma(e, x, 1.0 / 5040);
+  e = fma(e, x, 1.0 / 720);
+  e = fma(e, x, 1.0 / 120);
+  e = fma(e, x, 1.0 / 24);
+  e = fma(e, x, 1.0 / 6);
+  e = fma(e, x, 0.5);
+  e = fma(e, x, 1.0);
+  e = fma(e, x, 1.0);
+  return ldexp(e, (int)whole);
+}
+// x > 0 and a number
 __device__ __forceinline__ bool positive(float x) {
   const int bits = __builtin_bit_cast(int, x);
   return bits > 0 && bits <= 0x7f800000;
 }
 
-// Reductions over the S lanes of a pixel, neighbours within a row of 16.
+// Reductions over the S lanes of a pixel, neighbours: within a row of 16, or the whole wavefront (S = 64).
 template <int CTRL>
-__device__ __forceinline__ int move_i(int x) {
+__device__ __forceinline__ int move(int x) {
   return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
 }
 template <int CTRL>
 __device__ __forceinline__ float move(float x) {
-  return __builtin_bit_cast(float, move_i<CTRL>(__builtin_bit_cast(int, x)));
-}
-template <int CTRL>
-__device__ __forceinline__ int move(int x) {
-  return move_i<CTRL>(x);
+  return __builtin_bit_cast(float, move<CTRL>(__builtin_bit_cast(int, x)));
 }
 template <int CTRL>
 __device__ __forceinline__ double move(double x) {
   const int64_t bits = __builtin_bit_cast(int64_t, x);
-  const uint32_t lo = (uint32_t)move_i<CTRL>((int)(uint32_t)bits), hi = (uint32_t)move_i<CTRL>((int)(bits >> 32));
+  const uint32_t lo = (uint32_t)move<CTRL>((int)(uint32_t)bits), hi = (uint32_t)move<CTRL>((int)(bits >> 32));
   return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
 }
 template <int S, typename V, typename F>
@@ -75,15 +91,17 @@ __device__ __forceinline__ V over_lanes(V x, F f) {
   if (S > 2) x = f(x, move<0x4E>(x));   // the other pair of four
   if (S > 4) x = f(x, move<0x141>(x));  // the other four of eight
   if (S > 8) x = f(x, move<0x140>(x));  // the other eight
+  if (S > 16) x = f(x, __shfl_xor(x, 16));
+  if (S > 32) x = f(x, __shfl_xor(x, 32));
   return x;
 }
-template <int S>
-__device__ __forceinline__ float lanes_min(float x) {
-  return over_lanes<S>(x, [](float a, float b) { return b < a ? b : a; });
+template <int S, typename V>
+__device__ __forceinline__ V lanes_min(V x) {
+  return over_lanes<S>(x, [](V a, V b) { return b < a ? b : a; });
 }
-template <int S>
-__device__ __forceinline__ float lanes_max(float x) {
-  return over_lanes<S>(x, [](float a, float b) { return b > a ? b : a; });
+template <int S, typename V>
+__device__ __forceinline__ V lanes_max(V x) {
+  return over_lanes<S>(x, [](V a, V b) { return b > a ? b : a; });
 }
 template <int S, typename V>
 __device__ __forceinline__ V lanes_sum(V x) {
@@ -102,12 +120,34 @@ __device__ __forceinline__ V lanes_before(V x, int s) {
   return s == 0 ? V(0) : left;
 }
 
-// The least cost t of the pixel's with sum(of labels with v <= t) >= target, from `from` (the best) on; `to` (the
-// worst candidate) where no sum reaches it.
-template <int NV, int S, typename V, typename SumUpTo>
-__device__ __forceinline__ float threshold(const float (&v)[NV], float from, float to, V target, SumUpTo sum_up_to) {
-  float lo = from, hi = to;
-  for (int step = 0; __builtin_amdgcn_ballot_w64(lo < hi) != 0; ++step) {
+// The range lo <= t <= hi of the least cost t with sum(of labels with cost <= t) >= target; hi where no sum reaches it.
+// reached(sum) decides, or sets `unsure`, which ends the search where it is.
+//
+// narrow() halves it without looking for costs that occur, which takes less than half the instructions of a step of
+// threshold(), which closes it: there sum_upto(mid, below, above) also takes the greatest cost that is not above mid
+// and the least that is.  lo is a cost that occurs, or one that t is above.
+constexpr int kCoarse = 5;
+template <int S, typename SumUpTo, typename Reached>
+__device__ __forceinline__ void narrow(float& lo, float& hi, const bool& unsure, SumUpTo sum_upto, Reached reached) {
+#pragma unroll 1
+  for (int step = 0; step < kCoarse; ++step) {
+    const float mid = 0.5f * lo + 0.5f * hi;
+    const auto sum = lanes_sum<S>(sum_upto(mid));
+    if (mid > lo && mid < hi) {
+      const bool down = reached(sum);
+      if (!unsure) {
+        if (down)
+          hi = mid;
+        else
+          lo = mid;
+      }
+    }
+  }
+}
+template <int S, typename SumUpTo, typename Reached>
+__device__ __forceinline__ void threshold(float& lo, float& hi, const bool& unsure, SumUpTo sum_upto, Reached reached) {
+#pragma unroll 1
+  for (int step = 0; __builtin_amdgcn_ballot_w64(lo < hi && !unsure) != 0; ++step) {
     // Halves the costs, and after a while what lies between their bit patterns: costs that grow from one to the next
     // by factors would lose one a step.
     float mid = 0.5f * lo + 0.5f * hi;
@@ -117,152 +157,441 @@ __device__ __forceinline__ float threshold(const float (&v)[NV], float from, flo
     }
     if (!(mid >= lo && mid < hi)) mid = lo;
     float below = lo, above = hi;
-    V sum = V(0);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const bool in = v[j] <= mid;
-      if (in) below = v[j] > below ? v[j] : below;
-      if (!in) above = v[j] < above ? v[j] : above;
-      sum += in ? sum_up_to(j) : V(0);
-    }
-    sum = lanes_sum<S>(sum);
+    const auto sum = lanes_sum<S>(sum_upto(mid, below, above));
     below = lanes_max<S>(below);
     above = lanes_min<S>(above);
     if (lo < hi) {
-      if (sum >= target)
-        hi = below;
-      else
-        lo = above;
+      const bool down = reached(sum);
+      if (!unsure) {
+        if (down)
+          hi = below;
+        else
+          lo = above;
+      }
     }
   }
-  return hi;
+}
+
+// What the parameters of an image come to.
+struct Parameters {
+  float temperature, top_p, min_p;
+  int top_k;
+  bool warm;
+  double inv_t;
+};
+template <bool FILTER>
+__device__ __forceinline__ Parameters parameters(const Sample& p, int image) {
+  Parameters q;
+  q.temperature = p.temperature != nullptr ? p.temperature[image] : p.temperature_all;
+  q.warm = positive(q.temperature);
+  q.inv_t = q.warm ? 1.0 / (double)q.temperature : 0.0;
+  q.top_k = p.n;
+  q.top_p = 1.f;
+  q.min_p = 0.f;
+  if (FILTER) {
+    const int k = p.top_k != nullptr ? p.top_k[image] : p.top_k_all;
+    if (k > 0 && k < p.n) q.top_k = k;
+    if (!q.warm) q.top_k = 1;
+    if (q.warm) {
+      q.top_p = p.top_p != nullptr ? p.top_p[image] : p.top_p_all;
+      q.min_p = p.min_p != nullptr ? p.min_p[image] : p.min_p_all;
+    }
+  }
+  return q;
+}
+
+// The greatest cost that min_p leaves: the greatest float whose distance from the best is at most T * ln(1 / min_p).
+__device__ __forceinline__ float farthest(const Parameters& q, float best) {
+  if (best == -kInf) return best;
+  const double reach = q.min_p >= 1.f ? 0.0 : -(double)q.temperature * log((double)q.min_p);
+  const auto within = [&](float c) { return (double)c - (double)best <= reach; };
+  const float far = (float)((double)best + reach);
+  if (!(far < kInf)) return kInf;
+  const int key = float_key(__builtin_bit_cast(int, far));
+  const float next = __builtin_bit_cast(float, float_key(key + 1)), previous = __builtin_bit_cast(float, float_key(key - 1));
+  const float c = within(next) ? next : within(far) ? far : previous;
+  return c < best ? best : c;
+}
+
+// One pixel by a whole wavefront, four labels to a lane, in 64 bits: cost(l) gives its costs, at is its place in the
+// uniform numbers and the labels.
+template <bool FILTER, typename Cost>
+__device__ void draw_exactly(const Sample& p, const Parameters& q, int64_t at, Cost cost) {
+  const int lane = (int)(threadIdx.x & 63);
+  float v[4], best = kInf;
+  double w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int l = 4 * lane + j;
+    v[j] = l < p.n ? candidate(cost(l)) : kInf;
+    best = v[j] < best ? v[j] : best;
+  }
+  best = lanes_min<64>(best);
+  const auto weight = [&](float c) {
+    const double e = exp2_64(((double)best - (double)c) * (q.inv_t * 1.4426950408889634));
+    return !(c < kInf) ? 0.0 : c == best ? 1.0 : best == -kInf ? 0.0 : e;
+  };
+  if (FILTER) {
+    const auto worst = [&]() {
+      float m = best;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = v[j] < kInf && v[j] > m ? v[j] : m;
+      return lanes_max<64>(m);
+    };
+    // takes out what is worse than t, and of the labels at t those that do not stay by their rank
+    const auto cut = [&](float t, auto stays) {
+      int rank = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t ties = __builtin_amdgcn_ballot_w64(v[j] == t);
+        rank += __builtin_amdgcn_mbcnt_hi((uint32_t)(ties >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ties, 0));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool tie = v[j] == t;
+        if (v[j] > t || (tie && !stays(rank))) v[j] = kInf;
+        rank += tie ? 1 : 0;
+      }
+    };
+    constexpr bool unsure = false;
+    const auto search = [&](auto target, auto add) {
+      float lo = best, hi = worst();
+      threshold<64>(
+          lo, hi, unsure,
+          [&](float mid, float& below, float& above) {
+            auto sum = target;
+            sum = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              below = v[j] <= mid && v[j] > below ? v[j] : below;
+              above = v[j] > mid && v[j] < above ? v[j] : above;
+              if (v[j] <= mid) sum += add(j);
+            }
+            return sum;
+          },
+          [&](auto sum) { return sum >= target; });
+      return hi;
+    };
+    if (q.top_k < p.n) {
+      const float t = search(q.top_k, [](int) { return 1; });
+      int less = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) less += v[j] < t ? 1 : 0;
+      less = lanes_sum<64>(less);
+      cut(t, [&](int rank) { return less + rank < q.top_k; });
+    }
+    if (q.top_p < 1.f) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = weight(v[j]);
+      const double target = (double)q.top_p * lanes_sum<64>((w[0] + w[1]) + (w[2] + w[3]));
+      const float t = search(target, [&](int j) { return w[j]; });
+      double less = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) less += v[j] < t ? w[j] : 0.0;
+      less = lanes_sum<64>(less);
+      const double each = weight(t);
+      cut(t, [&](int rank) { return less + rank * each < target || (t == best && rank == 0); });
+    }
+    if (positive(q.min_p)) {
+      const float far = farthest(q, best);
+      cut(far, [](int) { return true; });
+    }
+  }
+  double sum = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    w[j] = weight(v[j]);
+    sum += w[j];
+  }
+  double upto = sum;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const double left = __shfl_up(upto, m);
+    if (lane >= m) upto += left;
+  }
+  const double total = __shfl(upto, 63), before = __shfl_up(upto, 1);
+  int last = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (w[j] > 0) last = 4 * lane + j;
+  last = lanes_max<64>(last);
+  for (int d = 0; d < p.n_draws; ++d) {
+    const float u = p.uniforms[d * p.items_pixels + at];
+    // (the lanes' sums may pass the total by a rounding)
+    const double target = positive(u) && u >= 1.f ? __builtin_huge_val() : (positive(u) ? (double)u : 0.0) * total;
+    double run = lane == 0 ? 0.0 : before;
+    int label = last;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      double to = run;
+#pragma unroll
+      for (int i = 0; i <= j; ++i) to += w[i];
+      // (a label that is out adds nothing, but the lanes' sums are formed in another order)
+      if (to > target && w[j] > 0) label = min(label, 4 * lane + j);
+    }
+    label = lanes_min<64>(label);
+    if (lane == 0) p.labels[d * p.items_pixels + at] = (uint8_t)label;
+  }
 }
 
 // S lanes per pixel, NV labels per lane: lane s owns labels s * NV ... s * NV + NV - 1.
+//
+// Weights and sums are formed in 32 bits, with a bound on how far they may be off, relative to the sum of all:
+//   a weight  3 roundings of its exponent a (2^-24 * 3 * a * w, and sum(a * w) <= ln(n) * sum(w): the entropy of n labels),
+//             1 ulp of the exponential: (2 + 3 * ln 256) * 2^-24 < 19 * 2^-24
+//   a sum     NV - 1 additions in a lane, S over the lanes: (NV + S) * 2^-24
+// and as much for a target, which is a product with such a sum (and is rounded itself).  Where a sum is as close to a
+// target as both (kNear), 32 bits do not tell, and draw_exactly() takes the pixel: with costs as a layer gives them one
+// draw in 400 of 192 labels, one in 4000 of 21.
 template <int NV, int S, bool FILTER, bool LAST>
 __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
   constexpr int kQuads = S * NV / 4, kJ = NV / 4;  // of four labels: in all, per lane
   constexpr int kStride = 4 * (kQuads | 1);
-  __shared__ __align__(16) float tile[kPixels * kStride];
-  const int64_t block = (int64_t)blockIdx.x;
-  const int64_t item = block / p.tiles, p0 = (block - item * p.tiles) * kPixels;
+  constexpr bool kTile = S > 1 || LAST;  // through LDS
+  constexpr float kNear = 2 * (NV + S + 25) * 0x1p-24f;
+  __shared__ __align__(16) float tile[kTile ? kPixels * kStride : 4];
+  __shared__ uint32_t left_over[2];  // pixels for draw_exactly()
+  const unsigned block = blockIdx.x, tiles = (unsigned)p.tiles;
+  const int64_t item = block / tiles, p0 = (int64_t)(block - (unsigned)item * tiles) * kPixels;
   const int count = (int)min((int64_t)kPixels, p.pixels - p0);
   const int tid = (int)threadIdx.x;
   const float* cost = p.cost + item * p.n * p.pixels;
-  // the quads of a pixel lie in the order in which its lanes read them: quad q, of lane q / kJ, at place q % kJ * S + q / kJ
-  const auto place = [](int l) { return ((l >> 2) % kJ * S + (l >> 2) / kJ) * 4 + (l & 3); };
-  if (LAST) {
-    for (int i = tid; i < count * p.n; i += kPixels * S) tile[i / p.n * kStride + place(i % p.n)] = cost[p0 * p.n + i];
-  } else {
-    const int px = tid % kPixels;
-    if (px < count)
-      for (int l = tid / kPixels; l < p.n; l += S) tile[px * kStride + place(l)] = cost[l * p.pixels + p0 + px];
-  }
-  __syncthreads();
-  const int px = tid / S, s = tid % S;
-  if (px >= count) return;  // (whole pixels: the lanes of one stay or go together)
   float v[NV];
+  const int px = tid / S, s = tid % S;
+  if (tid < 2) left_over[tid] = 0;
+  // The quads of a pixel lie in the order in which its lanes read them: quad q, of lane q / kJ, at place q % kJ * S + q / kJ.
+  const auto place = [](int q) { return (q % kJ * S + q / kJ) * 4; };
+  // Rows of labels: the labels behind the last and the pixels behind the last are read from the last's place, so that
+  // no branch lies between the loads.
+  const auto row = [&](int l) { return cost + (int64_t)min(l, p.n - 1) * p.pixels + p0; };
+  if (!kTile) {
+    const int of = min(px, count - 1);
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-    v[j] = s * NV + j < p.n ? candidate(tile[px * kStride + ((j >> 2) * S + s) * 4 + (j & 3)]) : kInf;
+    for (int j = 0; j < NV; ++j) v[j] = row(j)[of];
+  } else {
+    if (LAST) {
+      const unsigned n = (unsigned)p.n, total = (unsigned)count * n;
+      const float* from = cost + p0 * p.n;
+      if (p.quads) {
+        float4 c[kJ];
+#pragma unroll
+        for (int k = 0; k < kJ; ++k)
+          c[k] = *reinterpret_cast<const float4*>(from + min((unsigned)(tid + k * kPixels * S) * 4, total - 4));
+#pragma unroll
+        for (int k = 0; k < kJ; ++k) {
+          const unsigned i = min((unsigned)(tid + k * kPixels * S) * 4, total - 4);
+          const unsigned of = __umulhi(i, p.reciprocal), l = i - of * n;
+          *reinterpret_cast<float4*>(&tile[of * kStride + place((int)(l >> 2))]) = c[k];
+        }
+      } else {
+        float c[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) c[k] = from[min((unsigned)(tid + k * kPixels * S), total - 1)];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const unsigned i = min((unsigned)(tid + k * kPixels * S), total - 1);
+          const unsigned of = n == 1 ? i : __umulhi(i, p.reciprocal), l = i - of * n;
+          tile[of * kStride + place((int)(l >> 2)) + (l & 3)] = c[k];
+        }
+      }
+    } else {
+      const int of = min(tid % kPixels, count - 1), wave = uniform_i(tid / kPixels);
+      float4 c[kJ];
+#pragma unroll
+      for (int i = 0; i < kJ; ++i) {
+        const int l = 4 * (wave + i * S);
+        c[i] = float4{row(l)[of], row(l + 1)[of], row(l + 2)[of], row(l + 3)[of]};
+      }
+#pragma unroll
+      for (int i = 0; i < kJ; ++i)
+        *reinterpret_cast<float4*>(&tile[tid % kPixels * kStride + place(wave + i * S)]) = c[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = tile[px * kStride + ((j >> 2) * S + s) * 4 + (j & 3)];
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) v[j] = s * NV + j < p.n && px < count ? candidate(v[j]) : kInf;
   float best = v[0];
 #pragma unroll
   for (int j = 1; j < NV; ++j) best = v[j] < best ? v[j] : best;
   best = lanes_min<S>(best);
 
-  const int image = (int)(item / p.n_cv);
-  const float t32 = p.temperature != nullptr ? p.temperature[image] : p.temperature_all;
-  const bool warm = positive(t32);
-  const double inv_t = warm ? 1.0 / (double)t32 : 0.0;
-  double w[NV];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const double e = exp(((double)best - (double)v[j]) * inv_t);
-    w[j] = !(v[j] < kInf) ? 0.0 : v[j] == best ? 1.0 : best == -kInf ? 0.0 : e;
-  }
-
+  const Parameters q = parameters<FILTER>(p, (int)((unsigned)item / (unsigned)p.n_cv));
+  const bool empty = best == kInf;
+  // what the bound above needs: no overflow in the exponents, a best cost to subtract (or one label that stays)
+  bool unsure = !empty && q.warm && !(q.temperature > 1e-30f && q.temperature < 1e30f && best > -kInf);
+  const float to_exponent = (float)(q.inv_t * 1.4426950408889634);
+  const auto weight = [&](float c) {
+    const float e = __builtin_amdgcn_exp2f((best - c) * to_exponent);
+    return !FILTER || q.warm ? e : c < kInf ? 1.f : 0.f;
+  };
+  float w[NV];
   if (FILTER) {
     const auto worst = [&]() {
       float m = best;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (v[j] < kInf) m = v[j] > m ? v[j] : m;
+      for (int j = 0; j < NV; ++j) m = v[j] < kInf && v[j] > m ? v[j] : m;
       return lanes_max<S>(m);
     };
-    // takes out what is worse than t, and of the labels at t those behind the first `ties`
-    const auto cut = [&](float t, auto stays) {
-      int at = 0;
+    // takes out what is worse than t, and of the `at` labels at t those behind the first `ties`
+    const auto cut = [&](float t, int at, int ties) {
+      if (__builtin_amdgcn_ballot_w64(at > ties) == 0) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) at += v[j] == t ? 1 : 0;
-      int rank = lanes_before<S>(at, s);
+        for (int j = 0; j < NV; ++j) v[j] = v[j] > t ? kInf : v[j];
+        return;
+      }
+      int mine = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) mine += v[j] == t ? 1 : 0;
+      int rank = lanes_before<S>(mine, s);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const bool tie = v[j] == t;
-        if (v[j] > t || (tie && !stays(rank))) {
-          v[j] = kInf;
-          w[j] = 0.0;
-        }
+        if (v[j] > t || (tie && rank >= ties)) v[j] = kInf;
         rank += tie ? 1 : 0;
       }
     };
-    int k = p.top_k != nullptr ? p.top_k[image] : p.top_k_all;
-    if (k <= 0) k = p.n;
-    if (!warm) k = 1;
-    if (k < p.n) {
-      const float t = threshold<NV, S, int>(v, best, worst(), k, [](int) { return 1; });
-      int less = 0;
+    const auto labels_at = [&](float t) {
+      int at = 0;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) less += v[j] < t ? 1 : 0;
-      less = lanes_sum<S>(less);
-      cut(t, [&](int rank) { return less + rank < k; });
-    }
-    const float top_p = p.top_p != nullptr ? p.top_p[image] : p.top_p_all;
-    if (top_p < 1.f) {
-      double total = 0;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) total += w[j];
-      const double target = (double)top_p * lanes_sum<S>(total);
-      const float t = threshold<NV, S, double>(v, best, worst(), target, [&](int j) { return w[j]; });
-      double less = 0, at = 0;
+      for (int j = 0; j < NV; ++j) at += v[j] == t ? 1 : 0;
+      return lanes_sum<S>(at);
+    };
+    // the costs beside mid
+    const auto neighbours = [&](float mid, float& below, float& above) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        less += v[j] < t ? w[j] : 0.0;
-        if (v[j] == t) at = w[j];
+        const bool in = v[j] <= mid;
+        const float b = in ? v[j] : below, a = in ? above : v[j];
+        below = b > below ? b : below;
+        above = a < above ? a : above;
       }
-      less = lanes_sum<S>(less);
-      at = over_lanes<S>(at, [](double a, double b) { return a > b ? a : b; });
-      cut(t, [&](int rank) { return less + rank * at < target || (t == best && rank == 0); });
-    }
-    const float min_p = p.min_p != nullptr ? p.min_p[image] : p.min_p_all;
-    if (positive(min_p)) {
-      const double reach = min_p >= 1.f ? 0.0 : -(double)t32 * log((double)min_p);
+    };
+    if (q.top_k < p.n) {
+      constexpr bool whole = false;  // (whole numbers are never unsure)
+      const auto reached = [&](int labels) { return labels >= q.top_k; };
+      const auto labels_upto = [&](float mid) {
+        int labels = 0;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (v[j] != best && (double)v[j] - (double)best > reach) w[j] = 0.0;
+        for (int j = 0; j < NV; ++j) labels += v[j] <= mid ? 1 : 0;
+        return labels;
+      };
+      float lo = best, hi = q.top_k == 1 ? best : worst();
+      narrow<S>(lo, hi, whole, labels_upto, reached);
+      threshold<S>(
+          lo, hi, whole,
+          [&](float mid, float& below, float& above) {
+            neighbours(mid, below, above);
+            return labels_upto(mid);
+          },
+          reached);
+      const int at = labels_at(hi);
+      cut(hi, at, q.top_k - (lanes_sum<S>(labels_upto(hi)) - at));
     }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) w[j] = weight(v[j]);
+    float t = kInf;
+    int at = 0, ties = 0;
+    if (q.top_p < 1.f) {
+      float total = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) total += w[j];
+      total = lanes_sum<S>(total);
+      const float target = q.top_p * total, near = kNear * total;
+      const auto weight_upto = [&](float mid) {
+        float sum = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) sum += v[j] <= mid ? w[j] : 0.f;
+        return sum;
+      };
+      const auto reached = [&](float sum) {
+        unsure |= fabsf(sum - target) <= near;
+        return sum >= target;
+      };
+      float lo = best, hi = worst();
+      narrow<S>(lo, hi, unsure, weight_upto, reached);
+      threshold<S>(
+          lo, hi, unsure,
+          [&](float mid, float& below, float& above) {
+            neighbours(mid, below, above);
+            return weight_upto(mid);
+          },
+          reached);
+      t = hi;
+      at = ties = labels_at(t);
+      if (__builtin_amdgcn_ballot_w64(at > 1) != 0) {
+        const float each = weight(t);
+        const float left = target - (lanes_sum<S>(weight_upto(t)) - (float)at * each);
+        const float stay = ceilf(left / each);
+        if (at > 1) {
+          // the nearest of the sums that the ties give
+          unsure |= fabsf(left - rintf(left / each) * each) <= 2 * near || !(stay < 512.f);
+          ties = min(at, max(1, (int)stay));
+        }
+      }
+    }
+    if (positive(q.min_p)) {
+      const float far = farthest(q, best);
+      if (far < t) {
+        t = far;
+        at = ties = 0;
+      }
+    }
+    if (t < kInf || __builtin_amdgcn_ballot_w64(t < kInf) != 0) {
+      cut(t, at, ties);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) w[j] = v[j] < kInf ? w[j] : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) w[j] = weight(v[j]);
   }
 
-  int last = 0;
-  double sum = 0;
+  float sum = 0;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    if (w[j] > 0) last = s * NV + j;
     sum += w[j];
     w[j] = sum;
   }
-  const double before = lanes_before<S>(sum, s);
-  // (lanes_sum would add in another order)
-  const double total = over_lanes<S>(before + sum, [](double a, double b) { return a > b ? a : b; });
-  last = over_lanes<S>(last, [](int a, int b) { return a > b ? a : b; });
-  const int64_t at = item * p.pixels + p0 + px;
+  const float before = lanes_before<S>(sum, s);
+  const float total = lanes_max<S>(before + sum);  // (lanes_sum would add in another order)
+  const float near = kNear * total;
+  const int64_t at = item * p.pixels + p0;
+  const int of = min(px, count - 1);
   for (int d = 0; d < p.n_draws; ++d) {
-    const float u = p.uniforms[d * p.items_pixels + at];
-    const double target = (positive(u) ? (double)u : 0.0) * total;
-    int label = 0;
+    const float u = p.uniforms[d * p.items_pixels + at + of];
+    const float target = (positive(u) ? u : 0.f) * total - before;
+    const float low = target - near, high = target + near;
+    int label = 0, most = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) label += before + w[j] <= target ? 1 : 0;
+    for (int j = 0; j < NV; ++j) {
+      label += w[j] <= low ? 1 : 0;
+      most += w[j] <= high ? 1 : 0;
+    }
     label = lanes_sum<S>(label);
-    if (s == 0) p.labels[d * p.items_pixels + at] = (uint8_t)(label < last ? label : last);
+    unsure |= label != lanes_sum<S>(most) || label >= p.n;
+    if (s == 0 && px < count && (empty || !unsure)) p.labels[d * p.items_pixels + at + of] = (uint8_t)(empty ? 0 : label);
+  }
+
+  unsure = unsure && !empty && px < count;
+  if (S == 1) {
+    // (one wavefront)
+    for (uint64_t rest = __builtin_amdgcn_ballot_w64(unsure); rest != 0; rest &= rest - 1) {
+      const int of = __builtin_ctzll(rest);
+      draw_exactly<FILTER>(p, q, at + of, [&](int l) {
+        return LAST ? tile[of * kStride + place(l >> 2) + (l & 3)] : row(l)[of];
+      });
+    }
+  } else {
+    if (unsure && s == 0) atomicOr(&left_over[px >> 5], 1u << (px & 31));
+    __syncthreads();
+    int turn = 0;
+    for (uint64_t rest = (uint64_t)left_over[1] << 32 | left_over[0]; rest != 0; rest &= rest - 1)
+      if (turn++ % S == uniform_i(tid / 64)) {
+        const int of = __builtin_ctzll(rest);
+        draw_exactly<FILTER>(p, q, at + of, [&](int l) { return tile[of * kStride + place(l >> 2) + (l & 3)]; });
+      }
   }
 }
 
@@ -311,36 +640,33 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
   p.n = n_disp;
   p.n_cv = n_cv;
   p.n_draws = n_draws;
+  p.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
+  p.quads = n_disp % 4 == 0 && ((uintptr_t)cost & 15) == 0;
   const bool filter = temperatures != nullptr || !(temperature > 0) || top_ks != nullptr || (top_k > 0 && top_k < n_disp) ||
                       top_ps != nullptr || top_p < 1.f || min_ps != nullptr || min_p > 0.f;
   const unsigned blocks = (unsigned)(tiles * items);
   const hipStream_t st = (hipStream_t)stream;
   const bool lf = labels_first != 0;
-  // 16 labels a lane at most, in fours
-  if (n_disp <= 4)
-    launch<4, 1>(p, filter, lf, blocks, st);
-  else if (n_disp <= 8)
+  if (n_disp <= 8)
     launch<8, 1>(p, filter, lf, blocks, st);
-  else if (n_disp <= 12)
-    launch<12, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 16)
     launch<16, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 24)
-    launch<12, 2>(p, filter, lf, blocks, st);
+    launch<24, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 32)
-    launch<16, 2>(p, filter, lf, blocks, st);
+    launch<32, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 48)
-    launch<12, 4>(p, filter, lf, blocks, st);
+    launch<24, 2>(p, filter, lf, blocks, st);
   else if (n_disp <= 64)
-    launch<16, 4>(p, filter, lf, blocks, st);
+    launch<32, 2>(p, filter, lf, blocks, st);
   else if (n_disp <= 96)
-    launch<12, 8>(p, filter, lf, blocks, st);
+    launch<24, 4>(p, filter, lf, blocks, st);
   else if (n_disp <= 128)
-    launch<16, 8>(p, filter, lf, blocks, st);
+    launch<32, 4>(p, filter, lf, blocks, st);
   else if (n_disp <= 192)
-    launch<12, 16>(p, filter, lf, blocks, st);
+    launch<24, 8>(p, filter, lf, blocks, st);
   else
-    launch<16, 16>(p, filter, lf, blocks, st);
+    launch<32, 8>(p, filter, lf, blocks, st);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "sample_labels: %s", hipGetErrorString(e));
 }

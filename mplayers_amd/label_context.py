@@ -112,17 +112,23 @@ def label_buckets(n_classes, n_buckets, max_distance=None):
   return torch.tensor([min(k, n_classes) for k in starts] + [n_classes], dtype=torch.int32)
 
 
-def _bucket_call(name, src, starts, square, shape):
-  src = src.contiguous()
-  out = torch.empty(shape, dtype=torch.float32, device=src.device)
-  n_buckets, n = starts.numel() - 1, int(starts[-1])
-  lead = out.numel() // (n_buckets if name == 'mpl_bucket_sums' else n * n if square else n)
-  if lead == 0:
-    return out
-  with torch.cuda.device(src.device):
-    rc = getattr(_lib.load(), name)(src.data_ptr(), starts.data_ptr(), lead, n_buckets, n, square, out.data_ptr(),
-                                    torch.cuda.current_stream().cuda_stream)
-  _lib.check(rc, name[4:])
+def _expand(table, starts, n, square):
+  table = table.contiguous()
+  out = torch.empty(table.shape[:-1] + ((n, n) if square else (n,)), dtype=torch.float32, device=table.device)
+  n_buckets = table.size(-1)
+  if table.numel():
+    _lib.launch('mpl_bucket_context', table, table.data_ptr(), starts.data_ptr(), table.numel() // n_buckets, n_buckets,
+                n, square, out.data_ptr())
+  return out
+
+
+def _sums(grad, starts, n, square):
+  grad = grad.contiguous()
+  n_buckets = starts.numel() - 1
+  out = torch.empty(grad.shape[:-2 if square else -1] + (n_buckets,), dtype=torch.float32, device=grad.device)
+  if out.numel():
+    _lib.launch('mpl_bucket_sums', grad, grad.data_ptr(), starts.data_ptr(), out.numel() // n_buckets, n_buckets, n,
+                square, out.data_ptr())
   return out
 
 
@@ -130,29 +136,26 @@ class _BucketContext(torch.autograd.Function):
   """(..., n_buckets) -> (..., n) or (..., n, n)."""
 
   @staticmethod
-  def forward(ctx, table, starts, square):
-    ctx.rest = (starts, square)
-    n = int(starts[-1])
-    return _bucket_call('mpl_bucket_context', table, starts, square,
-                        tuple(table.shape[:-1]) + ((n, n) if square else (n,)))
+  def forward(ctx, table, starts, n, square):
+    ctx.rest = (starts, n, square)
+    return _expand(table, starts, n, square)
 
   @staticmethod
   def backward(ctx, grad):
-    return _BucketSums.apply(grad, *ctx.rest), None, None
+    return (_BucketSums.apply if torch.is_grad_enabled() else _sums)(grad, *ctx.rest), None, None, None
 
 
 class _BucketSums(torch.autograd.Function):
   """The gradient of _BucketContext; linear, so its gradient is _BucketContext."""
 
   @staticmethod
-  def forward(ctx, grad, starts, square):
-    ctx.rest = (starts, square)
-    return _bucket_call('mpl_bucket_sums', grad, starts, square,
-                        tuple(grad.shape[:-2 if square else -1]) + (starts.numel() - 1,))
+  def forward(ctx, grad, starts, n, square):
+    ctx.rest = (starts, n, square)
+    return _sums(grad, starts, n, square)
 
   @staticmethod
   def backward(ctx, grad):
-    return _BucketContext.apply(grad, *ctx.rest), None, None
+    return _BucketContext.apply(grad, *ctx.rest), None, None, None
 
 
 def bucket_context(table, starts, square=False, symmetric=True):
@@ -172,7 +175,8 @@ def bucket_context(table, starts, square=False, symmetric=True):
     raise RuntimeError('bucket_context: table has %s entries for %d buckets' %
                        (table.size(-1) if table.dim() else 'no', starts.numel() - 1))
   if table.is_cuda:
-    return _BucketContext.apply(table, starts, 0 if not square else 2 if symmetric else 1)
+    call = _BucketContext.apply if table.requires_grad and torch.is_grad_enabled() else _expand
+    return call(table, starts, int(starts[-1]), 0 if not square else 2 if symmetric else 1)
   if int(starts[0]) != 0 or bool((starts[1:] < starts[:-1]).any()):
     raise RuntimeError('bucket_context: the buckets must be in order, from distance 0')
   bucket = torch.repeat_interleave(torch.arange(starts.numel() - 1), (starts[1:] - starts[:-1]).long())

@@ -83,14 +83,24 @@ _DROPOUT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # MPL_
 _DROPOUT_SHARES = {"element": 0, "pixel": 1, "label": 2}  # MPL_DROPOUT_*
 
 
-def _dropout(call, dtype, share, p, state, src, dst, batch, n, pixels):
-  if src.numel() == 0:
-    return dst
-  with torch.cuda.device(src.device):
-    rc = getattr(_lib.load(), call)(_DROPOUT_TYPES[dtype], _DROPOUT_SHARES[share], p, state.data_ptr(), src.data_ptr(),
-                                    dst.data_ptr(), batch, n, pixels, torch.cuda.current_stream().cuda_stream)
-  _lib.check(rc, call[4:])
-  return dst
+def _dropout_last(x, state, p, share):
+  b, cv, n, h, w = x.shape
+  x = x.contiguous()
+  out = torch.empty((b, cv, h, w, n), dtype=torch.float32, device=x.device)
+  if out.numel():
+    _lib.launch("mpl_dropout_labels_last", x, _DROPOUT_TYPES[x.dtype], share, p, state.data_ptr(), x.data_ptr(),
+                out.data_ptr(), b * cv, n, h * w)
+  return out
+
+
+def _dropout_first(grad, state, p, share, dtype):
+  b, cv, h, w, n = grad.shape
+  grad = grad.contiguous()
+  out = torch.empty((b, cv, n, h, w), dtype=dtype, device=grad.device)
+  if out.numel():
+    _lib.launch("mpl_dropout_labels_first", grad, _DROPOUT_TYPES[dtype], share, p, state.data_ptr(), grad.data_ptr(),
+                out.data_ptr(), b * cv, n, h * w)
+  return out
 
 
 class _DropoutLast(torch.autograd.Function):
@@ -100,14 +110,12 @@ class _DropoutLast(torch.autograd.Function):
   def forward(ctx, x, state, p, share):
     ctx.save_for_backward(state)
     ctx.rest = (p, share, x.dtype)
-    b, cv, n, h, w = x.shape
-    return _dropout("mpl_dropout_labels_last", x.dtype, share, p, state, x.contiguous(),
-                    torch.empty((b, cv, h, w, n), dtype=torch.float32, device=x.device), b * cv, n, h * w)
+    return _dropout_last(x, state, p, share)
 
   @staticmethod
   def backward(ctx, grad):
-    p, share, dtype = ctx.rest
-    return _DropoutFirst.apply(grad, ctx.saved_tensors[0], p, share, dtype), None, None, None
+    call = _DropoutFirst.apply if torch.is_grad_enabled() else _dropout_first
+    return call(grad, ctx.saved_tensors[0], *ctx.rest), None, None, None
 
 
 class _DropoutFirst(torch.autograd.Function):
@@ -117,14 +125,11 @@ class _DropoutFirst(torch.autograd.Function):
   def forward(ctx, grad, state, p, share, dtype):
     ctx.save_for_backward(state)
     ctx.rest = (p, share)
-    b, cv, h, w, n = grad.shape
-    return _dropout("mpl_dropout_labels_first", dtype, share, p, state, grad.contiguous(),
-                    torch.empty((b, cv, n, h, w), dtype=dtype, device=grad.device), b * cv, n, h * w)
+    return _dropout_first(grad, state, p, share, dtype)
 
   @staticmethod
   def backward(ctx, grad):
-    p, share = ctx.rest
-    return _DropoutLast.apply(grad, ctx.saved_tensors[0], p, share), None, None, None, None
+    return _DropoutLast.apply(grad, ctx.saved_tensors[0], *ctx.rest), None, None, None, None
 
 
 def labels_last_dropout(x, p, state, share="element"):
@@ -151,4 +156,5 @@ def labels_last_dropout(x, p, state, share="element"):
     raise RuntimeError("labels_last_dropout: p must be in [0, 1], got %r" % (p,))
   if share not in _DROPOUT_SHARES:
     raise RuntimeError("labels_last_dropout: share must be 'element', 'pixel' or 'label', got %r" % (share,))
-  return _DropoutLast.apply(x, state, float(p), share)
+  call = _DropoutLast.apply if x.requires_grad and torch.is_grad_enabled() else _dropout_last
+  return call(x, state, float(p), _DROPOUT_SHARES[share])

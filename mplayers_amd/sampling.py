@@ -63,9 +63,6 @@ def sample_labels(cost, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
   ps, p = _parameter("top_p", top_p, batch, cost, f32, 0.0, 1.0)
   ms, m = _parameter("min_p", min_p, batch, cost, f32, 0.0, 1.0)
   labels = torch.empty(uniforms.shape, dtype=torch.uint8, device=cost.device)
-  with torch.cuda.device(cost.device):
-    rc = _lib.load().mpl_sample_labels(
-        int(bool(labels_first)), cost.data_ptr(), uniforms.data_ptr(), batch, cv, n, height * width, draws, ts, t, ks,
-        k, ps, p, ms, m, labels.data_ptr(), torch.cuda.current_stream().cuda_stream)
-  _lib.check(rc, "sample_labels")
+  _lib.launch("mpl_sample_labels", cost, int(bool(labels_first)), cost.data_ptr(), uniforms.data_ptr(), batch, cv, n,
+              height * width, draws, ts, t, ks, k, ps, p, ms, m, labels.data_ptr())
   return labels
