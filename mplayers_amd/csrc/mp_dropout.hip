@@ -23,11 +23,14 @@ enum Share { kElement = MPL_DROPOUT_ELEMENT, kPixel = MPL_DROPOUT_PIXEL, kLabel 
 
 struct Dropout {
   const int64_t* state;  // seed, offset
-  int64_t pixels, tiles;
-  int labels;
+  int64_t pixels;
+  int tiles, labels;
   uint32_t bound;  // words from this on stay
   int nothing;     // rate 1
   float scale;
+  uint32_t reciprocal;  // 2^32 / labels, rounded up
+  int whole_quads;      // the label-innermost side: labels in fours, all aligned
+  int xcd_group;        // tiles beside each other that go to one die (xcd_block)
 };
 
 struct Words {
@@ -50,16 +53,19 @@ __device__ __forceinline__ Words random_words(uint64_t group, uint64_t offset, u
   return Words{{c0, c1, c2, c3}};
 }
 
-// which labels of quad q of a pixel stay, as factors
+// Bits 0 to 3: which labels of quad q of a pixel stay.
 template <int SHARE>
-__device__ __forceinline__ void factors(const Dropout& d, int64_t item, int64_t pixel, int q, int quads, uint64_t seed,
-                                        uint64_t offset, bool keep[4]) {
+__device__ __forceinline__ int stays(const Dropout& d, int64_t item, int64_t pixel, int q, int quads, uint64_t seed,
+                                     uint64_t offset) {
   const uint64_t group = SHARE == kElement ? (uint64_t)(item * d.pixels + pixel) * (uint64_t)quads + (uint64_t)q
                          : SHARE == kPixel ? (uint64_t)(item * d.pixels + pixel)
                                            : (uint64_t)item * (uint64_t)quads + (uint64_t)q;
   const Words r = random_words(group, offset, seed);
+  if (SHARE == kPixel) return r.w[0] >= d.bound && !d.nothing ? 15 : 0;
+  int bits = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) keep[j] = r.w[SHARE == kPixel ? 0 : j] >= d.bound && !d.nothing;
+  for (int j = 0; j < 4; ++j) bits |= r.w[j] >= d.bound && !d.nothing ? 1 << j : 0;
+  return bits;
 }
 
 // An fp32 product, rounded as such before a narrower type rounds it again: the compiler would make one instruction
@@ -70,54 +76,127 @@ __device__ __forceinline__ float scaled(float x, float scale) {
   return y;
 }
 
-// One tile of kPixels pixels and all labels per workgroup of 64 x 4 threads.  LAST: into the label-innermost layout.
-template <typename T, int SHARE, bool LAST>
-__global__ void __launch_bounds__(256) dropout_kernel(Dropout d, const void* __restrict__ src, void* __restrict__ dst) {
-  extern __shared__ float tile[];  // [pixel][labels | 1]
-  const int64_t block = (int64_t)blockIdx.x;
-  const int64_t item = block / d.tiles, p0 = (block - item * d.tiles) * kPixels;
-  const int px = (int)threadIdx.x, ty = (int)threadIdx.y, tid = ty * kPixels + px;
-  const int n = d.labels, stride = n | 1, quads = (n + 3) >> 2;
+// One tile of kPixels pixels and all labels per workgroup of W wavefronts, so that the label-innermost side is one run
+// of memory whatever the number of labels.  Wavefront w takes the quads w + i * W, i < J, with a lane per pixel: 256
+// contiguous bytes of a label's row (fp32) to an instruction.  The tile lies in LDS with the labels of a pixel side by
+// side, an odd number of quads apart, which keeps the 16-byte accesses of either side off each other's banks.
+//
+// The random words are formed between the loads and their first use.  What lies behind the last label or pixel is
+// loaded from the last's place, so that there is no branch between the loads.
+//
+// LAST: into the label-innermost layout, else its gradient back.
+template <typename T, int SHARE, bool LAST, int W, int J>
+__global__ void __launch_bounds__(kPixels* W) dropout_kernel(Dropout d, const void* __restrict__ src,
+                                                             void* __restrict__ dst) {
+  constexpr int kStride = 4 * (W * J | 1);
+  __shared__ __align__(16) float tile[kPixels * kStride];
+  const unsigned block = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, d.xcd_group);
+  const unsigned of_item = block / (unsigned)d.tiles;
+  const int64_t item = of_item, p0 = (int64_t)(block - of_item * (unsigned)d.tiles) * kPixels;
+  const int tid = (int)threadIdx.x, px = tid % kPixels, wave = uniform_i(tid / kPixels);
+  const int n = d.labels, quads = (n + 3) >> 2;
   const int count = (int)min((int64_t)kPixels, d.pixels - p0);
-  const uint64_t seed = (uint64_t)d.state[0], offset = (uint64_t)d.state[1];
+  const unsigned total = (unsigned)(count * n);
   const int64_t first = item * n * d.pixels;
-  const float* last_in = (const float*)src + first + p0 * n;
-  float* last_out = (float*)dst + first + p0 * n;
-  const T* rows_in = (const T*)src + first + p0;
-  T* rows_out = (T*)dst + first + p0;
-  if (!LAST) {
-    for (int i = tid; i < count * n; i += 256) tile[i / n * stride + i % n] = last_in[i];
+  const uint64_t seed = (uint64_t)d.state[0], offset = (uint64_t)d.state[1];
+  const int of = min(px, count - 1);
+  const auto place = [&](unsigned i) {  // of entry i of the label-innermost run
+    const unsigned p = n == 1 ? i : __umulhi(i, d.reciprocal);
+    return p * kStride + (i - p * (unsigned)n);
+  };
+  int keep[J];
+  const auto form_masks = [&]() {
+    const int all = SHARE == kPixel ? stays<SHARE>(d, item, p0 + of, 0, quads, seed, offset) : 0;
+#pragma unroll
+    for (int i = 0; i < J; ++i)
+      keep[i] = SHARE == kPixel ? all : stays<SHARE>(d, item, p0 + of, wave + i * W, quads, seed, offset);
+  };
+  if (LAST) {
+    const T* from = (const T*)src + first + p0;
+    T x[J][4];
+#pragma unroll
+    for (int i = 0; i < J; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] = from[(int64_t)min(4 * (wave + i * W) + j, n - 1) * d.pixels + of];
+    form_masks();
+#pragma unroll
+    for (int i = 0; i < J; ++i) {
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = keep[i] >> j & 1 ? (float)x[i][j] * d.scale : 0.f;
+      *reinterpret_cast<float4*>(&tile[px * kStride + 4 * (wave + i * W)]) = float4{y[0], y[1], y[2], y[3]};
+    }
     __syncthreads();
-  }
-  if (px < count) {
-    for (int q = ty; q < quads; q += 4) {
-      bool keep[4];
-      factors<SHARE>(d, item, p0 + px, q, quads, seed, offset, keep);
-      for (int j = 0; j < 4 && 4 * q + j < n; ++j) {
-        const int l = 4 * q + j;
-        if (LAST)
-          tile[px * stride + l] = keep[j] ? (float)rows_in[l * d.pixels + px] * d.scale : 0.f;
-        else
-          rows_out[l * d.pixels + px] = (T)(keep[j] ? scaled(tile[px * stride + l], d.scale) : 0.f);
+    float* to = (float*)dst + first + p0 * n;
+    if (d.whole_quads) {
+      for (unsigned i = (unsigned)tid * 4; i < total; i += kPixels * W * 4)
+        *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(&tile[place(i)]);
+    } else {
+      for (unsigned i = (unsigned)tid; i < total; i += kPixels * W) to[i] = tile[place(i)];
+    }
+  } else {
+    const float* from = (const float*)src + first + p0 * n;
+    if (d.whole_quads) {
+      float4 x[J];
+#pragma unroll
+      for (int k = 0; k < J; ++k)
+        x[k] = *reinterpret_cast<const float4*>(from + min((unsigned)(tid + k * kPixels * W) * 4, total - 4));
+      form_masks();
+#pragma unroll
+      for (int k = 0; k < J; ++k)
+        *reinterpret_cast<float4*>(&tile[place(min((unsigned)(tid + k * kPixels * W) * 4, total - 4))]) = x[k];
+    } else {
+      float x[4 * J];
+#pragma unroll
+      for (int k = 0; k < 4 * J; ++k) x[k] = from[min((unsigned)(tid + k * kPixels * W), total - 1)];
+      form_masks();
+#pragma unroll
+      for (int k = 0; k < 4 * J; ++k) tile[place(min((unsigned)(tid + k * kPixels * W), total - 1))] = x[k];
+    }
+    __syncthreads();
+    if (px >= count) return;
+    T* to = (T*)dst + first + p0 + px;
+#pragma unroll
+    for (int i = 0; i < J; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(&tile[px * kStride + 4 * (wave + i * W)]);
+      const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int l = 4 * (wave + i * W) + j;
+        if (l < n) to[(int64_t)l * d.pixels] = (T)(keep[i] >> j & 1 ? scaled(y[j], d.scale) : 0.f);
       }
     }
   }
-  if (LAST) {
-    __syncthreads();
-    for (int i = tid; i < count * n; i += 256) last_out[i] = tile[i / n * stride + i % n];
-  }
 }
 
+template <typename T, int SHARE, bool LAST>
+void launch_share(const Dropout& d, const void* src, void* dst, unsigned blocks, hipStream_t st) {
+  const int n = d.labels;
+  if (n <= 8)
+    dropout_kernel<T, SHARE, LAST, 1, 2><<<blocks, kPixels, 0, st>>>(d, src, dst);
+  else if (n <= 16)
+    dropout_kernel<T, SHARE, LAST, 1, 4><<<blocks, kPixels, 0, st>>>(d, src, dst);
+  else if (n <= 24)
+    dropout_kernel<T, SHARE, LAST, 1, 6><<<blocks, kPixels, 0, st>>>(d, src, dst);
+  else if (n <= 48)
+    dropout_kernel<T, SHARE, LAST, 2, 6><<<blocks, 2 * kPixels, 0, st>>>(d, src, dst);
+  else if (n <= 96)
+    dropout_kernel<T, SHARE, LAST, 4, 6><<<blocks, 4 * kPixels, 0, st>>>(d, src, dst);
+  else if (n <= 128)
+    dropout_kernel<T, SHARE, LAST, 8, 4><<<blocks, 8 * kPixels, 0, st>>>(d, src, dst);
+  else if (n <= 192)
+    dropout_kernel<T, SHARE, LAST, 8, 6><<<blocks, 8 * kPixels, 0, st>>>(d, src, dst);
+  else
+    dropout_kernel<T, SHARE, LAST, 8, 8><<<blocks, 8 * kPixels, 0, st>>>(d, src, dst);
+}
 template <typename T, bool LAST>
 void launch(int share, const Dropout& d, const void* src, void* dst, unsigned blocks, hipStream_t st) {
-  const dim3 block(kPixels, 4);
-  const size_t lds = (size_t)kPixels * (size_t)(d.labels | 1) * sizeof(float);
   if (share == kElement)
-    dropout_kernel<T, kElement, LAST><<<blocks, block, lds, st>>>(d, src, dst);
+    launch_share<T, kElement, LAST>(d, src, dst, blocks, st);
   else if (share == kPixel)
-    dropout_kernel<T, kPixel, LAST><<<blocks, block, lds, st>>>(d, src, dst);
+    launch_share<T, kPixel, LAST>(d, src, dst, blocks, st);
   else
-    dropout_kernel<T, kLabel, LAST><<<blocks, block, lds, st>>>(d, src, dst);
+    launch_share<T, kLabel, LAST>(d, src, dst, blocks, st);
 }
 
 template <bool LAST>
@@ -130,16 +209,21 @@ int run(const char* what, int dtype, int share, double rate, const int64_t* stat
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
   if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
   if (batch == 0 || pixels == 0) return MPL_OK;
+  const int64_t tiles = (pixels + kPixels - 1) / kPixels;
+  if (pixels > ((int64_t)1 << 40) || tiles * batch > 0x7fffffff) return fail(MPL_EINVAL, "%s: too many pixels", what);
   Dropout d;
   d.state = state;
   d.pixels = pixels;
-  d.tiles = (pixels + kPixels - 1) / kPixels;
+  d.tiles = (int)tiles;
   d.labels = n_disp;
-  if (pixels > ((int64_t)1 << 40) || d.tiles * batch > 0x7fffffff) return fail(MPL_EINVAL, "%s: too many pixels", what);
+  d.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
+  d.whole_quads = n_disp % 4 == 0 && ((uintptr_t)(LAST ? dst : src) & 15) == 0;
+  // where rows are not whole cache lines the tiles beside each other share lines
+  d.xcd_group = pixels * (dtype == MPL_F32 ? 4 : 2) % kLineBytes != 0 ? 8 : 0;
   d.nothing = rate >= 1;
   d.bound = d.nothing ? 0u : (uint32_t)(rate * 4294967296.0);
   d.scale = d.nothing ? 0.f : (float)(1.0 / (1.0 - rate));
-  const unsigned blocks = (unsigned)(d.tiles * batch);
+  const unsigned blocks = (unsigned)(tiles * batch);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == MPL_F32)
     launch<float, LAST>(share, d, src, dst, blocks, st);
