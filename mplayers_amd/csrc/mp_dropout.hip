@@ -174,25 +174,32 @@ __global__ void __launch_bounds__(kPixels* W) dropout_kernel(Dropout d, const vo
   }
 }
 
+// Wavefronts W and quads J to a wavefront.  Small launches do not fill the chip: up to eight wavefronts share a tile
+// before one takes a second quad of each.
 template <typename T, int SHARE, bool LAST>
 void launch_share(const Dropout& d, const void* src, void* dst, unsigned blocks, hipStream_t st) {
+  const auto run = [&](auto kernel, int waves) { kernel<<<blocks, kPixels * waves, 0, st>>>(d, src, dst); };
   const int n = d.labels;
   if (n <= 8)
-    dropout_kernel<T, SHARE, LAST, 1, 2><<<blocks, kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 2, 1>, 2);
   else if (n <= 16)
-    dropout_kernel<T, SHARE, LAST, 1, 4><<<blocks, kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 4, 1>, 4);
   else if (n <= 24)
-    dropout_kernel<T, SHARE, LAST, 1, 6><<<blocks, kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 3, 2>, 3);
+  else if (n <= 32)
+    run(dropout_kernel<T, SHARE, LAST, 4, 2>, 4);
   else if (n <= 48)
-    dropout_kernel<T, SHARE, LAST, 2, 6><<<blocks, 2 * kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 6, 2>, 6);
+  else if (n <= 64)
+    run(dropout_kernel<T, SHARE, LAST, 8, 2>, 8);
   else if (n <= 96)
-    dropout_kernel<T, SHARE, LAST, 4, 6><<<blocks, 4 * kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 8, 3>, 8);
   else if (n <= 128)
-    dropout_kernel<T, SHARE, LAST, 8, 4><<<blocks, 8 * kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 8, 4>, 8);
   else if (n <= 192)
-    dropout_kernel<T, SHARE, LAST, 8, 6><<<blocks, 8 * kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 8, 6>, 8);
   else
-    dropout_kernel<T, SHARE, LAST, 8, 8><<<blocks, 8 * kPixels, 0, st>>>(d, src, dst);
+    run(dropout_kernel<T, SHARE, LAST, 8, 8>, 8);
 }
 template <typename T, bool LAST>
 void launch(int share, const Dropout& d, const void* src, void* dst, unsigned blocks, hipStream_t st) {
