@@ -20,6 +20,7 @@ using namespace mpl;
 namespace {
 
 constexpr int kPixels = 64;  // pixels of a workgroup
+constexpr int kSearchFrom = 2;
 
 struct Sample {
   const float* cost;
@@ -120,30 +121,10 @@ __device__ __forceinline__ V lanes_before(V x, int s) {
   return s == 0 ? V(0) : left;
 }
 
-// The range lo <= t <= hi of the least cost t with sum(of labels with cost <= t) >= target; hi where no sum reaches it.
-// reached(sum) decides, or sets `unsure`, which ends the search where it is.
-//
-// narrow() halves it without looking for costs that occur, which takes less than half the instructions of a step of
-// threshold(), which closes it: there sum_upto(mid, below, above) also takes the greatest cost that is not above mid
-// and the least that is.  lo is a cost that occurs, or one that t is above.
-constexpr int kCoarse = 5;
-template <int S, typename SumUpTo, typename Reached>
-__device__ __forceinline__ void narrow(float& lo, float& hi, const bool& unsure, SumUpTo sum_upto, Reached reached) {
-#pragma unroll 1
-  for (int step = 0; step < kCoarse; ++step) {
-    const float mid = 0.5f * lo + 0.5f * hi;
-    const auto sum = lanes_sum<S>(sum_upto(mid));
-    if (mid > lo && mid < hi) {
-      const bool down = reached(sum);
-      if (!unsure) {
-        if (down)
-          hi = mid;
-        else
-          lo = mid;
-      }
-    }
-  }
-}
+// Closes the range lo <= t <= hi of the least cost t with sum(of labels with cost <= t) >= target; hi where no sum
+// reaches it.  sum_upto(mid, below, above) gives the sum, the greatest cost that is not above mid and the least that
+// is; reached(sum) decides, or sets `unsure`, which ends the search where it is.  lo is a cost that occurs, or one
+// that t is above.
 template <int S, typename SumUpTo, typename Reached>
 __device__ __forceinline__ void threshold(float& lo, float& hi, const bool& unsure, SumUpTo sum_upto, Reached reached) {
 #pragma unroll 1
@@ -168,6 +149,85 @@ __device__ __forceinline__ void threshold(float& lo, float& hi, const bool& unsu
         else
           lo = above;
       }
+    }
+  }
+}
+
+// The same for the costs v of a lane, in steps of a third and half the instructions: a few that only halve the range,
+// then from its lower end up from one cost to the next.  What that leaves open, costs close together in a wide range,
+// threshold() closes.  On return t is the cost, `at` the number of labels at it, `less` the sum of those below.
+//   value(a)      what a label of cost a adds
+//   sum_upto(c)   this lane's sum of the labels with cost <= c
+constexpr int kHalves = 5, kSteps = 4;
+template <int NV, int S, typename V, typename Value, typename SumUpTo, typename Reached>
+__device__ __forceinline__ void find(const float (&v)[NV], float best, float worst, bool& unsure, Value value,
+                                     SumUpTo sum_upto, Reached reached, float& t, int& at, V& less) {
+  // t > lo, and less is the sum up to lo
+  float lo = best - (fabsf(best) * 0x1p-20f + 0x1p-100f), hi = worst;
+  less = V(0);
+#pragma unroll 1
+  for (int step = 0; step < kHalves; ++step) {
+    const float mid = 0.5f * lo + 0.5f * hi;
+    const V sum = lanes_sum<S>(sum_upto(mid));
+    if (mid > lo && mid < hi) {
+      const bool down = reached(sum);
+      hi = down && !unsure ? mid : hi;
+      lo = down || unsure ? lo : mid;
+      less = down || unsure ? less : sum;
+    }
+  }
+  bool open = true;
+  t = hi;
+  at = 0;
+#pragma unroll 1
+  for (int step = 0; step < kSteps && __builtin_amdgcn_ballot_w64(open && !unsure) != 0; ++step) {
+    float next = kInf;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const float above = v[j] > lo ? v[j] : kInf;
+      next = above < next ? above : next;
+    }
+    next = lanes_min<S>(next);
+    int labels = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) labels += v[j] == next ? 1 : 0;
+    labels = lanes_sum<S>(labels);
+    if (open) {
+      const V sum = less + (V)labels * value(next);
+      if (!(next < kInf) || reached(sum)) {
+        open = false;
+        t = next;
+        at = labels;
+      } else {
+        lo = next;
+        less = sum;
+      }
+    }
+  }
+  if (__builtin_amdgcn_ballot_w64(open && !unsure) != 0) {
+    if (!open) lo = hi = t;
+    threshold<S>(
+        lo, hi, unsure,
+        [&](float mid, float& below, float& above) {
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const bool in = v[j] <= mid;
+            const float b = in ? v[j] : below, a = in ? above : v[j];
+            below = b > below ? b : below;
+            above = a < above ? a : above;
+          }
+          return sum_upto(mid);
+        },
+        reached);
+    int labels = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) labels += v[j] == hi ? 1 : 0;
+    labels = lanes_sum<S>(labels);
+    const V sum = lanes_sum<S>(sum_upto(hi));
+    if (open) {
+      t = hi;
+      at = labels;
+      less = sum - (V)labels * value(hi);
     }
   }
 }
@@ -343,13 +403,13 @@ __device__ void draw_exactly(const Sample& p, const Parameters& q, int64_t at, C
 // and as much for a target, which is a product with such a sum (and is rounded itself).  Where a sum is as close to a
 // target as both (kNear), 32 bits do not tell, and draw_exactly() takes the pixel: with costs as a layer gives them one
 // draw in 400 of 192 labels, one in 4000 of 21.
-template <int NV, int S, bool FILTER, bool LAST>
+template <int NV, int S, bool FILTER, bool LAST, bool SEARCH>
 __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
   constexpr int kQuads = S * NV / 4, kJ = NV / 4;  // of four labels: in all, per lane
   constexpr int kStride = 4 * (kQuads | 1);
-  constexpr bool kTile = S > 1 || LAST;  // through LDS
+  constexpr bool kTile = S > 1 || LAST;  // costs through LDS
   constexpr float kNear = 2 * (NV + S + 25) * 0x1p-24f;
-  __shared__ __align__(16) float tile[kTile ? kPixels * kStride : 4];
+  __shared__ __align__(16) float tile[kTile || SEARCH ? kPixels * kStride : 4];
   __shared__ uint32_t left_over[2];  // pixels for draw_exactly()
   const unsigned block = blockIdx.x, tiles = (unsigned)p.tiles;
   const int64_t item = block / tiles, p0 = (int64_t)(block - (unsigned)item * tiles) * kPixels;
@@ -428,12 +488,6 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
   };
   float w[NV];
   if (FILTER) {
-    const auto worst = [&]() {
-      float m = best;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) m = v[j] < kInf && v[j] > m ? v[j] : m;
-      return lanes_max<S>(m);
-    };
     // takes out what is worse than t, and of the `at` labels at t those behind the first `ties`
     const auto cut = [&](float t, int at, int ties) {
       if (__builtin_amdgcn_ballot_w64(at > ties) == 0) {
@@ -452,42 +506,25 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
         rank += tie ? 1 : 0;
       }
     };
-    const auto labels_at = [&](float t) {
-      int at = 0;
+    float worst = best;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) at += v[j] == t ? 1 : 0;
-      return lanes_sum<S>(at);
-    };
-    // the costs beside mid
-    const auto neighbours = [&](float mid, float& below, float& above) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const bool in = v[j] <= mid;
-        const float b = in ? v[j] : below, a = in ? above : v[j];
-        below = b > below ? b : below;
-        above = a < above ? a : above;
-      }
-    };
+    for (int j = 0; j < NV; ++j) worst = v[j] < kInf && v[j] > worst ? v[j] : worst;
+    worst = lanes_max<S>(worst);
     if (q.top_k < p.n) {
-      constexpr bool whole = false;  // (whole numbers are never unsure)
-      const auto reached = [&](int labels) { return labels >= q.top_k; };
-      const auto labels_upto = [&](float mid) {
-        int labels = 0;
+      bool whole = false;  // (whole numbers are never unsure)
+      int at, less;
+      float t;
+      find<NV, S>(
+          v, best, q.top_k == 1 ? best : worst, whole, [](float) { return 1; },
+          [&](float mid) {
+            int labels = 0;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) labels += v[j] <= mid ? 1 : 0;
-        return labels;
-      };
-      float lo = best, hi = q.top_k == 1 ? best : worst();
-      narrow<S>(lo, hi, whole, labels_upto, reached);
-      threshold<S>(
-          lo, hi, whole,
-          [&](float mid, float& below, float& above) {
-            neighbours(mid, below, above);
-            return labels_upto(mid);
+            for (int j = 0; j < NV; ++j) labels += v[j] <= mid ? 1 : 0;
+            return labels;
           },
-          reached);
-      const int at = labels_at(hi);
-      cut(hi, at, q.top_k - (lanes_sum<S>(labels_upto(hi)) - at));
+          [&](int labels) { return labels >= q.top_k; }, t, at, less);
+      cut(t, at, q.top_k - less);
+      worst = t < worst ? t : worst;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) w[j] = weight(v[j]);
@@ -499,30 +536,26 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
       for (int j = 0; j < NV; ++j) total += w[j];
       total = lanes_sum<S>(total);
       const float target = q.top_p * total, near = kNear * total;
-      const auto weight_upto = [&](float mid) {
-        float sum = 0;
+      // Labels further than T * ln(2 n / (1 - top_p)) from the best weigh less than half of what may go.
+      const float rest = 1.f - q.top_p;
+      const float reach = rest > 1e-3f ? q.temperature * __logf(2.f * (float)p.n / rest) : kInf;
+      float less;
+      find<NV, S>(
+          v, best, best + reach < worst ? best + reach : worst, unsure, weight,
+          [&](float mid) {
+            float sum = 0;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) sum += v[j] <= mid ? w[j] : 0.f;
-        return sum;
-      };
-      const auto reached = [&](float sum) {
-        unsure |= fabsf(sum - target) <= near;
-        return sum >= target;
-      };
-      float lo = best, hi = worst();
-      narrow<S>(lo, hi, unsure, weight_upto, reached);
-      threshold<S>(
-          lo, hi, unsure,
-          [&](float mid, float& below, float& above) {
-            neighbours(mid, below, above);
-            return weight_upto(mid);
+            for (int j = 0; j < NV; ++j) sum += v[j] <= mid ? w[j] : 0.f;
+            return sum;
           },
-          reached);
-      t = hi;
-      at = ties = labels_at(t);
+          [&](float sum) {
+            unsure |= fabsf(sum - target) <= near;
+            return sum >= target;
+          },
+          t, at, less);
+      ties = at;
       if (__builtin_amdgcn_ballot_w64(at > 1) != 0) {
-        const float each = weight(t);
-        const float left = target - (lanes_sum<S>(weight_upto(t)) - (float)at * each);
+        const float each = weight(t), left = target - less;
         const float stay = ceilf(left / each);
         if (at > 1) {
           // the nearest of the sums that the ties give
@@ -559,49 +592,89 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
   const float near = kNear * total;
   const int64_t at = item * p.pixels + p0;
   const int of = min(px, count - 1);
-  for (int d = 0; d < p.n_draws; ++d) {
-    const float u = p.uniforms[d * p.items_pixels + at + of];
-    const float target = (positive(u) ? u : 0.f) * total - before;
-    const float low = target - near, high = target + near;
-    int label = 0, most = 0;
+  if (SEARCH) {
+    // Running sums to LDS (the lanes of a pixel are of one wavefront, and nobody else reads its costs any more), a draw
+    // to a lane, and the first sum above the target by halving.
+    float* sums = &tile[px * kStride];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      label += w[j] <= low ? 1 : 0;
-      most += w[j] <= high ? 1 : 0;
+    for (int j = 0; j < NV; j += 4)
+      *reinterpret_cast<float4*>(sums + s * NV + j) =
+          float4{before + w[j], before + w[j + 1], before + w[j + 2], before + w[j + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int top = 1 << (31 - __builtin_clz(p.n));
+    for (int d = s; d < p.n_draws; d += S) {
+      const float u = p.uniforms[d * p.items_pixels + at + of];
+      const float target = (positive(u) ? u : 0.f) * total;
+      int label = 0;
+      float least = -kInf;  // the last sum that is not above the target
+      for (int step = top; step > 0; step >>= 1) {
+        const int to = label + step;
+        const float sum = sums[min(to, p.n) - 1];
+        if (to <= p.n && sum <= target) {
+          label = to;
+          least = sum;
+        }
+      }
+      const float most = sums[min(label, p.n - 1)];
+      const bool near_one = !(least <= target - near && most > target + near) || label >= p.n;
+      unsure |= near_one;
+      if (px < count && (empty || !unsure)) p.labels[d * p.items_pixels + at + of] = (uint8_t)(empty ? 0 : label);
     }
-    label = lanes_sum<S>(label);
-    unsure |= label != lanes_sum<S>(most) || label >= p.n;
-    if (s == 0 && px < count && (empty || !unsure)) p.labels[d * p.items_pixels + at + of] = (uint8_t)(empty ? 0 : label);
+    unsure = lanes_max<S>(unsure ? 1 : 0) != 0;
+  } else {
+    for (int d = 0; d < p.n_draws; ++d) {
+      const float u = p.uniforms[d * p.items_pixels + at + of];
+      const float target = (positive(u) ? u : 0.f) * total - before;
+      const float low = target - near, high = target + near;
+      int label = 0, most = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        label += w[j] <= low ? 1 : 0;
+        most += w[j] <= high ? 1 : 0;
+      }
+      label = lanes_sum<S>(label);
+      unsure |= label != lanes_sum<S>(most) || label >= p.n;
+      if (s == 0 && px < count && (empty || !unsure)) p.labels[d * p.items_pixels + at + of] = (uint8_t)(empty ? 0 : label);
+    }
   }
 
   unsure = unsure && !empty && px < count;
+  const auto exactly = [&](int of) {
+    const float* c = cost + (LAST ? (p0 + of) * p.n : p0 + of);
+    const int64_t step = LAST ? 1 : p.pixels;
+    draw_exactly<FILTER>(p, q, at + of, [&](int l) { return c[l * step]; });
+  };
   if (S == 1) {
     // (one wavefront)
-    for (uint64_t rest = __builtin_amdgcn_ballot_w64(unsure); rest != 0; rest &= rest - 1) {
-      const int of = __builtin_ctzll(rest);
-      draw_exactly<FILTER>(p, q, at + of, [&](int l) {
-        return LAST ? tile[of * kStride + place(l >> 2) + (l & 3)] : row(l)[of];
-      });
-    }
+    for (uint64_t rest = __builtin_amdgcn_ballot_w64(unsure); rest != 0; rest &= rest - 1) exactly(__builtin_ctzll(rest));
   } else {
     if (unsure && s == 0) atomicOr(&left_over[px >> 5], 1u << (px & 31));
     __syncthreads();
     int turn = 0;
     for (uint64_t rest = (uint64_t)left_over[1] << 32 | left_over[0]; rest != 0; rest &= rest - 1)
-      if (turn++ % S == uniform_i(tid / 64)) {
-        const int of = __builtin_ctzll(rest);
-        draw_exactly<FILTER>(p, q, at + of, [&](int l) { return tile[of * kStride + place(l >> 2) + (l & 3)]; });
-      }
+      if (turn++ % S == uniform_i(tid / 64)) exactly(__builtin_ctzll(rest));
   }
 }
 
+template <int NV, int S, bool FILTER, bool LAST>
+void launch_draws(const Sample& p, unsigned blocks, hipStream_t st) {
+  if (p.n_draws >= kSearchFrom)
+    sample_kernel<NV, S, FILTER, LAST, true><<<blocks, kPixels * S, 0, st>>>(p);
+  else
+    sample_kernel<NV, S, FILTER, LAST, false><<<blocks, kPixels * S, 0, st>>>(p);
+}
 template <int NV, int S>
 void launch(const Sample& p, bool filter, bool labels_first, unsigned blocks, hipStream_t st) {
-  const auto run = [&](auto kernel) { kernel<<<blocks, kPixels * S, 0, st>>>(p); };
-  if (filter)
-    labels_first ? run(sample_kernel<NV, S, true, false>) : run(sample_kernel<NV, S, true, true>);
+  if (filter && labels_first)
+    launch_draws<NV, S, true, false>(p, blocks, st);
+  else if (filter)
+    launch_draws<NV, S, true, true>(p, blocks, st);
+  else if (labels_first)
+    launch_draws<NV, S, false, false>(p, blocks, st);
   else
-    labels_first ? run(sample_kernel<NV, S, false, false>) : run(sample_kernel<NV, S, false, true>);
+    launch_draws<NV, S, false, true>(p, blocks, st);
 }
 
 }  // namespace
