@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kPixels = 64;  // pixels of a workgroup
 constexpr int kSearchFrom = 2;
+constexpr int kFewDraws = 4;  // one after the other in draw_exactly
 
 struct Sample {
   const float* cost;
@@ -32,6 +33,7 @@ struct Sample {
   const float* min_p;
   float temperature_all, top_p_all, min_p_all;
   int top_k_all;
+  double reach_all;  // of min_p, where temperature and min_p are numbers
   int64_t pixels, tiles, items_pixels;
   int n, n_cv, n_draws;
   uint32_t reciprocal;  // 2^32 / n, rounded up
@@ -71,7 +73,8 @@ __device__ __forceinline__ bool positive(float x) {
   return bits > 0 && bits <= 0x7f800000;
 }
 
-// Reductions over the S lanes of a pixel, neighbours: within a row of 16, or the whole wavefront (S = 64).
+// Reductions over the S lanes of a pixel, neighbours: within a row of 16, or the whole wavefront (S = 64, all lanes at
+// work; the four rows meet in scalar registers).
 template <int CTRL>
 __device__ __forceinline__ int move(int x) {
   return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
@@ -86,14 +89,20 @@ __device__ __forceinline__ double move(double x) {
   const uint32_t lo = (uint32_t)move<CTRL>((int)(uint32_t)bits), hi = (uint32_t)move<CTRL>((int)(bits >> 32));
   return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
 }
+__device__ __forceinline__ int from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ float from_lane(float x, int lane) { return readlane_f(x, lane); }
+__device__ __forceinline__ double from_lane(double x, int lane) {
+  const int64_t bits = __builtin_bit_cast(int64_t, x);
+  const uint32_t lo = (uint32_t)from_lane((int)(uint32_t)bits, lane), hi = (uint32_t)from_lane((int)(bits >> 32), lane);
+  return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
+}
 template <int S, typename V, typename F>
 __device__ __forceinline__ V over_lanes(V x, F f) {
   if (S > 1) x = f(x, move<0xB1>(x));   // the other of a pair
   if (S > 2) x = f(x, move<0x4E>(x));   // the other pair of four
   if (S > 4) x = f(x, move<0x141>(x));  // the other four of eight
   if (S > 8) x = f(x, move<0x140>(x));  // the other eight
-  if (S > 16) x = f(x, __shfl_xor(x, 16));
-  if (S > 32) x = f(x, __shfl_xor(x, 32));
+  if (S > 16) x = f(f(from_lane(x, 0), from_lane(x, 16)), f(from_lane(x, 32), from_lane(x, 48)));
   return x;
 }
 template <int S, typename V>
@@ -107,6 +116,24 @@ __device__ __forceinline__ V lanes_max(V x) {
 template <int S, typename V>
 __device__ __forceinline__ V lanes_sum(V x) {
   return over_lanes<S>(x, [](V a, V b) { return a + b; });
+}
+// x of the lane that CTRL names, in the rows of MASK; 0 where there is none
+template <int CTRL, int MASK = 0xf>
+__device__ __forceinline__ double move_or_0(double x) {
+  const int64_t bits = __builtin_bit_cast(int64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CTRL, MASK, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, MASK, 0xf, false);
+  return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
+}
+// sum of the wavefront's lanes up to this one
+__device__ __forceinline__ double wave_upto(double x) {
+  x += move_or_0<0x111>(x);       // one lane up a row, two, four, eight
+  x += move_or_0<0x112>(x);
+  x += move_or_0<0x114>(x);
+  x += move_or_0<0x118>(x);
+  x += move_or_0<0x142, 0xa>(x);  // the last of a row to the next row: rows 1 and 3
+  x += move_or_0<0x143, 0xc>(x);  // the last of row 1 to rows 2 and 3
+  return x;
 }
 // sum of the lanes before this one, one after the other: a lane that adds nothing leaves the bits as they are
 template <int S, typename V>
@@ -158,10 +185,11 @@ __device__ __forceinline__ void threshold(float& lo, float& hi, const bool& unsu
 // threshold() closes.  On return t is the cost, `at` the number of labels at it, `less` the sum of those below.
 //   value(a)      what a label of cost a adds
 //   sum_upto(c)   this lane's sum of the labels with cost <= c
-constexpr int kHalves = 5, kSteps = 4;
+constexpr int kSteps = 6;
 template <int NV, int S, typename V, typename Value, typename SumUpTo, typename Reached>
 __device__ __forceinline__ void find(const float (&v)[NV], float best, float worst, bool& unsure, Value value,
                                      SumUpTo sum_upto, Reached reached, float& t, int& at, V& less) {
+  constexpr int kHalves = NV * S <= 32 ? 6 : 7;
   // t > lo, and less is the sum up to lo
   float lo = best - (fabsf(best) * 0x1p-20f + 0x1p-100f), hi = worst;
   less = V(0);
@@ -234,11 +262,14 @@ __device__ __forceinline__ void find(const float (&v)[NV], float best, float wor
 
 // What the parameters of an image come to.
 struct Parameters {
-  float temperature, top_p, min_p;
+  float temperature, top_p;
   int top_k;
-  bool warm;
-  double inv_t;
+  bool warm, bounded;  // T > 0; min_p > 0
+  double inv_t, reach;  // 1 / T; T * ln(1 / min_p)
 };
+__host__ __device__ __forceinline__ double reach_of(float temperature, float min_p) {
+  return min_p >= 1.f ? 0.0 : -(double)temperature * log((double)min_p);
+}
 template <bool FILTER>
 __device__ __forceinline__ Parameters parameters(const Sample& p, int image) {
   Parameters q;
@@ -247,14 +278,17 @@ __device__ __forceinline__ Parameters parameters(const Sample& p, int image) {
   q.inv_t = q.warm ? 1.0 / (double)q.temperature : 0.0;
   q.top_k = p.n;
   q.top_p = 1.f;
-  q.min_p = 0.f;
+  q.bounded = false;
+  q.reach = 0;
   if (FILTER) {
     const int k = p.top_k != nullptr ? p.top_k[image] : p.top_k_all;
     if (k > 0 && k < p.n) q.top_k = k;
     if (!q.warm) q.top_k = 1;
     if (q.warm) {
       q.top_p = p.top_p != nullptr ? p.top_p[image] : p.top_p_all;
-      q.min_p = p.min_p != nullptr ? p.min_p[image] : p.min_p_all;
+      const float min_p = p.min_p != nullptr ? p.min_p[image] : p.min_p_all;
+      q.bounded = positive(min_p);
+      if (q.bounded) q.reach = p.min_p != nullptr || p.temperature != nullptr ? reach_of(q.temperature, min_p) : p.reach_all;
     }
   }
   return q;
@@ -263,9 +297,8 @@ __device__ __forceinline__ Parameters parameters(const Sample& p, int image) {
 // The greatest cost that min_p leaves: the greatest float whose distance from the best is at most T * ln(1 / min_p).
 __device__ __forceinline__ float farthest(const Parameters& q, float best) {
   if (best == -kInf) return best;
-  const double reach = q.min_p >= 1.f ? 0.0 : -(double)q.temperature * log((double)q.min_p);
-  const auto within = [&](float c) { return (double)c - (double)best <= reach; };
-  const float far = (float)((double)best + reach);
+  const auto within = [&](float c) { return (double)c - (double)best <= q.reach; };
+  const float far = (float)((double)best + q.reach);
   if (!(far < kInf)) return kInf;
   const int key = float_key(__builtin_bit_cast(int, far));
   const float next = __builtin_bit_cast(float, float_key(key + 1)), previous = __builtin_bit_cast(float, float_key(key - 1));
@@ -278,6 +311,7 @@ __device__ __forceinline__ float farthest(const Parameters& q, float best) {
 template <bool FILTER, typename Cost>
 __device__ void draw_exactly(const Sample& p, const Parameters& q, int64_t at, Cost cost) {
   const int lane = (int)(threadIdx.x & 63);
+  const float mine = lane < p.n_draws ? p.uniforms[lane * p.items_pixels + at] : 0.f;  // of draw `lane`
   float v[4], best = kInf;
   double w[4];
 #pragma unroll
@@ -352,7 +386,7 @@ __device__ void draw_exactly(const Sample& p, const Parameters& q, int64_t at, C
       const double each = weight(t);
       cut(t, [&](int rank) { return less + rank * each < target || (t == best && rank == 0); });
     }
-    if (positive(q.min_p)) {
+    if (q.bounded) {
       const float far = farthest(q, best);
       cut(far, [](int) { return true; });
     }
@@ -363,34 +397,58 @@ __device__ void draw_exactly(const Sample& p, const Parameters& q, int64_t at, C
     w[j] = weight(v[j]);
     sum += w[j];
   }
-  double upto = sum;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double left = __shfl_up(upto, m);
-    if (lane >= m) upto += left;
-  }
-  const double total = __shfl(upto, 63), before = __shfl_up(upto, 1);
+  const double upto = wave_upto(sum), total = from_lane(upto, 63), before = move_or_0<0x138>(upto);
   int last = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (w[j] > 0) last = 4 * lane + j;
   last = lanes_max<64>(last);
-  for (int d = 0; d < p.n_draws; ++d) {
-    const float u = p.uniforms[d * p.items_pixels + at];
-    // (the lanes' sums may pass the total by a rounding)
-    const double target = positive(u) && u >= 1.f ? __builtin_huge_val() : (positive(u) ? (double)u : 0.0) * total;
-    double run = lane == 0 ? 0.0 : before;
-    int label = last;
+  // (the lanes' sums may pass the total by a rounding)
+  const auto target_of = [&](float u) {
+    return positive(u) && u >= 1.f ? __builtin_huge_val() : (positive(u) ? (double)u : 0.0) * total;
+  };
+  if (p.n_draws <= kFewDraws) {
+    for (int d = 0; d < p.n_draws; ++d) {
+      const double target = target_of(from_lane(mine, d));
+      double run = before;
+      int label = last;
+      bool found = false;
 #pragma unroll
-    for (int j = 3; j >= 0; --j) {
-      double to = run;
-#pragma unroll
-      for (int i = 0; i <= j; ++i) to += w[i];
-      // (a label that is out adds nothing, but the lanes' sums are formed in another order)
-      if (to > target && w[j] > 0) label = min(label, 4 * lane + j);
+      for (int j = 0; j < 4; ++j) {
+        run += w[j];
+        // (a label that is out adds nothing, but the lanes' sums are formed in another order)
+        if (!found && run > target && w[j] > 0) {
+          label = 4 * lane + j;
+          found = true;
+        }
+      }
+      label = lanes_min<64>(label);
+      if (lane == 0) p.labels[d * p.items_pixels + at] = (uint8_t)label;
     }
-    label = lanes_min<64>(label);
-    if (lane == 0) p.labels[d * p.items_pixels + at] = (uint8_t)label;
+    return;
+  }
+  // A draw to a lane.  The first lane whose labels' sum passes the target is found by halving; of its labels the first
+  // whose sum does.
+  for (int first = 0; first < p.n_draws; first += 64) {
+    const int d = first + lane;
+    const double target = target_of(first == 0 ? mine : d < p.n_draws ? p.uniforms[d * p.items_pixels + at] : 0.f);
+    int who = 0;
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1)
+      if (__shfl(upto, who + step - 1) <= target) who += step;
+    double run = __shfl(before, who);
+    int label = last;
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double e = __shfl(w[j], who);
+      run += e;
+      if (!found && e > 0) {
+        label = 4 * who + j;
+        found = run > target;
+      }
+    }
+    if (d < p.n_draws) p.labels[d * p.items_pixels + at] = (uint8_t)label;
   }
 }
 
@@ -507,9 +565,14 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
       }
     };
     float worst = best;
+    if (q.top_k < p.n || q.top_p < 1.f) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) worst = v[j] < kInf && v[j] > worst ? v[j] : worst;
-    worst = lanes_max<S>(worst);
+      for (int j = 0; j < NV; ++j) {
+        const float c = v[j] < kInf ? v[j] : best;
+        worst = c > worst ? c : worst;
+      }
+      worst = lanes_max<S>(worst);
+    }
     if (q.top_k < p.n) {
       bool whole = false;  // (whole numbers are never unsure)
       int at, less;
@@ -564,17 +627,17 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
         }
       }
     }
-    if (positive(q.min_p)) {
+    if (q.bounded) {
       const float far = farthest(q, best);
       if (far < t) {
         t = far;
         at = ties = 0;
       }
     }
-    if (t < kInf || __builtin_amdgcn_ballot_w64(t < kInf) != 0) {
-      cut(t, at, ties);
+    if (q.top_p < 1.f || q.bounded) {
+      if (__builtin_amdgcn_ballot_w64(at > ties) != 0) cut(t, at, ties);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) w[j] = v[j] < kInf ? w[j] : 0.f;
+      for (int j = 0; j < NV; ++j) w[j] = v[j] > t ? 0.f : w[j];
     }
   } else {
 #pragma unroll
@@ -642,9 +705,13 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
 
   unsure = unsure && !empty && px < count;
   const auto exactly = [&](int of) {
-    const float* c = cost + (LAST ? (p0 + of) * p.n : p0 + of);
-    const int64_t step = LAST ? 1 : p.pixels;
-    draw_exactly<FILTER>(p, q, at + of, [&](int l) { return c[l * step]; });
+    if (kTile && !SEARCH) {
+      draw_exactly<FILTER>(p, q, at + of, [&](int l) { return tile[of * kStride + place(l >> 2) + (l & 3)]; });
+    } else {  // (the tile has the running sums)
+      const float* c = cost + (LAST ? (p0 + of) * p.n : p0 + of);
+      const int64_t step = LAST ? 1 : p.pixels;
+      draw_exactly<FILTER>(p, q, at + of, [&](int l) { return c[l * step]; });
+    }
   };
   if (S == 1) {
     // (one wavefront)
@@ -707,6 +774,7 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
   p.top_k_all = top_k;
   p.top_p_all = top_p;
   p.min_p_all = min_p;
+  p.reach_all = temperature > 0 && min_p > 0 ? reach_of(temperature, min_p) : 0;
   p.pixels = pixels;
   p.tiles = tiles;
   p.items_pixels = items * pixels;
