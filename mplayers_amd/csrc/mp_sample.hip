@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kPixels = 64;  // pixels of a workgroup
 constexpr int kSearchFrom = 2;
+constexpr unsigned kFewTiles = 4096;
 constexpr int kFewDraws = 4;  // one after the other in draw_exactly
 
 struct Sample {
@@ -788,22 +789,28 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
   const unsigned blocks = (unsigned)(tiles * items);
   const hipStream_t st = (hipStream_t)stream;
   const bool lf = labels_first != 0;
+  // Labels per lane and lanes per pixel.  Many labels in a lane need fewer instructions, many lanes more wavefronts: up to
+  // kFewTiles workgroups a launch is short of those.  us, few lanes / many: no filter, all filters: 30 labels
+  // 129x129 (261 tiles) 5.3 / 4.5, 21.0 / 15.3; 60 labels 375x450, 16 draws, top-k (2637) 38.8 / 33.0; 45 labels 800x900
+  // (11 250) 30.8 / 34.2, 88.6 / 99.6; 128 labels 375x1242 (7277) 60.6 / 63.2, 141 / 154; 96 labels 384x1248 (7488) 41 / 48,
+  // 110 / 134.
+  const bool few = blocks <= kFewTiles;
   if (n_disp <= 8)
     launch<8, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 16)
-    launch<16, 1>(p, filter, lf, blocks, st);
+    few ? launch<8, 2>(p, filter, lf, blocks, st) : launch<16, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 24)
-    launch<24, 1>(p, filter, lf, blocks, st);
+    few ? launch<12, 2>(p, filter, lf, blocks, st) : launch<24, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 32)
-    launch<32, 1>(p, filter, lf, blocks, st);
+    few ? launch<16, 2>(p, filter, lf, blocks, st) : launch<32, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 48)
-    launch<24, 2>(p, filter, lf, blocks, st);
+    few ? launch<12, 4>(p, filter, lf, blocks, st) : launch<24, 2>(p, filter, lf, blocks, st);
   else if (n_disp <= 64)
-    launch<32, 2>(p, filter, lf, blocks, st);
+    few ? launch<16, 4>(p, filter, lf, blocks, st) : launch<32, 2>(p, filter, lf, blocks, st);
   else if (n_disp <= 96)
-    launch<24, 4>(p, filter, lf, blocks, st);
+    few ? launch<12, 8>(p, filter, lf, blocks, st) : launch<24, 4>(p, filter, lf, blocks, st);
   else if (n_disp <= 128)
-    launch<32, 4>(p, filter, lf, blocks, st);
+    few ? launch<16, 8>(p, filter, lf, blocks, st) : launch<32, 4>(p, filter, lf, blocks, st);
   else if (n_disp <= 192)
     launch<24, 8>(p, filter, lf, blocks, st);
   else
