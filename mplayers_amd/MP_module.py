@@ -220,8 +220,8 @@ class MPModule(torch.nn.Module):
   enable_min_a_dir, enable_sgm, enable_seg and, per call, training -- as the reference does.
 
   Not in the reference, and off unless the field is there: mpnet_unary_dropout (a rate; in training mode the
-  unary costs are dropped out by it, the masks seeded from torch's generator of the device) with
-  mpnet_unary_dropout_share ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has
+  unary costs, which may then be fp16 or bf16, are dropped out by it, the masks seeded from torch's generator of
+  the device; GPU only) with mpnet_unary_dropout_share ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has
   that many entries, which go by buckets of the label distance) with mpnet_smoothness_bucket_far (the distance
   from which on they share the last one).
   """
@@ -326,7 +326,7 @@ class MPModule(torch.nn.Module):
     if buckets is None:
       return label_context
     return bucket_context(label_context, buckets, square=self.args.enable_seg,
-                          symmetric=bool(self.args.enable_symmetric))
+                          symmetric=bool(getattr(self.args, "enable_symmetric", True)))
 
   def _reparameterised_label_context(self, weight_first):
     """Re-parameterisation of the learned context (MP_module.py:207-220).  weight_first: the term
@@ -359,8 +359,10 @@ class MPModule(torch.nn.Module):
   def _labels_last(self, unary):
     """The unary costs in the kernels' layout, in training mode with the dropout that args asks for."""
     rate = getattr(self.args, "mpnet_unary_dropout", None)
-    if not rate or not self.training:
+    if not rate:
       return labels_last(unary)
+    if not self.training:  # (as in training, a network's fp16 and bf16 costs are welcome)
+      return labels_last(unary.float() if unary.dtype in (torch.float16, torch.bfloat16) else unary)
     # (from torch's generator: it follows manual_seed, and a captured call has a new mask at every replay)
     state = torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), device=unary.device)
     return labels_last_dropout(unary, rate, state, getattr(self.args, "mpnet_unary_dropout_share", "element"))

@@ -222,7 +222,10 @@ int run(const char* what, int dtype, int share, double rate, const int64_t* stat
   if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
   if (batch == 0 || pixels == 0) return MPL_OK;
   const int64_t tiles = (pixels + kPixels - 1) / kPixels;
-  if (pixels > ((int64_t)1 << 40) || tiles * batch > 0x7fffffff) return fail(MPL_EINVAL, "%s: too many pixels", what);
+  // (a launch has less than 2^32 threads; these are the most per tile, see launch_share)
+  const int64_t threads = kPixels * (n_disp <= 8 ? 2 : n_disp <= 32 ? 4 : 8);
+  if (pixels > ((int64_t)1 << 40) || tiles > 0xffffffff / threads / batch)
+    return fail(MPL_EINVAL, "%s: too many pixels", what);
   Dropout d;
   d.state = state;
   d.pixels = pixels;

@@ -192,7 +192,7 @@ __device__ __forceinline__ void find(const float (&v)[NV], float best, float wor
                                      SumUpTo sum_upto, Reached reached, float& t, int& at, V& less) {
   constexpr int kHalves = NV * S <= 32 ? 6 : 7;
   // t > lo, and less is the sum up to lo
-  float lo = best - (fabsf(best) * 0x1p-20f + 0x1p-100f), hi = worst;
+  float lo = best < kInf ? best - (fabsf(best) * 0x1p-20f + 0x1p-100f) : best, hi = worst;
   less = V(0);
 #pragma unroll 1
   for (int step = 0; step < kHalves; ++step) {
@@ -761,7 +761,9 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
     return fail(MPL_EINVAL, "sample_labels: null pointer");
   const int64_t items = (int64_t)batch * n_cv;
   const int64_t tiles = (pixels + kPixels - 1) / kPixels;
-  if (items > 0x7fffffff || pixels > ((int64_t)1 << 40) || tiles * items > 0x7fffffff)
+  // (a launch has less than 2^32 threads, at most eight per pixel)
+  const int64_t threads = kPixels * (n_disp <= 32 ? 2 : 8);
+  if (items > 0x7fffffff || pixels > ((int64_t)1 << 40) || tiles > 0xffffffff / threads / items)
     return fail(MPL_EINVAL, "sample_labels: too many pixels");
   Sample p;
   p.cost = cost;

@@ -162,7 +162,7 @@ def bucket_context(table, starts, square=False, symmetric=True):
   """The pairwise table of a layer from one entry per bucket of label distances.
 
   table   (..., n_buckets) fp32; leading axes are tables of their own (one per direction, say)
-  starts  as label_buckets returns it
+  starts  as label_buckets returns it; read in either pass, so not to be written to between them
   square  False: (..., n) indexed by |a - b|; True: (..., n, n), with symmetric=False zeros below the diagonal
   -> the table, with autograd; the gradient of an entry is the sum over the distances of its bucket."""
   if not isinstance(table, torch.Tensor) or not isinstance(starts, torch.Tensor):
@@ -174,9 +174,12 @@ def bucket_context(table, starts, square=False, symmetric=True):
   if table.dim() < 1 or starts.numel() < 2 or table.size(-1) != starts.numel() - 1:
     raise RuntimeError('bucket_context: table has %s entries for %d buckets' %
                        (table.size(-1) if table.dim() else 'no', starts.numel() - 1))
+  n = int(starts[-1])
+  if not 1 <= n <= 256:
+    raise RuntimeError('bucket_context: 1 to 256 labels, got %d' % n)
   if table.is_cuda:
     call = _BucketContext.apply if table.requires_grad and torch.is_grad_enabled() else _expand
-    return call(table, starts, int(starts[-1]), 0 if not square else 2 if symmetric else 1)
+    return call(table, starts, n, 0 if not square else 2 if symmetric else 1)
   if int(starts[0]) != 0 or bool((starts[1:] < starts[:-1]).any()):
     raise RuntimeError('bucket_context: the buckets must be in order, from distance 0')
   bucket = torch.repeat_interleave(torch.arange(starts.numel() - 1), (starts[1:] - starts[:-1]).long())

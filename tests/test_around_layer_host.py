@@ -76,7 +76,9 @@ def test_bucket_context_refuses():
   table = torch.zeros(4)
   for t, s in [(torch.zeros(5), starts), (table.double(), starts), (table, starts.long()), (table, starts[None]),
                (table, torch.tensor([0, 3, 2, 4, 9], dtype=torch.int32)), (torch.zeros(()), starts),
-               (table, torch.tensor([1, 2, 3, 4, 9], dtype=torch.int32)), (table, starts[:1])]:
+               (table, torch.tensor([1, 2, 3, 4, 9], dtype=torch.int32)), (table, starts[:1]),
+               (table, torch.tensor([0, 2, 3, 4, 257], dtype=torch.int32)),
+               (table, torch.tensor([0, 0, 0, 0, 0], dtype=torch.int32))]:
     with pytest.raises(RuntimeError):
       bucket_context(t, s)
   with pytest.raises(TypeError):
@@ -116,6 +118,7 @@ def test_entry_points_refuse_before_any_launch():
     refused(call(0, 0, 0.5, one, one, one, 1, 257, 9, None), b"n_disp")
     refused(call(0, 0, 0.5, one, one, one, 1, 4, -9, None), b"negative")
     refused(call(0, 0, 0.5, one, one, one, 1 << 20, 4, 1 << 30, None), b"too many")
+    refused(call(0, 0, 0.5, one, one, one, 1, 1, 1 << 32, None), b"too many")  # 2^33 threads
     assert call(0, 0, 0.5, one, one, one, 0, 4, 9, None) == 0
 
   def sample(cost=one, uniforms=one, batch=1, n_cv=1, n=4, pixels=9, draws=1, labels=one):
@@ -129,6 +132,7 @@ def test_entry_points_refuse_before_any_launch():
   refused(sample(n=257), b"n_disp")
   refused(sample(draws=-1), b"negative")
   refused(sample(batch=1 << 20, pixels=1 << 30), b"too many")
+  refused(sample(n=200, pixels=1 << 30), b"too many")  # 2^33 threads
   assert sample(draws=0) == 0 and sample(batch=0) == 0 and sample(pixels=0) == 0
 
 

@@ -81,6 +81,27 @@ def test_a_bucketed_table_under_the_sigmoid(gpu):
   assert torch.allclose(context, bucket_context(entry, module.label_buckets), rtol=1e-6, atol=0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_half_precision_costs(gpu, dtype):
+  """A network's fp16 or bf16 costs with dropout, in training and in evaluation: the layer's costs are those of the
+  same values in fp32, the gradient comes in the network's type."""
+  from mplayers_amd import MPModule
+  module = MPModule(_module_args("ISGMR", 21, mpnet_unary_dropout=0.4), enable_create_label_context=True).cuda()
+  half = torch.randn(1, 1, 21, 7, 10, device="cuda").to(dtype).requires_grad_(True)
+  whole = half.detach().float().requires_grad_(True)
+  dcost = torch.randn(1, 1, 21, 7, 10, device="cuda")
+  got = []
+  for x in (half, whole):
+    torch.manual_seed(3)
+    module.train()
+    cost = module(x)[0]
+    (dx,) = torch.autograd.grad(cost, x, dcost)
+    module.eval()
+    got.append((cost, dx, module(x.detach())[0]))
+  assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][2], got[1][2])
+  assert got[0][1].dtype == dtype and torch.equal(got[0][1], got[1][1].to(dtype))
+
+
 def test_a_captured_step(gpu):
   """The whole step captured and replayed: every replay has a mask of its own, from torch's generator."""
   from mplayers_amd import MPModule

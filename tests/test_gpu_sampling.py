@@ -104,6 +104,40 @@ def test_parameters_of_each_image(gpu, n, labels_first):
         around_oracle.draw_labels(cost.astype(np.float32), u, top_p=parameters["top_p"], temperature=2.0))
 
 
+def test_temperatures_that_are_no_numbers(gpu):
+  rng = np.random.default_rng(2)
+  cost = rng.standard_normal((3, 1, 30, 4, 9))
+  u = _uniforms(rng, (2, 3, 1, 4, 9))
+  got = _draw(cost, u, temperature=[NAN, -NAN, -INF], top_k=[5, 0, 3], top_p=[0.5, 0.9, 1.0], min_p=[NAN, 0.5, NAN])
+  _same(got, np.broadcast_to(cost.astype(np.float32).argmin(2), u.shape))
+
+
+@pytest.mark.parametrize("masked", [0.0, 0.3, 0.97, 1.0])
+@pytest.mark.parametrize("n", [21, 96, 200])
+def test_masked_and_constant_images(gpu, n, masked):
+  """Images whose labels are mostly out, and whose costs are all the same: every sum is a whole number, and a target
+  may be one of them."""
+  rng = np.random.default_rng(int(100 * masked) + n)
+  cost = np.where(rng.random((1, 1, n, 6, 40)) < masked, INF, 0.75)
+  u = _uniforms(rng, (2, 1, 1, 6, 40))
+  u[1] = rng.integers(0, 8, u[1].shape) / 8
+  for parameters in (dict(), dict(top_p=0.5), dict(top_k=4, top_p=0.25), dict(min_p=1.0), dict(top_p=0.75, min_p=0.5)):
+    _same(_draw(cost, u, **parameters), around_oracle.draw_labels(cost.astype(np.float32), u, **parameters))
+
+
+@pytest.mark.parametrize("n", [21, 70, 256])
+def test_costs_close_together_in_a_wide_range(gpu, n):
+  """Most costs within 1e-3 of each other and a few far away, or growing by factors: the thresholds are not found by
+  halving the range."""
+  rng = np.random.default_rng(n)
+  cost = 1 + 1e-3 * rng.random((1, 1, n, 4, 33))
+  cost[:, :, ::7] = 50 * rng.random(cost[:, :, ::7].shape)
+  cost[..., 16:] = 2.0 ** rng.uniform(-100, 100, cost[..., 16:].shape)
+  u = _uniforms(rng, (3, 1, 1, 4, 33))
+  for parameters in (dict(top_k=n // 2), dict(top_p=0.6), dict(top_k=n - 1, top_p=0.3, min_p=0.2), dict(top_p=0.99, temperature=20)):
+    _same(_draw(cost, u, **parameters), around_oracle.draw_labels(cost.astype(np.float32), u, **parameters))
+
+
 @pytest.mark.parametrize("height,width", [(1, 1), (1, 63), (1, 64), (1, 65), (7, 19), (16, 16)])
 @pytest.mark.parametrize("n", [12, 21, 192])
 def test_image_sizes_and_items(gpu, n, height, width):
