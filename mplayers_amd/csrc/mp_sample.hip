@@ -78,7 +78,7 @@ __device__ __forceinline__ bool positive(float x) {
 // work; the four rows meet in scalar registers).
 template <int CTRL>
 __device__ __forceinline__ int move(int x) {
-  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
+  return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true);  // (0 where there is no such lane: part of what uses it)
 }
 template <int CTRL>
 __device__ __forceinline__ float move(float x) {
