@@ -184,18 +184,19 @@ __device__ __forceinline__ void threshold(float& lo, float& hi, const bool& unsu
 // The same for the costs v of a lane, in steps of a third and half the instructions: a few that only halve the range,
 // then from its lower end up from one cost to the next.  What that leaves open, costs close together in a wide range,
 // threshold() closes.  On return t is the cost, `at` the number of labels at it, `less` the sum of those below.
+//   labels        how many there are about: a halving for each time they can be halved leaves one or two
 //   value(a)      what a label of cost a adds
 //   sum_upto(c)   this lane's sum of the labels with cost <= c
 constexpr int kSteps = 6;
 template <int NV, int S, typename V, typename Value, typename SumUpTo, typename Reached>
-__device__ __forceinline__ void find(const float (&v)[NV], float best, float worst, bool& unsure, Value value,
+__device__ __forceinline__ void find(const float (&v)[NV], int labels, float best, float worst, bool& unsure, Value value,
                                      SumUpTo sum_upto, Reached reached, float& t, int& at, V& less) {
-  constexpr int kHalves = NV * S <= 32 ? 6 : 7;
+  const int halves = 32 - __builtin_clz(labels | 7);
   // t > lo, and less is the sum up to lo
   float lo = best < kInf ? best - (fabsf(best) * 0x1p-20f + 0x1p-100f) : best, hi = worst;
   less = V(0);
 #pragma unroll 1
-  for (int step = 0; step < kHalves; ++step) {
+  for (int step = 0; step < halves; ++step) {
     const float mid = 0.5f * lo + 0.5f * hi;
     const V sum = lanes_sum<S>(sum_upto(mid));
     if (mid > lo && mid < hi) {
@@ -217,16 +218,16 @@ __device__ __forceinline__ void find(const float (&v)[NV], float best, float wor
       next = above < next ? above : next;
     }
     next = lanes_min<S>(next);
-    int labels = 0;
+    int ties = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) labels += v[j] == next ? 1 : 0;
-    labels = lanes_sum<S>(labels);
+    for (int j = 0; j < NV; ++j) ties += v[j] == next ? 1 : 0;
+    ties = lanes_sum<S>(ties);
     if (open) {
-      const V sum = less + (V)labels * value(next);
+      const V sum = less + (V)ties * value(next);
       if (!(next < kInf) || reached(sum)) {
         open = false;
         t = next;
-        at = labels;
+        at = ties;
       } else {
         lo = next;
         less = sum;
@@ -248,15 +249,15 @@ __device__ __forceinline__ void find(const float (&v)[NV], float best, float wor
           return sum_upto(mid);
         },
         reached);
-    int labels = 0;
+    int ties = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) labels += v[j] == hi ? 1 : 0;
-    labels = lanes_sum<S>(labels);
+    for (int j = 0; j < NV; ++j) ties += v[j] == hi ? 1 : 0;
+    ties = lanes_sum<S>(ties);
     const V sum = lanes_sum<S>(sum_upto(hi));
     if (open) {
       t = hi;
-      at = labels;
-      less = sum - (V)labels * value(hi);
+      at = ties;
+      less = sum - (V)ties * value(hi);
     }
   }
 }
@@ -579,7 +580,7 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
       int at, less;
       float t;
       find<NV, S>(
-          v, best, q.top_k == 1 ? best : worst, whole, [](float) { return 1; },
+          v, p.n, best, q.top_k == 1 ? best : worst, whole, [](float) { return 1; },
           [&](float mid) {
             int labels = 0;
 #pragma unroll
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
       const float reach = rest > 1e-3f ? q.temperature * __logf(2.f * (float)p.n / rest) : kInf;
       float less;
       find<NV, S>(
-          v, best, best + reach < worst ? best + reach : worst, unsure, weight,
+          v, q.top_k, best, best + reach < worst ? best + reach : worst, unsure, weight,
           [&](float mid) {
             float sum = 0;
 #pragma unroll
