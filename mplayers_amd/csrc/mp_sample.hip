@@ -52,17 +52,22 @@ __device__ __forceinline__ float candidate(float c) {
 __device__ __forceinline__ double exp2_64(double y) {
   y = y > -2000.0 ? y : -2000.0;
   const double whole = rint(y), x = (y - whole) * 0.69314718055994530942;
-  double e = 1.0 / 6227020800;
-  e = fma(e, x, 1.0 / 479001600);
-  e = fma(e, x, 1.0 / 39916800);
-  e = fma(e, x, 1.0 / 3628800);
-  e = fma(e, x, 1.0 / 362880);
-  e = fma(e, x, 1.0 / 40320);
-  e = fma(e, x, 1.0 / 5040);
-  e = fma(e, x, 1.0 / 720);
-  e = fma(e, x, 1.0 / 120);
-  e = fma(e, x, 1.0 / 24);
-  e = fma(e, x, 1.0 / 6);
+  // (coefficients in scalar registers: the kernels have few others to spare, see sample_kernel)
+  const auto scalar = [](double c) {
+    asm("" : "+s"(c));
+    return c;
+  };
+  double e = scalar(1.0 / 6227020800);
+  e = fma(e, x, scalar(1.0 / 479001600));
+  e = fma(e, x, scalar(1.0 / 39916800));
+  e = fma(e, x, scalar(1.0 / 3628800));
+  e = fma(e, x, scalar(1.0 / 362880));
+  e = fma(e, x, scalar(1.0 / 40320));
+  e = fma(e, x, scalar(1.0 / 5040));
+  e = fma(e, x, scalar(1.0 / 720));
+  e = fma(e, x, scalar(1.0 / 120));
+  e = fma(e, x, scalar(1.0 / 24));
+  e = fma(e, x, scalar(1.0 / 6));
   e = fma(e, x, 0.5);
   e = fma(e, x, 1.0);
   e = fma(e, x, 1.0);
