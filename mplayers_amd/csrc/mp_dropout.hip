@@ -10,6 +10,12 @@
 // Four labels of a pixel share a counter (its four words): a thread owns a quad of labels of one pixel, so the words
 // it forms are all used (but for the last quad of a label count that is no multiple of four) wherever the pixel
 // lies, and the number of pixels may be odd.
+//
+// Bound by HBM: the mask costs no traffic and the change of layout is one the layer makes anyway.  us, forward /
+// backward: fp32, 192 labels 1500x2000 883 / 885 (5.2 TB/s; the change of layout alone, mpl_transpose, 1019); fp16, 128
+// labels 375x1242, whole pixels 74 / 75 (4.8 TB/s); bf16, 21 labels 12x129x129 9.6 / 8.7 (2.6 TB/s, a launch that is
+// over before memory is busy).  The generator takes 20 wide products and 20 exclusive ors for four labels, 420 vector
+// instructions to a wavefront of the first case in all.
 
 #include "mp_common.h"
 
@@ -175,7 +181,10 @@ __global__ void __launch_bounds__(kPixels* W) dropout_kernel(Dropout d, const vo
 }
 
 // Wavefronts W and quads J to a wavefront.  Small launches do not fill the chip: up to eight wavefronts share a tile
-// before one takes a second quad of each.
+// before one takes a third quad.  us forward / backward with one to four wavefronts of six quads -> this: 16 labels 64x96
+// 3.2 / 3.6 -> 2.4 / 2.5, 21 labels 129x129 4.7 / 4.6 -> 3.5 / 3.4, 64 labels 375x450 16.7 / 20.8 -> 15.4 / 15.9, 96 labels
+// 384x1248 70.1 / 72.5 -> 70.2 / 70.9; a wavefront to every quad: 64 labels 15.6 / 16.9, 21 labels 600x800 17.8 / 16.4 (14.9 /
+// 14.7 this).
 template <typename T, int SHARE, bool LAST>
 void launch_share(const Dropout& d, const void* src, void* dst, unsigned blocks, hipStream_t st) {
   const auto run = [&](auto kernel, int waves) { kernel<<<blocks, kPixels * waves, 0, st>>>(d, src, dst); };
@@ -233,8 +242,11 @@ int run(const char* what, int dtype, int share, double rate, const int64_t* stat
   d.labels = n_disp;
   d.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
   d.whole_quads = n_disp % 4 == 0 && ((uintptr_t)(LAST ? dst : src) & 15) == 0;
-  // where rows are not whole cache lines the tiles beside each other share lines
-  d.xcd_group = pixels * (dtype == MPL_F32 ? 4 : 2) % kLineBytes != 0 ? 8 : 0;
+  // Where rows are not whole cache lines the tiles beside each other share lines, which one die's L2 can join.  us forward
+  // / backward, tiles dealt out one by one -> groups of 8 -> 16: fp32 192 labels 377x501 57.5 / 64.2 -> 52.2 / 59.4 -> 51.1 /
+  // 58.3, 97 labels 301x803 40.6 / 38.5 -> 34.7 / 36.3 -> 34.4 / 35.3, fp16 128 labels 375x1242 77.7 / 82.6 -> 74.9 / 73.7 ->
+  // 74.9 / 73.9, bf16 21 labels 12x129x129 9.2 / 8.8 -> 9.7 / 8.9 -> 9.7 / 8.8.
+  d.xcd_group = pixels * (dtype == MPL_F32 ? 4 : 2) % kLineBytes != 0 ? 16 : 0;
   d.nothing = rate >= 1;
   d.bound = d.nothing ? 0u : (uint32_t)(rate * 4294967296.0);
   d.scale = d.nothing ? 0.f : (float)(1.0 / (1.0 - rate));

@@ -6,12 +6,19 @@
 //
 // All three filters keep the best labels down to a threshold (a cost, and how many of the labels that have exactly
 // that cost): top_k the cost of the k-th best, top_p the least cost whose labels down to it weigh enough, min_p
-// best + T * ln(1 / min_p).  So no sort: the threshold is found by halving the range of costs, each step moving an
-// end to a cost that occurs.
+// best + T * ln(1 / min_p).  So no sort: the threshold is found by halving the range of costs and then going from one
+// cost that occurs to the next (find).
+//
+// The costs are read once: a tile of 64 pixels lies in registers, a pixel's labels over one to eight lanes beside each
+// other.  (Tiles in the operators' layout, and of more than one lane to a pixel, get there through LDS, which turns rows of
+// labels into labels of a pixel.)  Without filters that bounds the call: 192 labels 1500x2000 0.45 ms, 5.1 TB/s, where a
+// large copy moves 4.7.  The filters are bound by the instructions they issue: 96 labels 384x1248 with all three and 4 draws
+// 131 us, 2650 vector instructions to a wavefront of 16 pixels, which issue 97 % of the time.
 //
 // Which label is drawn must not depend on how the sums are formed, or two correct programs would disagree on the
-// pixels whose target falls next to a border: weights and sums are held in 64 bits, which leaves borders of a
-// relative width of 2^-52.
+// pixels whose target falls next to a border.  So the borders are those of sums in 64 bits, which are off by 2^-50 or
+// so, and 32 bits, which take a third of the time, only where they tell (see sample_kernel): with 64 bits throughout 192
+// labels 1500x2000 took 1.42 ms.
 
 #include "mp_common.h"
 
@@ -20,9 +27,12 @@ using namespace mpl;
 namespace {
 
 constexpr int kPixels = 64;  // pixels of a workgroup
+// Draws from which on each has a lane of its own that halves the running sums in LDS; below, all lanes of a pixel count the
+// sums up to the target.  us, counting / halving: 1 draw: 60 labels 375x450 13.7 / 15.0, 192 labels 256x512 25.0 / 28.2; 2:
+// 15.9 / 15.5, 29.1 / 30.1; 4: 19.7 / 16.5, 38.4 / 33.2; 16: 39.2 / 23.9, 77.3 / 42.0.
 constexpr int kSearchFrom = 2;
-constexpr unsigned kFewTiles = 4096;
-constexpr int kFewDraws = 4;  // one after the other in draw_exactly
+constexpr unsigned kFewTiles = 4096;  // see mpl_sample_labels
+constexpr int kFewDraws = 4;          // one after the other in draw_exactly, more a lane each
 
 struct Sample {
   const float* cost;
@@ -39,6 +49,7 @@ struct Sample {
   int n, n_cv, n_draws;
   uint32_t reciprocal;  // 2^32 / n, rounded up
   int quads;            // labels last: whole and aligned quads
+  int xcd_group;        // tiles beside each other that go to one die (xcd_block)
 };
 
 constexpr float kInf = __builtin_huge_valf();
@@ -467,7 +478,8 @@ __device__ void draw_exactly(const Sample& p, const Parameters& q, int64_t at, C
 //   a sum     NV - 1 additions in a lane, S over the lanes: (NV + S) * 2^-24
 // and as much for a target, which is a product with such a sum (and is rounded itself).  Where a sum is as close to a
 // target as both (kNear), 32 bits do not tell, and draw_exactly() takes the pixel: with costs as a layer gives them one
-// draw in 400 of 192 labels, one in 4000 of 21.
+// draw in 400 of 192 labels, one in 4000 of 21.  (One wavefront for all pixels it had in registers took longer: its 64-bit
+// weights cost every call the registers of a third of its wavefronts, and each of its pixels waited for one.)
 template <int NV, int S, bool FILTER, bool LAST, bool SEARCH>
 __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
   constexpr int kQuads = S * NV / 4, kJ = NV / 4;  // of four labels: in all, per lane
@@ -476,7 +488,7 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
   constexpr float kNear = 2 * (NV + S + 25) * 0x1p-24f;
   __shared__ __align__(16) float tile[kTile || SEARCH ? kPixels * kStride : 4];
   __shared__ uint32_t left_over[2];  // pixels for draw_exactly()
-  const unsigned block = blockIdx.x, tiles = (unsigned)p.tiles;
+  const unsigned block = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.xcd_group), tiles = (unsigned)p.tiles;
   const int64_t item = block / tiles, p0 = (int64_t)(block - (unsigned)item * tiles) * kPixels;
   const int count = (int)min((int64_t)kPixels, p.pixels - p0);
   const int tid = (int)threadIdx.x;
@@ -792,6 +804,10 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
   p.n_draws = n_draws;
   p.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
   p.quads = n_disp % 4 == 0 && ((uintptr_t)cost & 15) == 0;
+  // Where rows are not whole cache lines the tiles beside each other share lines, which one die's L2 can join.  us, tiles dealt
+  // out one by one -> groups of 16: 60 labels 375x451 14.0 -> 12.8, 16 labels 601x803 11.2 -> 10.1, 192 labels 1501x1999 479 ->
+  // 465, 97 labels 301x803 28.5 -> 29.6.
+  p.xcd_group = labels_first && pixels * 4 % kLineBytes != 0 ? 16 : 0;
   const bool filter = temperatures != nullptr || !(temperature > 0) || top_ks != nullptr || (top_k > 0 && top_k < n_disp) ||
                       top_ps != nullptr || top_p < 1.f || min_ps != nullptr || min_p > 0.f;
   const unsigned blocks = (unsigned)(tiles * items);
