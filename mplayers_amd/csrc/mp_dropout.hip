@@ -23,7 +23,8 @@ using namespace mpl;
 
 namespace {
 
-constexpr int kPixels = 64;  // pixels of a tile: one wavefront along a label's row
+
+constexpr int64_t kFewTiles = 4096;  // of 64 pixels, see launch_share
 
 enum Share { kElement = MPL_DROPOUT_ELEMENT, kPixel = MPL_DROPOUT_PIXEL, kLabel = MPL_DROPOUT_LABEL };
 
@@ -87,26 +88,26 @@ __device__ __forceinline__ float scaled(float x, float scale) {
   return y;
 }
 
-// One tile of kPixels pixels and all labels per workgroup of W wavefronts, so that the label-innermost side is one run
-// of memory whatever the number of labels.  Wavefront w takes the quads w + i * W, i < J, with a lane per pixel: 256
-// contiguous bytes of a label's row (fp32) to an instruction.  The tile lies in LDS with the labels of a pixel side by
+// One tile of P pixels (P / 64 wavefronts beside each other) and all labels per workgroup of W times as many, so that the
+// label-innermost side is one run of memory whatever the number of labels.  Those of wavefront w of W take the quads
+// w + i * W, i < J, with a lane per pixel: 256 contiguous bytes of a label's row (fp32) to an instruction.  The tile lies in LDS with the labels of a pixel side by
 // side, an odd number of quads apart, which keeps the 16-byte accesses of either side off each other's banks.
 //
 // The random words are formed between the loads and their first use.  What lies behind the last label or pixel is
 // loaded from the last's place, so that there is no branch between the loads.
 //
 // LAST: into the label-innermost layout, else its gradient back.
-template <typename T, int SHARE, bool LAST, int W, int J>
-__global__ void __launch_bounds__(kPixels* W) dropout_kernel(Dropout d, const void* __restrict__ src,
+template <typename T, int SHARE, bool LAST, int W, int J, int P>
+__global__ void __launch_bounds__(P* W) dropout_kernel(Dropout d, const void* __restrict__ src,
                                                              void* __restrict__ dst) {
   constexpr int kStride = 4 * (W * J | 1);
-  __shared__ __align__(16) float tile[kPixels * kStride];
+  __shared__ __align__(16) float tile[P * kStride];
   const unsigned block = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, d.xcd_group);
   const unsigned of_item = block / (unsigned)d.tiles;
-  const int64_t item = of_item, p0 = (int64_t)(block - of_item * (unsigned)d.tiles) * kPixels;
-  const int tid = (int)threadIdx.x, px = tid % kPixels, wave = uniform_i(tid / kPixels);
+  const int64_t item = of_item, p0 = (int64_t)(block - of_item * (unsigned)d.tiles) * P;
+  const int tid = (int)threadIdx.x, px = tid % P, wave = uniform_i(tid / P);
   const int n = d.labels, quads = (n + 3) >> 2;
-  const int count = (int)min((int64_t)kPixels, d.pixels - p0);
+  const int count = (int)min((int64_t)P, d.pixels - p0);
   const unsigned total = (unsigned)(count * n);
   const int64_t first = item * n * d.pixels;
   const uint64_t seed = (uint64_t)d.state[0], offset = (uint64_t)d.state[1];
@@ -140,10 +141,10 @@ __global__ void __launch_bounds__(kPixels* W) dropout_kernel(Dropout d, const vo
     __syncthreads();
     float* to = (float*)dst + first + p0 * n;
     if (d.whole_quads) {
-      for (unsigned i = (unsigned)tid * 4; i < total; i += kPixels * W * 4)
+      for (unsigned i = (unsigned)tid * 4; i < total; i += P * W * 4)
         *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(&tile[place(i)]);
     } else {
-      for (unsigned i = (unsigned)tid; i < total; i += kPixels * W) to[i] = tile[place(i)];
+      for (unsigned i = (unsigned)tid; i < total; i += P * W) to[i] = tile[place(i)];
     }
   } else {
     const float* from = (const float*)src + first + p0 * n;
@@ -151,18 +152,18 @@ __global__ void __launch_bounds__(kPixels* W) dropout_kernel(Dropout d, const vo
       float4 x[J];
 #pragma unroll
       for (int k = 0; k < J; ++k)
-        x[k] = *reinterpret_cast<const float4*>(from + min((unsigned)(tid + k * kPixels * W) * 4, total - 4));
+        x[k] = *reinterpret_cast<const float4*>(from + min((unsigned)(tid + k * P * W) * 4, total - 4));
       form_masks();
 #pragma unroll
       for (int k = 0; k < J; ++k)
-        *reinterpret_cast<float4*>(&tile[place(min((unsigned)(tid + k * kPixels * W) * 4, total - 4))]) = x[k];
+        *reinterpret_cast<float4*>(&tile[place(min((unsigned)(tid + k * P * W) * 4, total - 4))]) = x[k];
     } else {
       float x[4 * J];
 #pragma unroll
-      for (int k = 0; k < 4 * J; ++k) x[k] = from[min((unsigned)(tid + k * kPixels * W), total - 1)];
+      for (int k = 0; k < 4 * J; ++k) x[k] = from[min((unsigned)(tid + k * P * W), total - 1)];
       form_masks();
 #pragma unroll
-      for (int k = 0; k < 4 * J; ++k) tile[place(min((unsigned)(tid + k * kPixels * W), total - 1))] = x[k];
+      for (int k = 0; k < 4 * J; ++k) tile[place(min((unsigned)(tid + k * P * W), total - 1))] = x[k];
     }
     __syncthreads();
     if (px >= count) return;
@@ -180,44 +181,46 @@ __global__ void __launch_bounds__(kPixels* W) dropout_kernel(Dropout d, const vo
   }
 }
 
-// Wavefronts W and quads J to a wavefront.  Small launches do not fill the chip: up to eight wavefronts share a tile
-// before one takes a third quad.  us forward / backward with one to four wavefronts of six quads -> this: 16 labels 64x96
-// 3.2 / 3.6 -> 2.4 / 2.5, 21 labels 129x129 4.7 / 4.6 -> 3.5 / 3.4, 64 labels 375x450 16.7 / 20.8 -> 15.4 / 15.9, 96 labels
-// 384x1248 70.1 / 72.5 -> 70.2 / 70.9; a wavefront to every quad: 64 labels 15.6 / 16.9, 21 labels 600x800 17.8 / 16.4 (14.9 /
-// 14.7 this).
+// Wavefronts W and quads J to a wavefront, pixels P of a tile.  Small launches do not fill the chip: up to eight wavefronts
+// share a tile before one takes a third quad.  us forward / backward with one to four wavefronts of six quads -> this: 16
+// labels 64x96 3.2 / 3.6 -> 2.4 / 2.5, 21 labels 129x129 4.7 / 4.6 -> 3.5 / 3.4, 64 labels 375x450 16.7 / 20.8 -> 15.4 / 15.9,
+// 96 labels 384x1248 70.1 / 72.5 -> 70.2 / 70.9; a wavefront to every quad: 64 labels 15.6 / 16.9, 21 labels 600x800 17.8 /
+// 16.4 (14.9 / 14.7 this).  Large launches of few labels are bound by the workgroups that start: wider tiles, from kFewTiles
+// on, with 64 pixels -> this: bf16 2 labels 7x1217x1930 158 / 140 -> 89 / 81, 5 labels 182 / 153 -> 128 / 115, 13 labels
+// 4x387x672 25.5 / 22.6 -> 20.0 / 18.1, fp32 4 labels 173 / 151 -> 99 / 93, 8 labels 191 / 186 -> 188 / 186.
 template <typename T, int SHARE, bool LAST>
-void launch_share(const Dropout& d, const void* src, void* dst, unsigned blocks, hipStream_t st) {
-  const auto run = [&](auto kernel, int waves) { kernel<<<blocks, kPixels * waves, 0, st>>>(d, src, dst); };
+int launch_share(const char* what, Dropout& d, int batch, const void* src, void* dst, hipStream_t st) {
+  const auto run = [&](auto kernel, int waves, int pixels) {
+    const int64_t tiles = (d.pixels + pixels - 1) / pixels;
+    // (a launch has less than 2^32 threads)
+    if (tiles > (int64_t)0xffffffff / (pixels * waves) / batch) return fail(MPL_EINVAL, "%s: too many pixels", what);
+    d.tiles = (int)tiles;
+    kernel<<<(unsigned)(tiles * batch), pixels * waves, 0, st>>>(d, src, dst);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
+  };
   const int n = d.labels;
+  const bool few = d.pixels / 64 * batch <= kFewTiles;
+  if (n <= 4)
+    return few ? run(dropout_kernel<T, SHARE, LAST, 1, 1, 64>, 1, 64) : run(dropout_kernel<T, SHARE, LAST, 1, 1, 512>, 1, 512);
   if (n <= 8)
-    run(dropout_kernel<T, SHARE, LAST, 2, 1>, 2);
-  else if (n <= 16)
-    run(dropout_kernel<T, SHARE, LAST, 4, 1>, 4);
-  else if (n <= 24)
-    run(dropout_kernel<T, SHARE, LAST, 3, 2>, 3);
-  else if (n <= 32)
-    run(dropout_kernel<T, SHARE, LAST, 4, 2>, 4);
-  else if (n <= 48)
-    run(dropout_kernel<T, SHARE, LAST, 6, 2>, 6);
-  else if (n <= 64)
-    run(dropout_kernel<T, SHARE, LAST, 8, 2>, 8);
-  else if (n <= 96)
-    run(dropout_kernel<T, SHARE, LAST, 8, 3>, 8);
-  else if (n <= 128)
-    run(dropout_kernel<T, SHARE, LAST, 8, 4>, 8);
-  else if (n <= 192)
-    run(dropout_kernel<T, SHARE, LAST, 8, 6>, 8);
-  else
-    run(dropout_kernel<T, SHARE, LAST, 8, 8>, 8);
+    return few ? run(dropout_kernel<T, SHARE, LAST, 2, 1, 64>, 2, 64) : run(dropout_kernel<T, SHARE, LAST, 1, 2, 256>, 1, 256);
+  if (n <= 16)
+    return few ? run(dropout_kernel<T, SHARE, LAST, 4, 1, 64>, 4, 64) : run(dropout_kernel<T, SHARE, LAST, 2, 2, 128>, 2, 128);
+  if (n <= 24) return run(dropout_kernel<T, SHARE, LAST, 3, 2, 64>, 3, 64);
+  if (n <= 32) return run(dropout_kernel<T, SHARE, LAST, 4, 2, 64>, 4, 64);
+  if (n <= 48) return run(dropout_kernel<T, SHARE, LAST, 6, 2, 64>, 6, 64);
+  if (n <= 64) return run(dropout_kernel<T, SHARE, LAST, 8, 2, 64>, 8, 64);
+  if (n <= 96) return run(dropout_kernel<T, SHARE, LAST, 8, 3, 64>, 8, 64);
+  if (n <= 128) return run(dropout_kernel<T, SHARE, LAST, 8, 4, 64>, 8, 64);
+  if (n <= 192) return run(dropout_kernel<T, SHARE, LAST, 8, 6, 64>, 8, 64);
+  return run(dropout_kernel<T, SHARE, LAST, 8, 8, 64>, 8, 64);
 }
 template <typename T, bool LAST>
-void launch(int share, const Dropout& d, const void* src, void* dst, unsigned blocks, hipStream_t st) {
-  if (share == kElement)
-    launch_share<T, kElement, LAST>(d, src, dst, blocks, st);
-  else if (share == kPixel)
-    launch_share<T, kPixel, LAST>(d, src, dst, blocks, st);
-  else
-    launch_share<T, kLabel, LAST>(d, src, dst, blocks, st);
+int launch(const char* what, int share, Dropout& d, int batch, const void* src, void* dst, hipStream_t st) {
+  return share == kElement ? launch_share<T, kElement, LAST>(what, d, batch, src, dst, st)
+         : share == kPixel ? launch_share<T, kPixel, LAST>(what, d, batch, src, dst, st)
+                           : launch_share<T, kLabel, LAST>(what, d, batch, src, dst, st);
 }
 
 template <bool LAST>
@@ -230,15 +233,10 @@ int run(const char* what, int dtype, int share, double rate, const int64_t* stat
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
   if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
   if (batch == 0 || pixels == 0) return MPL_OK;
-  const int64_t tiles = (pixels + kPixels - 1) / kPixels;
-  // (a launch has less than 2^32 threads; these are the most per tile, see launch_share)
-  const int64_t threads = kPixels * (n_disp <= 8 ? 2 : n_disp <= 32 ? 4 : 8);
-  if (pixels > ((int64_t)1 << 40) || tiles > 0xffffffff / threads / batch)
-    return fail(MPL_EINVAL, "%s: too many pixels", what);
+  if (pixels > ((int64_t)1 << 40)) return fail(MPL_EINVAL, "%s: too many pixels", what);
   Dropout d;
   d.state = state;
   d.pixels = pixels;
-  d.tiles = (int)tiles;
   d.labels = n_disp;
   d.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
   d.whole_quads = n_disp % 4 == 0 && ((uintptr_t)(LAST ? dst : src) & 15) == 0;
@@ -250,16 +248,10 @@ int run(const char* what, int dtype, int share, double rate, const int64_t* stat
   d.nothing = rate >= 1;
   d.bound = d.nothing ? 0u : (uint32_t)(rate * 4294967296.0);
   d.scale = d.nothing ? 0.f : (float)(1.0 / (1.0 - rate));
-  const unsigned blocks = (unsigned)(tiles * batch);
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == MPL_F32)
-    launch<float, LAST>(share, d, src, dst, blocks, st);
-  else if (dtype == MPL_F16)
-    launch<_Float16, LAST>(share, d, src, dst, blocks, st);
-  else
-    launch<__bf16, LAST>(share, d, src, dst, blocks, st);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
+  return dtype == MPL_F32   ? launch<float, LAST>(what, share, d, batch, src, dst, st)
+         : dtype == MPL_F16 ? launch<_Float16, LAST>(what, share, d, batch, src, dst, st)
+                            : launch<__bf16, LAST>(what, share, d, batch, src, dst, st);
 }
 
 }  // namespace
