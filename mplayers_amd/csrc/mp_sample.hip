@@ -44,7 +44,7 @@ struct Sample {
   const float* min_p;
   float temperature_all, top_p_all, min_p_all;
   int top_k_all;
-  double reach_all;  // of min_p, where temperature and min_p are numbers
+  double inv_t_all, reach_all;  // 1 / T; of min_p, where temperature and min_p are numbers
   int64_t pixels, tiles, items_pixels;
   int n, n_cv, n_draws;
   uint32_t reciprocal;  // 2^32 / n, rounded up
@@ -293,7 +293,7 @@ __device__ __forceinline__ Parameters parameters(const Sample& p, int image) {
   Parameters q;
   q.temperature = p.temperature != nullptr ? p.temperature[image] : p.temperature_all;
   q.warm = positive(q.temperature);
-  q.inv_t = q.warm ? 1.0 / (double)q.temperature : 0.0;
+  q.inv_t = p.temperature == nullptr ? p.inv_t_all : q.warm ? 1.0 / (double)q.temperature : 0.0;
   q.top_k = p.n;
   q.top_p = 1.f;
   q.bounded = false;
@@ -795,6 +795,7 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
   p.top_k_all = top_k;
   p.top_p_all = top_p;
   p.min_p_all = min_p;
+  p.inv_t_all = temperature > 0 ? 1.0 / (double)temperature : 0.0;
   p.reach_all = temperature > 0 && min_p > 0 ? reach_of(temperature, min_p) : 0;
   p.pixels = pixels;
   p.tiles = tiles;
@@ -819,7 +820,9 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
   // (11 250) 30.8 / 34.2, 88.6 / 99.6; 128 labels 375x1242 (7277) 60.6 / 63.2, 141 / 154; 96 labels 384x1248 (7488) 41 / 48,
   // 110 / 134.
   const bool few = blocks <= kFewTiles;
-  if (n_disp <= 8)
+  if (n_disp <= 4)
+    launch<4, 1>(p, filter, lf, blocks, st);
+  else if (n_disp <= 8)
     launch<8, 1>(p, filter, lf, blocks, st);
   else if (n_disp <= 16)
     few ? launch<8, 2>(p, filter, lf, blocks, st) : launch<16, 1>(p, filter, lf, blocks, st);
