@@ -17,11 +17,11 @@ def _parameter(name, value, batch, cost, dtype, low, high):
       raise RuntimeError("sample_labels: %s must be a number or a contiguous %s tensor of one per image (%d)" %
                          (name, dtype, batch))
     return value.data_ptr(), 0
-  if dtype == torch.int32 and (isinstance(value, bool) or not isinstance(value, int)):
+  if dtype == torch.int32 and (isinstance(value, bool) or not hasattr(value, "__index__")):
     raise RuntimeError("sample_labels: %s must be a whole number" % name)
   if not low <= value <= high:
     raise RuntimeError("sample_labels: %s must be in [%g, %g], got %r" % (name, low, high, value))
-  return None, value
+  return None, int(value) if dtype == torch.int32 else float(value)
 
 
 def sample_labels(cost, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, labels_first=True):

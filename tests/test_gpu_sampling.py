@@ -258,5 +258,6 @@ def test_refusals(gpu):
                 dict(cost=torch.zeros(2, 1, 0, 3, 3, device="cuda"))]:
     with pytest.raises(RuntimeError):
       sample_labels(**{**dict(cost=cost, uniforms=u), **wrong})
+  assert torch.equal(sample_labels(cost, u, temperature=np.float32(2), top_k=np.int64(2)), sample_labels(cost, u, temperature=2, top_k=2))
   assert sample_labels(cost[:0], u[:0]).shape == (0, 1, 3, 3)
   assert sample_labels(cost, u[None][:0]).shape == (0, 2, 1, 3, 3)
