@@ -1,6 +1,6 @@
 """Compiles the HIP sources under csrc/ into libmplayers_hip.so (gfx950 only) with hipcc, and the
 measurement probes (csrc/mp_probe.hip) into libmplayers_probe.so, which only the benchmark and the
-tests load.
+tests load; and csrc/torch/mp_autograd.cpp into the Python module _autograd.
 
 The scan kernels are instantiated once per R (labels per lane, 1..4; the reverse scans with four
 wavefronts per chain from 2 on), the forward scans also once
@@ -56,6 +56,25 @@ HOST_UNITS = [("mp_cpu", os.path.join("cpu", "mp_cpu.cpp"))]
 HOST_FLAGS = ["-O3", "-ffp-contract=off", "-std=c++17", "-fPIC", "-pthread", "-Wall", "-Wextra"]
 
 
+# the operators around the layers for torch: host code against torch's headers, a Python module of its own that is
+# handed the library's entry points (no link between the two)
+AUTOGRAD = os.path.join(HERE, "_autograd.so")
+
+
+def _autograd_command(out=AUTOGRAD):
+  import sysconfig
+  import torch
+  from torch.utils import cpp_extension
+  torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+  include = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(HERE), "include"),
+                                             "/opt/rocm/include"]
+  return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_autograd", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] + ["-I" + path for path in include] +
+          [os.path.join(CSRC, "torch", "mp_autograd.cpp"), "-L" + torch_lib, "-Wl,-rpath," + torch_lib, "-lc10", "-lc10_hip",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-o", out])
+
+
 def _run(cmd):
   proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
   out = "\n".join(l for l in proc.stdout.splitlines() if "packed-fp32-ops" not in l)
@@ -80,6 +99,8 @@ def build(verbose=False, extra_flags=(), lib_path=LIB, jobs=None):
   for name, src in HOST_UNITS:
     cmds.append([cxx] + HOST_FLAGS + ["-c", os.path.join(CSRC, src), "-o",
                                       os.path.join(obj_dir, name + ".o")])
+  if lib_path == LIB:
+    cmds.insert(0, _autograd_command())
   with ThreadPoolExecutor(max_workers=jobs) as pool:
     for cmd, out in zip(cmds, pool.map(_run, cmds)):
       if verbose:

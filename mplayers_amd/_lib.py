@@ -2,8 +2,6 @@
 import ctypes
 import os
 
-import torch
-
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MPLAYERS_HIP_LIB", os.path.join(HERE, "libmplayers_hip.so"))
 
@@ -153,16 +151,22 @@ def check(rc, what):
     raise RuntimeError("%s failed (%d): %s" % (what, rc, load().mpl_last_error().decode()))
 
 
-def launch(name, like, *args):
-  """Calls an entry point whose last argument is the stream, on the device and the current stream of the tensor
-  `like`.  (Where that is the current device, as nearly always, without the context manager's two microseconds.)"""
-  call = getattr(_lib or load(), name)
-  index = like.device.index
-  stream = torch._C._cuda_getCurrentRawStream(index)
-  if torch.cuda.current_device() == index:
-    rc = call(*args, stream)
-  else:
-    with torch.cuda.device(index):
-      rc = call(*args, stream)
-  if rc != 0:
-    check(rc, name[4:])
+_autograd = None
+
+
+def autograd():
+  """The module of the operators around the layers (csrc/torch/mp_autograd.cpp), on the library that load() loads;
+  raises if it has not been built."""
+  global _autograd
+  if _autograd is None:
+    lib = load()
+    try:
+      from . import _autograd as module
+    except ImportError as e:
+      raise RuntimeError("mplayers_amd/_autograd.so is missing or of another torch (%s): build it with "
+                         "`python -m mplayers_amd._build`" % e)
+    module.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
+                 ("mpl_bucket_context", "mpl_bucket_sums", "mpl_dropout_labels_last", "mpl_dropout_labels_first",
+                  "mpl_sample_labels", "mpl_last_error")])
+    _autograd = module
+  return _autograd

@@ -14,7 +14,6 @@ says which distances share an entry, bucket_context makes the table of a layer o
 through mpl_bucket_context with mpl_bucket_sums as its gradient, and create_bucket_table the parameter.
 """
 import argparse
-import ctypes
 
 import numpy as np
 import torch
@@ -113,61 +112,17 @@ def label_buckets(n_classes, n_buckets, max_distance=None):
   return torch.tensor([min(k, n_classes) for k in starts] + [n_classes], dtype=torch.int32)
 
 
-def _expand(table, starts, n, square):
-  table = table.contiguous()
-  out = table.new_empty(table.shape[:-1] + ((n, n) if square else (n,)))
-  n_buckets = table.size(-1)
-  if table.numel():
-    _lib.launch('mpl_bucket_context', table, table.data_ptr(), starts.data_ptr(), table.numel() // n_buckets, n_buckets,
-                n, square, out.data_ptr())
-  return out
-
-
-def _sums(grad, starts, n, square):
-  grad = grad.contiguous()
-  n_buckets = starts.numel() - 1
-  out = grad.new_empty(grad.shape[:-2 if square else -1] + (n_buckets,))
-  if out.numel():
-    _lib.launch('mpl_bucket_sums', grad, grad.data_ptr(), starts.data_ptr(), out.numel() // n_buckets, n_buckets, n,
-                square, out.data_ptr())
-  return out
-
-
-class _BucketContext(torch.autograd.Function):
-  """(..., n_buckets) -> (..., n) or (..., n, n)."""
-
-  @staticmethod
-  def forward(ctx, table, starts, n, square):
-    ctx.rest = (starts, n, square)
-    return _expand(table, starts, n, square)
-
-  @staticmethod
-  def backward(ctx, grad):
-    return (_BucketSums.apply if torch.is_grad_enabled() else _sums)(grad, *ctx.rest), None, None, None
-
-
-class _BucketSums(torch.autograd.Function):
-  """The gradient of _BucketContext; linear, so its gradient is _BucketContext."""
-
-  @staticmethod
-  def forward(ctx, grad, starts, n, square):
-    ctx.rest = (starts, n, square)
-    return _sums(grad, starts, n, square)
-
-  @staticmethod
-  def backward(ctx, grad):
-    return _BucketContext.apply(grad, *ctx.rest), None, None, None
-
-
 def bucket_context(table, starts, square=False, symmetric=True):
   """The pairwise table of a layer from one entry per bucket of label distances.
 
   table   (..., n_buckets) fp32; leading axes are tables of their own (one per direction, say)
-  starts  as label_buckets returns it; read in either pass, so not to be written to between them
+  starts  as label_buckets returns it
   square  False: (..., n) indexed by |a - b|; True: (..., n, n), with symmetric=False zeros below the diagonal
   -> the table, with autograd; the gradient of an entry is the sum over the distances of its bucket."""
   if not isinstance(table, torch.Tensor) or not isinstance(starts, torch.Tensor):
     raise TypeError('bucket_context: table and starts must be tensors')
+  if table.is_cuda:
+    return _lib.autograd().bucket_context(table, starts, square, symmetric)
   if starts.is_cuda or starts.dtype != torch.int32 or starts.dim() != 1 or not starts.is_contiguous():
     raise RuntimeError('bucket_context: starts must be an int32 CPU tensor, as label_buckets returns it')
   if table.dtype != torch.float32:
@@ -175,13 +130,8 @@ def bucket_context(table, starts, square=False, symmetric=True):
   if table.dim() < 1 or starts.numel() < 2 or table.size(-1) != starts.numel() - 1:
     raise RuntimeError('bucket_context: table has %s entries for %d buckets' %
                        (table.size(-1) if table.dim() else 'no', starts.numel() - 1))
-  # (starts[-1], in a third of the time)
-  n = ctypes.c_int32.from_address(starts.data_ptr() + 4 * table.size(-1)).value
-  if not 1 <= n <= 256:
-    raise RuntimeError('bucket_context: 1 to 256 labels, got %d' % n)
-  if table.is_cuda:
-    call = _BucketContext.apply if table.requires_grad and torch.is_grad_enabled() else _expand
-    return call(table, starts, n, 0 if not square else 2 if symmetric else 1)
+  if not 1 <= int(starts[-1]) <= 256:
+    raise RuntimeError('bucket_context: 1 to 256 labels, got %d' % int(starts[-1]))
   if int(starts[0]) != 0 or bool((starts[1:] < starts[:-1]).any()):
     raise RuntimeError('bucket_context: the buckets must be in order, from distance 0')
   bucket = torch.repeat_interleave(torch.arange(starts.numel() - 1), (starts[1:] - starts[:-1]).long())
