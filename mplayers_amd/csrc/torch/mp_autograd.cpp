@@ -3,8 +3,8 @@
 //
 // Their kernels take a few microseconds, and autograd runs a gradient in a thread of its own.  A node in Python has to
 // get the interpreter there and give it back; these do not touch it.  Host time, us, in Python -> here: a forward call of a
-// bucketed table 11 -> 5.5, with its gradient 40 -> 28 where the two threads share a cache and 82 -> 50 where they do not,
-// dropout of 16 labels 64x96 with its gradient 40 -> 37 and 88 -> 52, a draw of as many 9.9 -> 5.0.
+// bucketed table 11 -> 5.5, with its gradient 40 -> 28 (82 -> 50 where the machine takes longer to wake the thread), dropout
+// of 16 labels 64x96 with its gradient 40 -> 37 (88 -> 52), a draw of as many 9.9 -> 5.0.
 //
 // The entry points are those of the library that the ctypes binding has loaded (bind), not of one found by the linker.
 #include <torch/extension.h>
@@ -43,6 +43,11 @@ void bind(const std::vector<uintptr_t>& at) {
 
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void check(int rc, const char* what) { TORCH_CHECK(rc == MPL_OK, what, " failed (", rc, "): ", lib.last_error()); }
+// a size that the entry points take as an int
+int small(int64_t size) {
+  TORCH_CHECK(size <= std::numeric_limits<int>::max(), "a size of ", size, " is too large");
+  return (int)size;
+}
 // whether a gradient is itself to be differentiated
 bool recorded(const at::Tensor& grad) { return at::GradMode::is_enabled() && grad.requires_grad(); }
 
@@ -56,7 +61,7 @@ at::Tensor expand(const at::Tensor& table_in, const at::Tensor& starts, int64_t 
   at::Tensor out = at::empty(size, table.options());
   if (out.numel() == 0) return out;
   const c10::DeviceGuard guard(table.device());
-  check(lib.bucket_context(table.data_ptr<float>(), starts.data_ptr<int32_t>(), (int)(table.numel() / buckets),
+  check(lib.bucket_context(table.data_ptr<float>(), starts.data_ptr<int32_t>(), small(table.numel() / buckets),
                            (int)buckets, (int)n, (int)square, out.data_ptr<float>(), stream_of(table)),
         "bucket_context");
   return out;
@@ -71,7 +76,7 @@ at::Tensor sums(const at::Tensor& grad_in, const at::Tensor& starts, int64_t n, 
   at::Tensor out = at::empty(size, grad.options());
   if (out.numel() == 0) return out;
   const c10::DeviceGuard guard(grad.device());
-  check(lib.bucket_sums(grad.data_ptr<float>(), starts.data_ptr<int32_t>(), (int)(out.numel() / buckets), (int)buckets,
+  check(lib.bucket_sums(grad.data_ptr<float>(), starts.data_ptr<int32_t>(), small(out.numel() / buckets), small(buckets),
                         (int)n, (int)square, out.data_ptr<float>(), stream_of(grad)),
         "bucket_sums");
   return out;
@@ -130,7 +135,7 @@ at::Tensor dropout_last(const at::Tensor& x_in, const at::Tensor& state, double 
   if (out.numel() == 0) return out;
   const c10::DeviceGuard guard(x.device());
   check(lib.dropout_labels_last(mpl_type(x.scalar_type()), (int)share, p, state.data_ptr<int64_t>(), x.data_ptr(),
-                                out.data_ptr<float>(), (int)(s[0] * s[1]), (int)s[2], s[3] * s[4], stream_of(x)),
+                                out.data_ptr<float>(), small(s[0] * s[1]), (int)s[2], s[3] * s[4], stream_of(x)),
         "dropout_labels_last");
   return out;
 }
@@ -142,7 +147,7 @@ at::Tensor dropout_first(const at::Tensor& grad_in, const at::Tensor& state, dou
   if (out.numel() == 0) return out;
   const c10::DeviceGuard guard(grad.device());
   check(lib.dropout_labels_first(mpl_type(type), (int)share, p, state.data_ptr<int64_t>(), grad.data_ptr<float>(),
-                                 out.data_ptr(), (int)(s[0] * s[1]), (int)s[4], s[2] * s[3], stream_of(grad)),
+                                 out.data_ptr(), small(s[0] * s[1]), (int)s[4], s[2] * s[3], stream_of(grad)),
         "dropout_labels_first");
   return out;
 }
@@ -244,8 +249,8 @@ at::Tensor sample_labels(const at::Tensor& cost, const at::Tensor& uniforms, con
   const Parameter<float> p("top_p", top_p, batch, cost, at::kFloat, 1), m("min_p", min_p, batch, cost, at::kFloat, 1);
   at::Tensor labels = at::empty(uniforms.sizes(), uniforms.options().dtype(at::kByte));
   const c10::DeviceGuard guard(cost.device());
-  check(lib.sample_labels(labels_first, cost.data_ptr<float>(), uniforms.data_ptr<float>(), (int)batch, (int)cv, (int)n,
-                          height * width, at == 1 ? (int)uniforms.size(0) : 1, t.each, t.all, k.each, k.all, p.each, p.all,
+  check(lib.sample_labels(labels_first, cost.data_ptr<float>(), uniforms.data_ptr<float>(), small(batch), small(cv), small(n),
+                          height * width, at == 1 ? small(uniforms.size(0)) : 1, t.each, t.all, k.each, k.all, p.each, p.all,
                           m.each, m.all, labels.data_ptr<uint8_t>(), stream_of(cost)),
         "sample_labels");
   return labels;

@@ -135,6 +135,37 @@ def test_a_captured_step(gpu):
   assert all(abs(d - 0.5) <= 5 * 0.5 / 4320 ** 0.5 for d in dropped), dropped
 
 
+def test_inference_mode_and_two_streams(gpu):
+  """The three without autograd, and on two streams at once: the results of a call alone."""
+  from mplayers_amd import bucket_context, label_buckets, labels_last_dropout, sample_labels
+  starts = label_buckets(60, 9)
+  table = torch.randn(9, device="cuda", requires_grad=True)
+  x = torch.randn(1, 1, 60, 200, 300, device="cuda", requires_grad=True)
+  u = torch.rand(2, 1, 1, 200, 300, device="cuda")
+  states = [torch.tensor([k, 5], device="cuda") for k in range(2)]
+
+  def step(state):
+    context = bucket_context(table, starts)
+    y = labels_last_dropout(x, 0.2, state)
+    return context, y, sample_labels((y + context).detach(), u, top_p=0.8, top_k=20, labels_first=False)
+
+  want = [step(state) for state in states]
+  with torch.inference_mode():
+    got = step(states[0])
+  assert not got[0].requires_grad and not got[1].requires_grad
+  assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+  streams = [torch.cuda.Stream() for _ in states]
+  torch.cuda.synchronize()
+  for _ in range(3):
+    got = []
+    for stream, state in zip(streams, states):
+      with torch.cuda.stream(stream):
+        got.append(step(state))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+      assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 def test_the_energy_minimiser_draws(gpu, tmp_path):
   import scipy.io as scio
   from mplayers_amd import energy_min
