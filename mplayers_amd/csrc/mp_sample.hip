@@ -556,8 +556,8 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
 
   const Parameters q = parameters<FILTER>(p, (int)((unsigned)item / (unsigned)p.n_cv));
   const bool empty = best == kInf;
-  // what the bound above needs: no overflow in the exponents, a best cost to subtract (or one label that stays)
-  bool unsure = !empty && q.warm && !(q.temperature > 1e-30f && q.temperature < 1e30f && best > -kInf);
+  // what the bound above needs: no overflow in the exponents; and find() a cost below the best
+  bool unsure = !empty && (!(best > -kInf) || (q.warm && !(q.temperature > 1e-30f && q.temperature < 1e30f)));
   const float to_exponent = (float)(q.inv_t * 1.4426950408889634);
   const auto weight = [&](float c) {
     const float e = __builtin_amdgcn_exp2f((best - c) * to_exponent);

@@ -91,6 +91,27 @@ def test_costs_that_are_no_numbers(gpu, n, parameters):
     _same(_draw(cost, u, labels_first, **parameters), want)
 
 
+@pytest.mark.parametrize("parameters", [dict(), dict(top_k=2), dict(top_p=0.7), dict(min_p=0.2), dict(top_k=1, min_p=0.5),
+                                        dict(top_k=4, top_p=0.9, min_p=0.01, temperature=0.5), dict(temperature=0.0),
+                                        dict(temperature=[0.0], top_k=[3])])
+@pytest.mark.parametrize("n", [2, 9, 21, 70, 150, 256])
+def test_the_same_costs_with_ordinary_numbers(gpu, n, parameters):
+  """Costs as above, but uniform numbers inside their range: those outside have a pixel drawn in 64 bits throughout."""
+  rng = np.random.default_rng(n + 1)
+  big = float(np.finfo(np.float32).max)
+  odd = np.arange(n) % 2
+  rows = [np.full(n, -INF), np.where(odd, -INF, 1.0), np.where(odd, 1.0, -INF), np.where(np.arange(n) == n - 1, -INF, np.arange(n)),
+          np.where(odd, INF, -INF), np.where(odd, -INF, NAN), np.where(odd, -INF, -big), np.full(n, NAN), np.full(n, big),
+          np.full(n, -big), np.where(odd, big, -big), np.where(odd, -big, INF), np.where(odd, big, 0.0), np.where(odd, 0.0, -0.0),
+          np.arange(n) * 1e-42, np.where(odd, NAN, 0.5), 2.0 ** (np.arange(n) % 126 - 60), -2.0 ** (np.arange(n) % 126 - 60)]
+  cost = np.stack(rows, -1).astype(np.float32).reshape(1, 1, n, 1, len(rows))
+  for draws in (1, 3):
+    u = _uniforms(rng, (draws, 1, 1, 1, len(rows)))
+    want = around_oracle.draw_labels(cost, u, **parameters)
+    for labels_first in (True, False):
+      _same(_draw(cost, u, labels_first, **parameters), want)
+
+
 @pytest.mark.parametrize("n,labels_first", [(21, True), (21, False), (130, True)])
 def test_parameters_of_each_image(gpu, n, labels_first):
   rng = np.random.default_rng(n)
