@@ -650,7 +650,8 @@ __global__ void __launch_bounds__(kPixels* S) sample_kernel(Sample p) {
       const float far = farthest(q, best);
       if (far < t) {
         t = far;
-        at = ties = 0;
+        at = 0;
+        ties = p.n;  // all stay, also where another pixel has the wavefront cut
       }
     }
     if (q.top_p < 1.f || q.bounded) {

@@ -112,6 +112,20 @@ def test_the_same_costs_with_ordinary_numbers(gpu, n, parameters):
       _same(_draw(cost, u, labels_first, **parameters), want)
 
 
+@pytest.mark.parametrize("parameters", [dict(top_p=0.999, min_p=0.6), dict(top_p=0.95, min_p=0.8, temperature=0.3),
+                                        dict(top_k=5, top_p=0.8, min_p=0.5), dict(top_p=0.5, temperature=20.0, min_p=0.99)])
+@pytest.mark.parametrize("n", [4, 14, 41, 99, 250])
+def test_min_p_at_a_cost_that_occurs(gpu, n, parameters):
+  """Costs so large that all floats between them occur: the last cost that min_p leaves is one of them, beside pixels
+  whose ties top_p cuts."""
+  rng = np.random.default_rng(n)
+  for offset in (1e6, -1e6, 3e4):
+    cost = (offset + rng.standard_normal((1, 1, n, 3, 40))).astype(np.float32)
+    for draws in (1, 2):
+      u = _uniforms(rng, (draws, 1, 1, 3, 40))
+      _same(_draw(cost, u, **parameters), around_oracle.draw_labels(cost, u, **parameters))
+
+
 @pytest.mark.parametrize("n,labels_first", [(21, True), (21, False), (130, True)])
 def test_parameters_of_each_image(gpu, n, labels_first):
   rng = np.random.default_rng(n)
