@@ -142,14 +142,15 @@ __device__ __forceinline__ double move_or_0(double x) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, MASK, 0xf, false);
   return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
 }
-// sum of the wavefront's lanes up to this one
-__device__ __forceinline__ double wave_upto(double x) {
-  x += move_or_0<0x111>(x);       // one lane up a row, two, four, eight
-  x += move_or_0<0x112>(x);
-  x += move_or_0<0x114>(x);
-  x += move_or_0<0x118>(x);
-  x += move_or_0<0x142, 0xa>(x);  // the last of a row to the next row: rows 1 and 3
-  x += move_or_0<0x143, 0xc>(x);  // the last of row 1 to rows 2 and 3
+// f over the wavefront's lanes up to this one, where f(x, 0) is x
+template <typename F>
+__device__ __forceinline__ double wave_upto(double x, F f) {
+  x = f(x, move_or_0<0x111>(x));       // one lane up a row, two, four, eight
+  x = f(x, move_or_0<0x112>(x));
+  x = f(x, move_or_0<0x114>(x));
+  x = f(x, move_or_0<0x118>(x));
+  x = f(x, move_or_0<0x142, 0xa>(x));  // the last of a row to the next row: rows 1 and 3
+  x = f(x, move_or_0<0x143, 0xc>(x));  // the last of row 1 to rows 2 and 3
   return x;
 }
 // sum of the lanes before this one, one after the other: a lane that adds nothing leaves the bits as they are
@@ -415,57 +416,55 @@ __device__ void draw_exactly(const Sample& p, const Parameters& q, int64_t at, C
     w[j] = weight(v[j]);
     sum += w[j];
   }
-  const double upto = wave_upto(sum), total = from_lane(upto, 63), before = move_or_0<0x138>(upto);
+  // Each lane adds up in an order of its own, so that a sum may fall by a rounding from one lane to the next, or rise over
+  // a lane whose labels weigh nothing, where a target may come to lie.  So they are made to rise at lanes that weigh only.
+  const double ragged = wave_upto(sum, [](double a, double b) { return a + b; });
+  const double upto = wave_upto(sum > 0 ? ragged : 0.0, [](double a, double b) { return b > a ? b : a; });
+  const double total = from_lane(upto, 63), before = move_or_0<0x138>(upto);
   int last = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (w[j] > 0) last = 4 * lane + j;
   last = lanes_max<64>(last);
-  // (the lanes' sums may pass the total by a rounding)
+  // (a label's sum may pass the total by a rounding)
   const auto target_of = [&](float u) {
     return positive(u) && u >= 1.f ? __builtin_huge_val() : (positive(u) ? (double)u : 0.0) * total;
   };
+  // of lane `who`, `run` before it and e its weights: the first label whose sum passes the target, or the last that weighs
+  const auto within = [&](int who, double run, const double (&e)[4], double target) {
+    int label = last;
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      run += e[j];
+      if (!found && e[j] > 0) {
+        label = 4 * who + j;
+        found = run > target;
+      }
+    }
+    return label;
+  };
+  // The label is of the first lane whose sum, which is `before` of the next, passes the target; with many draws one to a
+  // lane, which finds it by halving.
   if (p.n_draws <= kFewDraws) {
     for (int d = 0; d < p.n_draws; ++d) {
       const double target = target_of(from_lane(mine, d));
-      double run = before;
-      int label = last;
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        run += w[j];
-        // (a label that is out adds nothing, but the lanes' sums are formed in another order)
-        if (!found && run > target && w[j] > 0) {
-          label = 4 * lane + j;
-          found = true;
-        }
-      }
-      label = lanes_min<64>(label);
-      if (lane == 0) p.labels[d * p.items_pixels + at] = (uint8_t)label;
+      const int label = within(lane, before, w, target);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before > target) >> 1 | (uint64_t)(total > target) << 63;
+      const int drawn = past != 0 ? from_lane(label, __builtin_ctzll(past)) : last;
+      if (lane == 0) p.labels[d * p.items_pixels + at] = (uint8_t)drawn;
     }
     return;
   }
-  // A draw to a lane.  The first lane whose labels' sum passes the target is found by halving; of its labels the first
-  // whose sum does.
   for (int first = 0; first < p.n_draws; first += 64) {
     const int d = first + lane;
     const double target = target_of(first == 0 ? mine : d < p.n_draws ? p.uniforms[d * p.items_pixels + at] : 0.f);
     int who = 0;
 #pragma unroll
     for (int step = 32; step > 0; step >>= 1)
-      if (__shfl(upto, who + step - 1) <= target) who += step;
-    double run = __shfl(before, who);
-    int label = last;
-    bool found = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double e = __shfl(w[j], who);
-      run += e;
-      if (!found && e > 0) {
-        label = 4 * who + j;
-        found = run > target;
-      }
-    }
+      if (__shfl(before, who + step) <= target) who += step;
+    const double e[4] = {__shfl(w[0], who), __shfl(w[1], who), __shfl(w[2], who), __shfl(w[3], who)};
+    const int label = within(who, __shfl(before, who), e, target);
     if (d < p.n_draws) p.labels[d * p.items_pixels + at] = (uint8_t)label;
   }
 }
