@@ -220,10 +220,10 @@ class MPModule(torch.nn.Module):
   enable_min_a_dir, enable_sgm, enable_seg and, per call, training -- as the reference does.
 
   Not in the reference, and off unless the field is there: mpnet_unary_dropout (a rate; in training mode the
-  unary costs, which may then be fp16 or bf16, are dropped out by it, the masks seeded from torch's generator of
-  the device; GPU only) with mpnet_unary_dropout_share ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has
-  that many entries, which go by buckets of the label distance) with mpnet_smoothness_bucket_far (the distance
-  from which on they share the last one).
+  unary costs are dropped out by it, the masks seeded from torch's generator of the device, on the GPU only; with the
+  field there, at a rate of 0 and in evaluation too, the costs may be fp16 or bf16) with mpnet_unary_dropout_share
+  ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has that many entries, which go by
+  buckets of the label distance) with mpnet_smoothness_bucket_far (the distance from which on they share the last one).
   """
 
   def __init__(self, args, enable_create_label_context=False, enable_saving_label=False,
@@ -359,9 +359,9 @@ class MPModule(torch.nn.Module):
   def _labels_last(self, unary):
     """The unary costs in the kernels' layout, in training mode with the dropout that args asks for."""
     rate = getattr(self.args, "mpnet_unary_dropout", None)
-    if not rate:
+    if rate is None:
       return labels_last(unary)
-    if not self.training:  # (as in training, a network's fp16 and bf16 costs are welcome)
+    if not self.training or rate == 0:  # (as at any other rate, a network's fp16 and bf16 costs are welcome)
       return labels_last(unary.float() if unary.dtype in (torch.float16, torch.bfloat16) else unary)
     # (from torch's generator: it follows manual_seed, and a captured call has a new mask at every replay)
     state = torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), device=unary.device)

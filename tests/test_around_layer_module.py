@@ -1,0 +1,33 @@
+"""The modules with dropout and bucketed tables, on the CPU: half-precision costs at a rate of 0."""
+import pytest
+import torch
+
+from tests.test_capi_host import _args
+
+
+def _module(soft=False, **fields):
+  from mplayers_amd import MPModule, MP_module_hard_soft
+  kind = MP_module_hard_soft.MPModule if soft else MPModule
+  return kind(_args(mpnet_smoothness_mode="TL", mpnet_smoothness_trunct_value=3, **fields), enable_create_label_context=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rate", [0, 0.0])
+def test_half_precision_costs_at_a_rate_of_0(rate, dtype):
+  """A rate that is scheduled from or to 0: the same network runs at 0, without dropout, as at any other rate."""
+  half = torch.randn(2, 1, 9, 4, 5).to(dtype)
+  for soft in (False, True):
+    module = _module(soft, n_classes=9, mpnet_unary_dropout=rate)
+    for training in (True, False):
+      for x in (half, half.float()):
+        last = module.train(training)._labels_last(x)
+        assert last.dtype == torch.float32 and torch.equal(last, half.float().permute(0, 1, 3, 4, 2))
+  # (the CPU operators take a table of all pairs of labels for each direction)
+  table = (torch.arange(9)[:, None] - torch.arange(9)).abs().clamp(max=3).float().expand(4, 9, 9).contiguous()
+  modules = [_module(n_classes=9, mpnet_unary_dropout=rate).eval(), _module(n_classes=9).eval()]
+  for module in modules:
+    module.set_label_context(torch.nn.Parameter(table), None, None)
+  assert torch.equal(modules[0](half)[0], modules[1](half.float())[0])
+  # without the field the costs are the operators' fp32 ones, as ever
+  with pytest.raises(RuntimeError, match="float32"):
+    modules[1](half)
