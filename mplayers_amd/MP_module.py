@@ -222,8 +222,9 @@ class MPModule(torch.nn.Module):
   Not in the reference, and off unless the field is there: mpnet_unary_dropout (a rate; in training mode the
   unary costs are dropped out by it, the masks seeded from torch's generator of the device, on the GPU only; with the
   field there, at a rate of 0 and in evaluation too, the costs may be fp16 or bf16) with mpnet_unary_dropout_share
-  ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has that many entries, which go by
-  buckets of the label distance) with mpnet_smoothness_bucket_far (the distance from which on they share the last one).
+  ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has that many entries, two at least,
+  which go by buckets of the label distance) with mpnet_smoothness_bucket_far (the distance from which on they share
+  the last one).
   """
 
   def __init__(self, args, enable_create_label_context=False, enable_saving_label=False,

@@ -144,8 +144,12 @@ def bucket_context(table, starts, square=False, symmetric=True):
 
 def create_bucket_table(args, n_buckets, max_distance=None):
   """(nn.Parameter (n_buckets,), loc, diag_loc, starts): create_label_context's vector at the first distance of
-  each bucket; the reads of args are its own."""
+  each bucket; the reads of args are its own.  The first entry is the pinned one, so a single bucket of all distances
+  is refused."""
   starts = label_buckets(args.n_classes, n_buckets, max_distance)
+  if starts[1] != 1:
+    raise ValueError('create_bucket_table: the first bucket must hold distance 0 alone, two buckets at least, got %r' %
+                     (n_buckets,))
   plain = argparse.Namespace(**vars(args))
   vector, _, _ = create_label_context(plain, enable_seg=False)
   first = starts[:-1].long().clamp(max=args.n_classes - 1).to(vector.device)

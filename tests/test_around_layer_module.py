@@ -31,3 +31,18 @@ def test_half_precision_costs_at_a_rate_of_0(rate, dtype):
   # without the field the costs are the operators' fp32 ones, as ever
   with pytest.raises(RuntimeError, match="float32"):
     modules[1](half)
+
+
+@pytest.mark.parametrize("train", ["", "on", "sigmoid", "softmax"])
+def test_one_bucket_is_refused(train):
+  """The first entry is pinned, as the table's of distance 0 is: it has to be of that distance alone."""
+  from mplayers_amd.label_context import create_bucket_table
+  with pytest.raises(ValueError, match="distance 0"):
+    _module(n_classes=9, mpnet_smoothness_train=train, mpnet_smoothness_buckets=1)
+  with pytest.raises(ValueError, match="distance 0"):
+    create_bucket_table(_args(n_classes=21, mpnet_smoothness_train=train), 1)
+  module = _module(n_classes=9, mpnet_smoothness_train=train, mpnet_smoothness_buckets=2)
+  context = module._effective_label_context()
+  assert context.shape == (9,) and float(context[0]) == 0 and bool((context[1:] == context[1]).all())
+  # (one label has no other distance)
+  assert create_bucket_table(_args(n_classes=1, mpnet_smoothness_train=train), 1)[3].tolist() == [0, 1]
