@@ -350,8 +350,9 @@ class MPModule(torch.nn.Module):
       label_context[self.label_context_loc] = scale * torch.sigmoid(valid)
     elif mode == 'softmax':
       valid = label_context[self.label_context_loc].flatten()
-      norm = nn.Softmax(dim=0)(valid)
-      label_context[self.label_context_loc] = norm * valid.max() / norm.max()
+      if valid.numel() > 0:  # (a single label has the pinned entry only)
+        norm = nn.Softmax(dim=0)(valid)
+        label_context[self.label_context_loc] = norm * valid.max() / norm.max()
     if mode in {'sigmoid', 'softmax'}:
       diag = self.label_context_diag_loc
       label_context[tuple(diag) if isinstance(diag, list) else diag] = self.args.mpnet_diag_value

@@ -144,7 +144,7 @@ def bucket_context(table, starts, square=False, symmetric=True):
 
 def create_bucket_table(args, n_buckets, max_distance=None):
   """(nn.Parameter (n_buckets,), loc, diag_loc, starts): create_label_context's vector at the first distance of
-  each bucket; the reads of args are its own.  The first entry is the pinned one, so a single bucket of all distances
+  each bucket, loc the buckets that hold a distance; the reads of args are its own.  The first entry is the pinned one, so a single bucket of all distances
   is refused."""
   starts = label_buckets(args.n_classes, n_buckets, max_distance)
   if starts[1] != 1:
@@ -153,5 +153,6 @@ def create_bucket_table(args, n_buckets, max_distance=None):
   plain = argparse.Namespace(**vars(args))
   vector, _, _ = create_label_context(plain, enable_seg=False)
   first = starts[:-1].long().clamp(max=args.n_classes - 1).to(vector.device)
-  return (nn.Parameter(vector.detach()[first].clone(), requires_grad=vector.requires_grad), range(1, n_buckets),
-          range(1), starts)
+  # (what an empty bucket's entry holds reaches no label: it is not to weigh in a softmax over the others)
+  loc = [b for b in range(1, n_buckets) if starts[b] < starts[b + 1]]
+  return nn.Parameter(vector.detach()[first].clone(), requires_grad=vector.requires_grad), loc, range(1), starts

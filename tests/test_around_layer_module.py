@@ -43,6 +43,41 @@ def test_one_bucket_is_refused(train):
     create_bucket_table(_args(n_classes=21, mpnet_smoothness_train=train), 1)
   module = _module(n_classes=9, mpnet_smoothness_train=train, mpnet_smoothness_buckets=2)
   context = module._effective_label_context()
+  context = context.detach()
   assert context.shape == (9,) and float(context[0]) == 0 and bool((context[1:] == context[1]).all())
   # (one label has no other distance)
   assert create_bucket_table(_args(n_classes=1, mpnet_smoothness_train=train), 1)[3].tolist() == [0, 1]
+
+
+@pytest.mark.parametrize("n,buckets,far", [(5, 8, None), (40, 9, 2), (40, 9, 20), (21, 30, None), (1, 3, None)])
+def test_entries_of_empty_buckets_take_no_part(n, buckets, far):
+  """The softmax is over the entries that a distance has: whatever the others hold, the table is the same, and they have
+  no gradient."""
+  module = _module(n_classes=n, mpnet_smoothness_train="softmax", mpnet_smoothness_buckets=buckets,
+                   mpnet_smoothness_bucket_far=far)
+  starts = module.label_buckets
+  full = (starts[1:] > starts[:-1]).tolist()
+  learned = [b for b in range(1, buckets) if full[b]]
+  assert list(module.label_context_loc) == learned and list(module.label_context_diag_loc) == [0]
+  entries = torch.linspace(-1, 1, buckets).double().tolist()
+  module.label_context.data.copy_(torch.tensor(entries))
+  # by the definition: e_b / max(e) * max of what is stored, e the softmax
+  stored = [entries[b] for b in learned]
+  want = torch.zeros(buckets, dtype=torch.float64)
+  if learned:
+    e = torch.exp(torch.tensor(stored, dtype=torch.float64))
+    want[learned] = e / e.max() * max(stored)
+  distance = torch.arange(n)
+  bucket = (distance[:, None] >= starts[None, 1:-1]).sum(-1)
+  want = want[bucket]
+  if n == 21:
+    want = want[(distance[:, None] - distance).abs()]
+  for other in (0.0, 100.0):
+    for b in range(buckets):
+      if not full[b]:
+        module.label_context.data[b] = other
+    context = module._effective_label_context()
+    # (fp32: a softmax of at most 30 entries and two products, some tens of roundings of 2^-24 of values up to 1)
+    assert torch.allclose(context.detach().double(), want, rtol=0, atol=64 * 2.0 ** -24)
+    (grad,) = torch.autograd.grad(context.sum(), module.label_context)
+    assert all(float(grad[b]) == 0 for b in range(buckets) if not full[b])
