@@ -283,6 +283,24 @@ class MPModule(torch.nn.Module):
     state.pop("_kept_masks", None)
     return state
 
+  def _save_to_state_dict(self, destination, prefix, keep_vars):
+    """A bucketed table's borders go with its entries, which mean nothing under others."""
+    super()._save_to_state_dict(destination, prefix, keep_vars)
+    if getattr(self, "label_buckets", None) is not None:
+      destination[prefix + "label_buckets"] = self.label_buckets
+
+  def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+    key = prefix + "label_buckets"
+    if key in state_dict:
+      own, saved = getattr(self, "label_buckets", None), state_dict[key].cpu()
+      if own is None or not torch.equal(own, saved):
+        error_msgs.append("%s: the saved table has buckets of label distances from %s, this module's %s" %
+                          (key, saved.tolist(), "has none" if own is None else own.tolist()))
+        return  # (nothing is loaded)
+    super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+    if key in unexpected_keys:
+      unexpected_keys.remove(key)
+
   def _location_masks(self, label_context):
     """Masks of label_context_loc and label_context_diag_loc on the table's device, None where a location is
     not a list of different entries that numpy reads as torch does, or more than one value is pinned, and in

@@ -1,4 +1,5 @@
-"""The modules with dropout and bucketed tables, on the CPU: half-precision costs at a rate of 0."""
+"""The modules with dropout and bucketed tables, on the CPU: half-precision costs at a rate of 0, which entries of a
+table are learned, and tables that are saved and loaded."""
 import pytest
 import torch
 
@@ -81,3 +82,37 @@ def test_entries_of_empty_buckets_take_no_part(n, buckets, far):
     assert torch.allclose(context.detach().double(), want, rtol=0, atol=64 * 2.0 ** -24)
     (grad,) = torch.autograd.grad(context.sum(), module.label_context)
     assert all(float(grad[b]) == 0 for b in range(buckets) if not full[b])
+
+
+@pytest.mark.parametrize("strict", [True, False])
+def test_a_learned_table_is_loaded_with_its_borders(strict):
+  """Entries that were learned for other distances are refused; a state without borders, or of a table without buckets,
+  is loaded as ever."""
+  from mplayers_amd import MP_module_hard_soft, label_buckets
+  fields = dict(n_classes=40, mpnet_smoothness_train="on", mpnet_smoothness_buckets=8)
+  module = _module(mpnet_smoothness_bucket_far=30, **fields)
+  module.label_context.data.copy_(torch.rand(8))
+  network = torch.nn.Sequential(torch.nn.Linear(2, 3), module)
+  state = network.state_dict()
+  assert torch.equal(state["1.label_buckets"], label_buckets(40, 8, 30))
+
+  def other(**more):
+    return torch.nn.Sequential(torch.nn.Linear(2, 3), _module(**{**fields, **more}))
+
+  for soft in (False, True):
+    same = torch.nn.Sequential(torch.nn.Linear(2, 3), _module(soft, mpnet_smoothness_bucket_far=30, **fields))
+    same.load_state_dict(state, strict=strict)
+    assert torch.equal(same[1].label_context, module.label_context) and isinstance(same[1], MP_module_hard_soft.MPModule) == soft
+  for wrong in (other(mpnet_smoothness_bucket_far=20), other(n_classes=50, mpnet_smoothness_bucket_far=30),
+                other(n_classes=8, mpnet_smoothness_buckets=0)):
+    kept = wrong[1].label_context.detach().clone()
+    with pytest.raises(RuntimeError, match="buckets"):
+      wrong.load_state_dict(state, strict=strict)
+    assert torch.equal(wrong[1].label_context, kept)
+  before = {k: v for k, v in state.items() if k != "1.label_buckets"}
+  loaded = other(mpnet_smoothness_bucket_far=30)
+  loaded.load_state_dict(before, strict=strict)
+  assert torch.equal(loaded[1].label_context, module.label_context)
+  plain = other(mpnet_smoothness_buckets=0)
+  assert set(plain.state_dict()) == {"0.weight", "0.bias", "1.label_context"}
+  plain.load_state_dict(plain.state_dict(), strict=strict)
