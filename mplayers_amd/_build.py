@@ -8,6 +8,7 @@ with and once without argmin labels; each instantiation is its own translation u
 compile in parallel.
 """
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -66,13 +67,27 @@ def _autograd_command(out=AUTOGRAD):
   import torch
   from torch.utils import cpp_extension
   torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-  include = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(HERE), "include"),
-                                             "/opt/rocm/include"]
-  return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__=1",
+  # (others' headers as the system's: what -Wall and -Wextra find is the unit's own)
+  include = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], _rocm_include()]
+  return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__=1",
            "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_autograd", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] + ["-I" + path for path in include] +
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+           "-I" + os.path.join(os.path.dirname(HERE), "include")] + [arg for path in include for arg in ("-isystem", path)] +
           [os.path.join(CSRC, "torch", "mp_autograd.cpp"), "-L" + torch_lib, "-Wl,-rpath," + torch_lib, "-lc10", "-lc10_hip",
            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-o", out])
+
+
+def _hipcc():
+  return os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+
+
+def _rocm_include():
+  """The headers beside the compiler, or the usual ones where it has none (a wrapper, say)."""
+  hipcc = shutil.which(_hipcc()) or _hipcc()
+  for root in (os.path.dirname(os.path.dirname(os.path.realpath(hipcc))), "/opt/rocm"):
+    if os.path.exists(os.path.join(root, "include", "hip", "hip_runtime.h")):
+      break
+  return os.path.join(root, "include")
 
 
 def _run(cmd):
@@ -85,7 +100,7 @@ def _run(cmd):
 
 def build(verbose=False, extra_flags=(), lib_path=LIB, jobs=None):
   """Always recompiles; returns the path of the shared library."""
-  hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+  hipcc = _hipcc()
   obj_dir = OBJ if lib_path == LIB else lib_path + ".build"
   os.makedirs(obj_dir, exist_ok=True)
   jobs = jobs or min(8, os.cpu_count() or 1)
@@ -113,7 +128,7 @@ def build(verbose=False, extra_flags=(), lib_path=LIB, jobs=None):
 
 def link(lib_path=LIB, verbose=False):
   """Links the objects that are there into the product library and the probe library."""
-  hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+  hipcc = _hipcc()
   obj_dir = OBJ if lib_path == LIB else lib_path + ".build"
   probe_path = PROBE_LIB if lib_path == LIB else lib_path.replace(".so", "_probe.so")
   names = [name for name, _, _ in _units()]
