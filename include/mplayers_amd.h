@@ -337,8 +337,8 @@ int mpl_dropout_labels_first(int dtype, int share, double rate, const int64_t* s
 
 /* Pairwise tables whose entries go by buckets of the label distance k = |a - b|, for the layers' `context`; no
  * counterpart in the reference.  Bucket b is the distances starts[b] <= k < starts[b + 1]; starts is a HOST array of
- * n_buckets + 1 numbers in order, from 0 to n_disp, read during the call (a bucket may be empty).  table
- * (n_tables, n_buckets) -> context (n_tables, n_disp) with square = 0, (n_tables, n_disp, n_disp) otherwise: with
+ * n_buckets + 1 numbers in order, from 0 to n_disp, read during the call (a bucket may be empty).  At most
+ * MPL_MAX_LABELS labels and buckets and 65 535 tables.  table (n_tables, n_buckets) -> context (n_tables, n_disp) with square = 0, (n_tables, n_disp, n_disp) otherwise: with
  * square = 1 the entries b >= a, zeros below the diagonal, with square = 2 both triangles.  mpl_bucket_sums is the
  * gradient: dtable[t][b] = the sum of dcontext over the entries that table[t][b] went to, in fp64 and in a fixed
  * order, rounded once. */
@@ -357,8 +357,11 @@ int mpl_bucket_sums(const float* dcontext, const int32_t* starts, int n_tables, 
  *   min_p  of these the ones of at least min_p of the best one's weight (off: <= 0)
  * The label drawn is the first, in label order, whose running sum of what stays exceeds uniform * (sum of what stays),
  * or the last that stays where none does (a uniform of 1 or more); a uniform below 0 or NaN counts as 0.  A
- * temperature that is not above 0 takes the label of least cost, the lowest of equals; a pixel without candidates
- * gets label 0.  Weights and sums are formed in fp64.  temperatures, top_ks, top_ps, min_ps: batch numbers each in
+ * temperature that is not above 0 takes the label of least cost, the lowest of equals; at an infinite one all
+ * candidates weigh the same.  min_p of 1 or more leaves the labels of the best cost at any temperature, an infinite one
+ * too (as at the ever greater ones before it).  A pixel without candidates gets label 0.  The label is that of weights
+ * and sums in fp64: they are formed in fp32 with a bound on their error, and in fp64 where a target is as close to a
+ * sum as that.  It does not depend on n_draws.  temperatures, top_ks, top_ps, min_ps: batch numbers each in
  * DEVICE memory, one per image, or NULL for the number beside. */
 int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms, int batch, int n_cv, int n_disp,
                       int64_t pixels, int n_draws, const float* temperatures, float temperature, const int32_t* top_ks,

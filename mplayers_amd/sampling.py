@@ -15,7 +15,8 @@ def sample_labels(cost, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
   temperature, top_k, top_p, min_p
              numbers, or tensors of one per image on the device of the costs (fp32, top_k int32; these are not
              looked at).  top_k best labels (0: all), of these the best ones that weigh top_p together, of
-             these the ones of min_p of the best one's weight.  temperature 0: the label of least cost.
+             these the ones of min_p of the best one's weight (1: those of the best cost, at any temperature).
+             temperature 0: the label of least cost; infinite: all candidates weigh the same.
   -> uint8 labels of the shape of uniforms.
 
   Equal costs order by label.  A pixel without candidates gets label 0."""

@@ -79,3 +79,27 @@ def test_whole_sums_and_many_draws(gpu, n, draws, masked):
   for parameters in (dict(), dict(top_p=0.5), dict(top_k=4, top_p=0.25), dict(min_p=1.0)):
     want = around_oracle.draw_labels(cost.astype(np.float32), u, **parameters)
     assert np.array_equal(_draw(cost, u, **parameters), want), parameters
+
+
+@pytest.mark.parametrize("n", [3, 16, 21, 60, 200])
+def test_min_p_of_1_at_any_temperature(gpu, n):
+  """min_p of 1 leaves the labels of the best cost, whatever the temperature: at an infinite one too, where a lesser min_p
+  leaves all candidates."""
+  from mplayers_amd import sample_labels
+  rng = np.random.default_rng(n)
+  cost = np.round(rng.standard_normal((2, 1, n, 2, 33)) * 3) / 2
+  cost[rng.random(cost.shape) < 0.2] = INF
+  cost = cost.astype(np.float32)
+  u = rng.integers(0, 2 ** 24, (3, 2, 1, 2, 33)).astype(np.float32) * np.float32(2.0 ** -24)
+  best = cost.min(2)
+  for temperature in (INF, 1e30, 1.0, 1e-30):
+    for more in (dict(), dict(top_p=0.5), dict(top_k=2)):
+      parameters = dict(temperature=temperature, min_p=1.0, **more)
+      got = _draw(cost, u, **parameters)
+      assert np.array_equal(got, around_oracle.draw_labels(cost, u, **parameters)), parameters
+      assert (np.take_along_axis(cost[None], got[:, :, :, None].astype(np.int64), 3)[:, :, :, 0] == best).all()
+  # per image: an infinite temperature with min_p of 1 and just below it
+  below = float(np.nextafter(np.float32(1), np.float32(0)))
+  got = sample_labels(torch.from_numpy(cost).cuda(), torch.from_numpy(u).cuda(), temperature=torch.tensor([INF, INF]).cuda(),
+                      min_p=torch.tensor([1.0, below]).cuda()).cpu().numpy()
+  assert np.array_equal(got, around_oracle.draw_labels(cost, u, temperature=[INF, INF], min_p=[1.0, below]))
