@@ -13,9 +13,11 @@
 //
 // Bound by HBM: the mask costs no traffic and the change of layout is one the layer makes anyway.  us, forward /
 // backward: fp32, 192 labels 1500x2000 883 / 885 (5.2 TB/s; the change of layout alone, mpl_transpose, 1019); fp16, 128
-// labels 375x1242, whole pixels 74 / 75 (4.8 TB/s); bf16, 21 labels 12x129x129 9.6 / 8.7 (2.6 TB/s, a launch that is
-// over before memory is busy).  The generator takes 20 wide products and 20 exclusive ors for four labels, 420 vector
-// instructions to a wavefront of the first case in all.
+// labels 375x1242, whole pixels 74 / 80 (4.8 and 4.5 TB/s; in turn, one in the cache that the other filled, 62 / 95);
+// bf16, 21 labels 12x129x129 9.7 / 8.7 (2.5 and 2.8 TB/s; what bounds it is not shown: vector issue is 0.3 of it, so not
+// the generator; its accesses are 2 bytes to a lane, 4 on the operators' side, as its labels are no multiple of four).
+// The generator takes 20 wide products and 20 exclusive ors for four labels, 420 vector instructions to a wavefront of
+// the first case in all.
 
 #include "mp_common.h"
 
