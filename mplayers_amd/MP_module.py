@@ -287,7 +287,7 @@ class MPModule(torch.nn.Module):
     """A bucketed table's borders go with its entries, which mean nothing under others."""
     super()._save_to_state_dict(destination, prefix, keep_vars)
     if getattr(self, "label_buckets", None) is not None:
-      destination[prefix + "label_buckets"] = self.label_buckets
+      destination[prefix + "label_buckets"] = self.label_buckets.clone()  # (layers may share it)
 
   def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
     key = prefix + "label_buckets"

@@ -116,3 +116,16 @@ def test_a_learned_table_is_loaded_with_its_borders(strict):
   plain = other(mpnet_smoothness_buckets=0)
   assert set(plain.state_dict()) == {"0.weight", "0.bias", "1.label_context"}
   plain.load_state_dict(plain.state_dict(), strict=strict)
+
+
+def test_layers_that_share_their_borders_are_saved(tmp_path):
+  """Formats that refuse tensors of one memory under two names take them."""
+  safetensors = pytest.importorskip("safetensors.torch")
+  fields = dict(n_classes=40, mpnet_smoothness_train="on", mpnet_smoothness_buckets=8)
+  first, second = _module(**fields), _module(**fields)
+  second.set_label_context(second.label_context, second.label_context_loc, second.label_context_diag_loc, first.label_buckets)
+  network = torch.nn.ModuleList([first, second])
+  safetensors.save_file(network.state_dict(), str(tmp_path / "net.safetensors"))
+  first.label_context.data.add_(1)
+  network.load_state_dict(safetensors.load_file(str(tmp_path / "net.safetensors")))
+  assert torch.equal(first.label_context, second.label_context)
