@@ -16,7 +16,7 @@ import torch.nn as nn
 
 from . import _lib, lib_seg, lib_stereo
 from .label_context import bucket_context, create_bucket_table, create_label_context
-from .layout import gradient_labels_last, labels_first, labels_last, labels_last_dropout
+from .layout import gradient_labels_last, labels_first, labels_last, labels_last_dropout, labels_last_norm
 
 
 def _ops_for(n_disp):
@@ -224,7 +224,9 @@ class MPModule(torch.nn.Module):
   field there, at a rate of 0 and in evaluation too, the costs may be fp16 or bf16) with mpnet_unary_dropout_share
   ('element' | 'pixel' | 'label'); mpnet_smoothness_buckets (the pairwise table has that many entries, two at least,
   which go by buckets of the label distance) with mpnet_smoothness_bucket_far (the distance from which on they share
-  the last one).
+  the last one); mpnet_unary_norm (if true, the unary costs are normalised over the labels of each pixel, after dropout, with
+  a weight and a bias per label that are learned, unary_norm_weight and unary_norm_bias; the costs may be fp16 or bf16) with
+  mpnet_unary_norm_eps (1e-5).
   """
 
   def __init__(self, args, enable_create_label_context=False, enable_saving_label=False,
@@ -236,6 +238,10 @@ class MPModule(torch.nn.Module):
     self.args.enable_min_a_dir = enable_min_a_dir
     self.args.enable_sgm = args.mpnet_mrf_mode == 'SGM'
     self.args.enable_seg = True if (args.n_classes == 21) else False
+    if getattr(args, "mpnet_unary_norm", False):
+      like = dict(device="cuda" if getattr(args, "enable_cuda", False) else "cpu")
+      self.unary_norm_weight = torch.nn.Parameter(torch.ones(args.n_classes, **like))
+      self.unary_norm_bias = torch.nn.Parameter(torch.zeros(args.n_classes, **like))
     if enable_create_label_context:
       self.create_label_context()
 
@@ -377,15 +383,23 @@ class MPModule(torch.nn.Module):
     return label_context
 
   def _labels_last(self, unary):
-    """The unary costs in the kernels' layout, in training mode with the dropout that args asks for."""
+    """The unary costs in the kernels' layout, in training mode with the dropout that args asks for, and normalised if it
+    asks for that."""
     rate = getattr(self.args, "mpnet_unary_dropout", None)
-    if rate is None:
-      return labels_last(unary)
-    if not self.training or rate == 0:  # (as at any other rate, a network's fp16 and bf16 costs are welcome)
-      return labels_last(unary.float() if unary.dtype in (torch.float16, torch.bfloat16) else unary)
-    # (from torch's generator: it follows manual_seed, and a captured call has a new mask at every replay)
-    state = torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), device=unary.device)
-    return labels_last_dropout(unary, rate, state, getattr(self.args, "mpnet_unary_dropout_share", "element"))
+    norm = getattr(self, "unary_norm_weight", None) is not None
+    if rate and self.training:
+      # (from torch's generator: it follows manual_seed, and a captured call has a new mask at every replay)
+      state = torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), device=unary.device)
+      unary = labels_last_dropout(unary, rate, state, getattr(self.args, "mpnet_unary_dropout_share", "element"))
+      return self._normalised(unary, False) if norm else unary
+    if norm:
+      return self._normalised(unary, True)
+    # (as at any other rate, a network's fp16 and bf16 costs are welcome)
+    return labels_last(unary.float() if rate is not None and unary.dtype in (torch.float16, torch.bfloat16) else unary)
+
+  def _normalised(self, unary, first):
+    return labels_last_norm(unary, self.unary_norm_weight, self.unary_norm_bias,
+                            getattr(self.args, "mpnet_unary_norm_eps", 1e-5), labels_first=first)
 
   def forward(self, unary, edge_weights=None):
     # label axis innermost for the kernels; direction axis outermost for the edge weights

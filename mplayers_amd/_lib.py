@@ -13,7 +13,7 @@ SYMBOLS = ("mpl_trwp_forward", "mpl_trwp_backward", "mpl_isgmr_forward", "mpl_is
            "mpl_trwp_soft_backward", "mpl_soft_weighted_message", "mpl_soft_weighted_message_back", "mpl_set_option",
            "mpl_stereo_data_cost", "mpl_gradient_cues", "mpl_mrf_energy", "mpl_transpose",
            "mpl_dropout_labels_last", "mpl_dropout_labels_first", "mpl_bucket_context", "mpl_bucket_sums",
-           "mpl_sample_labels")
+           "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace")
 
 KERNEL_KINDS = ("fwd_sweep", "bwd_sweep", "belief", "aggregate", "label", "combine", "other",
                 "fwd_sweep_all", "bwd_sweep_all", "unary_all")
@@ -81,6 +81,9 @@ def load():
   lib.mpl_bucket_context.argtypes = [vp, vp, ci, ci, ci, ci, vp, vp]
   lib.mpl_bucket_sums.argtypes = [vp, vp, ci, ci, ci, ci, vp, vp]
   lib.mpl_sample_labels.argtypes = [ci, vp, vp, ci, ci, ci, i64, ci, vp, cf, vp, ci, vp, cf, vp, cf, vp, vp]
+  lib.mpl_norm_labels_last.argtypes = [ci, ci, vp, vp, vp, cf, vp, vp, ci, ci, i64, vp]
+  lib.mpl_norm_labels_last_grad.argtypes = [ci, ci] + [vp] * 8 + [ci, ci, i64, vp]
+  lib.mpl_norm_workspace.argtypes = [ci, ci, i64]
   lib.mpl_n_chains.argtypes = [ci, ci, ci]
   lib.mpl_dcontext_copies.argtypes = [sp, ci]
   lib.mpl_table_is_dense.argtypes = [vp, ci]
@@ -88,6 +91,7 @@ def load():
   lib.mpl_profile_end.argtypes = [ctypes.POINTER(KernelStat), ci]
   for name in SYMBOLS:
     getattr(lib, name).restype = ci
+  lib.mpl_norm_workspace.restype = i64
   lib.mpl_last_error.restype = ctypes.c_char_p
   if lib.mpl_version() // 100 != 2:
     raise RuntimeError("libmplayers_hip.so has ABI version %d, this package needs 2xx: rebuild it "
@@ -167,6 +171,6 @@ def autograd():
                          "`python -m mplayers_amd._build`" % e)
     module.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
                  ("mpl_bucket_context", "mpl_bucket_sums", "mpl_dropout_labels_last", "mpl_dropout_labels_first",
-                  "mpl_sample_labels", "mpl_last_error")])
+                  "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace", "mpl_last_error")])
     _autograd = module
   return _autograd

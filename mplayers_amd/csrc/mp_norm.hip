@@ -1,0 +1,411 @@
+// Layer norm of the unary costs over the labels of a pixel, within the change to the layers' layout, for gfx950.
+//
+// x in the network's layout (items, labels, pixels) or in the operators' (items, pixels, labels), fp32, fp16 or bf16
+//   ->  y (items, pixels, labels) fp32:   y[l] = xhat[l] * weight[l] + bias[l],   xhat[l] = (x[l] - mean) * r,
+//   r = 1 / sqrt(var + eps), mean and var over the labels of the pixel; and its gradient, with g[l] = dy[l] * weight[l]:
+//   dx[l] = r * (g[l] - mean(g) - xhat[l] * mean(g * xhat)),   dweight[l] = sum over pixels of dy[l] * xhat[l],
+//   dbias[l] = sum over pixels of dy[l].
+//
+// The variance is that of the differences from the mean, in registers: each wavefront's own labels first, and those of
+// the W wavefronts of a tile joined as sum(M2_w + n_w * (mean_w - mean)^2).  mean and r are kept for the gradient, 8 bytes a
+// pixel.
+//
+// Bound by HBM: a pixel's labels are read once, and the change of layout is one that the layer makes anyway.  The sums over
+// pixels stay in registers while a workgroup goes from tile to tile: a fp32 sum for each lane and label, then over the 64
+// lanes, and the workgroups' sums in 64 bits and in their order by a second kernel, so that the same call gives the same bits.
+
+#include "mp_pixels.h"
+
+using namespace mpl;
+
+namespace {
+
+constexpr int kSumRows = 2048;  // workgroups of a gradient, at most
+
+struct Norm {
+  Tiles t;
+  const void* x;
+  const float* weight;  // or nullptr: 1
+  const float* bias;    // or nullptr: 0
+  float* y;
+  float* stats;  // mean and r of each pixel
+  const float* dy;
+  void* dx;      // or nullptr
+  float* sums;   // of each workgroup: dweight, dbias
+  float eps;
+  int x_quads, y_quads;  // whole and aligned quads in the operators' layout
+};
+
+// labels that wavefront w of W has
+template <int W, int I>
+__device__ __forceinline__ int labels_of(int w, int n) {
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < I; ++i) count += min(max(n - 4 * (w + i * W), 0), 4);
+  return count;
+}
+
+template <typename T, bool FIRST, int W, int I, int G>
+__global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
+  static_assert(W == 1 || G == 1, "wavefronts that share a tile meet at the workgroup's barrier");
+  constexpr int kStride = tile_stride(W * I);
+  __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
+  __shared__ __align__(16) float affine[2][4 * W * I];
+  __shared__ float2 part[W > 1 ? W : 1][kTilePixels];
+  const int tid = (int)threadIdx.x % (64 * W), group = uniform_i((int)threadIdx.x / (64 * W));
+  const int lane = tid % 64, w = uniform_i(tid / 64), n = p.t.labels;
+  const unsigned at = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.t.xcd_group) * G + group;
+  const bool work = at < p.t.total;
+  const unsigned item = at / p.t.per_item;
+  const int64_t p0 = (int64_t)(at - item * p.t.per_item) * kTilePixels;
+  const int count = work ? (int)min((int64_t)kTilePixels, p.t.pixels - p0) : 0;
+  const unsigned total = (unsigned)(count * n);
+  const int of = min(lane, count - 1);
+  const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n;
+  float* const tile = tiles + group * kTilePixels * kStride;
+  float* const mine = tile + lane * kStride;
+  float x[I][4];
+  if (work) {
+    if (FIRST) {
+      load_rows<W, I>((const T*)p.x + first + p0, p.t, w, of, x);
+    } else {
+      Run<I, T> r;
+      load_run<W, I>((const T*)p.x + run, total, p.x_quads, tid, r);
+      run_to_tile<W, I>(r, total, p.x_quads, tid, p.t, tile);
+    }
+  }
+  for (int i = (int)threadIdx.x; i < 4 * W * I; i += 64 * W * G) {
+    affine[0][i] = i >= n ? 0.f : p.weight != nullptr ? p.weight[i] : 1.f;
+    affine[1][i] = i >= n || p.bias == nullptr ? 0.f : p.bias[i];
+  }
+  __syncthreads();
+  if (!work) return;
+  if (!FIRST) from_tile<W, I>(mine, w, x);
+  const auto is = [&](int i, int j) { return 4 * (w + i * W) + j < n; };
+  const float labels = (float)n;
+  float sum = 0;
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += is(i, j) ? x[i][j] : 0.f;
+  const int here = labels_of<W, I>(w, n);
+  float mean = here > 0 ? sum / (float)here : 0.f, m2 = 0;
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = is(i, j) ? x[i][j] - mean : 0.f;
+      m2 += d * d;
+    }
+  if (W > 1) {
+    part[w][lane] = float2{mean, m2};
+    tile_sync<W>();
+    float2 of_wave[W];
+    sum = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      of_wave[k] = part[k][lane];
+      sum += of_wave[k].x * (float)labels_of<W, I>(k, n);
+    }
+    mean = sum / labels;
+    m2 = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const float d = of_wave[k].x - mean;
+      m2 += of_wave[k].y + (float)labels_of<W, I>(k, n) * d * d;
+    }
+  }
+  const float r = 1.f / sqrtf(m2 / labels + p.eps);
+  if (p.stats != nullptr && w == 0 && lane < count)
+    reinterpret_cast<float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + lane] = float2{mean, r};
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int l = 4 * (w + i * W) + j;
+      x[i][j] = (x[i][j] - mean) * r * affine[0][l] + affine[1][l];
+    }
+  to_tile<W, I>(mine, w, x);
+  tile_sync<W>();
+  store_run<W, I>(p.y + run, total, p.y_quads, tid, p.t, tile);
+}
+
+// SUMS: with the sums over pixels that dweight and dbias are made of.
+template <typename T, bool FIRST, bool SUMS, int W, int I, int G>
+__global__ void __launch_bounds__(64 * W * G) norm_grad_kernel(Norm p) {
+  constexpr int kStride = tile_stride(W * I);
+  __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
+  __shared__ __align__(16) float weight[4 * W * I];
+  __shared__ float2 part[W > 1 ? W : 1][kTilePixels];
+  const int tid = (int)threadIdx.x % (64 * W), group = uniform_i((int)threadIdx.x / (64 * W));
+  const int lane = tid % 64, w = uniform_i(tid / 64), n = p.t.labels;
+  float* const tile = tiles + group * kTilePixels * kStride;
+  float* const mine = tile + lane * kStride;
+  for (int i = (int)threadIdx.x; i < 4 * W * I; i += 64 * W * G)
+    weight[i] = i >= n ? 0.f : p.weight != nullptr ? p.weight[i] : 1.f;
+  __syncthreads();
+  const float per_label = 1.f / (float)n;
+  float dw[SUMS ? I : 1][4] = {}, db[SUMS ? I : 1][4] = {};
+  for (unsigned at = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.t.xcd_group) * G + group; at < p.t.total;
+       at += gridDim.x * G) {
+    const unsigned item = at / p.t.per_item;
+    const int64_t p0 = (int64_t)(at - item * p.t.per_item) * kTilePixels;
+    const int count = (int)min((int64_t)kTilePixels, p.t.pixels - p0);
+    const unsigned total = (unsigned)(count * n);
+    const int of = min(lane, count - 1);
+    const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n;
+    float x[I][4], d[I][4];
+    Run<I, float> dy;
+    load_run<W, I>(p.dy + run, total, p.y_quads, tid, dy);
+    const float2 stats = reinterpret_cast<const float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + of];
+    if (FIRST) {
+      load_rows<W, I>((const T*)p.x + first + p0, p.t, w, of, x);
+    } else {
+      Run<I, T> rx;
+      load_run<W, I>((const T*)p.x + run, total, p.x_quads, tid, rx);
+      run_to_tile<W, I>(rx, total, p.x_quads, tid, p.t, tile);
+      tile_sync<W>();
+      from_tile<W, I>(mine, w, x);
+      tile_sync<W>();
+    }
+    run_to_tile<W, I>(dy, total, p.y_quads, tid, p.t, tile);
+    tile_sync<W>();
+    from_tile<W, I>(mine, w, d);
+    float s1 = 0, s2 = 0;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int l = 4 * (w + i * W) + j;
+        // (behind the last label or pixel of a tile in LDS lies an earlier one's, or no number at all)
+        const bool in = l < n && lane < count;
+        d[i][j] = in ? d[i][j] : 0.f;
+        x[i][j] = in ? (x[i][j] - stats.x) * stats.y : 0.f;
+        if (SUMS) {
+          dw[i][j] += d[i][j] * x[i][j];
+          db[i][j] += d[i][j];
+        }
+        d[i][j] *= weight[l];
+        s1 += d[i][j];
+        s2 += d[i][j] * x[i][j];
+      }
+    if (W > 1) {
+      part[w][lane] = float2{s1, s2};
+      tile_sync<W>();
+      s1 = s2 = 0;
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const float2 of_wave = part[k][lane];
+        s1 += of_wave.x;
+        s2 += of_wave.y;
+      }
+    }
+    if (p.dx != nullptr) {
+      s1 *= per_label;
+      s2 *= per_label;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = stats.y * (d[i][j] - s1 - x[i][j] * s2);
+      if (FIRST) {
+        if (lane < count) store_rows<W, I>((T*)p.dx + first + p0, p.t, w, lane, x);
+      } else {
+        to_tile<W, I>(mine, w, x);
+        tile_sync<W>();
+        store_run<W, I>((T*)p.dx + run, total, p.x_quads, tid, p.t, tile);
+      }
+    }
+    tile_sync<W>();  // (the next tile overwrites this one and its parts)
+  }
+  if (SUMS) {
+    // over the lanes, and the G wavefronts that had tiles of their own
+    __shared__ float ends[G][2][4 * W * I];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = wave_sum(dw[i][j]), b = wave_sum(db[i][j]);
+        if (lane == 0) {
+          ends[group][0][4 * (w + i * W) + j] = a;
+          ends[group][1][4 * (w + i * W) + j] = b;
+        }
+      }
+    __syncthreads();
+    for (int i = (int)threadIdx.x; i < 2 * n; i += 64 * W * G) {
+      float sum = 0;
+#pragma unroll
+      for (int g = 0; g < G; ++g) sum += i < n ? ends[g][0][i] : ends[g][1][i - n];
+      p.sums[(int64_t)blockIdx.x * 2 * n + i] = sum;
+    }
+  }
+}
+
+// The workgroups' rows of 2 * n sums, a column to every 16th thread, in 64 bits.
+__global__ void __launch_bounds__(256) norm_sums_kernel(const float* __restrict__ sums, int rows, int n, float* __restrict__ dweight,
+                                                       float* __restrict__ dbias) {
+  __shared__ double part[16][17];
+  const int of = (int)threadIdx.x % 16, by = (int)threadIdx.x / 16, column = (int)blockIdx.x * 16 + of;
+  double sum = 0;
+  if (column < 2 * n) {
+#pragma unroll 8
+    for (int row = by; row < rows; row += 16) sum += (double)sums[(int64_t)row * 2 * n + column];
+  }
+  part[by][of] = sum;
+  __syncthreads();
+  if (by == 0 && column < 2 * n) {
+    sum = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum += part[k][of];
+    if (column < n) {
+      if (dweight != nullptr) dweight[column] = (float)sum;
+    } else if (dbias != nullptr) {
+      dbias[column - n] = (float)sum;
+    }
+  }
+}
+
+int status(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+
+// f(wavefronts of a tile, quads of a wavefront, tiles of a workgroup)
+template <int W, int I, int G>
+struct Shape {
+  static constexpr int kW = W, kI = I, kG = G;
+};
+template <typename F>
+void with_shape(int n, F f) {
+  if (n <= 4)
+    f(Shape<1, 1, 4>());
+  else if (n <= 8)
+    f(Shape<1, 2, 4>());
+  else if (n <= 16)
+    f(Shape<1, 4, 4>());
+  else if (n <= 24)
+    f(Shape<1, 6, 4>());
+  else if (n <= 32)
+    f(Shape<1, 8, 4>());
+  else if (n <= 48)
+    f(Shape<2, 6, 1>());
+  else if (n <= 64)
+    f(Shape<4, 4, 1>());
+  else if (n <= 96)
+    f(Shape<4, 6, 1>());
+  else if (n <= 128)
+    f(Shape<8, 4, 1>());
+  else if (n <= 192)
+    f(Shape<8, 6, 1>());
+  else
+    f(Shape<8, 8, 1>());
+}
+
+unsigned grad_blocks(unsigned tiles, int per_block) {
+  const unsigned blocks = (tiles + (unsigned)per_block - 1) / (unsigned)per_block;
+  return blocks < (unsigned)kSumRows ? blocks : (unsigned)kSumRows;
+}
+
+template <typename T, bool FIRST>
+void launch(const Norm& p, hipStream_t st) {
+  with_shape(p.t.labels, [&](auto s) {
+    constexpr int W = s.kW, I = s.kI, G = s.kG;
+    norm_kernel<T, FIRST, W, I, G><<<(p.t.total + G - 1) / G, 64 * W * G, 0, st>>>(p);
+  });
+}
+template <typename T, bool FIRST>
+void launch_grad(const Norm& p, float* dweight, float* dbias, hipStream_t st) {
+  with_shape(p.t.labels, [&](auto s) {
+    constexpr int W = s.kW, I = s.kI, G = s.kG;
+    const unsigned blocks = grad_blocks(p.t.total, G);
+    if (p.sums == nullptr) {
+      norm_grad_kernel<T, FIRST, false, W, I, G><<<blocks, 64 * W * G, 0, st>>>(p);
+      return;
+    }
+    norm_grad_kernel<T, FIRST, true, W, I, G><<<blocks, 64 * W * G, 0, st>>>(p);
+    norm_sums_kernel<<<(2 * p.t.labels + 15) / 16, 256, 0, st>>>(p.sums, (int)blocks, p.t.labels, dweight, dbias);
+  });
+}
+template <typename F>
+void with_type(int dtype, bool labels_first, F f) {
+  const auto by_layout = [&](auto type) {
+    labels_first ? f(type, std::true_type()) : f(type, std::false_type());
+  };
+  if (dtype == MPL_F32)
+    by_layout(float());
+  else if (dtype == MPL_F16)
+    by_layout((_Float16)0);
+  else
+    by_layout((__bf16)0);
+}
+
+int prepare(const char* what, Norm& p, int dtype, bool labels_first, int batch, int n_disp, int64_t pixels) {
+  if (dtype < 0 || dtype > MPL_BF16) return fail(MPL_EINVAL, "%s: unknown data type %d", what, dtype);
+  if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
+  if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
+  if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels, 512)) return fail(MPL_EINVAL, "%s: too many pixels", what);
+  return MPL_OK;
+}
+int whole_quads(const void* at, int n_disp, int dtype) {
+  return n_disp % 4 == 0 && ((uintptr_t)at & (dtype == MPL_F32 ? 15 : 7)) == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels) {
+  if (batch <= 0 || pixels <= 0 || n_disp < 1 || n_disp > kMaxL) return 0;
+  const int64_t per_item = (pixels + kTilePixels - 1) / kTilePixels;
+  const int64_t rows = per_item > kSumRows / batch ? kSumRows : per_item * batch;
+  return rows * 2 * n_disp;
+}
+
+int mpl_norm_labels_last(int dtype, int labels_first, const void* src, const float* weight, const float* bias, float eps,
+                         float* dst, float* stats, int batch, int n_disp, int64_t pixels, void* stream) {
+  Norm p = {};
+  const int rc = prepare("norm_labels_last", p, dtype, labels_first != 0, batch, n_disp, pixels);
+  if (rc != MPL_OK) return rc;
+  if (!(eps >= 0 && eps < __builtin_huge_valf())) return fail(MPL_EINVAL, "norm_labels_last: eps must be finite and not below 0");
+  if (batch == 0 || pixels == 0) return MPL_OK;
+  if (src == nullptr || dst == nullptr) return fail(MPL_EINVAL, "norm_labels_last: null pointer");
+  p.x = src;
+  p.weight = weight;
+  p.bias = bias;
+  p.y = dst;
+  p.stats = stats;
+  p.eps = eps;
+  p.x_quads = whole_quads(src, n_disp, dtype);
+  p.y_quads = whole_quads(dst, n_disp, MPL_F32);
+  with_type(dtype, labels_first != 0, [&](auto type, auto first) { launch<decltype(type), first.value>(p, (hipStream_t)stream); });
+  return status("norm_labels_last");
+}
+
+int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, const float* weight, const float* stats,
+                              const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace, int batch, int n_disp,
+                              int64_t pixels, void* stream) {
+  Norm p = {};
+  const int rc = prepare("norm_labels_last_grad", p, dtype, labels_first != 0, batch, n_disp, pixels);
+  if (rc != MPL_OK) return rc;
+  const bool sums = dweight != nullptr || dbias != nullptr;
+  if (batch == 0 || pixels == 0) {
+    // (a sum of nothing)
+    if (sums) norm_sums_kernel<<<(2 * n_disp + 15) / 16, 256, 0, (hipStream_t)stream>>>(nullptr, 0, n_disp, dweight, dbias);
+    return sums ? status("norm_labels_last_grad") : MPL_OK;
+  }
+  if (src == nullptr || stats == nullptr || ddst == nullptr || (sums && workspace == nullptr))
+    return fail(MPL_EINVAL, "norm_labels_last_grad: null pointer");
+  if (dsrc == nullptr && !sums) return MPL_OK;
+  p.x = src;
+  p.weight = weight;
+  p.stats = const_cast<float*>(stats);
+  p.dy = ddst;
+  p.dx = dsrc;
+  p.sums = sums ? workspace : nullptr;
+  p.x_quads = whole_quads(src, n_disp, dtype) && whole_quads(dsrc, n_disp, dtype);
+  p.y_quads = whole_quads(ddst, n_disp, MPL_F32);
+  with_type(dtype, labels_first != 0,
+            [&](auto type, auto first) { launch_grad<decltype(type), first.value>(p, dweight, dbias, (hipStream_t)stream); });
+  return status("norm_labels_last_grad");
+}
+
+}  // extern "C"

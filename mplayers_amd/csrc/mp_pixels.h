@@ -1,0 +1,165 @@
+// Tiles of 64 pixels with a lane to a pixel, for the operators that stand around the layers.
+//
+// W wavefronts share the labels of a tile: wavefront w owns the quads (four labels) w, w + W, ..., I of them at most, so
+// that every one has as many labels as the others but for one quad.  With W = 1 the G wavefronts of a workgroup have a tile
+// each and meet nobody.
+//
+// In the network's layout (labels in front of the pixels) a lane reads its pixel in the row of each of its labels: 256 bytes to
+// an instruction in fp32.  In the operators' layout (labels innermost) a tile is one run of memory, which goes through LDS: the
+// labels of a pixel side by side, an odd number of quads apart, which keeps the 16-byte accesses of either side off each
+// other's banks.
+#ifndef MPLAYERS_AMD_MP_PIXELS_H_
+#define MPLAYERS_AMD_MP_PIXELS_H_
+
+#include "mp_common.h"
+
+namespace mpl {
+
+constexpr int kTilePixels = 64;
+
+struct Tiles {
+  int64_t pixels;       // of an item
+  unsigned per_item;    // tiles
+  unsigned total;
+  int labels;
+  uint32_t reciprocal;  // 2^32 / labels, rounded up
+  int xcd_group;        // workgroups beside each other that go to one die (xcd_block)
+};
+
+// Tiles of 64 pixels and `threads` threads each; false where a launch would have too many.
+inline bool make_tiles(Tiles& t, int items, int n_disp, int64_t pixels, int threads) {
+  if (pixels > ((int64_t)1 << 40)) return false;
+  const int64_t per_item = (pixels + kTilePixels - 1) / kTilePixels;
+  // (less than 2^31 threads, so that tiles and workgroups are ints as well)
+  if (per_item > 0x7fffffff / threads / items) return false;
+  t.pixels = pixels;
+  t.per_item = (unsigned)per_item;
+  t.total = (unsigned)per_item * (unsigned)items;
+  t.labels = n_disp;
+  t.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
+  t.xcd_group = 0;
+  return true;
+}
+
+constexpr int tile_stride(int quads) { return 4 * (quads | 1); }  // floats from pixel to pixel in LDS
+
+// What the wavefronts of a tile wait for each other with.
+template <int W>
+__device__ __forceinline__ void tile_sync() {
+  if (W > 1) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// Rows of the network's layout: from = the item's first label at the tile's first pixel.  Labels behind the last are read
+// from the last's place, so that there is no branch between the loads.
+template <int W, int I, typename T>
+__device__ __forceinline__ void load_rows(const T* from, const Tiles& t, int w, int of, float (&x)[I][4]) {
+  T raw[I][4];
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[i][j] = from[(int64_t)min(4 * (w + i * W) + j, t.labels - 1) * t.pixels + of];
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[i][j] = (float)raw[i][j];
+}
+
+template <int W, int I, typename T>
+__device__ __forceinline__ void store_rows(T* to, const Tiles& t, int w, int of, const float (&x)[I][4]) {
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int l = 4 * (w + i * W) + j;
+      if (l < t.labels) to[(int64_t)l * t.pixels + of] = (T)x[i][j];
+    }
+}
+
+// A run of the operators' layout, `total` labels of whole pixels, as the threads of a tile hold it on its way.
+template <int I, typename T>
+struct Run {
+  T x[4 * I];
+};
+template <typename T>
+struct alignas(4 * sizeof(T)) Quad {
+  T x[4];
+};
+
+// Entry i of a run in the tile.
+template <int STRIDE>
+__device__ __forceinline__ unsigned tile_place(unsigned i, const Tiles& t) {
+  const unsigned p = t.labels == 1 ? i : __umulhi(i, t.reciprocal);
+  return p * STRIDE + (i - p * (unsigned)t.labels);
+}
+
+// quads: the labels are whole quads and the run is aligned to them.  tid: of the 64 * W threads of the tile.
+template <int W, int I, typename T>
+__device__ __forceinline__ void load_run(const T* from, unsigned total, bool quads, int tid, Run<I, T>& r) {
+  constexpr int kThreads = 64 * W;
+  if (quads) {
+#pragma unroll
+    for (int k = 0; k < I; ++k) {
+      const Quad<T> q = *reinterpret_cast<const Quad<T>*>(from + min((unsigned)(tid + k * kThreads) * 4, total - 4));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.x[4 * k + j] = q.x[j];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4 * I; ++k) r.x[k] = from[min((unsigned)(tid + k * kThreads), total - 1)];
+  }
+}
+template <int W, int I, typename T>
+__device__ __forceinline__ void run_to_tile(const Run<I, T>& r, unsigned total, bool quads, int tid, const Tiles& t, float* tile) {
+  constexpr int kThreads = 64 * W, kStride = tile_stride(W * I);
+  if (quads) {
+#pragma unroll
+    for (int k = 0; k < I; ++k)
+      *reinterpret_cast<float4*>(&tile[tile_place<kStride>(min((unsigned)(tid + k * kThreads) * 4, total - 4), t)]) =
+          float4{(float)r.x[4 * k], (float)r.x[4 * k + 1], (float)r.x[4 * k + 2], (float)r.x[4 * k + 3]};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4 * I; ++k)
+      tile[tile_place<kStride>(min((unsigned)(tid + k * kThreads), total - 1), t)] = (float)r.x[k];
+  }
+}
+template <int W, int I, typename T>
+__device__ __forceinline__ void store_run(T* to, unsigned total, bool quads, int tid, const Tiles& t, const float* tile) {
+  constexpr int kThreads = 64 * W, kStride = tile_stride(W * I);
+  if (quads) {
+    for (unsigned i = (unsigned)tid * 4; i < total; i += kThreads * 4) {
+      const float4 x = *reinterpret_cast<const float4*>(&tile[tile_place<kStride>(i, t)]);
+      *reinterpret_cast<Quad<T>*>(to + i) = Quad<T>{{(T)x.x, (T)x.y, (T)x.z, (T)x.w}};
+    }
+  } else {
+    for (unsigned i = (unsigned)tid; i < total; i += kThreads) to[i] = (T)tile[tile_place<kStride>(i, t)];
+  }
+}
+
+// A lane's labels in the tile: tile = its pixel's.
+template <int W, int I>
+__device__ __forceinline__ void from_tile(const float* tile, int w, float (&x)[I][4]) {
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const float4 q = *reinterpret_cast<const float4*>(&tile[4 * (w + i * W)]);
+    x[i][0] = q.x;
+    x[i][1] = q.y;
+    x[i][2] = q.z;
+    x[i][3] = q.w;
+  }
+}
+template <int W, int I>
+__device__ __forceinline__ void to_tile(float* tile, int w, const float (&x)[I][4]) {
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+    *reinterpret_cast<float4*>(&tile[4 * (w + i * W)]) = float4{x[i][0], x[i][1], x[i][2], x[i][3]};
+}
+
+}  // namespace mpl
+
+#endif  // MPLAYERS_AMD_MP_PIXELS_H_

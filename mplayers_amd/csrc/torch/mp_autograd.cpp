@@ -28,17 +28,23 @@ struct EntryPoints {
   decltype(&mpl_dropout_labels_last) dropout_labels_last;
   decltype(&mpl_dropout_labels_first) dropout_labels_first;
   decltype(&mpl_sample_labels) sample_labels;
+  decltype(&mpl_norm_labels_last) norm_labels_last;
+  decltype(&mpl_norm_labels_last_grad) norm_labels_last_grad;
+  decltype(&mpl_norm_workspace) norm_workspace;
   decltype(&mpl_last_error) last_error;
 } lib;
 
 void bind(const std::vector<uintptr_t>& at) {
-  TORCH_CHECK(at.size() == 6, "bind: six entry points");
+  TORCH_CHECK(at.size() == 9, "bind: nine entry points");
   lib.bucket_context = reinterpret_cast<decltype(lib.bucket_context)>(at[0]);
   lib.bucket_sums = reinterpret_cast<decltype(lib.bucket_sums)>(at[1]);
   lib.dropout_labels_last = reinterpret_cast<decltype(lib.dropout_labels_last)>(at[2]);
   lib.dropout_labels_first = reinterpret_cast<decltype(lib.dropout_labels_first)>(at[3]);
   lib.sample_labels = reinterpret_cast<decltype(lib.sample_labels)>(at[4]);
-  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at[5]);
+  lib.norm_labels_last = reinterpret_cast<decltype(lib.norm_labels_last)>(at[5]);
+  lib.norm_labels_last_grad = reinterpret_cast<decltype(lib.norm_labels_last_grad)>(at[6]);
+  lib.norm_workspace = reinterpret_cast<decltype(lib.norm_workspace)>(at[7]);
+  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at[8]);
 }
 
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -201,6 +207,126 @@ at::Tensor labels_last_dropout(const at::Tensor& x, double p, const at::Tensor& 
   return DropoutLast::apply(x, state, p, kind);
 }
 
+// ------------------------------------------------------------------------------------------------------ layer norm
+// (batch, cv, H, W, labels) of a tensor in either layout
+struct Layout {
+  int64_t batch, cv, n, height, width;
+  Layout(const at::Tensor& t, bool labels_first) {
+    const auto s = t.sizes();
+    batch = s[0];
+    cv = s[1];
+    n = s[labels_first ? 2 : 4];
+    height = s[labels_first ? 3 : 2];
+    width = s[labels_first ? 4 : 3];
+  }
+  int64_t pixels() const { return height * width; }
+};
+template <typename T>
+T* or_null(const at::Tensor& t) {
+  return t.defined() ? t.data_ptr<T>() : nullptr;
+}
+void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// y, and the statistics that its gradient takes (undefined where they are not asked for)
+std::pair<at::Tensor, at::Tensor> norm_last(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double eps,
+                                            bool labels_first, bool with_stats) {
+  const Layout s(x, labels_first);
+  const auto single = x.options().dtype(at::kFloat);
+  at::Tensor y = at::empty({s.batch, s.cv, s.height, s.width, s.n}, single), stats;
+  if (with_stats) stats = at::empty({s.batch, s.cv, s.height, s.width, 2}, single);
+  const c10::DeviceGuard guard(x.device());
+  check(lib.norm_labels_last(mpl_type(x.scalar_type()), labels_first, x.data_ptr(), or_null<float>(weight), or_null<float>(bias),
+                             (float)eps, y.data_ptr<float>(), or_null<float>(stats), small(s.batch * s.cv), (int)s.n, s.pixels(),
+                             stream_of(x)),
+        "labels_last_norm");
+  return {y, stats};
+}
+
+// dx, dweight, dbias, undefined where they are not asked for
+variable_list norm_grad(const at::Tensor& grad_in, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& stats,
+                        bool labels_first, bool with_x, bool with_weight, bool with_bias) {
+  const at::Tensor grad = grad_in.contiguous();
+  const Layout s(x, labels_first);
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor dx, dweight, dbias, workspace;
+  if (with_x) dx = at::empty_like(x);
+  if (with_weight) dweight = at::empty({s.n}, grad.options());
+  if (with_bias) dbias = at::empty({s.n}, grad.options());
+  const int items = small(s.batch * s.cv);
+  if (with_weight || with_bias) workspace = at::empty({lib.norm_workspace(items, (int)s.n, s.pixels())}, grad.options());
+  check(lib.norm_labels_last_grad(mpl_type(x.scalar_type()), labels_first, x.data_ptr(), or_null<float>(weight),
+                                  stats.data_ptr<float>(), grad.data_ptr<float>(), data_or_null(dx), or_null<float>(dweight),
+                                  or_null<float>(dbias), or_null<float>(workspace), items, (int)s.n, s.pixels(), stream_of(x)),
+        "labels_last_norm's gradient");
+  return {dx, dweight, dbias};
+}
+
+// The gradient where it is recorded for another one, which there is none of: an error when that is asked for, not before.
+struct NormGrad : Function<NormGrad> {
+  static variable_list forward(AutogradContext*, const at::Tensor& grad, const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                               const at::Tensor& stats, bool labels_first, bool with_x, bool with_weight, bool with_bias) {
+    variable_list out = norm_grad(grad, x, weight.value_or(at::Tensor()), stats, labels_first, with_x, with_weight, with_bias);
+    for (at::Tensor& t : out)
+      if (!t.defined()) t = at::empty({0}, grad.options());
+    return out;
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    TORCH_CHECK(false, "labels_last_norm cannot be differentiated twice");
+  }
+};
+struct NormLast : Function<NormLast> {
+  // (an input that is not there takes no place among those that may need a gradient)
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x_in, const std::optional<at::Tensor>& weight_in,
+                            const std::optional<at::Tensor>& bias_in, double eps, bool labels_first) {
+    const at::Tensor x = x_in.contiguous(), weight = weight_in ? weight_in->contiguous() : at::Tensor(),
+                     bias = bias_in ? bias_in->contiguous() : at::Tensor();
+    ctx->saved_data["weight"] = weight_in.has_value();
+    ctx->saved_data["bias"] = bias_in.has_value();
+    const auto [y, stats] = norm_last(x, weight, bias, eps, labels_first, true);
+    ctx->save_for_backward({x, weight, stats});
+    ctx->saved_data["labels_first"] = labels_first;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const bool labels_first = ctx->saved_data["labels_first"].toBool();
+    const bool weighted = ctx->saved_data["weight"].toBool();
+    const bool wanted[] = {ctx->needs_input_grad(0), weighted && ctx->needs_input_grad(1),
+                           ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(weighted ? 2 : 1)};
+    variable_list out;
+    if (at::GradMode::is_enabled()) {
+      out = NormGrad::apply(grads[0], saved[0], weighted ? std::optional<at::Tensor>(saved[1]) : std::nullopt, saved[2],
+                            labels_first, wanted[0], wanted[1], wanted[2]);
+      for (int k = 0; k < 3; ++k)
+        if (!wanted[k]) out[k] = at::Tensor();
+    } else {
+      out = norm_grad(grads[0], saved[0], saved[1], saved[2], labels_first, wanted[0], wanted[1], wanted[2]);
+    }
+    return {out[0], out[1], out[2], {}, {}};
+  }
+};
+
+at::Tensor labels_last_norm(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
+                            double eps, bool labels_first) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 5, "labels_last_norm: x must be a (batch, cv, labels, H, W) or (batch, cv, H, W, labels) "
+              "GPU tensor");
+  TORCH_CHECK(mpl_type(x.scalar_type()) >= 0, "labels_last_norm: x must be float32, float16 or bfloat16, got ", x.scalar_type());
+  const int64_t n = Layout(x, labels_first).n;
+  TORCH_CHECK(n >= 1 && n <= MPL_MAX_LABELS, "labels_last_norm: 1 to 256 labels, got ", n);
+  bool recorded = at::GradMode::is_enabled() && x.requires_grad();
+  const std::pair<const char*, const std::optional<at::Tensor>*> given[] = {{"weight", &weight}, {"bias", &bias}};
+  for (const auto& [name, t] : given) {
+    if (!t->has_value()) continue;
+    TORCH_CHECK((*t)->device() == x.device() && (*t)->scalar_type() == at::kFloat && (*t)->dim() == 1 && (*t)->size(0) == n,
+                "labels_last_norm: ", name, " must be ", n, " float32 numbers on the device of x");
+    recorded |= at::GradMode::is_enabled() && (*t)->requires_grad();
+  }
+  TORCH_CHECK(eps >= 0 && eps <= std::numeric_limits<float>::max(), "labels_last_norm: eps must be finite and not below 0, got ", eps);
+  if (recorded) return NormLast::apply(x, weight, bias, eps, labels_first);
+  return norm_last(x.contiguous(), weight ? weight->contiguous() : at::Tensor(), bias ? bias->contiguous() : at::Tensor(), eps,
+                   labels_first, false).first;
+}
+
 // -------------------------------------------------------------------------------------------------- sampled labels
 // A parameter: a number, or a tensor of one per image (not looked at).
 template <typename T>
@@ -262,5 +388,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
   m.def("bucket_context", &bucket_context);
   m.def("labels_last_dropout", &labels_last_dropout);
+  m.def("labels_last_norm", &labels_last_norm);
   m.def("sample_labels", &sample_labels);
 }

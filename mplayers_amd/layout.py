@@ -8,6 +8,9 @@ passes are the opposite transposes.
 `labels_last_dropout` is dropout of the unary costs within that change (no counterpart in the
 reference, whose networks have their dropout in front of the layer): mpl_dropout_labels_last and
 mpl_dropout_labels_first, which form the mask anew from a seed instead of storing it.
+
+`labels_last_norm` is layer norm over the labels of a pixel within it (no counterpart either):
+mpl_norm_labels_last and mpl_norm_labels_last_grad.
 """
 import ctypes
 
@@ -90,3 +93,22 @@ def labels_last_dropout(x, p, state, share="element"):
   share  'element': every entry by itself; 'pixel': all labels of a pixel (its neighbours' messages then
          decide); 'label': all pixels of a label's plane"""
   return _lib.autograd().labels_last_dropout(x, p, state, share)
+
+
+def labels_last_norm(x, weight=None, bias=None, eps=1e-5, labels_first=True):
+  """labels_last(layer norm of x over its labels) in one pass over the costs, in fp32.
+
+  A network's unary costs have whatever scale a pixel gives them, a layer's pairwise costs have one for all.
+
+  x       (batch, cv, labels, H, W), or (batch, cv, H, W, labels) with labels_first=False, fp32, fp16 or bf16, at most
+          256 labels
+  weight, bias
+          fp32, one number per label, or None (1 and 0)
+  -> (batch, cv, H, W, labels) fp32, (x - mean) / sqrt(var + eps) * weight + bias with the mean and the variance of each
+     pixel's labels.  Gradients come in x's layout and type; those of weight and bias are the same bits in every call.
+
+  An infinite cost or NaN makes its pixel's results NaN.  CPU tensors go through torch."""
+  if x.is_cuda:
+    return _lib.autograd().labels_last_norm(x, weight, bias, eps, labels_first)
+  x = (x.movedim(2, -1) if labels_first else x).float()
+  return torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps).contiguous()

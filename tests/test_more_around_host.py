@@ -1,0 +1,129 @@
+"""Layer norm in the layout change, a teacher's best labels, the divergence from them and verified labels on the CPU: the
+refusals of the entry points, the plain forms that the GPU tests compare with, and the modules with them."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import more_around_oracle as oracle
+from tests.test_capi_host import _args
+
+
+@pytest.fixture(scope="module")
+def lib():
+  from mplayers_amd import _lib
+  return _lib.load()
+
+
+def _refused(lib, rc, words):
+  assert rc == -1 and words in lib.mpl_last_error(), (rc, lib.mpl_last_error())
+
+
+# (refused before a pointer is looked at, and nothing is launched)
+ONE = ctypes.c_void_p(1 << 20)
+
+
+def test_norm_refusals(lib):
+  def last(dtype=0, src=ONE, eps=1e-5, dst=ONE, batch=1, n=4, pixels=9):
+    return lib.mpl_norm_labels_last(dtype, 1, src, None, None, eps, dst, None, batch, n, pixels, None)
+
+  def grad(dtype=0, src=ONE, stats=ONE, ddst=ONE, dsrc=ONE, dweight=None, workspace=None, batch=1, n=4, pixels=9):
+    return lib.mpl_norm_labels_last_grad(dtype, 1, src, None, stats, ddst, dsrc, dweight, None, workspace, batch, n, pixels, None)
+
+  for call in (last, grad):
+    _refused(lib, call(src=None), b"null")
+    _refused(lib, call(dtype=3), b"type")
+    _refused(lib, call(dtype=-1), b"type")
+    _refused(lib, call(n=0), b"n_disp")
+    _refused(lib, call(n=257), b"n_disp")
+    _refused(lib, call(pixels=-1), b"negative")
+    _refused(lib, call(batch=-1), b"negative")
+    _refused(lib, call(batch=1 << 20, pixels=1 << 30), b"too many")
+    _refused(lib, call(pixels=1 << 32), b"too many")
+    assert call(batch=0) == 0 and call(pixels=0) == 0
+  _refused(lib, last(dst=None), b"null")
+  for eps in (-1e-9, math.nan, math.inf):
+    _refused(lib, last(eps=eps), b"eps")
+  _refused(lib, grad(stats=None), b"null")
+  _refused(lib, grad(ddst=None), b"null")
+  _refused(lib, grad(dweight=ONE), b"null")  # no workspace
+  assert grad(dsrc=None) == 0  # nothing wanted
+  # a row of 2 * n sums for each workgroup, 2048 at most
+  assert lib.mpl_norm_workspace(1, 21, 64) == 42 and lib.mpl_norm_workspace(3, 21, 65) == 6 * 42
+  assert lib.mpl_norm_workspace(1, 256, 1 << 30) == 2048 * 512 and lib.mpl_norm_workspace(1 << 30, 2, 1 << 30) == 2048 * 4
+  assert lib.mpl_norm_workspace(0, 21, 9) == 0 and lib.mpl_norm_workspace(1, 21, 0) == 0
+
+
+def test_norm_of_the_plain_form():
+  x = np.array([[1.0, 3.0], [5.0, 5.0]])
+  y, xhat, r = oracle.norm(x, [2.0, 1.0], [0.0, 10.0], 0.0 + 1e-30)
+  assert np.allclose(y[0], [-2, 11]) and np.allclose(xhat[1], 0) and np.isclose(r[0, 0], 1)
+  # against torch's, in 64 bits
+  g = torch.Generator().manual_seed(1)
+  x, w, b, dy = (torch.randn(s, dtype=torch.float64, generator=g, requires_grad=True) for s in ((7, 5), (5,), (5,), (7, 5)))
+  y = torch.nn.functional.layer_norm(x, (5,), w, b, 1e-5)
+  grads = torch.autograd.grad(y, (x, w, b), dy)
+  x, w, b, dy = (t.detach().numpy() for t in (x, w, b, dy))
+  assert np.allclose(oracle.norm(x, w, b, 1e-5)[0], y.detach().numpy(), rtol=0, atol=1e-12)
+  for got, want in zip(oracle.norm_grad(x, w, 1e-5, dy), grads):
+    assert np.allclose(got, want.numpy(), rtol=0, atol=1e-12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_norm_of_cpu_tensors(dtype):
+  from mplayers_amd import labels_last_norm
+  x = torch.randn(2, 1, 6, 3, 4).to(dtype).requires_grad_(True)
+  w, b = torch.rand(6).requires_grad_(True), torch.rand(6)
+  y = labels_last_norm(x, w, b, 1e-3)
+  assert y.shape == (2, 1, 3, 4, 6) and y.dtype == torch.float32 and y.is_contiguous()
+  flat = np.moveaxis(x.detach().double().numpy(), 2, -1)
+  want = oracle.norm(flat.reshape(-1, 6), w.detach().numpy(), b.numpy(), 1e-3)[0]
+  # fp32: some tens of roundings of values below 32
+  assert np.abs(y.detach().double().numpy().reshape(-1, 6) - want).max() <= 64 * 2.0 ** -24 * 32
+  assert torch.equal(labels_last_norm(x.movedim(2, -1), w, b, 1e-3, labels_first=False), y)
+  dx, dw = torch.autograd.grad(y.sum(), (x, w))
+  assert dx.shape == x.shape and dx.dtype == dtype and dw.shape == (6,)
+
+
+@pytest.mark.parametrize("soft", [False, True])
+def test_a_module_that_normalises(soft):
+  """mpnet_unary_norm: learned weights in the module's state, fp16 and bf16 costs taken, after dropout where there is any."""
+  from mplayers_amd import MPModule, MP_module_hard_soft, labels_last_norm
+  kind = MP_module_hard_soft.MPModule if soft else MPModule
+  fields = dict(mpnet_smoothness_mode="TL", mpnet_smoothness_trunct_value=3, n_classes=9)
+  module = kind(_args(mpnet_unary_norm=True, mpnet_unary_norm_eps=1e-2, **fields), enable_create_label_context=True)
+  assert {"unary_norm_weight", "unary_norm_bias"} <= {name for name, _ in module.named_parameters()}
+  with torch.no_grad():
+    module.unary_norm_weight.copy_(torch.rand(9))
+    module.unary_norm_bias.copy_(torch.rand(9))
+  x = torch.randn(2, 1, 9, 4, 5)
+  want = labels_last_norm(x, module.unary_norm_weight, module.unary_norm_bias, 1e-2)
+  for training in (True, False):
+    assert torch.equal(module.train(training)._labels_last(x), want)
+  assert module._labels_last(x.half()).dtype == torch.float32
+  other = kind(_args(mpnet_unary_norm=True, **fields), enable_create_label_context=True)
+  other.load_state_dict(module.state_dict())
+  assert torch.equal(other.unary_norm_weight, module.unary_norm_weight)
+  for off in (dict(), dict(mpnet_unary_norm=False), dict(mpnet_unary_norm=None)):
+    plain = kind(_args(**fields, **off), enable_create_label_context=True)
+    assert set(plain.state_dict()) == {"label_context"} and torch.equal(plain._labels_last(x), x.permute(0, 1, 3, 4, 2))
+  # in evaluation a rate of dropout changes nothing
+  dropped = kind(_args(mpnet_unary_norm=True, mpnet_unary_norm_eps=1e-2, mpnet_unary_dropout=0.5, **fields),
+                 enable_create_label_context=True).eval()
+  dropped.load_state_dict(module.state_dict())
+  assert torch.equal(dropped._labels_last(x), want)
+
+
+def test_a_cpu_layer_on_normalised_costs():
+  """The CPU operators run on them as on any costs."""
+  from mplayers_amd import MPModule
+  fields = dict(mpnet_smoothness_mode="TL", mpnet_smoothness_trunct_value=3, n_classes=9)
+  table = (torch.arange(9)[:, None] - torch.arange(9)).abs().clamp(max=3).float().expand(4, 9, 9).contiguous()
+  modules = [MPModule(_args(mpnet_unary_norm=on, **fields), enable_create_label_context=True).eval() for on in (True, False)]
+  for module in modules:
+    module.set_label_context(torch.nn.Parameter(table), None, None)
+  x = torch.randn(1, 1, 9, 4, 5)
+  normalised = torch.nn.functional.layer_norm(x.movedim(2, -1), (9,)).movedim(-1, 2)
+  assert torch.allclose(modules[0](x)[0], modules[1](normalised)[0], rtol=1e-5, atol=1e-5)
