@@ -353,6 +353,37 @@ int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, cons
                               int n_disp, int64_t pixels, void* stream);
 int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels);
 
+/* What is kept of a teacher: the n_kept labels of least cost of every pixel, in order of cost, equal costs in order of label.
+ * cost of `dtype`, (items, n_disp, pixels) with labels_first, else (items, pixels, n_disp); +inf and NaN are no candidates,
+ * beside a cost of -inf only others of -inf are -> kept_labels, uint8, and kept_costs of `kept_dtype`, (items, n_kept,
+ * pixels) or (items, pixels, n_kept): the costs relative to the pixel's least one (a difference in fp32, rounded to the type).
+ * A place whose difference is +inf or that no candidate is left for has label 0 and cost +inf.  rest: NULL, or (items, pixels)
+ * fp32: -T log(sum of exp(-c / T)) over the other candidates' relative costs c, +inf where there are none.  The temperature T
+ * is for it alone, finite and above 0.  1 <= n_kept <= n_disp <= MPL_MAX_LABELS.  No counterpart in the reference. */
+int mpl_best_labels(int dtype, int labels_first, const void* cost, int n_kept, float temperature, int kept_dtype,
+                    uint8_t* kept_labels, void* kept_costs, float* rest, int items, int n_disp, int64_t pixels, void* stream);
+
+/* The divergence (Kullback and Leibler's) of the layers' costs from a teacher's, of whose labels a list is kept (as
+ * mpl_best_labels writes it, or of the caller's own), for every pixel; no counterpart in the reference.  cost (the student's)
+ * and the list in the layouts and types of mpl_best_labels, the list with 1 to MPL_MAX_LABELS entries in any order; rest as
+ * there, or NULL -> loss (items, pixels) fp32.  With q = softmax(-cost / T) over the labels (a cost of +inf: none), the
+ * teacher's classes are the entries (label, t) of the list, and the rest of the labels as one class where rest is given:
+ * p = softmax(-t / T) over the classes that are there, loss = sum p (log p - log q of the class), q of the rest being the
+ * sum of q over the labels that the list does not name.  An entry is there where t is not +inf, its label is below
+ * n_disp (one that is not there names nothing) and the student's cost of that label is not +inf; the rest is there where its
+ * cost is not +inf and the student has a label left for it.  A pixel without classes has loss 0 and no gradient.  A label that
+ * the list has twice counts with either entry's p.  NaN or -inf among a pixel's costs that take part makes its loss NaN, and
+ * its gradient but for labels of cost +inf.
+ * mpl_distill_costs_grad: dcost, in cost's layout and type, = dloss * (p - q) / T of the label, p being the entries' or, for
+ * a label of the rest, p(rest) q / q(rest); 0 for a label of cost +inf.  Everything is formed in fp32.  T finite and above
+ * 0. */
+int mpl_distill_costs(int dtype, int labels_first, const void* cost, int kept_dtype, const uint8_t* kept_labels,
+                      const void* kept_costs, const float* rest, float temperature, float* loss, int items, int n_disp,
+                      int n_kept, int64_t pixels, void* stream);
+int mpl_distill_costs_grad(int dtype, int labels_first, const void* cost, int kept_dtype, const uint8_t* kept_labels,
+                           const void* kept_costs, const float* rest, float temperature, const float* dloss, void* dcost,
+                           int items, int n_disp, int n_kept, int64_t pixels, void* stream);
+
 /* Pairwise tables whose entries go by buckets of the label distance k = |a - b|, for the layers' `context`; no
  * counterpart in the reference.  Bucket b is the distances starts[b] <= k < starts[b + 1]; starts is a HOST array of
  * n_buckets + 1 numbers in order, from 0 to n_disp, read during the call (a bucket may be empty).  At most

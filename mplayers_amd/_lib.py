@@ -13,7 +13,8 @@ SYMBOLS = ("mpl_trwp_forward", "mpl_trwp_backward", "mpl_isgmr_forward", "mpl_is
            "mpl_trwp_soft_backward", "mpl_soft_weighted_message", "mpl_soft_weighted_message_back", "mpl_set_option",
            "mpl_stereo_data_cost", "mpl_gradient_cues", "mpl_mrf_energy", "mpl_transpose",
            "mpl_dropout_labels_last", "mpl_dropout_labels_first", "mpl_bucket_context", "mpl_bucket_sums",
-           "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace")
+           "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace",
+           "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad")
 
 KERNEL_KINDS = ("fwd_sweep", "bwd_sweep", "belief", "aggregate", "label", "combine", "other",
                 "fwd_sweep_all", "bwd_sweep_all", "unary_all")
@@ -84,6 +85,9 @@ def load():
   lib.mpl_norm_labels_last.argtypes = [ci, ci, vp, vp, vp, cf, vp, vp, ci, ci, i64, vp]
   lib.mpl_norm_labels_last_grad.argtypes = [ci, ci] + [vp] * 8 + [ci, ci, i64, vp]
   lib.mpl_norm_workspace.argtypes = [ci, ci, i64]
+  lib.mpl_best_labels.argtypes = [ci, ci, vp, ci, cf, ci, vp, vp, vp, ci, ci, i64, vp]
+  lib.mpl_distill_costs.argtypes = [ci, ci, vp, ci, vp, vp, vp, cf, vp, ci, ci, ci, i64, vp]
+  lib.mpl_distill_costs_grad.argtypes = [ci, ci, vp, ci, vp, vp, vp, cf, vp, vp, ci, ci, ci, i64, vp]
   lib.mpl_n_chains.argtypes = [ci, ci, ci]
   lib.mpl_dcontext_copies.argtypes = [sp, ci]
   lib.mpl_table_is_dense.argtypes = [vp, ci]
@@ -169,8 +173,10 @@ def autograd():
     except ImportError as e:
       raise RuntimeError("mplayers_amd/_autograd.so is missing or of another torch (%s): build it with "
                          "`python -m mplayers_amd._build`" % e)
+    # (in the order of its EntryPoints)
     module.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
                  ("mpl_bucket_context", "mpl_bucket_sums", "mpl_dropout_labels_last", "mpl_dropout_labels_first",
-                  "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace", "mpl_last_error")])
+                  "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace",
+                  "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_last_error")])
     _autograd = module
   return _autograd

@@ -1,0 +1,171 @@
+// The labels of least cost of every pixel, in order, their costs, and what the others weigh: what is kept of a teacher.
+// For gfx950.
+//
+// cost -> k labels by cost, equal ones by label, with their costs relative to the best one (what a softmax of them needs, and what
+// fits a narrow type), and rest = -T log(sum over the other candidates of exp(-(c - best) / T)).  +inf and NaN are no candidates.
+//
+// The costs are read once, a pixel's labels over S lanes (mp_lanes.h).  A label is found as the least cost that is left and the
+// first label that has it, over the lane's registers and the lanes of the pixel, and taken out: about 4.5 instructions for each
+// label and place of the list, no sort.  So a short list is bound by HBM and a long one by the instructions.
+
+#include "mp_lanes.h"
+
+using namespace mpl;
+
+namespace {
+
+constexpr int kChunk = 16;  // places of the list that wait in LDS for whole rows
+
+struct Best {
+  LaneTiles t;
+  const void* cost;
+  uint8_t* labels;
+  void* costs;
+  float* rest;  // or nullptr
+  int k, kept;  // places of the list, type of their costs
+  float temperature, to_exponent;  // T, log2(e) / T
+  int quads;
+};
+
+template <typename T, int NV, int S, bool LAST>
+__global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
+  __shared__ __align__(16) float tile[kLanePixels * LaneTile<NV, S>::kStride];
+  __shared__ float found_cost[kChunk][kLanePixels];
+  __shared__ uint8_t found_label[kChunk][kLanePixels];
+  const unsigned block = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.t.xcd_group), tiles = (unsigned)p.t.tiles;
+  const int64_t item = block / tiles, p0 = (int64_t)(block - (unsigned)item * tiles) * kLanePixels;
+  const int count = (int)min((int64_t)kLanePixels, p.t.pixels - p0);
+  const int tid = (int)threadIdx.x, px = tid / S, s = tid % S;
+  {
+    LaneLoads<NV, S, LAST, T> loads;
+    loads.load((const T*)p.cost + item * p.t.n * p.t.pixels, p.t, p0, count, p.quads, tid);
+    loads.to_tile(tile, p.t, count, p.quads, tid);
+  }
+  __syncthreads();
+  float v[NV];
+  lane_costs<NV, S>(tile, px, s, p.t.n, v);
+  const auto least = [&]() {
+    float m = v[0];
+#pragma unroll
+    for (int j = 1; j < NV; ++j) m = v[j] < m ? v[j] : m;
+    return lanes_min<S>(m);
+  };
+  float best = least();
+  if (__builtin_amdgcn_ballot_w64(best == -kInf) != 0 && best == -kInf) {
+    // beside a cost of -inf only others of -inf are candidates
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = v[j] == -kInf ? 0.f : kInf;
+    best = 0;
+  }
+  for (int first = 0; first < p.k; first += kChunk) {
+    const int here = min(kChunk, p.k - first);
+    for (int k = 0; k < here; ++k) {
+      const float m = least();
+      int place = NV;
+#pragma unroll
+      for (int j = NV - 1; j >= 0; --j) place = v[j] == m ? j : place;
+      const int label = lanes_min<S>(place < NV ? s * NV + place : S * NV);
+      place = label - s * NV;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) v[j] = j == place ? kInf : v[j];
+      if (s == 0) {
+        const float c = m < kInf ? m - best : kInf;
+        found_cost[k][px] = c;
+        found_label[k][px] = (uint8_t)(c < kInf ? label : 0);
+      }
+    }
+    __syncthreads();
+    // whole rows of pixels, or of places
+    for (int i = tid; i < here * kLanePixels; i += kLanePixels * S) {
+      const int k = LAST ? i % here : i / kLanePixels, of = LAST ? i / here : i % kLanePixels;
+      if (of < count) {
+        const int64_t at = LAST ? (item * p.t.pixels + p0 + of) * p.k + first + k : (item * p.k + first + k) * p.t.pixels + p0 + of;
+        const float c = found_cost[k][of];
+        p.labels[at] = found_label[k][of];
+        if (p.kept == MPL_F32)
+          ((float*)p.costs)[at] = c;
+        else if (p.kept == MPL_F16)
+          ((_Float16*)p.costs)[at] = (_Float16)c;
+        else
+          ((__bf16*)p.costs)[at] = (__bf16)c;
+      }
+    }
+    __syncthreads();
+  }
+  if (p.rest != nullptr) {
+    const float m = least();
+    float sum = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) sum += v[j] < kInf ? __builtin_amdgcn_exp2f((m - v[j]) * p.to_exponent) : 0.f;
+    sum = lanes_sum<S>(sum);
+    if (s == 0 && px < count) p.rest[item * p.t.pixels + p0 + px] = m < kInf ? (m - best) - p.temperature * logf(sum) : kInf;
+  }
+}
+
+template <typename T, bool LAST>
+void launch(const Best& p, unsigned blocks, hipStream_t st) {
+  const int n = p.t.n;
+  if (n <= 4)
+    best_kernel<T, 4, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 8)
+    best_kernel<T, 8, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 16)
+    best_kernel<T, 8, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 24)
+    best_kernel<T, 12, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 32)
+    best_kernel<T, 16, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 48)
+    best_kernel<T, 12, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 64)
+    best_kernel<T, 16, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 96)
+    best_kernel<T, 24, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 128)
+    best_kernel<T, 32, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 192)
+    best_kernel<T, 24, 8, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
+  else
+    best_kernel<T, 32, 8, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
+}
+
+}  // namespace
+
+extern "C" int mpl_best_labels(int dtype, int labels_first, const void* cost, int n_kept, float temperature, int kept_dtype,
+                               uint8_t* kept_labels, void* kept_costs, float* rest, int items, int n_disp, int64_t pixels,
+                               void* stream) {
+  if (dtype < 0 || dtype > MPL_BF16) return fail(MPL_EINVAL, "best_labels: unknown data type %d", dtype);
+  if (kept_dtype < 0 || kept_dtype > MPL_BF16) return fail(MPL_EINVAL, "best_labels: unknown data type %d of the list", kept_dtype);
+  if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "best_labels: n_disp must be in [1, %d], got %d", kMaxL, n_disp);
+  if (n_kept < 1 || n_kept > n_disp)
+    return fail(MPL_EINVAL, "best_labels: the list must have 1 to n_disp = %d places, got %d", n_disp, n_kept);
+  if (!(temperature > 0 && temperature < kInf && 1.f / temperature < kInf))
+    return fail(MPL_EINVAL, "best_labels: the temperature must be finite and above 0");
+  if (items < 0 || pixels < 0) return fail(MPL_EINVAL, "best_labels: negative size");
+  if (items == 0 || pixels == 0) return MPL_OK;
+  if (cost == nullptr || kept_labels == nullptr || kept_costs == nullptr) return fail(MPL_EINVAL, "best_labels: null pointer");
+  Best p = {};
+  if (!make_lane_tiles(p.t, items, n_disp, pixels)) return fail(MPL_EINVAL, "best_labels: too many pixels");
+  p.cost = cost;
+  p.labels = kept_labels;
+  p.costs = kept_costs;
+  p.rest = rest;
+  p.k = n_kept;
+  p.kept = kept_dtype;
+  p.temperature = temperature;
+  p.to_exponent = (float)(1.4426950408889634 / (double)temperature);
+  p.quads = n_disp % 4 == 0 && ((uintptr_t)cost & (dtype == MPL_F32 ? 15 : 7)) == 0;
+  const unsigned blocks = (unsigned)(p.t.tiles * items);
+  const auto by_type = [&](auto type) {
+    using T = decltype(type);
+    labels_first != 0 ? launch<T, false>(p, blocks, (hipStream_t)stream) : launch<T, true>(p, blocks, (hipStream_t)stream);
+  };
+  if (dtype == MPL_F32)
+    by_type(float());
+  else if (dtype == MPL_F16)
+    by_type((_Float16)0);
+  else
+    by_type((__bf16)0);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "best_labels: %s", hipGetErrorString(e));
+}

@@ -47,7 +47,6 @@ __device__ __forceinline__ int labels_of(int w, int n) {
 
 template <typename T, bool FIRST, int W, int I, int G>
 __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
-  static_assert(W == 1 || G == 1, "wavefronts that share a tile meet at the workgroup's barrier");
   constexpr int kStride = tile_stride(W * I);
   __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
   __shared__ __align__(16) float affine[2][4 * W * I];
@@ -269,37 +268,6 @@ int status(const char* what) {
   return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
 }
 
-// f(wavefronts of a tile, quads of a wavefront, tiles of a workgroup)
-template <int W, int I, int G>
-struct Shape {
-  static constexpr int kW = W, kI = I, kG = G;
-};
-template <typename F>
-void with_shape(int n, F f) {
-  if (n <= 4)
-    f(Shape<1, 1, 4>());
-  else if (n <= 8)
-    f(Shape<1, 2, 4>());
-  else if (n <= 16)
-    f(Shape<1, 4, 4>());
-  else if (n <= 24)
-    f(Shape<1, 6, 4>());
-  else if (n <= 32)
-    f(Shape<1, 8, 4>());
-  else if (n <= 48)
-    f(Shape<2, 6, 1>());
-  else if (n <= 64)
-    f(Shape<4, 4, 1>());
-  else if (n <= 96)
-    f(Shape<4, 6, 1>());
-  else if (n <= 128)
-    f(Shape<8, 4, 1>());
-  else if (n <= 192)
-    f(Shape<8, 6, 1>());
-  else
-    f(Shape<8, 8, 1>());
-}
-
 unsigned grad_blocks(unsigned tiles, int per_block) {
   const unsigned blocks = (tiles + (unsigned)per_block - 1) / (unsigned)per_block;
   return blocks < (unsigned)kSumRows ? blocks : (unsigned)kSumRows;
@@ -342,7 +310,7 @@ int prepare(const char* what, Norm& p, int dtype, bool labels_first, int batch, 
   if (dtype < 0 || dtype > MPL_BF16) return fail(MPL_EINVAL, "%s: unknown data type %d", what, dtype);
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
   if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
-  if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels, 512)) return fail(MPL_EINVAL, "%s: too many pixels", what);
+  if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels)) return fail(MPL_EINVAL, "%s: too many pixels", what);
   return MPL_OK;
 }
 int whole_quads(const void* at, int n_disp, int dtype) {

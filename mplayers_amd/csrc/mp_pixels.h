@@ -26,8 +26,42 @@ struct Tiles {
   int xcd_group;        // workgroups beside each other that go to one die (xcd_block)
 };
 
-// Tiles of 64 pixels and `threads` threads each; false where a launch would have too many.
-inline bool make_tiles(Tiles& t, int items, int n_disp, int64_t pixels, int threads) {
+// W wavefronts of I quads each to a tile, G tiles to a workgroup.
+template <int W, int I, int G>
+struct TileShape {
+  static_assert(W == 1 || G == 1, "wavefronts that share a tile meet at the workgroup's barrier");
+  static constexpr int kW = W, kI = I, kG = G;
+};
+template <typename F>
+inline void with_shape(int n, F f) {
+  if (n <= 4)
+    f(TileShape<1, 1, 4>());
+  else if (n <= 8)
+    f(TileShape<1, 2, 4>());
+  else if (n <= 16)
+    f(TileShape<1, 4, 4>());
+  else if (n <= 24)
+    f(TileShape<1, 6, 4>());
+  else if (n <= 32)
+    f(TileShape<1, 8, 4>());
+  else if (n <= 48)
+    f(TileShape<2, 6, 1>());
+  else if (n <= 64)
+    f(TileShape<4, 4, 1>());
+  else if (n <= 96)
+    f(TileShape<4, 6, 1>());
+  else if (n <= 128)
+    f(TileShape<8, 4, 1>());
+  else if (n <= 192)
+    f(TileShape<8, 6, 1>());
+  else
+    f(TileShape<8, 8, 1>());
+}
+
+// False where a launch would have too many threads.
+inline bool make_tiles(Tiles& t, int items, int n_disp, int64_t pixels) {
+  int threads = 0;
+  with_shape(n_disp, [&](auto s) { threads = kTilePixels * s.kW; });
   if (pixels > ((int64_t)1 << 40)) return false;
   const int64_t per_item = (pixels + kTilePixels - 1) / kTilePixels;
   // (less than 2^31 threads, so that tiles and workgroups are ints as well)

@@ -20,7 +20,7 @@
 // so, and 32 bits, which take a third of the time, only where they tell (see sample_kernel): with 64 bits throughout 192
 // labels 1500x2000 took 1.42 ms.
 
-#include "mp_common.h"
+#include "mp_lanes.h"
 
 using namespace mpl;
 
@@ -51,120 +51,6 @@ struct Sample {
   int quads;            // labels last: whole and aligned quads
   int xcd_group;        // tiles beside each other that go to one die (xcd_block)
 };
-
-constexpr float kInf = __builtin_huge_valf();
-
-// +inf for what is no candidate.  By bits: the library is compiled for code without NaNs.
-__device__ __forceinline__ float candidate(float c) {
-  return (__builtin_bit_cast(int, c) & 0x7fffffff) > 0x7f800000 ? kInf : c;
-}
-
-// 2^y, y <= 0, to about 2^-51: the exponential series of the fraction, whose 14th term is below 2^-52 of the first.
-__device__ __forceinline__ double exp2_64(double y) {
-  y = y > -2000.0 ? y : -2000.0;
-  const double whole = rint(y), x = (y - whole) * 0.69314718055994530942;
-  // (coefficients in scalar registers: the kernels have few others to spare, see sample_kernel)
-  const auto scalar = [](double c) {
-    asm("" : "+s"(c));
-    return c;
-  };
-  double e = scalar(1.0 / 6227020800);
-  e = fma(e, x, scalar(1.0 / 479001600));
-  e = fma(e, x, scalar(1.0 / 39916800));
-  e = fma(e, x, scalar(1.0 / 3628800));
-  e = fma(e, x, scalar(1.0 / 362880));
-  e = fma(e, x, scalar(1.0 / 40320));
-  e = fma(e, x, scalar(1.0 / 5040));
-  e = fma(e, x, scalar(1.0 / 720));
-  e = fma(e, x, scalar(1.0 / 120));
-  e = fma(e, x, scalar(1.0 / 24));
-  e = fma(e, x, scalar(1.0 / 6));
-  e = fma(e, x, 0.5);
-  e = fma(e, x, 1.0);
-  e = fma(e, x, 1.0);
-  return ldexp(e, (int)whole);
-}
-// x > 0 and a number
-__device__ __forceinline__ bool positive(float x) {
-  const int bits = __builtin_bit_cast(int, x);
-  return bits > 0 && bits <= 0x7f800000;
-}
-
-// Reductions over the S lanes of a pixel, neighbours: within a row of 16, or the whole wavefront (S = 64, all lanes at
-// work; the four rows meet in scalar registers).
-template <int CTRL>
-__device__ __forceinline__ int move(int x) {
-  return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true);  // (0 where there is no such lane: part of what uses it)
-}
-template <int CTRL>
-__device__ __forceinline__ float move(float x) {
-  return __builtin_bit_cast(float, move<CTRL>(__builtin_bit_cast(int, x)));
-}
-template <int CTRL>
-__device__ __forceinline__ double move(double x) {
-  const int64_t bits = __builtin_bit_cast(int64_t, x);
-  const uint32_t lo = (uint32_t)move<CTRL>((int)(uint32_t)bits), hi = (uint32_t)move<CTRL>((int)(bits >> 32));
-  return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
-}
-__device__ __forceinline__ int from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
-__device__ __forceinline__ float from_lane(float x, int lane) { return readlane_f(x, lane); }
-__device__ __forceinline__ double from_lane(double x, int lane) {
-  const int64_t bits = __builtin_bit_cast(int64_t, x);
-  const uint32_t lo = (uint32_t)from_lane((int)(uint32_t)bits, lane), hi = (uint32_t)from_lane((int)(bits >> 32), lane);
-  return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
-}
-template <int S, typename V, typename F>
-__device__ __forceinline__ V over_lanes(V x, F f) {
-  if (S > 1) x = f(x, move<0xB1>(x));   // the other of a pair
-  if (S > 2) x = f(x, move<0x4E>(x));   // the other pair of four
-  if (S > 4) x = f(x, move<0x141>(x));  // the other four of eight
-  if (S > 8) x = f(x, move<0x140>(x));  // the other eight
-  if (S > 16) x = f(f(from_lane(x, 0), from_lane(x, 16)), f(from_lane(x, 32), from_lane(x, 48)));
-  return x;
-}
-template <int S, typename V>
-__device__ __forceinline__ V lanes_min(V x) {
-  return over_lanes<S>(x, [](V a, V b) { return b < a ? b : a; });
-}
-template <int S, typename V>
-__device__ __forceinline__ V lanes_max(V x) {
-  return over_lanes<S>(x, [](V a, V b) { return b > a ? b : a; });
-}
-template <int S, typename V>
-__device__ __forceinline__ V lanes_sum(V x) {
-  return over_lanes<S>(x, [](V a, V b) { return a + b; });
-}
-// x of the lane that CTRL names, in the rows of MASK; 0 where there is none
-template <int CTRL, int MASK = 0xf>
-__device__ __forceinline__ double move_or_0(double x) {
-  const int64_t bits = __builtin_bit_cast(int64_t, x);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CTRL, MASK, 0xf, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, MASK, 0xf, false);
-  return __builtin_bit_cast(double, (int64_t)(((uint64_t)hi << 32) | lo));
-}
-// f over the wavefront's lanes up to this one, where f(x, 0) is x
-template <typename F>
-__device__ __forceinline__ double wave_upto(double x, F f) {
-  x = f(x, move_or_0<0x111>(x));       // one lane up a row, two, four, eight
-  x = f(x, move_or_0<0x112>(x));
-  x = f(x, move_or_0<0x114>(x));
-  x = f(x, move_or_0<0x118>(x));
-  x = f(x, move_or_0<0x142, 0xa>(x));  // the last of a row to the next row: rows 1 and 3
-  x = f(x, move_or_0<0x143, 0xc>(x));  // the last of row 1 to rows 2 and 3
-  return x;
-}
-// sum of the lanes before this one, one after the other: a lane that adds nothing leaves the bits as they are
-template <int S, typename V>
-__device__ __forceinline__ V lanes_before(V x, int s) {
-  V upto = x;
-#pragma unroll
-  for (int i = 1; i < S; ++i) {
-    const V left = move<0x111>(upto);
-    if (s == i) upto = left + x;
-  }
-  const V left = S > 1 ? move<0x111>(upto) : x;
-  return s == 0 ? V(0) : left;
-}
 
 // Closes the range lo <= t <= hi of the least cost t with sum(of labels with cost <= t) >= target; hi where no sum
 // reaches it.  sum_upto(mid, below, above) gives the sum, the greatest cost that is not above mid and the least that

@@ -31,20 +31,31 @@ struct EntryPoints {
   decltype(&mpl_norm_labels_last) norm_labels_last;
   decltype(&mpl_norm_labels_last_grad) norm_labels_last_grad;
   decltype(&mpl_norm_workspace) norm_workspace;
+  decltype(&mpl_best_labels) best_labels;
+  decltype(&mpl_distill_costs) distill_costs;
+  decltype(&mpl_distill_costs_grad) distill_costs_grad;
   decltype(&mpl_last_error) last_error;
 } lib;
 
 void bind(const std::vector<uintptr_t>& at) {
-  TORCH_CHECK(at.size() == 9, "bind: nine entry points");
-  lib.bucket_context = reinterpret_cast<decltype(lib.bucket_context)>(at[0]);
-  lib.bucket_sums = reinterpret_cast<decltype(lib.bucket_sums)>(at[1]);
-  lib.dropout_labels_last = reinterpret_cast<decltype(lib.dropout_labels_last)>(at[2]);
-  lib.dropout_labels_first = reinterpret_cast<decltype(lib.dropout_labels_first)>(at[3]);
-  lib.sample_labels = reinterpret_cast<decltype(lib.sample_labels)>(at[4]);
-  lib.norm_labels_last = reinterpret_cast<decltype(lib.norm_labels_last)>(at[5]);
-  lib.norm_labels_last_grad = reinterpret_cast<decltype(lib.norm_labels_last_grad)>(at[6]);
-  lib.norm_workspace = reinterpret_cast<decltype(lib.norm_workspace)>(at[7]);
-  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at[8]);
+  size_t next = 0;
+  const auto take = [&](auto& entry) {
+    TORCH_CHECK(next < at.size(), "bind: ", at.size(), " entry points are too few");
+    entry = reinterpret_cast<std::remove_reference_t<decltype(entry)>>(at[next++]);
+  };
+  take(lib.bucket_context);
+  take(lib.bucket_sums);
+  take(lib.dropout_labels_last);
+  take(lib.dropout_labels_first);
+  take(lib.sample_labels);
+  take(lib.norm_labels_last);
+  take(lib.norm_labels_last_grad);
+  take(lib.norm_workspace);
+  take(lib.best_labels);
+  take(lib.distill_costs);
+  take(lib.distill_costs_grad);
+  take(lib.last_error);
+  TORCH_CHECK(next == at.size(), "bind: ", at.size(), " entry points are too many");
 }
 
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -327,6 +338,130 @@ at::Tensor labels_last_norm(const at::Tensor& x, const std::optional<at::Tensor>
                    labels_first, false).first;
 }
 
+// ---------------------------------------------------------------------------------------- a teacher's best labels
+void check_costs(const char* what, const at::Tensor& cost, bool labels_first) {
+  TORCH_CHECK(cost.is_cuda() && cost.dim() == 5, what, ": cost must be a (batch, cv, labels, H, W) or (batch, cv, H, W, labels) "
+              "GPU tensor");
+  TORCH_CHECK(mpl_type(cost.scalar_type()) >= 0, what, ": cost must be float32, float16 or bfloat16, got ", cost.scalar_type());
+  const int64_t n = Layout(cost, labels_first).n;
+  TORCH_CHECK(n >= 1 && n <= MPL_MAX_LABELS, what, ": 1 to 256 labels, got ", n);
+}
+void check_temperature(const char* what, double t) {
+  const float single = (float)t;
+  TORCH_CHECK(single > 0 && single <= std::numeric_limits<float>::max() && 1.f / single <= std::numeric_limits<float>::max(), what,
+              ": temperature must be finite and above 0, got ", t);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> best_labels(const at::Tensor& cost_in, int64_t k, double temperature,
+                                                           bool labels_first, at::ScalarType type) {
+  check_costs("best_labels", cost_in, labels_first);
+  TORCH_CHECK(mpl_type(type) >= 0, "best_labels: dtype must be float32, float16 or bfloat16, got ", type);
+  check_temperature("best_labels", temperature);
+  const Layout s(cost_in, labels_first);
+  TORCH_CHECK(k >= 1 && k <= s.n, "best_labels: k must be in [1, ", s.n, "], got ", k);
+  const c10::DeviceGuard guard(cost_in.device());
+  const at::Tensor cost = cost_in.detach().contiguous();
+  const std::vector<int64_t> size = labels_first ? std::vector<int64_t>{s.batch, s.cv, k, s.height, s.width}
+                                                 : std::vector<int64_t>{s.batch, s.cv, s.height, s.width, k};
+  const at::Tensor labels = at::empty(size, cost.options().dtype(at::kByte)), costs = at::empty(size, cost.options().dtype(type)),
+                   rest = at::empty({s.batch, s.cv, s.height, s.width}, cost.options().dtype(at::kFloat));
+  check(lib.best_labels(mpl_type(cost.scalar_type()), labels_first, cost.data_ptr(), (int)k, (float)temperature, mpl_type(type),
+                        labels.data_ptr<uint8_t>(), costs.data_ptr(), rest.data_ptr<float>(), small(s.batch * s.cv), (int)s.n,
+                        s.pixels(), stream_of(cost)),
+        "best_labels");
+  return {labels, costs, rest};
+}
+
+// ------------------------------------------------------------------------------------- the divergence from a teacher
+// cost, labels, costs and rest are contiguous; rest may be undefined
+at::Tensor distill_loss(const at::Tensor& cost, const at::Tensor& labels, const at::Tensor& costs, const at::Tensor& rest,
+                        double temperature, bool labels_first) {
+  const Layout s(cost, labels_first);
+  const c10::DeviceGuard guard(cost.device());
+  at::Tensor loss = at::empty({s.batch, s.cv, s.height, s.width}, cost.options().dtype(at::kFloat));
+  check(lib.distill_costs(mpl_type(cost.scalar_type()), labels_first, cost.data_ptr(), mpl_type(costs.scalar_type()),
+                          labels.data_ptr<uint8_t>(), costs.data_ptr(), or_null<float>(rest), (float)temperature,
+                          loss.data_ptr<float>(), small(s.batch * s.cv), (int)s.n, (int)Layout(labels, labels_first).n, s.pixels(),
+                          stream_of(cost)),
+        "distill_costs");
+  return loss;
+}
+at::Tensor distill_grad(const at::Tensor& grad_in, const at::Tensor& cost, const at::Tensor& labels, const at::Tensor& costs,
+                        const at::Tensor& rest, double temperature, bool labels_first) {
+  const Layout s(cost, labels_first);
+  const c10::DeviceGuard guard(cost.device());
+  const at::Tensor grad = grad_in.contiguous();
+  at::Tensor out = at::empty_like(cost);
+  check(lib.distill_costs_grad(mpl_type(cost.scalar_type()), labels_first, cost.data_ptr(), mpl_type(costs.scalar_type()),
+                               labels.data_ptr<uint8_t>(), costs.data_ptr(), or_null<float>(rest), (float)temperature,
+                               grad.data_ptr<float>(), out.data_ptr(), small(s.batch * s.cv), (int)s.n,
+                               (int)Layout(labels, labels_first).n, s.pixels(), stream_of(cost)),
+        "distill_costs' gradient");
+  return out;
+}
+
+struct DistillGrad : Function<DistillGrad> {  // (as NormGrad)
+  static at::Tensor forward(AutogradContext*, const at::Tensor& grad, const at::Tensor& cost, const at::Tensor& labels,
+                            const at::Tensor& costs, const std::optional<at::Tensor>& rest, double temperature, bool labels_first) {
+    return distill_grad(grad, cost, labels, costs, rest.value_or(at::Tensor()), temperature, labels_first);
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    TORCH_CHECK(false, "distill_costs cannot be differentiated twice");
+  }
+};
+struct Distill : Function<Distill> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& cost_in, const at::Tensor& labels_in, const at::Tensor& costs_in,
+                            const std::optional<at::Tensor>& rest_in, double temperature, bool labels_first) {
+    const at::Tensor cost = cost_in.contiguous(), labels = labels_in.contiguous(), costs = costs_in.contiguous(),
+                     rest = rest_in ? rest_in->contiguous() : at::Tensor();
+    ctx->save_for_backward({cost, labels, costs, rest});
+    ctx->saved_data["rest"] = rest.defined();
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["labels_first"] = labels_first;
+    return distill_loss(cost, labels, costs, rest, temperature, labels_first);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const double temperature = ctx->saved_data["temperature"].toDouble();
+    const bool labels_first = ctx->saved_data["labels_first"].toBool(), with_rest = ctx->saved_data["rest"].toBool();
+    return {at::GradMode::is_enabled()
+                ? DistillGrad::apply(grads[0], s[0], s[1], s[2], with_rest ? std::optional<at::Tensor>(s[3]) : std::nullopt,
+                                     temperature, labels_first)
+                : distill_grad(grads[0], s[0], s[1], s[2], s[3], temperature, labels_first),
+            {}, {}, {}, {}, {}};
+  }
+};
+
+at::Tensor distill_costs(const at::Tensor& cost, const at::Tensor& labels, const at::Tensor& costs,
+                         const std::optional<at::Tensor>& rest, double temperature, bool labels_first) {
+  check_costs("distill_costs", cost, labels_first);
+  check_temperature("distill_costs", temperature);
+  const Layout s(cost, labels_first);
+  const std::pair<const char*, const at::Tensor*> lists[] = {{"labels", &labels}, {"costs", &costs}};
+  for (const auto& [name, t] : lists) {
+    TORCH_CHECK(t->device() == cost.device() && t->dim() == 5, "distill_costs: ", name, " must be a list for every pixel, in the layout "
+                "of cost and on its device");
+    const Layout l(*t, labels_first);
+    TORCH_CHECK(l.batch == s.batch && l.cv == s.cv && l.height == s.height && l.width == s.width && l.n >= 1 && l.n <= MPL_MAX_LABELS,
+                "distill_costs: ", name, " must have 1 to 256 entries for each of ", s.batch, "x", s.cv, "x", s.height, "x", s.width,
+                " pixels");
+    TORCH_CHECK(!t->requires_grad() || !at::GradMode::is_enabled(), "distill_costs: the teacher's ", name, " have no gradient");
+  }
+  TORCH_CHECK(labels.scalar_type() == at::kByte, "distill_costs: labels must be uint8, got ", labels.scalar_type());
+  TORCH_CHECK(mpl_type(costs.scalar_type()) >= 0, "distill_costs: costs must be float32, float16 or bfloat16, got ",
+              costs.scalar_type());
+  TORCH_CHECK(labels.sizes() == costs.sizes(), "distill_costs: labels and costs must be of the same size");
+  if (rest) {
+    TORCH_CHECK(rest->device() == cost.device() && rest->scalar_type() == at::kFloat && rest->dim() == 4 && rest->size(0) == s.batch &&
+                    rest->size(1) == s.cv && rest->size(2) == s.height && rest->size(3) == s.width,
+                "distill_costs: rest must be a float32 (batch, cv, H, W) tensor on the device of cost");
+    TORCH_CHECK(!rest->requires_grad() || !at::GradMode::is_enabled(), "distill_costs: the teacher's rest has no gradient");
+  }
+  if (at::GradMode::is_enabled() && cost.requires_grad()) return Distill::apply(cost, labels, costs, rest, temperature, labels_first);
+  return distill_loss(cost.contiguous(), labels.contiguous(), costs.contiguous(), rest ? rest->contiguous() : at::Tensor(), temperature,
+                      labels_first);
+}
+
 // -------------------------------------------------------------------------------------------------- sampled labels
 // A parameter: a number, or a tensor of one per image (not looked at).
 template <typename T>
@@ -389,5 +524,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bucket_context", &bucket_context);
   m.def("labels_last_dropout", &labels_last_dropout);
   m.def("labels_last_norm", &labels_last_norm);
+  m.def("best_labels", [](const at::Tensor& cost, int64_t k, double temperature, bool labels_first, const py::object& dtype) {
+    TORCH_CHECK(THPDtype_Check(dtype.ptr()), "best_labels: dtype must be a torch.dtype");
+    return best_labels(cost, k, temperature, labels_first, reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type);
+  });
+  m.def("distill_costs", &distill_costs);
   m.def("sample_labels", &sample_labels);
 }

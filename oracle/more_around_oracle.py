@@ -42,7 +42,9 @@ def best_labels(cost, k, temperature):
   if order and order[0][0] == -math.inf:
     order = [(0.0, l) for c, l in order if c == -math.inf]
   elif order:
-    order = [(c - order[0][0], l) for c, l in order]
+    with np.errstate(over="ignore"):  # (the difference is one of fp32)
+      order = [(float(np.float32(c) - np.float32(order[0][0])), l) for c, l in order]
+    order = [(c, l) for c, l in order if c < math.inf]
   kept, others = order[:k], order[k:]
   labels = [l for _, l in kept] + [0] * (k - len(kept))
   return labels, [c for c, _ in kept] + [math.inf] * (k - len(kept)), softmin([c for c, _ in others], temperature)
@@ -50,7 +52,8 @@ def best_labels(cost, k, temperature):
 
 # ------------------------------------------------------------------------------------- the divergence from a teacher
 def distill(cost, labels, costs, rest, temperature):
-  """One pixel: the loss and its gradient with respect to the costs; rest None: no such class."""
+  """One pixel: the loss, its gradient with respect to the costs, and the sizes of what each of those is a difference of;
+  rest None: no such class."""
   n = len(cost)
   cost = [float(c) for c in cost]
   candidates = [l for l in range(n) if cost[l] != math.inf]
@@ -61,20 +64,23 @@ def distill(cost, labels, costs, rest, temperature):
   if rest is not None and rest != math.inf and left:
     classes.append((left, float(rest)))
   if not classes:
-    return 0.0, [0.0] * n
+    return 0.0, [0.0] * n, [0.0] * n
   if any(c != c or c == -math.inf for c in [cost[l] for l in candidates] + [c for _, c in classes]):
-    return math.nan, [0.0 if c == math.inf else math.nan for c in cost]
+    return math.nan, [0.0 if c == math.inf else math.nan for c in cost], [0.0] * n
   total, mass = softmin([cost[l] for l in candidates], temperature), softmin([c for _, c in classes], temperature)
-  loss, grad = [], [0.0] * n
+  loss, grad, size = [], [0.0] * n, [0.0] * n
   for l in candidates:
-    grad[l] -= math.exp(-(cost[l] - total) / temperature) / temperature
+    size[l] = math.exp(-(cost[l] - total) / temperature) / temperature
+    grad[l] -= size[l]
   for members, c in classes:
     p, own = math.exp(-(c - mass) / temperature), softmin([cost[l] for l in members], temperature)
     if p > 0:
       loss.append(p * ((mass - c) - (total - own)) / temperature)
     for l in members:
-      grad[l] += p * math.exp(-(cost[l] - own) / temperature) / temperature
-  return math.fsum(loss), grad
+      share = p * math.exp(-(cost[l] - own) / temperature) / temperature
+      grad[l] += share
+      size[l] += share
+  return math.fsum(loss), grad, size
 
 
 # ------------------------------------------------------------------------------------------------- verified labels

@@ -127,3 +127,74 @@ def test_a_cpu_layer_on_normalised_costs():
   x = torch.randn(1, 1, 9, 4, 5)
   normalised = torch.nn.functional.layer_norm(x.movedim(2, -1), (9,)).movedim(-1, 2)
   assert torch.allclose(modules[0](x)[0], modules[1](normalised)[0], rtol=1e-5, atol=1e-5)
+
+
+def test_distill_refusals(lib):
+  def best(dtype=0, cost=ONE, k=2, t=1.0, kept=0, labels=ONE, costs=ONE, batch=1, n=4, pixels=9):
+    return lib.mpl_best_labels(dtype, 1, cost, k, t, kept, labels, costs, None, batch, n, pixels, None)
+
+  def loss(dtype=0, cost=ONE, k=2, t=1.0, kept=0, labels=ONE, costs=ONE, batch=1, n=4, pixels=9, out=ONE):
+    return lib.mpl_distill_costs(dtype, 1, cost, kept, labels, costs, None, t, out, batch, n, k, pixels, None)
+
+  def grad(dtype=0, cost=ONE, k=2, t=1.0, kept=0, labels=ONE, costs=ONE, batch=1, n=4, pixels=9, dloss=ONE, out=ONE):
+    return lib.mpl_distill_costs_grad(dtype, 1, cost, kept, labels, costs, None, t, dloss, out, batch, n, k, pixels, None)
+
+  for call in (best, loss, grad):
+    for name in ("cost", "labels", "costs"):
+      _refused(lib, call(**{name: None}), b"null")
+    for wrong in (3, -1):
+      _refused(lib, call(dtype=wrong), b"type")
+      _refused(lib, call(kept=wrong), b"type")
+    for n in (0, 257):
+      _refused(lib, call(n=n), b"n_disp")
+    for t in (0.0, -1.0, math.inf, math.nan, 1e-45):
+      _refused(lib, call(t=t), b"temperature")
+    _refused(lib, call(k=0), b"list")
+    _refused(lib, call(k=257), b"list")
+    _refused(lib, call(batch=-1), b"negative")
+    _refused(lib, call(pixels=-1), b"negative")
+    _refused(lib, call(batch=1 << 20, pixels=1 << 30), b"too many")
+    _refused(lib, call(pixels=1 << 41), b"too many")
+    assert call(batch=0) == 0 and call(pixels=0) == 0
+  _refused(lib, best(k=5), b"list")
+  _refused(lib, loss(out=None), b"null")
+  _refused(lib, grad(out=None), b"null")
+  _refused(lib, grad(dloss=None), b"null")
+
+
+def test_best_labels_of_the_plain_form():
+  inf, nan = math.inf, math.nan
+  assert oracle.best_labels([3, 1, 1, nan, 2], 3, 1.0)[:2] == ([1, 2, 4], [0, 0, 1])
+  assert oracle.best_labels([3, 1, 1, nan, 2], 3, 1.0)[2] == 2
+  assert oracle.best_labels([inf, 1, nan], 2, 1.0) == ([1, 0], [0, inf], inf)
+  assert oracle.best_labels([5, -inf, 0, -inf], 1, 1.0) == ([1], [0.0], 0.0)
+  assert abs(oracle.best_labels([0, 2, 2, 2], 1, 0.5)[2] - (2 - 0.5 * math.log(3))) < 1e-12
+
+
+@pytest.mark.parametrize("with_rest", [True, False])
+def test_distill_of_the_plain_form(with_rest):
+  """Against autograd through the definition, in 64 bits."""
+  g = torch.Generator().manual_seed(2)
+  for _ in range(30):
+    n, k, t = 9, 3, 1.7
+    cost = torch.randn(n, dtype=torch.float64, generator=g).mul(2).requires_grad_(True)
+    labels = torch.randperm(n, generator=g)[:k]
+    costs, rest = torch.rand(k, dtype=torch.float64, generator=g) * 3, 2.0
+    log_q = torch.log_softmax(-cost / t, 0)
+    log_class, class_cost = log_q[labels], costs
+    if with_rest:
+      left = [l for l in range(n) if l not in labels.tolist()]
+      log_class = torch.cat([log_class, torch.logsumexp(log_q[left], 0)[None]])
+      class_cost = torch.cat([costs, torch.tensor([rest], dtype=torch.float64)])
+    log_p = torch.log_softmax(-class_cost / t, 0)
+    want = (log_p.exp() * (log_p - log_class)).sum()
+    (grad,) = torch.autograd.grad(want, cost)
+    loss, got, _ = oracle.distill(cost.tolist(), labels.tolist(), costs.tolist(), rest if with_rest else None, t)
+    assert abs(loss - float(want.detach())) <= 1e-12 and np.allclose(got, grad.numpy(), rtol=0, atol=1e-12)
+  inf, nan = math.inf, math.nan
+  # entries that are not there; a pixel without any; what is no number
+  assert oracle.distill([0, 1], [0, 1], [inf, inf], None, 1.0)[0] == 0
+  assert oracle.distill([0, inf], [1, 7], [0, 0], None, 1.0)[:2] == (0.0, [0.0, 0.0])
+  assert oracle.distill([0, 1], [0, 1], [0, 1], 5.0, 1.0)[0] == oracle.distill([0, 1], [0, 1], [0, 1], None, 1.0)[0]
+  loss, grad, _ = oracle.distill([0, nan, inf], [0], [0], None, 1.0)
+  assert math.isnan(loss) and math.isnan(grad[0]) and grad[2] == 0
