@@ -417,6 +417,21 @@ int mpl_sample_labels(int labels_first, const float* cost, const float* uniforms
                       int top_k, const float* top_ps, float top_p, const float* min_ps, float min_p, uint8_t* labels,
                       void* stream);
 
+/* Labels drafted from other costs (of fewer iterations, of the last frame), kept or drawn anew so that they are distributed as
+ * the layers' costs say, and are the drafted ones as often as that can be; no counterpart in the reference.  cost and
+ * draft_cost in the layout of mpl_sample_labels, draft_cost NULL for a draft that is certain of its labels; draft (n_drafts,
+ * batch, n_cv, pixels) uint8; uniforms (2, n_drafts, batch, n_cv, pixels) fp32 in [0, 1) -> labels and kept (0 or 1) of the
+ * draft's shape, uint8.  p and q are the distributions that mpl_sample_labels draws from without filters at temperature and
+ * draft_temperature (candidates and temperatures as there); without draft_cost q is 1 at the drafted label.  The label d stays
+ * where uniforms[0] * q[d] < p[d].  Where it does not, the label is drawn from max(p - q, 0) as there with uniforms[1]; from p
+ * where nothing is left of that, and where q[d] is 0 or d is not below n_disp, that is nothing was drafted: kept is 0 for
+ * these.  A pixel without candidates gets label 0, not kept.  Labels and kept are those of weights and sums in fp64, and do not
+ * depend on n_drafts.  temperatures, draft_temperatures: batch numbers each in DEVICE memory, one per image, or NULL for
+ * the number beside. */
+int mpl_verify_labels(int labels_first, const float* cost, const uint8_t* draft, const float* draft_cost, const float* uniforms,
+                      int batch, int n_cv, int n_disp, int64_t pixels, int n_drafts, const float* temperatures, float temperature,
+                      const float* draft_temperatures, float draft_temperature, uint8_t* labels, uint8_t* kept, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* mpl_last_error(void);
 

@@ -39,7 +39,7 @@ def _units():
            ("mp_sample", "mp_sample.hip", []),
            # (a network's costs may be NaN: what becomes of one is part of what these say)
            ("mp_norm", "mp_norm.hip", ["-fhonor-nans"]), ("mp_distill", "mp_distill.hip", ["-fhonor-nans"]),
-           ("mp_best", "mp_best.hip", [])]
+           ("mp_best", "mp_best.hip", []), ("mp_verify", "mp_verify.hip", [])]
   for r in (4, 3, 2, 1):  # (the largest units first)
     for t in (1, 0):
       units.append(("mp_fwd_r%d_t%d" % (r, t), "mp_fwd.hip",

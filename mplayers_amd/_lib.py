@@ -14,7 +14,7 @@ SYMBOLS = ("mpl_trwp_forward", "mpl_trwp_backward", "mpl_isgmr_forward", "mpl_is
            "mpl_stereo_data_cost", "mpl_gradient_cues", "mpl_mrf_energy", "mpl_transpose",
            "mpl_dropout_labels_last", "mpl_dropout_labels_first", "mpl_bucket_context", "mpl_bucket_sums",
            "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace",
-           "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad")
+           "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_verify_labels")
 
 KERNEL_KINDS = ("fwd_sweep", "bwd_sweep", "belief", "aggregate", "label", "combine", "other",
                 "fwd_sweep_all", "bwd_sweep_all", "unary_all")
@@ -88,6 +88,7 @@ def load():
   lib.mpl_best_labels.argtypes = [ci, ci, vp, ci, cf, ci, vp, vp, vp, ci, ci, i64, vp]
   lib.mpl_distill_costs.argtypes = [ci, ci, vp, ci, vp, vp, vp, cf, vp, ci, ci, ci, i64, vp]
   lib.mpl_distill_costs_grad.argtypes = [ci, ci, vp, ci, vp, vp, vp, cf, vp, vp, ci, ci, ci, i64, vp]
+  lib.mpl_verify_labels.argtypes = [ci, vp, vp, vp, vp, ci, ci, ci, i64, ci, vp, cf, vp, cf, vp, vp, vp]
   lib.mpl_n_chains.argtypes = [ci, ci, ci]
   lib.mpl_dcontext_copies.argtypes = [sp, ci]
   lib.mpl_table_is_dense.argtypes = [vp, ci]
@@ -177,6 +178,6 @@ def autograd():
     module.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
                  ("mpl_bucket_context", "mpl_bucket_sums", "mpl_dropout_labels_last", "mpl_dropout_labels_first",
                   "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace",
-                  "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_last_error")])
+                  "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_verify_labels", "mpl_last_error")])
     _autograd = module
   return _autograd

@@ -34,6 +34,7 @@ struct EntryPoints {
   decltype(&mpl_best_labels) best_labels;
   decltype(&mpl_distill_costs) distill_costs;
   decltype(&mpl_distill_costs_grad) distill_costs_grad;
+  decltype(&mpl_verify_labels) verify_labels;
   decltype(&mpl_last_error) last_error;
 } lib;
 
@@ -54,6 +55,7 @@ void bind(const std::vector<uintptr_t>& at) {
   take(lib.best_labels);
   take(lib.distill_costs);
   take(lib.distill_costs_grad);
+  take(lib.verify_labels);
   take(lib.last_error);
   TORCH_CHECK(next == at.size(), "bind: ", at.size(), " entry points are too many");
 }
@@ -469,20 +471,20 @@ struct Parameter {
   const T* each = nullptr;
   T all = 0;
 
+  // name: with the call's, as errors give it
   Parameter(const char* name, const py::object& value, int64_t batch, const at::Tensor& cost, at::ScalarType type, double high) {
     if (THPVariable_Check(value.ptr())) {
       const at::Tensor& t = THPVariable_Unpack(value.ptr());
-      TORCH_CHECK(t.device() == cost.device(), "sample_labels: ", name, " must be on the device of the costs");
-      TORCH_CHECK(t.scalar_type() == type && t.dim() == 1 && t.size(0) == batch && t.is_contiguous(), "sample_labels: ", name,
+      TORCH_CHECK(t.device() == cost.device(), name, " must be on the device of the costs");
+      TORCH_CHECK(t.scalar_type() == type && t.dim() == 1 && t.size(0) == batch && t.is_contiguous(), name,
                   " must be a number or a contiguous ", type, " tensor of one per image (", batch, ")");
       each = t.data_ptr<T>();
       return;
     }
-    TORCH_CHECK(type != at::kInt || (PyIndex_Check(value.ptr()) && !PyBool_Check(value.ptr())), "sample_labels: ", name,
-                " must be a whole number");
+    TORCH_CHECK(type != at::kInt || (PyIndex_Check(value.ptr()) && !PyBool_Check(value.ptr())), name, " must be a whole number");
     const double number = PyFloat_AsDouble(value.ptr());
     if (PyErr_Occurred()) throw py::error_already_set();
-    TORCH_CHECK(number >= 0 && number <= high, "sample_labels: ", name, " must be in [0, ", high, "], got ", number);
+    TORCH_CHECK(number >= 0 && number <= high, name, " must be in [0, ", high, "], got ", number);
     all = (T)number;
   }
 };
@@ -505,9 +507,9 @@ at::Tensor sample_labels(const at::Tensor& cost, const at::Tensor& uniforms, con
                   uniforms.size(at + 2) == height && uniforms.size(at + 3) == width,
               "sample_labels: uniforms must be ([n,] ", batch, ", ", cv, ", ", height, ", ", width, ")");
   const double inf = std::numeric_limits<double>::infinity();
-  const Parameter<float> t("temperature", temperature, batch, cost, at::kFloat, inf);
-  const Parameter<int32_t> k("top_k", top_k, batch, cost, at::kInt, 2147483647.0);
-  const Parameter<float> p("top_p", top_p, batch, cost, at::kFloat, 1), m("min_p", min_p, batch, cost, at::kFloat, 1);
+  const Parameter<float> t("sample_labels: temperature", temperature, batch, cost, at::kFloat, inf);
+  const Parameter<int32_t> k("sample_labels: top_k", top_k, batch, cost, at::kInt, 2147483647.0);
+  const Parameter<float> p("sample_labels: top_p", top_p, batch, cost, at::kFloat, 1), m("sample_labels: min_p", min_p, batch, cost, at::kFloat, 1);
   at::Tensor labels = at::empty(uniforms.sizes(), uniforms.options().dtype(at::kByte));
   const c10::DeviceGuard guard(cost.device());
   check(lib.sample_labels(labels_first, cost.data_ptr<float>(), uniforms.data_ptr<float>(), small(batch), small(cv), small(n),
@@ -515,6 +517,43 @@ at::Tensor sample_labels(const at::Tensor& cost, const at::Tensor& uniforms, con
                           m.each, m.all, labels.data_ptr<uint8_t>(), stream_of(cost)),
         "sample_labels");
   return labels;
+}
+
+// ------------------------------------------------------------------------------------------------- verified labels
+std::pair<at::Tensor, at::Tensor> verify_labels(const at::Tensor& cost, const at::Tensor& draft, const at::Tensor& uniforms,
+                                                const std::optional<at::Tensor>& draft_cost, const py::object& temperature,
+                                                const py::object& draft_temperature, bool labels_first) {
+  const std::tuple<const char*, const at::Tensor*, at::ScalarType> all[] = {
+      {"cost", &cost, at::kFloat}, {"draft", &draft, at::kByte}, {"uniforms", &uniforms, at::kFloat},
+      {"draft_cost", draft_cost ? &*draft_cost : nullptr, at::kFloat}};
+  for (const auto& [name, t, type] : all) {
+    if (t == nullptr) continue;
+    TORCH_CHECK(t->is_cuda(), "verify_labels: ", name, " must be a GPU tensor");
+    TORCH_CHECK(t->scalar_type() == type, "verify_labels: ", name, " must be ", type, ", got ", t->scalar_type());
+    TORCH_CHECK(t->is_contiguous(), "verify_labels: ", name, " must be contiguous");
+    TORCH_CHECK(t->device() == cost.device(), "verify_labels: ", name, " must be on the device of the costs");
+  }
+  TORCH_CHECK(cost.dim() == 5, "verify_labels: cost must be (batch, cv, labels, H, W) or (batch, cv, H, W, labels)");
+  TORCH_CHECK(!draft_cost || draft_cost->sizes() == cost.sizes(), "verify_labels: draft_cost must be of the size of cost");
+  const Layout s(cost, labels_first);
+  const int64_t at = draft.dim() - 4;
+  TORCH_CHECK((at == 0 || at == 1) && draft.size(at) == s.batch && draft.size(at + 1) == s.cv && draft.size(at + 2) == s.height &&
+                  draft.size(at + 3) == s.width,
+              "verify_labels: draft must be ([n,] ", s.batch, ", ", s.cv, ", ", s.height, ", ", s.width, ")");
+  TORCH_CHECK(uniforms.dim() == draft.dim() + 1 && uniforms.size(0) == 2 && uniforms.sizes().slice(1) == draft.sizes(),
+              "verify_labels: uniforms must be two for each drafted label, (2, ...) of draft's size");
+  const double inf = std::numeric_limits<double>::infinity();
+  const Parameter<float> t("verify_labels: temperature", temperature, s.batch, cost, at::kFloat, inf),
+      dt("verify_labels: draft_temperature", draft_temperature.is_none() ? temperature : draft_temperature, s.batch, cost, at::kFloat,
+         inf);
+  at::Tensor labels = at::empty(draft.sizes(), draft.options()), kept = at::empty(draft.sizes(), draft.options().dtype(at::kBool));
+  const c10::DeviceGuard guard(cost.device());
+  check(lib.verify_labels(labels_first, cost.data_ptr<float>(), draft.data_ptr<uint8_t>(),
+                          draft_cost ? draft_cost->data_ptr<float>() : nullptr, uniforms.data_ptr<float>(), small(s.batch), small(s.cv),
+                          small(s.n), s.pixels(), at == 1 ? small(draft.size(0)) : 1, t.each, t.all, dt.each, dt.all,
+                          labels.data_ptr<uint8_t>(), reinterpret_cast<uint8_t*>(kept.data_ptr<bool>()), stream_of(cost)),
+        "verify_labels");
+  return {labels, kept};
 }
 
 }  // namespace
@@ -530,4 +569,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("distill_costs", &distill_costs);
   m.def("sample_labels", &sample_labels);
+  m.def("verify_labels", &verify_labels);
 }

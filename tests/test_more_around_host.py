@@ -198,3 +198,45 @@ def test_distill_of_the_plain_form(with_rest):
   assert oracle.distill([0, 1], [0, 1], [0, 1], 5.0, 1.0)[0] == oracle.distill([0, 1], [0, 1], [0, 1], None, 1.0)[0]
   loss, grad, _ = oracle.distill([0, nan, inf], [0], [0], None, 1.0)
   assert math.isnan(loss) and math.isnan(grad[0]) and grad[2] == 0
+
+
+def test_verify_refusals(lib):
+  def call(cost=ONE, draft=ONE, uniforms=ONE, batch=1, n_cv=1, n=4, pixels=9, drafts=1, labels=ONE, kept=ONE):
+    return lib.mpl_verify_labels(1, cost, draft, None, uniforms, batch, n_cv, n, pixels, drafts, None, 1.0, None, 1.0, labels, kept,
+                                 None)
+
+  for name in ("cost", "draft", "uniforms", "labels", "kept"):
+    _refused(lib, call(**{name: None}), b"null")
+  for n in (0, 257):
+    _refused(lib, call(n=n), b"n_disp")
+  for name in ("batch", "n_cv", "pixels", "drafts"):
+    _refused(lib, call(**{name: -1}), b"negative")
+    assert call(**{name: 0}) == 0
+  _refused(lib, call(batch=1 << 20, pixels=1 << 30), b"too many")
+  _refused(lib, call(n=200, pixels=1 << 30), b"too many")
+
+
+def test_verified_labels_of_the_plain_form():
+  inf = math.inf
+  verify = oracle.verify_label
+  log = [0.0, math.log(2), math.log(4), inf]  # p: 4/7, 2/7, 1/7
+  assert verify(log, 1, 0.28, 0.5) == (1, True) and verify(log, 1, 0.29, 0.79) == (0, False)
+  assert verify(log, 1, 0.29, 0.81) == (2, False) and verify(log, 3, 0.0, 0.9) == (2, False)
+  # nothing drafted: from p
+  assert [verify(log, 9, 0.0, u)[0] for u in (0.5, 0.6, 0.9, 1.0)] == [0, 1, 2, 2]
+  assert verify(log, 1, 0.0, 0.6, [0, inf, 0, 0]) == (1, False)
+  # q 1/2 each of labels 1 and 2: what is left is label 0 alone
+  assert verify(log, 1, 0.57, 0.99, [inf, 0, 0, inf]) == (1, True) and verify(log, 1, 0.58, 0.99, [inf, 0, 0, inf]) == (0, False)
+  assert verify([inf, inf], 1, 0.0, 0.5) == (0, False) and verify([1, 0], 0, 0.5, 0.5, temperature=0.0) == (1, False)
+  assert verify([0, 1], 0, 0.999, 0.5, [0, 1]) == (0, True)
+
+
+def test_python_entry_points_refuse_cpu_tensors():
+  from mplayers_amd import best_labels, distill_costs, verify_labels
+  cost = torch.zeros(1, 1, 4, 2, 2)
+  with pytest.raises(RuntimeError, match="GPU"):
+    best_labels(cost, 2)
+  with pytest.raises(RuntimeError, match="GPU"):
+    distill_costs(cost, torch.zeros(1, 1, 2, 2, 2, dtype=torch.uint8), torch.zeros(1, 1, 2, 2, 2))
+  with pytest.raises(RuntimeError, match="GPU"):
+    verify_labels(cost, torch.zeros(1, 1, 2, 2, dtype=torch.uint8), torch.zeros(2, 1, 1, 2, 2))
