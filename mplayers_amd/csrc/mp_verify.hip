@@ -13,6 +13,7 @@ using namespace mpl;
 namespace {
 
 struct Verify {
+  LaneTiles t;
   const float* cost;
   const float* draft_cost;  // or nullptr
   const uint8_t* draft;
@@ -22,8 +23,9 @@ struct Verify {
   const float* temperature;  // one per image, or nullptr for the number below
   const float* draft_temperature;
   float temperature_all, draft_temperature_all;
-  int64_t pixels, items_pixels;
-  int n, n_cv, n_drafts, labels_first;
+  int64_t items_pixels;
+  int n_cv, n_drafts;
+  int quads;  // both volumes in whole and aligned quads, labels last
 };
 
 __device__ __forceinline__ double inverse(float temperature) { return positive(temperature) ? 1.0 / (double)temperature : 0.0; }
@@ -102,7 +104,7 @@ __device__ void verify_exactly(const Verify& p, int image, int64_t at, Cost cost
   float v[4];
   double a[4], b[4] = {}, left[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < p.n ? candidate(cost(4 * lane + j)) : kInf;
+  for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < p.t.n ? candidate(cost(4 * lane + j)) : kInf;
   weights64(v, p.temperature != nullptr ? p.temperature[image] : p.temperature_all, a);
   const double total = total64(a), total_or_1 = total > 0 ? total : 1.0;
 #pragma unroll
@@ -111,7 +113,7 @@ __device__ void verify_exactly(const Verify& p, int image, int64_t at, Cost cost
   Running rest = all;
   if (COSTS) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < p.n ? candidate(draft_cost(4 * lane + j)) : kInf;
+    for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < p.t.n ? candidate(draft_cost(4 * lane + j)) : kInf;
     weights64(v, p.draft_temperature != nullptr ? p.draft_temperature[image] : p.draft_temperature_all, b);
     const double of_draft = total64(b), of_draft_or_1 = of_draft > 0 ? of_draft : 1.0;
 #pragma unroll
@@ -126,7 +128,7 @@ __device__ void verify_exactly(const Verify& p, int image, int64_t at, Cost cost
     const int64_t place = k * p.items_pixels + at;
     const int d = uniform_i(p.draft[place]);
     const float u0 = uniform_f(p.uniforms[place]), u1 = uniform_f(p.uniforms[drafts + place]);
-    const bool exists = d < p.n;
+    const bool exists = d < p.t.n;
     const double p_d = of_label(a, exists ? d : 0), q_d = !exists ? 0.0 : COSTS ? of_label(b, d) : 1.0;
     const bool stays = total > 0 && exists && q_d > 0 && (positive(u0) ? (double)u0 : 0.0) * q_d < p_d;
     int label = d;
@@ -146,15 +148,251 @@ __device__ void verify_exactly(const Verify& p, int image, int64_t at, Cost cost
   }
 }
 
-template <bool COSTS>
-__global__ void __launch_bounds__(256) verify_kernel(Verify p) {
-  for (int64_t at = (int64_t)blockIdx.x * 4 + uniform_i((int)threadIdx.x / 64); at < p.items_pixels; at += (int64_t)gridDim.x * 4) {
-    const int64_t item = at / p.pixels, pixel = at - item * p.pixels;
-    const int64_t first = item * p.n * p.pixels + (p.labels_first ? pixel : pixel * p.n), step = p.labels_first ? p.pixels : 1;
-    verify_exactly<COSTS>(
-        p, (int)(item / p.n_cv), at, [&](int l) { return p.cost[first + l * step]; },
-        [&](int l) { return p.draft_cost[first + l * step]; });
+// A temperature as 32 bits use it.
+struct Scale {
+  float to_exponent;  // log2(e) / T
+  bool cold, far;     // T not above 0; beyond what fp32 exponents are sure of (an infinite one too)
+};
+__device__ __forceinline__ Scale scale_of(const float* each, float all, int image) {
+  const float t = each != nullptr ? each[image] : all;
+  Scale s;
+  s.cold = !positive(t);
+  s.far = !s.cold && !(t > 1e-30f && t < 1e30f);
+  s.to_exponent = s.cold ? 0.f : (float)(inverse(t) * 1.4426950408889634);
+  return s;
+}
+
+// The weights of a pixel's labels in its S lanes, in place of the costs.
+struct Weights {
+  float best, total;  // the least cost, +inf where there is no candidate
+  int first;          // cold: the first label that has it, the only one that weighs
+};
+template <int NV, int S>
+__device__ __forceinline__ Weights weights32(float (&v)[NV], const Scale& scale, int s) {
+  Weights w = {v[0], 0.f, S * NV};
+#pragma unroll
+  for (int j = 1; j < NV; ++j) w.best = v[j] < w.best ? v[j] : w.best;
+  w.best = lanes_min<S>(w.best);
+  if (scale.cold) {
+#pragma unroll
+    for (int j = NV - 1; j >= 0; --j) w.first = v[j] == w.best && w.best < kInf ? s * NV + j : w.first;
+    w.first = lanes_min<S>(w.first);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = s * NV + j == w.first ? 1.f : 0.f;
+    w.total = 1.f;
+    return w;
   }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    v[j] = v[j] < kInf ? __builtin_amdgcn_exp2f((w.best - v[j]) * scale.to_exponent) : 0.f;
+    w.total += v[j];
+  }
+  w.total = lanes_sum<S>(w.total);
+  return w;
+}
+
+// S lanes per pixel, NV labels per lane.  p and q are formed in 32 bits, with a bound on how far they may be off, all relative to
+// a sum of 1 and u = 2^-24:
+//   weights   3 roundings of an exponent a (3 u a w, and sum(a w) <= ln(n) sum(w): the entropy of n labels) and an ulp of the
+//             exponential: (2 + 3 ln 256) u < 19 u of their sum
+//   p         those, the sum's own additions, (NV + S) u, its weights again, a reciprocal and a product: (40 + NV + S) u over
+//             all labels
+//   a running sum of max(p - q, 0): both of these, a rounding each, its own additions: (81 + 3 (NV + S)) u
+// and as much for a target, which is a product with such a sum.  Where a target is as close to a sum as both (kNear), 32 bits
+// do not tell, and verify_exactly() takes the pixel.  So it does where u0 q[d] is as close to p[d] as (3 a + 45 + NV + S) u of
+// either, a being their exponents.
+template <int NV, int S, bool COSTS, bool LAST>
+__global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
+  using Tile = LaneTile<NV, S>;
+  constexpr float kU = 0x1p-24f, kNear = 2 * (82 + 3 * (NV + S)) * kU;
+  constexpr float kLeast = 1e-30f;  // below it fp32 is not what the bounds say
+  __shared__ __align__(16) float tile[kLanePixels * Tile::kStride];
+  __shared__ uint32_t left_over[2];  // pixels for verify_exactly()
+  const unsigned block = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.t.xcd_group), tiles = (unsigned)p.t.tiles;
+  const int64_t item = block / tiles, p0 = (int64_t)(block - (unsigned)item * tiles) * kLanePixels;
+  const int count = (int)min((int64_t)kLanePixels, p.t.pixels - p0), n = p.t.n;
+  const int tid = (int)threadIdx.x, px = tid / S, s = tid % S, of = min(px, count - 1);
+  const int64_t first = item * n * p.t.pixels, at = item * p.t.pixels + p0 + of, drafts = p.items_pixels * p.n_drafts;
+  const int64_t pixel = first + (LAST ? (p0 + of) * n : p0 + of), step = LAST ? 1 : p.t.pixels;
+  if (tid < 2) left_over[tid] = 0;
+  // A draft to a lane: its label and uniform numbers, and the costs of that label.
+  struct Drafted {
+    int64_t place;
+    int label;
+    float u0, u1, cost, draft_cost;
+  };
+  const auto fetch_label = [&](int k) {
+    Drafted d;
+    d.place = min(k, p.n_drafts - 1) * p.items_pixels + at;
+    d.label = p.draft[d.place];
+    d.u0 = p.uniforms[d.place];
+    d.u1 = p.uniforms[drafts + d.place];
+    return d;
+  };
+  const auto fetch_costs = [&](Drafted& d) {
+    const int64_t from = pixel + min(d.label, n - 1) * step;
+    d.cost = p.cost[from];
+    d.draft_cost = COSTS ? p.draft_cost[from] : 0.f;
+  };
+  Drafted d = fetch_label(s);
+  float a[NV], b[NV];
+  {
+    LaneLoads<NV, S, LAST, float> target, draft;
+    target.load(p.cost + first, p.t, p0, count, p.quads, tid);
+    if (COSTS) draft.load(p.draft_cost + first, p.t, p0, count, p.quads, tid);
+    fetch_costs(d);
+    target.to_tile(tile, p.t, count, p.quads, tid);
+    __syncthreads();
+    lane_costs<NV, S>(tile, px, s, n, a);
+    if (COSTS) {
+      __syncthreads();
+      draft.to_tile(tile, p.t, count, p.quads, tid);
+      __syncthreads();
+      lane_costs<NV, S>(tile, px, s, n, b);
+    }
+  }
+  const int image = (int)((unsigned)item / (unsigned)p.n_cv);
+  const Scale scale = scale_of(p.temperature, p.temperature_all, image),
+              draft_scale = COSTS ? scale_of(p.draft_temperature, p.draft_temperature_all, image) : scale;
+  const Weights wa = weights32<NV, S>(a, scale, s), wb = COSTS ? weights32<NV, S>(b, draft_scale, s) : wa;
+  const bool empty = wa.best == kInf;
+  bool unsure = !(wa.best > -kInf) || scale.far || (COSTS && wb.best < kInf && (!(wb.best > -kInf) || draft_scale.far));
+  const float per_a = empty ? 0.f : 1.f / wa.total, per_b = COSTS && wb.best < kInf ? 1.f / wb.total : 0.f;
+  // running sums: of p, and of what the draft leaves
+  float sum_a = 0, sum_b = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const float of_target = a[j] * per_a;
+    sum_a += of_target;
+    a[j] = sum_a;
+    if (COSTS) {
+      const float rest = of_target - b[j] * per_b;
+      sum_b += rest > 0 ? rest : 0.f;
+      b[j] = sum_b;
+    }
+  }
+  const float before_a = lanes_before<S>(sum_a, s), before_b = COSTS ? lanes_before<S>(sum_b, s) : 0.f;
+  const float all_a = lanes_max<S>(before_a + sum_a), all_b = COSTS ? lanes_max<S>(before_b + sum_b) : 0.f;
+
+  // The sums to LDS: the lanes of a pixel are of one wavefront, and nobody else reads its place any more.
+  float* const sums = &tile[px * Tile::kStride];
+  const auto to_lds = [&](const float (&x)[NV], float before) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < NV; j += 4)
+      *reinterpret_cast<float4*>(sums + s * NV + j) = float4{before + x[j], before + x[j + 1], before + x[j + 2], before + x[j + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  // The first label whose sum is above the target, by halving; `taken` of the sums from label `from` on does not count.
+  const int top = 1 << (31 - __builtin_clz(n));
+  const auto find = [&](float target, int from, float taken, bool& near) {
+    int label = 0;
+    float least = -kInf;  // the last sum that is not above the target
+    for (int step = top; step > 0; step >>= 1) {
+      const int to = label + step;
+      const float sum = sums[min(to, n) - 1] - (to > from ? taken : 0.f);
+      if (to <= n && sum <= target) {
+        label = to;
+        least = sum;
+      }
+    }
+    const float most = sums[min(label, n - 1)] - (label >= from ? taken : 0.f);
+    near = !(least <= target - kNear && most > target + kNear) || label >= n;
+    return label;
+  };
+  if (COSTS)
+    to_lds(b, before_b);
+  else
+    to_lds(a, before_a);
+  for (int base = 0; base < p.n_drafts; base += S) {
+    if (base > 0) {
+      d = fetch_label(base + s);
+      fetch_costs(d);
+    }
+    const bool mine = base + s < p.n_drafts && px < count;
+    const bool exists = d.label < n;
+    const float c = candidate(d.cost), dc = candidate(d.draft_cost);
+    const bool has_p = exists && (scale.cold ? d.label == wa.first : c < kInf);
+    const bool has_q = exists && (!COSTS || (draft_scale.cold ? d.label == wb.first : dc < kInf));
+    const float far_a = scale.cold || !has_p ? 0.f : (wa.best - c) * scale.to_exponent;
+    const float far_b = !COSTS || draft_scale.cold || !has_q ? 0.f : (wb.best - dc) * draft_scale.to_exponent;
+    const float p_d = has_p ? __builtin_amdgcn_exp2f(far_a) * per_a : 0.f;
+    const float q_d = !has_q ? 0.f : COSTS ? __builtin_amdgcn_exp2f(far_b) * per_b : 1.f;
+    const float u0 = positive(d.u0) ? (d.u0 < 1.f ? d.u0 : 1.f) : 0.f, u1 = positive(d.u1) ? (d.u1 < 2.f ? d.u1 : 2.f) : 0.f;
+    const float least = u0 * q_d, off = (48 + NV + S - 3 * (far_a < far_b ? far_a : far_b)) * kU;
+    const bool kept = has_q && least < p_d;
+    bool near = has_q && (q_d < kLeast || fabsf(least - p_d) <= off * (least + p_d) + kLeast || (positive(d.u0) && d.u0 > 1.f));
+    int label = d.label;
+    // what the draft leaves, or all of p
+    const bool draws = mine && !empty && !kept && !near;
+    const bool draws_left = draws && (has_q || !COSTS), draws_all = draws && !has_q && COSTS;
+    if (__builtin_amdgcn_ballot_w64(draws_left) != 0) {
+      const float taken = !COSTS && exists ? p_d : 0.f, all = COSTS ? all_b : all_a - taken;
+      bool close;
+      const int drawn = find(u1 * all, d.label, taken, close);
+      label = draws_left ? drawn : label;
+      near |= draws_left && close;
+    }
+    if (COSTS && __builtin_amdgcn_ballot_w64(draws_all) != 0) {
+      to_lds(a, before_a);
+      bool close;
+      const int drawn = find(u1 * all_a, 0, 0.f, close);
+      label = draws_all ? drawn : label;
+      near |= draws_all && close;
+      to_lds(b, before_b);
+    }
+    unsure |= near && mine;
+    if (mine && (empty || !unsure)) {
+      p.labels[d.place] = (uint8_t)(empty ? 0 : label);
+      p.kept[d.place] = kept && !empty ? 1 : 0;
+    }
+  }
+  unsure = lanes_max<S>(unsure ? 1 : 0) != 0 && !empty && px < count;
+  const auto exactly = [&](int of) {
+    const int64_t from = first + (LAST ? (p0 + of) * n : p0 + of);
+    verify_exactly<COSTS>(
+        p, image, item * p.t.pixels + p0 + of, [&](int l) { return p.cost[from + l * step]; },
+        [&](int l) { return p.draft_cost[from + l * step]; });
+  };
+  if (S == 1) {
+    // (one wavefront)
+    for (uint64_t rest = __builtin_amdgcn_ballot_w64(unsure); rest != 0; rest &= rest - 1) exactly(__builtin_ctzll(rest));
+  } else {
+    if (unsure && s == 0) atomicOr(&left_over[px >> 5], 1u << (px & 31));
+    __syncthreads();
+    int turn = 0;
+    for (uint64_t rest = (uint64_t)left_over[1] << 32 | left_over[0]; rest != 0; rest &= rest - 1)
+      if (turn++ % S == uniform_i(tid / 64)) exactly(__builtin_ctzll(rest));
+  }
+}
+
+template <bool COSTS, bool LAST>
+void launch(const Verify& p, unsigned blocks, hipStream_t st) {
+  const int n = p.t.n;
+  if (n <= 4)
+    verify_kernel<4, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 8)
+    verify_kernel<8, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 16)
+    verify_kernel<8, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 24)
+    verify_kernel<12, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 32)
+    verify_kernel<16, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 48)
+    verify_kernel<12, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 64)
+    verify_kernel<16, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 96)
+    verify_kernel<24, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 128)
+    verify_kernel<32, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 192)
+    verify_kernel<24, 8, COSTS, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
+  else
+    verify_kernel<32, 8, COSTS, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
 }
 
 }  // namespace
@@ -169,9 +407,8 @@ extern "C" int mpl_verify_labels(int labels_first, const float* cost, const uint
   if (batch == 0 || n_cv == 0 || pixels == 0 || n_drafts == 0) return MPL_OK;
   if (cost == nullptr || draft == nullptr || uniforms == nullptr || labels == nullptr || kept == nullptr)
     return fail(MPL_EINVAL, "verify_labels: null pointer");
-  LaneTiles t;
-  if (!make_lane_tiles(t, (int64_t)batch * n_cv, n_disp, pixels)) return fail(MPL_EINVAL, "verify_labels: too many pixels");
   Verify p;
+  if (!make_lane_tiles(p.t, (int64_t)batch * n_cv, n_disp, pixels)) return fail(MPL_EINVAL, "verify_labels: too many pixels");
   p.cost = cost;
   p.draft_cost = draft_cost;
   p.draft = draft;
@@ -182,17 +419,18 @@ extern "C" int mpl_verify_labels(int labels_first, const float* cost, const uint
   p.draft_temperature = draft_temperatures;
   p.temperature_all = temperature;
   p.draft_temperature_all = draft_temperature;
-  p.pixels = pixels;
   p.items_pixels = (int64_t)batch * n_cv * pixels;
-  p.n = n_disp;
   p.n_cv = n_cv;
   p.n_drafts = n_drafts;
-  p.labels_first = labels_first != 0;
-  const unsigned blocks = (unsigned)(p.items_pixels < (4 << 16) ? (p.items_pixels + 3) / 4 : 1 << 16);
+  p.quads = n_disp % 4 == 0 && (((uintptr_t)cost | (uintptr_t)draft_cost) & 15) == 0;
+  // (tiles that share cache lines: see mpl_sample_labels)
+  p.t.xcd_group = labels_first && pixels * 4 % kLineBytes != 0 ? 16 : 0;
+  const unsigned blocks = (unsigned)(p.t.tiles * batch * n_cv);
+  const hipStream_t st = (hipStream_t)stream;
   if (draft_cost != nullptr)
-    verify_kernel<true><<<blocks, 256, 0, (hipStream_t)stream>>>(p);
+    labels_first ? launch<true, false>(p, blocks, st) : launch<true, true>(p, blocks, st);
   else
-    verify_kernel<false><<<blocks, 256, 0, (hipStream_t)stream>>>(p);
+    labels_first ? launch<false, false>(p, blocks, st) : launch<false, true>(p, blocks, st);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "verify_labels: %s", hipGetErrorString(e));
 }
