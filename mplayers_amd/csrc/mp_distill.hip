@@ -13,9 +13,10 @@
 // An entry is there where its cost is not +inf, its label exists and the student's cost of that label is not +inf; the rest
 // where its cost is not +inf and a label is left.  NaN (and -inf) goes through to the loss and the gradients of its pixel.
 //
-// A tile of 64 pixels, a lane to each (mp_pixels.h); the costs lie in LDS too, where the entries find the student's cost of
-// their label.  Every wavefront of a tile goes through the whole list: W times as many instructions as one alone, but no
-// further meeting.  Bound by HBM.
+// A tile of 64 pixels, a lane to each (mp_pixels.h).  The costs lie in LDS too, where the entries find the student's cost of
+// their label; the wavefronts of a tile share the list, and each has weights of its own labels that serve the student's sum, the
+// others' and the gradient, so there is one exponential to a label.
+// Bound by HBM.
 
 #include "mp_pixels.h"
 
@@ -39,20 +40,20 @@ struct Distill {
   int quads;                 // whole and aligned quads in the operators' layout
 };
 
-__device__ __forceinline__ float kept_cost(const Distill& p, int64_t at) {
-  return p.kept == MPL_F32   ? ((const float*)p.costs)[at]
-         : p.kept == MPL_F16 ? (float)((const _Float16*)p.costs)[at]
-                             : (float)((const __bf16*)p.costs)[at];
+__device__ __forceinline__ float kept_cost(const Distill& p, int64_t base, unsigned of) {
+  return p.kept == MPL_F32   ? ((const float*)p.costs + base)[of]
+         : p.kept == MPL_F16 ? (float)((const _Float16*)p.costs + base)[of]
+                             : (float)((const __bf16*)p.costs + base)[of];
 }
 
-// The least of some costs and the sum of their weights relative to it, (+inf, 0) of none.
+// A cost not above any of some costs, and the sum of their weights relative to it; (+inf, 0) of none.
 struct Mass {
   float least, sum;
 };
 __device__ __forceinline__ float weight(float least, float c, float to_exponent) {
   return c == kInf ? 0.f : __builtin_amdgcn_exp2f((least - c) * to_exponent);
 }
-// Those of the W wavefronts of a tile; part: two floats for each and lane.
+// Those of the W wavefronts of a tile.
 template <int W>
 __device__ __forceinline__ Mass join(Mass own, float2 (*part)[kTilePixels], int w, int lane, float to_exponent) {
   if (W == 1) return own;
@@ -70,11 +71,16 @@ __device__ __forceinline__ Mass join(Mass own, float2 (*part)[kTilePixels], int 
   return all;
 }
 
+constexpr float kFaint = 0x1p-60f;  // others that weigh less than this beside the best label: see distill_kernel
+
 template <typename T, bool FIRST, bool GRAD, int W, int I, int G>
 __global__ void __launch_bounds__(64 * W * G) distill_kernel(Distill p) {
-  constexpr int kStride = tile_stride(W * I), kShift = W == 1 ? 0 : W == 2 ? 1 : W == 4 ? 2 : 3;
+  constexpr int kStride = tile_stride(W * I), kShift = W == 1 ? 0 : W == 2 ? 1 : W == 4 ? 2 : 3, kParts = W > 1 ? W : 1;
   __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
-  __shared__ float2 part[2][W > 1 ? W : 1][kTilePixels];
+  __shared__ float2 part[2][kParts][kTilePixels];
+  __shared__ float part_far[kParts][kTilePixels];
+  __shared__ uint32_t named_by[kParts][kTilePixels];  // of each wavefront's labels, those that the list names
+  __shared__ uint32_t twice;                          // whether a list of the tile names one twice
   const int tid = (int)threadIdx.x % (64 * W), group = uniform_i((int)threadIdx.x / (64 * W));
   const int lane = tid % 64, w = uniform_i(tid / 64), n = p.t.labels;
   const unsigned at = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.t.xcd_group) * G + group;
@@ -85,10 +91,25 @@ __global__ void __launch_bounds__(64 * W * G) distill_kernel(Distill p) {
   const unsigned total = (unsigned)(count * n);
   const int of = min(lane, count - 1);
   const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n, pixel = (int64_t)item * p.t.pixels + p0 + of;
-  // of entry e of the lane's list
-  const int64_t entry = FIRST ? (int64_t)item * p.k * p.t.pixels + p0 + of : pixel * p.k, step = FIRST ? p.t.pixels : 1;
   float* const tile = tiles + group * kTilePixels * kStride;
   float* const mine = tile + lane * kStride;
+
+  // Entry e of the lane's list.  This wavefront has the entries w, w + W, ..., of which the first stays in registers.
+  struct Entry {
+    int label;
+    float cost;
+  };
+  const auto fetch = [&](int e) {
+    const int64_t base = FIRST ? ((int64_t)item * p.k + e) * p.t.pixels + p0 : ((int64_t)item * p.t.pixels + p0) * p.k + e;
+    const unsigned at = (unsigned)(FIRST ? of : of * p.k);
+    return Entry{p.labels[base + at], kept_cost(p, base, at)};
+  };
+  const Entry front = fetch(min(w, p.k - 1));
+  const auto entries = [&](auto f) {
+    if (w < p.k) f(front);
+    for (int e = w + W; e < p.k; e += W) f(fetch(e));
+  };
+
   float c[I][4];
   if (FIRST) {
     load_rows<W, I>((const T*)p.cost + first + p0, p.t, w, of, c);
@@ -100,88 +121,148 @@ __global__ void __launch_bounds__(64 * W * G) distill_kernel(Distill p) {
     tile_sync<W>();
     from_tile<W, I>(mine, w, c);
   }
-  // (labels behind the last are no candidates)
-  const auto mass_of = [&](auto leave_out) {
-    Mass m = {kInf, 0.f};
-#pragma unroll
-    for (int i = 0; i < I; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) m.least = c[i][j] < m.least && !leave_out(i, j) ? c[i][j] : m.least;
-#pragma unroll
-    for (int i = 0; i < I; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) m.sum += leave_out(i, j) ? 0.f : weight(m.least, c[i][j], p.to_exponent);
-    return m;
-  };
+  // weights of this wavefront's labels beside the least cost of them; labels behind the last are no candidates
+  float a[I][4], least = kInf, sum = 0;
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[i][j] = 4 * (w + i * W) + j < n ? c[i][j] : kInf;
-  const Mass student = join<W>(mass_of([](int, int) { return false; }), part[0], w, lane, p.to_exponent);
-
-  // the list: its least cost, and which of this wavefront's labels it names
-  const auto exists = [&](int label, float t) { return t != kInf && label < n; };
-  const auto cost_at = [&](int label) { return mine[min(label, n - 1)]; };
-  const auto place = [&](int label) { return (label >> 2 >> kShift) * 4 + (label & 3); };
-  const auto is_mine = [&](int label) { return W == 1 || ((label >> 2) & (W - 1)) == w; };
-  float least = kInf;
-  uint32_t named = 0;
-  for (int e = 0; e < p.k; ++e) {
-    const int label = p.labels[entry + e * step];
-    const float t = kept_cost(p, entry + e * step);
-    const bool is = exists(label, t);
-    if (is && is_mine(label)) named |= 1u << place(label);
-    least = is && cost_at(label) != kInf && t < least ? t : least;
+    for (int j = 0; j < 4; ++j) {
+      c[i][j] = 4 * (w + i * W) + j < n ? c[i][j] : kInf;
+      least = c[i][j] < least ? c[i][j] : least;
+    }
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += a[i][j] = weight(least, c[i][j], p.to_exponent);
+  if (W > 1) {
+    named_by[w][lane] = 0;
+    if (tid == 0) twice = 0;
   }
+  const Mass student = join<W>(Mass{least, sum}, part[0], w, lane, p.to_exponent);
+
+  // the list: what this wavefront's entries weigh, and that times log p - log q but for the logarithms of sums
+  const auto cost_at = [&](int label) { return mine[min(label, n - 1)]; };
+  const auto exists = [&](const Entry& e) { return e.cost != kInf && e.label < n; };
+  const auto place = [&](int label) { return (label >> 2 >> kShift) * 4 + (label & 3); };
+  Mass list = {kInf, 0.f};
+  float far = 0;
+  uint32_t named = 0;
+  bool again = false;
+  entries([&](const Entry& e) {
+    if (!exists(e)) return;
+    const uint32_t bit = 1u << place(e.label);
+    if (W == 1) {
+      again |= (named & bit) != 0;
+      named |= bit;
+    } else {
+      again |= (atomicOr(&named_by[e.label >> 2 & (W - 1)][lane], bit) & bit) != 0;
+    }
+    list.least = cost_at(e.label) != kInf && e.cost < list.least ? e.cost : list.least;
+  });
+  entries([&](const Entry& e) {
+    const float own = cost_at(e.label);
+    const float x = exists(e) && own != kInf ? weight(list.least, e.cost, p.to_exponent) : 0.f;
+    list.sum += x;
+    if (!GRAD) far += x > 0 ? x * ((own - student.least) - (e.cost - list.least)) : 0.f;
+  });
+  if (W > 1) {
+    if (GRAD && again) twice = 1;
+    if (!GRAD) part_far[w][lane] = far;
+    list = join<W>(list, part[1], w, lane, p.to_exponent);
+    named = named_by[w][lane];
+    if (!GRAD) {
+      far = 0;
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const float2 of_wave = part[1][k][lane];
+        const float x = weight(list.least, of_wave.x, p.to_exponent);
+        far += x > 0 ? x * (part_far[k][lane] - of_wave.y * (of_wave.x - list.least)) : 0.f;
+      }
+    }
+  }
+  // the rest: the labels that the list does not name
   const auto is_named = [&](int i, int j) { return (named >> (4 * i + j) & 1) != 0; };
   Mass others = {kInf, 0.f};
   float rest = kInf;
   if (p.rest != nullptr) {
-    others = join<W>(mass_of(is_named), part[1], w, lane, p.to_exponent);
-    rest = others.sum == 0.f ? kInf : p.rest[pixel];
-    least = rest < least ? rest : least;
-  }
-  // the sum of the classes' weights, and of weight * (log p - log q) but for the logarithms of the sums
-  float sum = 0, far = 0;
-  for (int e = 0; e < p.k; ++e) {
-    const int label = p.labels[entry + e * step];
-    const float t = kept_cost(p, entry + e * step), own = cost_at(label);
-    const float a = exists(label, t) && own != kInf ? weight(least, t, p.to_exponent) : 0.f;
-    sum += a;
-    if (!GRAD) far += a > 0 ? a * ((own - student.least) - (t - least)) : 0.f;
-  }
-  const float rest_weight = weight(least, rest, p.to_exponent);
-  sum += rest_weight;
-  if (!GRAD) {
-    far *= p.inv_t;
-    if (rest_weight > 0)
-      far += rest_weight * (((others.least - student.least) - (rest - least)) * p.inv_t - logf(others.sum));
-    const float loss = far / sum + (logf(student.sum) - logf(sum));
-    if (w == 0 && lane < count) p.loss[pixel] = sum == 0.f ? 0.f : loss;
-  } else {
-    // p of the list's labels: each wavefront adds up its own, entry by entry
-    const float per_sum = 1.f / sum;
-    if (W > 1) tile_sync<W>();  // (the costs in LDS are done with)
-    const float none[I][4] = {};
-    to_tile<W, I>(mine, w, none);
-    for (int e = 0; e < p.k; ++e) {
-      const int label = p.labels[entry + e * step];
-      const float t = kept_cost(p, entry + e * step);
-      if (exists(label, t) && is_mine(label)) mine[label] += weight(least, t, p.to_exponent) * per_sum;
+    rest = p.rest[pixel];
+    Mass own = {least, 0.f};
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) own.sum += is_named(i, j) ? 0.f : a[i][j];
+    others = join<W>(own, part[0], w, lane, p.to_exponent);  // (the list's join: the student's parts are read)
+    // Beside the best label they may weigh next to nothing in fp32, where they are to be told from each other: then they
+    // are weighed beside the least cost of theirs.  (Every wavefront of the tile finds the same.)
+    const bool faint = !(others.sum >= kFaint);
+    if (__builtin_amdgcn_ballot_w64(faint) != 0) {
+      if (W > 1) tile_sync<W>();  // (the parts are read)
+      float next = kInf, weigh = 0;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) next = !is_named(i, j) && c[i][j] < next ? c[i][j] : next;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) weigh += is_named(i, j) ? 0.f : weight(next, c[i][j], p.to_exponent);
+      const Mass nearer = join<W>(Mass{next, weigh}, part[0], w, lane, p.to_exponent);
+      others = faint ? nearer : others;
     }
+    rest = others.sum == 0.f ? kInf : rest;
+  }
+  const float top = rest < list.least ? rest : list.least;  // the least cost of all classes
+  const float list_scale = weight(top, list.least, p.to_exponent), rest_weight = weight(top, rest, p.to_exponent);
+  const float mass = (list.least == kInf ? list.sum : list.sum * list_scale) + rest_weight;
+  if (!GRAD) {
+    far = list_scale > 0 ? list_scale * (far - list.sum * (list.least - top)) * p.inv_t : 0.f;
+    if (rest_weight > 0) far += rest_weight * (((others.least - student.least) - (rest - top)) * p.inv_t - logf(others.sum));
+    const float loss = far / mass + (logf(student.sum) - logf(mass));
+    if (w == 0 && lane < count) p.loss[pixel] = mass == 0.f ? 0.f : loss;
+  } else {
+    // p of the list's labels, in LDS where the costs were
+    const float per_mass = 1.f / mass;
+    const float none[I][4] = {};
+    to_tile<W, I>(mine, w, none);  // (the list's join: all entries have found their costs)
+    tile_sync<W>();
+    const bool in_turn = W == 1 || twice != 0;
+    if (!in_turn) {
+      entries([&](const Entry& e) {
+        if (exists(e)) mine[e.label] = weight(top, e.cost, p.to_exponent) * per_mass;
+      });
+    } else {
+      // a label's entries one after the other, in their order, by the wavefront whose label it is
+      for (int e = 0; e < p.k; ++e) {
+        const Entry x = fetch(e);
+        if (exists(x) && (x.label >> 2 & (W - 1)) == w) mine[x.label] += weight(top, x.cost, p.to_exponent) * per_mass;
+      }
+    }
+    tile_sync<W>();
     float d[I][4];
     from_tile<W, I>(mine, w, d);
-    const float scale = p.dloss[pixel] * p.inv_t, per_student = 1.f / student.sum;
-    const float share = rest_weight > 0 ? rest_weight * per_sum / others.sum : 0.f;
-    const float nan = sum - sum;  // 0, or NaN where the teacher has one
+    const float scale = p.dloss[pixel] * p.inv_t, of_student = weight(student.least, least, p.to_exponent) / student.sum;
+    const float share = rest_weight > 0 ? rest_weight * per_mass / others.sum : 0.f;
+    const bool beside = others.least == student.least;  // (the others' weights are those of a)
+    const float of_rest = beside ? share * weight(student.least, least, p.to_exponent) : 0.f;
+    const float nan = mass - mass;  // 0, or NaN where the teacher has one
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float q = weight(student.least, c[i][j], p.to_exponent) * per_student;
-        const float r = share > 0 && !is_named(i, j) ? share * weight(others.least, c[i][j], p.to_exponent) : 0.f;
-        d[i][j] = c[i][j] == kInf || sum == 0.f ? 0.f : ((d[i][j] + r) - q + nan) * scale;
+        const float r = is_named(i, j) ? 0.f : of_rest;
+        d[i][j] += a[i][j] * (r - of_student) + nan;
       }
+    if (__builtin_amdgcn_ballot_w64(!beside && share > 0) != 0) {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          d[i][j] += beside || !(share > 0) || is_named(i, j) ? 0.f : share * weight(others.least, c[i][j], p.to_exponent);
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[i][j] = c[i][j] == kInf || mass == 0.f ? 0.f : d[i][j] * scale;
     if (FIRST) {
       if (lane < count) store_rows<W, I>((T*)p.dcost + first + p0, p.t, w, lane, d);
     } else {
