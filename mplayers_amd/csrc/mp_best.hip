@@ -4,9 +4,10 @@
 // cost -> k labels by cost, equal ones by label, with their costs relative to the best one (what a softmax of them needs, and what
 // fits a narrow type), and rest = -T log(sum over the other candidates of exp(-(c - best) / T)).  +inf and NaN are no candidates.
 //
-// The costs are read once, a pixel's labels over S lanes (mp_lanes.h).  A label is found as the least cost that is left and the
-// first label that has it, over the lane's registers and the lanes of the pixel, and taken out: about 4.5 instructions for each
-// label and place of the list, no sort.  So a short list is bound by HBM and a long one by the instructions.
+// The costs are read once, a pixel's labels over S lanes (mp_lanes.h), and stay in LDS; a lane has the least cost of each quad of
+// its labels in registers.  A place of the list is the least of those over the lanes: the first lane that has it looks its
+// quad up, takes the label out and finds the quad's next.  So a place costs the instructions of the quads and not of the
+// labels, and no sort is needed.
 
 #include "mp_lanes.h"
 
@@ -14,7 +15,9 @@ using namespace mpl;
 
 namespace {
 
-constexpr int kChunk = 16;  // places of the list that wait in LDS for whole rows
+// Places of the list that wait in LDS for whole rows.  us for 48 M costs, lists of 8, with 16 / 8 / 4: 21 labels 86 / 68 / 73, 192
+// labels 66 / 55 / 57; lists of 32, 192 labels 377x501 124 / 109 / 116.
+constexpr int kChunk = 8;
 
 struct Best {
   LaneTiles t;
@@ -36,42 +39,64 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
   const int64_t item = block / tiles, p0 = (int64_t)(block - (unsigned)item * tiles) * kLanePixels;
   const int count = (int)min((int64_t)kLanePixels, p.t.pixels - p0);
   const int tid = (int)threadIdx.x, px = tid / S, s = tid % S;
+  using Tile = LaneTile<NV, S>;
+  constexpr int kJ = Tile::kJ;
   {
     LaneLoads<NV, S, LAST, T> loads;
     loads.load((const T*)p.cost + item * p.t.n * p.t.pixels, p.t, p0, count, p.quads, tid);
-    loads.to_tile(tile, p.t, count, p.quads, tid);
+    loads.template to_tile<true>(tile, p.t, count, p.quads, tid);
   }
   __syncthreads();
-  float v[NV];
-  lane_costs<NV, S>(tile, px, s, p.t.n, v);
-  const auto least = [&]() {
-    float m = v[0];
-#pragma unroll
-    for (int j = 1; j < NV; ++j) m = v[j] < m ? v[j] : m;
-    return lanes_min<S>(m);
+  // quad g of this lane is at own[g * 4 * S]; nobody else reads or writes it from here on
+  float* const own = &tile[px * Tile::kStride + s * 4];
+  const auto quad = [&](int g) { return *reinterpret_cast<const float4*>(own + g * 4 * S); };
+  const auto least_of = [](const float4& q) {
+    const float a = q.x < q.y ? q.x : q.y, b = q.z < q.w ? q.z : q.w;
+    return a < b ? a : b;
   };
-  float best = least();
-  if (__builtin_amdgcn_ballot_w64(best == -kInf) != 0 && best == -kInf) {
-    // beside a cost of -inf only others of -inf are candidates
+  float least[kJ];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = v[j] == -kInf ? 0.f : kInf;
-    best = 0;
+  for (int g = 0; g < kJ; ++g) least[g] = least_of(quad(g));
+  const auto mine = [&]() {
+    float m = least[0];
+#pragma unroll
+    for (int g = 1; g < kJ; ++g) m = least[g] < m ? least[g] : m;
+    return m;
+  };
+  float best = lanes_min<S>(mine());
+  if (__builtin_amdgcn_ballot_w64(best == -kInf) != 0) {
+    // beside a cost of -inf only others of -inf are candidates
+    if (best == -kInf) {
+      for (int g = 0; g < kJ; ++g)
+        for (int j = 0; j < 4; ++j) own[g * 4 * S + j] = own[g * 4 * S + j] == -kInf ? 0.f : kInf;
+#pragma unroll
+      for (int g = 0; g < kJ; ++g) least[g] = least[g] == -kInf ? 0.f : kInf;
+      best = 0;
+    }
   }
   for (int first = 0; first < p.k; first += kChunk) {
     const int here = min(kChunk, p.k - first);
     for (int k = 0; k < here; ++k) {
-      const float m = least();
-      int place = NV;
+      const float m = mine(), all = lanes_min<S>(m);
+      const int who = S == 1 ? 0 : lanes_min<S>(m == all ? s : S);
+      int g = 0;
 #pragma unroll
-      for (int j = NV - 1; j >= 0; --j) place = v[j] == m ? j : place;
-      const int label = lanes_min<S>(place < NV ? s * NV + place : S * NV);
-      place = label - s * NV;
+      for (int i = kJ - 1; i >= 0; --i) g = least[i] == all ? i : g;
+      if (s == who) {
+        float* const at = own + g * 4 * S;
+        float4 q = *reinterpret_cast<const float4*>(at);
+        const int j = q.x == all ? 0 : q.y == all ? 1 : q.z == all ? 2 : 3;
+        at[j] = kInf;
+        q.x = j == 0 ? kInf : q.x;
+        q.y = j == 1 ? kInf : q.y;
+        q.z = j == 2 ? kInf : q.z;
+        q.w = j == 3 ? kInf : q.w;
+        const float next = least_of(q);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) v[j] = j == place ? kInf : v[j];
-      if (s == 0) {
-        const float c = m < kInf ? m - best : kInf;
+        for (int i = 0; i < kJ; ++i) least[i] = i == g ? next : least[i];
+        const float c = all < kInf ? all - best : kInf;
         found_cost[k][px] = c;
-        found_label[k][px] = (uint8_t)(c < kInf ? label : 0);
+        found_label[k][px] = (uint8_t)(c < kInf ? s * NV + 4 * g + j : 0);
       }
     }
     __syncthreads();
@@ -93,30 +118,35 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
     __syncthreads();
   }
   if (p.rest != nullptr) {
-    const float m = least();
+    const float m = lanes_min<S>(mine());
     float sum = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) sum += v[j] < kInf ? __builtin_amdgcn_exp2f((m - v[j]) * p.to_exponent) : 0.f;
+    for (int g = 0; g < kJ; ++g) {
+      const float4 q = quad(g);
+      const float c[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += c[j] < kInf ? __builtin_amdgcn_exp2f((m - c[j]) * p.to_exponent) : 0.f;
+    }
     sum = lanes_sum<S>(sum);
     if (s == 0 && px < count) p.rest[item * p.t.pixels + p0 + px] = m < kInf ? (m - best) - p.temperature * logf(sum) : kInf;
   }
 }
 
+// Labels per lane and lanes per pixel.  us for 48 M costs, lists of 8: 16 labels 74 (a lane) / 86 (two), 24: 82 / 87, 32: 70 / 73,
+// 48: 69 / 63, 64: 61 (two) / 61 (four), 96: 64 / 55, 128: 67 / 54, 192: 72 (four) / 67 (eight), 256: 68 / 60.
 template <typename T, bool LAST>
 void launch(const Best& p, unsigned blocks, hipStream_t st) {
   const int n = p.t.n;
-  if (n <= 4)
-    best_kernel<T, 4, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
-  else if (n <= 8)
+  if (n <= 8)
     best_kernel<T, 8, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 16)
-    best_kernel<T, 8, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+    best_kernel<T, 16, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 24)
-    best_kernel<T, 12, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+    best_kernel<T, 24, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 32)
-    best_kernel<T, 16, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+    best_kernel<T, 32, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 48)
-    best_kernel<T, 12, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+    best_kernel<T, 24, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
   else if (n <= 64)
     best_kernel<T, 16, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
   else if (n <= 96)
@@ -145,7 +175,7 @@ extern "C" int mpl_best_labels(int dtype, int labels_first, const void* cost, in
   if (items == 0 || pixels == 0) return MPL_OK;
   if (cost == nullptr || kept_labels == nullptr || kept_costs == nullptr) return fail(MPL_EINVAL, "best_labels: null pointer");
   Best p = {};
-  if (!make_lane_tiles(p.t, items, n_disp, pixels)) return fail(MPL_EINVAL, "best_labels: too many pixels");
+  if (!make_lane_tiles(p.t, items, n_disp, pixels, labels_first != 0, dtype == MPL_F32 ? 4 : 2)) return fail(MPL_EINVAL, "best_labels: too many pixels");
   p.cost = cost;
   p.labels = kept_labels;
   p.costs = kept_costs;

@@ -294,7 +294,7 @@ int run(const char* what, int dtype, int labels_first, Distill& p, int kept_dtyp
   if (p.cost == nullptr || p.labels == nullptr || p.costs == nullptr ||
       (GRAD ? p.dloss == nullptr || p.dcost == nullptr : p.loss == nullptr))
     return fail(MPL_EINVAL, "%s: null pointer", what);
-  if (!make_tiles(p.t, items, n_disp, pixels)) return fail(MPL_EINVAL, "%s: too many pixels", what);
+  if (!make_tiles(p.t, items, n_disp, pixels, labels_first != 0, dtype == MPL_F32 ? 4 : 2)) return fail(MPL_EINVAL, "%s: too many pixels", what);
   p.k = k;
   p.kept = kept_dtype;
   p.to_exponent = (float)(1.4426950408889634 / (double)temperature);

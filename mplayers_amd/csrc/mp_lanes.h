@@ -132,8 +132,9 @@ struct LaneTiles {
   uint32_t reciprocal;    // 2^32 / n, rounded up
   int xcd_group;          // tiles beside each other that go to one die (xcd_block)
 };
-// False where a launch would have too many threads, eight to a pixel at most.
-inline bool make_lane_tiles(LaneTiles& t, int64_t items, int n_disp, int64_t pixels) {
+// False where a launch would have too many threads, eight to a pixel at most.  bytes: of a cost; rows: in the network's layout,
+// where tiles share the cache lines of rows that are not whole ones.
+inline bool make_lane_tiles(LaneTiles& t, int64_t items, int n_disp, int64_t pixels, bool rows, int bytes) {
   const int64_t threads = kLanePixels * (n_disp <= 32 ? 2 : 8);
   if (items > 0x7fffffff || pixels > ((int64_t)1 << 40)) return false;
   t.pixels = pixels;
@@ -141,7 +142,7 @@ inline bool make_lane_tiles(LaneTiles& t, int64_t items, int n_disp, int64_t pix
   if (t.tiles > 0xffffffff / threads / items) return false;
   t.n = n_disp;
   t.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
-  t.xcd_group = 0;
+  t.xcd_group = rows && pixels * bytes % kLineBytes != 0 ? 16 : 0;
   return true;
 }
 
@@ -190,9 +191,15 @@ struct LaneLoads {
           c[4 * i + j] = cost[(int64_t)min(4 * (wave + i * S) + j, n - 1) * t.pixels + p0 + of];
     }
   }
+  // CLEAN: what is no candidate as +inf, labels behind the last too.
+  template <bool CLEAN = false>
   __device__ __forceinline__ void to_tile(float* tile, const LaneTiles& t, int count, bool quads, int tid) const {
     using Tile = LaneTile<NV, S>;
     constexpr int kJ = NV / 4, kThreads = kLanePixels * S;
+    const auto cost = [&](int k) { return CLEAN ? candidate((float)c[k]) : (float)c[k]; };
+    if (CLEAN && LAST) {
+      for (int l = t.n + tid % S; l < S * NV; l += S) tile[tid / S * Tile::kStride + Tile::place(l >> 2) + (l & 3)] = kInf;
+    }
     if (LAST) {
       const unsigned n = (unsigned)t.n, total = (unsigned)count * n;
       if (quads) {
@@ -201,22 +208,25 @@ struct LaneLoads {
           const unsigned i = min((unsigned)(tid + k * kThreads) * 4, total - 4);
           const unsigned of = __umulhi(i, t.reciprocal), l = i - of * n;
           *reinterpret_cast<float4*>(&tile[of * Tile::kStride + Tile::place((int)(l >> 2))]) =
-              float4{(float)c[4 * k], (float)c[4 * k + 1], (float)c[4 * k + 2], (float)c[4 * k + 3]};
+              float4{cost(4 * k), cost(4 * k + 1), cost(4 * k + 2), cost(4 * k + 3)};
         }
       } else {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
           const unsigned i = min((unsigned)(tid + k * kThreads), total - 1);
           const unsigned of = n == 1 ? i : __umulhi(i, t.reciprocal), l = i - of * n;
-          tile[of * Tile::kStride + Tile::place((int)(l >> 2)) + (l & 3)] = (float)c[k];
+          tile[of * Tile::kStride + Tile::place((int)(l >> 2)) + (l & 3)] = cost(k);
         }
       }
     } else {
       const int wave = uniform_i(tid / kLanePixels);
 #pragma unroll
-      for (int i = 0; i < kJ; ++i)
+      for (int i = 0; i < kJ; ++i) {
+        const int l = 4 * (wave + i * S);
+        const auto of = [&](int j) { return CLEAN && l + j >= t.n ? kInf : cost(4 * i + j); };
         *reinterpret_cast<float4*>(&tile[tid % kLanePixels * Tile::kStride + Tile::place(wave + i * S)]) =
-            float4{(float)c[4 * i], (float)c[4 * i + 1], (float)c[4 * i + 2], (float)c[4 * i + 3]};
+            float4{of(0), of(1), of(2), of(3)};
+      }
     }
   }
 };

@@ -20,7 +20,7 @@ using namespace mpl;
 
 namespace {
 
-constexpr int kSumRows = 2048;  // workgroups of a gradient, at most
+constexpr unsigned kSumRows = 2048;  // workgroups of a gradient, at most
 
 struct Norm {
   Tiles t;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
 
 // SUMS: with the sums over pixels that dweight and dbias are made of.
 template <typename T, bool FIRST, bool SUMS, int W, int I, int G>
-__global__ void __launch_bounds__(64 * W * G) norm_grad_kernel(Norm p) {
+__global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(Norm p) {
   constexpr int kStride = tile_stride(W * I);
   __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
   __shared__ __align__(16) float weight[4 * W * I];
@@ -240,21 +240,21 @@ __global__ void __launch_bounds__(64 * W * G) norm_grad_kernel(Norm p) {
 }
 
 // The workgroups' rows of 2 * n sums, a column to every 16th thread, in 64 bits.
-__global__ void __launch_bounds__(256) norm_sums_kernel(const float* __restrict__ sums, int rows, int n, float* __restrict__ dweight,
+__global__ void __launch_bounds__(1024) norm_sums_kernel(const float* __restrict__ sums, int rows, int n, float* __restrict__ dweight,
                                                        float* __restrict__ dbias) {
-  __shared__ double part[16][17];
+  __shared__ double part[64][17];
   const int of = (int)threadIdx.x % 16, by = (int)threadIdx.x / 16, column = (int)blockIdx.x * 16 + of;
   double sum = 0;
   if (column < 2 * n) {
 #pragma unroll 8
-    for (int row = by; row < rows; row += 16) sum += (double)sums[(int64_t)row * 2 * n + column];
+    for (int row = by; row < rows; row += 64) sum += (double)sums[(int64_t)row * 2 * n + column];
   }
   part[by][of] = sum;
   __syncthreads();
   if (by == 0 && column < 2 * n) {
     sum = 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) sum += part[k][of];
+    for (int k = 0; k < 64; ++k) sum += part[k][of];
     if (column < n) {
       if (dweight != nullptr) dweight[column] = (float)sum;
     } else if (dbias != nullptr) {
@@ -268,9 +268,37 @@ int status(const char* what) {
   return e == hipSuccess ? MPL_OK : fail(MPL_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
 }
 
-unsigned grad_blocks(unsigned tiles, int per_block) {
-  const unsigned blocks = (tiles + (unsigned)per_block - 1) / (unsigned)per_block;
-  return blocks < (unsigned)kSumRows ? blocks : (unsigned)kSumRows;
+// The gradient's shapes: quarter as many labels of a wavefront, whose sums over the pixels take two registers each.
+template <typename F>
+void with_grad_shape(int n, F f) {
+  if (n <= 4)
+    f(TileShape<1, 1, 4>());
+  else if (n <= 8)
+    f(TileShape<2, 1, 1>());
+  else if (n <= 16)
+    f(TileShape<4, 1, 1>());
+  else if (n <= 24)
+    f(TileShape<3, 2, 1>());
+  else if (n <= 32)
+    f(TileShape<4, 2, 1>());
+  else if (n <= 48)
+    f(TileShape<6, 2, 1>());
+  else if (n <= 64)
+    f(TileShape<8, 2, 1>());
+  else if (n <= 96)
+    f(TileShape<8, 3, 1>());
+  else if (n <= 128)
+    f(TileShape<8, 4, 1>());
+  else if (n <= 192)
+    f(TileShape<8, 6, 1>());
+  else
+    f(TileShape<8, 8, 1>());
+}
+// Workgroups of a gradient, each with as many tiles as the others.
+unsigned grad_blocks(unsigned tiles, int waves, int per_block) {
+  const unsigned most = waves >= 8 ? kSumRows / 4 : kSumRows, groups = (tiles + (unsigned)per_block - 1) / (unsigned)per_block;
+  const unsigned rounds = (groups + most - 1) / most;
+  return (groups + rounds - 1) / rounds;
 }
 
 template <typename T, bool FIRST>
@@ -282,15 +310,15 @@ void launch(const Norm& p, hipStream_t st) {
 }
 template <typename T, bool FIRST>
 void launch_grad(const Norm& p, float* dweight, float* dbias, hipStream_t st) {
-  with_shape(p.t.labels, [&](auto s) {
+  with_grad_shape(p.t.labels, [&](auto s) {
     constexpr int W = s.kW, I = s.kI, G = s.kG;
-    const unsigned blocks = grad_blocks(p.t.total, G);
+    const unsigned blocks = grad_blocks(p.t.total, W * G, G);
     if (p.sums == nullptr) {
       norm_grad_kernel<T, FIRST, false, W, I, G><<<blocks, 64 * W * G, 0, st>>>(p);
       return;
     }
     norm_grad_kernel<T, FIRST, true, W, I, G><<<blocks, 64 * W * G, 0, st>>>(p);
-    norm_sums_kernel<<<(2 * p.t.labels + 15) / 16, 256, 0, st>>>(p.sums, (int)blocks, p.t.labels, dweight, dbias);
+    norm_sums_kernel<<<(2 * p.t.labels + 15) / 16, 1024, 0, st>>>(p.sums, (int)blocks, p.t.labels, dweight, dbias);
   });
 }
 template <typename F>
@@ -310,7 +338,7 @@ int prepare(const char* what, Norm& p, int dtype, bool labels_first, int batch, 
   if (dtype < 0 || dtype > MPL_BF16) return fail(MPL_EINVAL, "%s: unknown data type %d", what, dtype);
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
   if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
-  if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels)) return fail(MPL_EINVAL, "%s: too many pixels", what);
+  if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels, labels_first, dtype == MPL_F32 ? 4 : 2)) return fail(MPL_EINVAL, "%s: too many pixels", what);
   return MPL_OK;
 }
 int whole_quads(const void* at, int n_disp, int dtype) {
@@ -324,7 +352,7 @@ extern "C" {
 int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels) {
   if (batch <= 0 || pixels <= 0 || n_disp < 1 || n_disp > kMaxL) return 0;
   const int64_t per_item = (pixels + kTilePixels - 1) / kTilePixels;
-  const int64_t rows = per_item > kSumRows / batch ? kSumRows : per_item * batch;
+  const int64_t rows = per_item > (int64_t)kSumRows / batch ? (int64_t)kSumRows : per_item * batch;
   return rows * 2 * n_disp;
 }
 
@@ -357,7 +385,7 @@ int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, cons
   const bool sums = dweight != nullptr || dbias != nullptr;
   if (batch == 0 || pixels == 0) {
     // (a sum of nothing)
-    if (sums) norm_sums_kernel<<<(2 * n_disp + 15) / 16, 256, 0, (hipStream_t)stream>>>(nullptr, 0, n_disp, dweight, dbias);
+    if (sums) norm_sums_kernel<<<(2 * n_disp + 15) / 16, 1024, 0, (hipStream_t)stream>>>(nullptr, 0, n_disp, dweight, dbias);
     return sums ? status("norm_labels_last_grad") : MPL_OK;
   }
   if (src == nullptr || stats == nullptr || ddst == nullptr || (sums && workspace == nullptr))

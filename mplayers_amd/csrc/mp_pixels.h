@@ -58,8 +58,12 @@ inline void with_shape(int n, F f) {
     f(TileShape<8, 8, 1>());
 }
 
-// False where a launch would have too many threads.
-inline bool make_tiles(Tiles& t, int items, int n_disp, int64_t pixels) {
+// False where a launch would have too many threads.  bytes: of a cost; rows: in the network's layout.
+// Where rows are not whole cache lines the tiles beside each other share lines, which one die's L2 can join.  us, tiles dealt
+// out one by one -> groups of 8 -> 16: layer norm forward 192 labels 377x501 69 -> 63 -> 63, 60 labels 375x451 16.6 -> 15.8 ->
+// 15.1, its gradient 126 -> 115 -> 116, 28.6 -> 26.8 -> 26.4, 97 labels 301x803 68 -> 62 -> 63, bf16 21 labels 12x129x129 12.3 ->
+// 12.4 -> 12.9; distillation's gradient 192 labels 76 -> 68 -> 66, 97 labels 63 -> 58 -> 57.
+inline bool make_tiles(Tiles& t, int items, int n_disp, int64_t pixels, bool rows, int bytes) {
   int threads = 0;
   with_shape(n_disp, [&](auto s) { threads = kTilePixels * s.kW; });
   if (pixels > ((int64_t)1 << 40)) return false;
@@ -71,7 +75,7 @@ inline bool make_tiles(Tiles& t, int items, int n_disp, int64_t pixels) {
   t.total = (unsigned)per_item * (unsigned)items;
   t.labels = n_disp;
   t.reciprocal = n_disp > 1 ? (uint32_t)((((uint64_t)1 << 32) + (uint64_t)n_disp - 1) / (uint64_t)n_disp) : 0u;
-  t.xcd_group = 0;
+  t.xcd_group = rows && pixels * bytes % kLineBytes != 0 ? 16 : 0;
   return true;
 }
 

@@ -408,7 +408,7 @@ extern "C" int mpl_verify_labels(int labels_first, const float* cost, const uint
   if (cost == nullptr || draft == nullptr || uniforms == nullptr || labels == nullptr || kept == nullptr)
     return fail(MPL_EINVAL, "verify_labels: null pointer");
   Verify p;
-  if (!make_lane_tiles(p.t, (int64_t)batch * n_cv, n_disp, pixels)) return fail(MPL_EINVAL, "verify_labels: too many pixels");
+  if (!make_lane_tiles(p.t, (int64_t)batch * n_cv, n_disp, pixels, labels_first != 0, 4)) return fail(MPL_EINVAL, "verify_labels: too many pixels");
   p.cost = cost;
   p.draft_cost = draft_cost;
   p.draft = draft;
@@ -423,8 +423,6 @@ extern "C" int mpl_verify_labels(int labels_first, const float* cost, const uint
   p.n_cv = n_cv;
   p.n_drafts = n_drafts;
   p.quads = n_disp % 4 == 0 && (((uintptr_t)cost | (uintptr_t)draft_cost) & 15) == 0;
-  // (tiles that share cache lines: see mpl_sample_labels)
-  p.t.xcd_group = labels_first && pixels * 4 % kLineBytes != 0 ? 16 : 0;
   const unsigned blocks = (unsigned)(p.t.tiles * batch * n_cv);
   const hipStream_t st = (hipStream_t)stream;
   if (draft_cost != nullptr)
