@@ -223,21 +223,28 @@ struct LaneLoads {
 #pragma unroll
       for (int i = 0; i < kJ; ++i) {
         const int l = 4 * (wave + i * S);
-        const auto of = [&](int j) { return CLEAN && l + j >= t.n ? kInf : cost(4 * i + j); };
-        *reinterpret_cast<float4*>(&tile[tid % kLanePixels * Tile::kStride + Tile::place(wave + i * S)]) =
-            float4{of(0), of(1), of(2), of(3)};
+        float4* const to = reinterpret_cast<float4*>(&tile[tid % kLanePixels * Tile::kStride + Tile::place(wave + i * S)]);
+        if (!CLEAN || l + 3 < t.n) {
+          *to = float4{cost(4 * i), cost(4 * i + 1), cost(4 * i + 2), cost(4 * i + 3)};
+        } else {
+          const auto of = [&](int j) { return l + j < t.n ? cost(4 * i + j) : kInf; };
+          *to = float4{of(0), of(1), of(2), of(3)};
+        }
       }
     }
   }
 };
 
-// The lane's costs out of LDS, +inf where there is no candidate.
+// The lane's costs out of LDS.
 template <int NV, int S>
-__device__ __forceinline__ void lane_costs(const float* tile, int px, int s, int n, float (&v)[NV]) {
+__device__ __forceinline__ void from_lane_tile(const float* tile, int px, int s, float (&v)[NV]) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const float c = tile[px * LaneTile<NV, S>::kStride + ((j >> 2) * S + s) * 4 + (j & 3)];
-    v[j] = s * NV + j < n ? candidate(c) : kInf;
+  for (int g = 0; g < NV / 4; ++g) {
+    const float4 q = *reinterpret_cast<const float4*>(&tile[px * LaneTile<NV, S>::kStride + (g * S + s) * 4]);
+    v[4 * g] = q.x;
+    v[4 * g + 1] = q.y;
+    v[4 * g + 2] = q.z;
+    v[4 * g + 3] = q.w;
   }
 }
 

@@ -182,29 +182,31 @@ __device__ __forceinline__ Weights weights32(float (&v)[NV], const Scale& scale,
     w.total = 1.f;
     return w;
   }
+  const float best = w.best < kInf ? w.best : 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    v[j] = v[j] < kInf ? __builtin_amdgcn_exp2f((w.best - v[j]) * scale.to_exponent) : 0.f;
+    v[j] = __builtin_amdgcn_exp2f((best - v[j]) * scale.to_exponent);  // (0 of +inf)
     w.total += v[j];
   }
   w.total = lanes_sum<S>(w.total);
   return w;
 }
 
-// S lanes per pixel, NV labels per lane.  p and q are formed in 32 bits, with a bound on how far they may be off, all relative to
-// a sum of 1 and u = 2^-24:
-//   weights   3 roundings of an exponent a (3 u a w, and sum(a w) <= ln(n) sum(w): the entropy of n labels) and an ulp of the
+// S lanes per pixel, NV labels per lane.  The weights stay as they are, those of the draft are brought to the target's scale: p is
+// a[l] / A and q is b[l] / B, so b[l] * (A / B) stands beside a[l].  They are formed in 32 bits, with a bound on how far they
+// may be off, all relative to A and u = 2^-24:
+//   weights   3 roundings of an exponent x (3 u x w, and sum(x w) <= ln(n) sum(w): the entropy of n labels) and an ulp of the
 //             exponential: (2 + 3 ln 256) u < 19 u of their sum
-//   p         those, the sum's own additions, (NV + S) u, its weights again, a reciprocal and a product: (40 + NV + S) u over
-//             all labels
-//   a running sum of max(p - q, 0): both of these, a rounding each, its own additions: (81 + 3 (NV + S)) u
+//   b A / B   those, of A and B as much and their own additions, (NV + S) u each, a quotient and a product: (59 + 2 (NV + S)) u
+//             over all labels
+//   a running sum of max(a - b A / B, 0): both of these, a rounding each, its own additions: (80 + 3 (NV + S)) u
 // and as much for a target, which is a product with such a sum.  Where a target is as close to a sum as both (kNear), 32 bits
-// do not tell, and verify_exactly() takes the pixel.  So it does where u0 q[d] is as close to p[d] as (3 a + 45 + NV + S) u of
-// either, a being their exponents.
+// do not tell, and verify_exactly() takes the pixel.  So it does where u0 q[d] is as close to p[d] as (3 x + 64 + 2 (NV + S)) u
+// of either, x being their exponents.
 template <int NV, int S, bool COSTS, bool LAST>
 __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   using Tile = LaneTile<NV, S>;
-  constexpr float kU = 0x1p-24f, kNear = 2 * (82 + 3 * (NV + S)) * kU;
+  constexpr float kU = 0x1p-24f, kNear = 2 * (81 + 3 * (NV + S)) * kU;
   constexpr float kLeast = 1e-30f;  // below it fp32 is not what the bounds say
   __shared__ __align__(16) float tile[kLanePixels * Tile::kStride];
   __shared__ uint32_t left_over[2];  // pixels for verify_exactly()
@@ -241,14 +243,14 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
     target.load(p.cost + first, p.t, p0, count, p.quads, tid);
     if (COSTS) draft.load(p.draft_cost + first, p.t, p0, count, p.quads, tid);
     fetch_costs(d);
-    target.to_tile(tile, p.t, count, p.quads, tid);
+    target.template to_tile<true>(tile, p.t, count, p.quads, tid);
     __syncthreads();
-    lane_costs<NV, S>(tile, px, s, n, a);
+    from_lane_tile<NV, S>(tile, px, s, a);
     if (COSTS) {
       __syncthreads();
-      draft.to_tile(tile, p.t, count, p.quads, tid);
+      draft.template to_tile<true>(tile, p.t, count, p.quads, tid);
       __syncthreads();
-      lane_costs<NV, S>(tile, px, s, n, b);
+      from_lane_tile<NV, S>(tile, px, s, b);
     }
   }
   const int image = (int)((unsigned)item / (unsigned)p.n_cv);
@@ -257,36 +259,42 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   const Weights wa = weights32<NV, S>(a, scale, s), wb = COSTS ? weights32<NV, S>(b, draft_scale, s) : wa;
   const bool empty = wa.best == kInf;
   bool unsure = !(wa.best > -kInf) || scale.far || (COSTS && wb.best < kInf && (!(wb.best > -kInf) || draft_scale.far));
-  const float per_a = empty ? 0.f : 1.f / wa.total, per_b = COSTS && wb.best < kInf ? 1.f / wb.total : 0.f;
-  // running sums: of p, and of what the draft leaves
-  float sum_a = 0, sum_b = 0;
+  const float to_target = COSTS && wb.total > 0 ? wa.total / wb.total : 0.f;
+  if (COSTS) {
+    // what the draft leaves
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const float of_target = a[j] * per_a;
-    sum_a += of_target;
-    a[j] = sum_a;
-    if (COSTS) {
-      const float rest = of_target - b[j] * per_b;
-      sum_b += rest > 0 ? rest : 0.f;
-      b[j] = sum_b;
+    for (int j = 0; j < NV; ++j) {
+      const float rest = a[j] - b[j] * to_target;
+      b[j] = rest > 0 ? rest : 0.f;
     }
   }
-  const float before_a = lanes_before<S>(sum_a, s), before_b = COSTS ? lanes_before<S>(sum_b, s) : 0.f;
-  const float all_a = lanes_max<S>(before_a + sum_a), all_b = COSTS ? lanes_max<S>(before_b + sum_b) : 0.f;
 
-  // The sums to LDS: the lanes of a pixel are of one wavefront, and nobody else reads its place any more.
+  // Running sums to LDS, and the last of them: the lanes of a pixel are of one wavefront, and nobody else reads its place any
+  // more.
   float* const sums = &tile[px * Tile::kStride];
-  const auto to_lds = [&](const float (&x)[NV], float before) {
+  const auto sum_up = [&](const float (&x)[NV]) {
+    float sum = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) sum += x[j];
+    sum = lanes_before<S>(sum, s);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int j = 0; j < NV; j += 4)
-      *reinterpret_cast<float4*>(sums + s * NV + j) = float4{before + x[j], before + x[j + 1], before + x[j + 2], before + x[j + 3]};
+    for (int j = 0; j < NV; j += 4) {
+      float4 q;
+      q.x = sum += x[j];
+      q.y = sum += x[j + 1];
+      q.z = sum += x[j + 2];
+      q.w = sum += x[j + 3];
+      *reinterpret_cast<float4*>(sums + s * NV + j) = q;
+    }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    return lanes_max<S>(sum);
   };
   // The first label whose sum is above the target, by halving; `taken` of the sums from label `from` on does not count.
   const int top = 1 << (31 - __builtin_clz(n));
+  const float too_near = kNear * wa.total;
   const auto find = [&](float target, int from, float taken, bool& near) {
     int label = 0;
     float least = -kInf;  // the last sum that is not above the target
@@ -299,13 +307,11 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
       }
     }
     const float most = sums[min(label, n - 1)] - (label >= from ? taken : 0.f);
-    near = !(least <= target - kNear && most > target + kNear) || label >= n;
+    near = !(least <= target - too_near && most > target + too_near) || label >= n;
     return label;
   };
-  if (COSTS)
-    to_lds(b, before_b);
-  else
-    to_lds(a, before_a);
+  bool ready = false;  // whether the sums in LDS are those that labels are drawn from
+  float left = 0;
   for (int base = 0; base < p.n_drafts; base += S) {
     if (base > 0) {
       d = fetch_label(base + s);
@@ -318,10 +324,10 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
     const bool has_q = exists && (!COSTS || (draft_scale.cold ? d.label == wb.first : dc < kInf));
     const float far_a = scale.cold || !has_p ? 0.f : (wa.best - c) * scale.to_exponent;
     const float far_b = !COSTS || draft_scale.cold || !has_q ? 0.f : (wb.best - dc) * draft_scale.to_exponent;
-    const float p_d = has_p ? __builtin_amdgcn_exp2f(far_a) * per_a : 0.f;
-    const float q_d = !has_q ? 0.f : COSTS ? __builtin_amdgcn_exp2f(far_b) * per_b : 1.f;
+    const float p_d = has_p ? __builtin_amdgcn_exp2f(far_a) : 0.f;
+    const float q_d = !has_q ? 0.f : COSTS ? __builtin_amdgcn_exp2f(far_b) * to_target : wa.total;
     const float u0 = positive(d.u0) ? (d.u0 < 1.f ? d.u0 : 1.f) : 0.f, u1 = positive(d.u1) ? (d.u1 < 2.f ? d.u1 : 2.f) : 0.f;
-    const float least = u0 * q_d, off = (48 + NV + S - 3 * (far_a < far_b ? far_a : far_b)) * kU;
+    const float least = u0 * q_d, off = (64 + 2 * (NV + S) - 3 * (far_a < far_b ? far_a : far_b)) * kU;
     const bool kept = has_q && least < p_d;
     bool near = has_q && (q_d < kLeast || fabsf(least - p_d) <= off * (least + p_d) + kLeast || (positive(d.u0) && d.u0 > 1.f));
     int label = d.label;
@@ -329,19 +335,21 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
     const bool draws = mine && !empty && !kept && !near;
     const bool draws_left = draws && (has_q || !COSTS), draws_all = draws && !has_q && COSTS;
     if (__builtin_amdgcn_ballot_w64(draws_left) != 0) {
-      const float taken = !COSTS && exists ? p_d : 0.f, all = COSTS ? all_b : all_a - taken;
+      if (!ready) left = sum_up(COSTS ? b : a);
+      ready = true;
+      const float taken = !COSTS && exists ? p_d : 0.f;
       bool close;
-      const int drawn = find(u1 * all, d.label, taken, close);
+      const int drawn = find(u1 * (left - taken), d.label, taken, close);
       label = draws_left ? drawn : label;
       near |= draws_left && close;
     }
     if (COSTS && __builtin_amdgcn_ballot_w64(draws_all) != 0) {
-      to_lds(a, before_a);
+      const float all = sum_up(a);
+      ready = false;
       bool close;
-      const int drawn = find(u1 * all_a, 0, 0.f, close);
+      const int drawn = find(u1 * all, 0, 0.f, close);
       label = draws_all ? drawn : label;
       near |= draws_all && close;
-      to_lds(b, before_b);
     }
     unsure |= near && mine;
     if (mine && (empty || !unsure)) {
