@@ -97,14 +97,31 @@ __device__ __forceinline__ double of_label(const double (&w)[4], int label) {
   return from_lane(x, label >> 2);
 }
 
-// One pixel by a wavefront: cost(l) and draft_cost(l) give its costs, at is its place in the drafts.
+// One pixel by a wavefront: cost(l) and draft_cost(l) give its costs, at is its place in the drafts, of which those k whose bit
+// k % 32 is set are asked for.
 template <bool COSTS, typename Cost, typename DraftCost>
-__device__ void verify_exactly(const Verify& p, int image, int64_t at, Cost cost, DraftCost draft_cost) {
+__device__ void verify_exactly(const Verify& p, int image, int64_t at, uint32_t asked, Cost cost, DraftCost draft_cost) {
   const int lane = (int)(threadIdx.x & 63);
-  float v[4];
+  const int64_t drafts = p.items_pixels * p.n_drafts;
+  // a draft to a lane, for the next 64
+  int d_of_lane = 0;
+  float u0_of_lane = 0, u1_of_lane = 0;
+  const auto fetch = [&](int k) {
+    const int64_t mine = min(k + lane, p.n_drafts - 1) * p.items_pixels + at;
+    d_of_lane = p.draft[mine];
+    u0_of_lane = p.uniforms[mine];
+    u1_of_lane = p.uniforms[drafts + mine];
+  };
+  fetch(0);
+  // (all that comes from memory is on its way before the first of it is waited for)
+  float v[4], y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = cost(min(4 * lane + j, p.t.n - 1));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = COSTS ? draft_cost(min(4 * lane + j, p.t.n - 1)) : 0.f;
   double a[4], b[4] = {}, left[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < p.t.n ? candidate(cost(4 * lane + j)) : kInf;
+  for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < p.t.n ? candidate(v[j]) : kInf;
   weights64(v, p.temperature != nullptr ? p.temperature[image] : p.temperature_all, a);
   const double total = total64(a), total_or_1 = total > 0 ? total : 1.0;
 #pragma unroll
@@ -113,8 +130,8 @@ __device__ void verify_exactly(const Verify& p, int image, int64_t at, Cost cost
   Running rest = all;
   if (COSTS) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = 4 * lane + j < p.t.n ? candidate(draft_cost(4 * lane + j)) : kInf;
-    weights64(v, p.draft_temperature != nullptr ? p.draft_temperature[image] : p.draft_temperature_all, b);
+    for (int j = 0; j < 4; ++j) y[j] = 4 * lane + j < p.t.n ? candidate(y[j]) : kInf;
+    weights64(y, p.draft_temperature != nullptr ? p.draft_temperature[image] : p.draft_temperature_all, b);
     const double of_draft = total64(b), of_draft_or_1 = of_draft > 0 ? of_draft : 1.0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -123,11 +140,12 @@ __device__ void verify_exactly(const Verify& p, int image, int64_t at, Cost cost
     }
     rest = running64(left);
   }
-  const int64_t drafts = p.items_pixels * p.n_drafts;
   for (int k = 0; k < p.n_drafts; ++k) {
+    if (k > 0 && k % 64 == 0) fetch(k);
+    if ((asked >> (k % 32) & 1) == 0) continue;
     const int64_t place = k * p.items_pixels + at;
-    const int d = uniform_i(p.draft[place]);
-    const float u0 = uniform_f(p.uniforms[place]), u1 = uniform_f(p.uniforms[drafts + place]);
+    const int d = from_lane(d_of_lane, k % 64);
+    const float u0 = from_lane(u0_of_lane, k % 64), u1 = from_lane(u1_of_lane, k % 64);
     const bool exists = d < p.t.n;
     const double p_d = of_label(a, exists ? d : 0), q_d = !exists ? 0.0 : COSTS ? of_label(b, d) : 1.0;
     const bool stays = total > 0 && exists && q_d > 0 && (positive(u0) ? (double)u0 : 0.0) * q_d < p_d;
@@ -162,6 +180,18 @@ __device__ __forceinline__ Scale scale_of(const float* each, float all, int imag
   return s;
 }
 
+// The sum of a lane's numbers, fours first: of NV / 4 + 1 additions on the way of any of them.
+template <int NV>
+__device__ __forceinline__ float tree_sum(const float (&v)[NV]) {
+  float sum = 0;
+#pragma unroll
+  for (int j = 0; j < NV; j += 4) {
+    const float four = (v[j] + v[j + 1]) + (v[j + 2] + v[j + 3]);
+    sum = j == 0 ? four : sum + four;
+  }
+  return sum;
+}
+
 // The weights of a pixel's labels in its S lanes, in place of the costs.
 struct Weights {
   float best, total;  // the least cost, +inf where there is no candidate
@@ -184,11 +214,8 @@ __device__ __forceinline__ Weights weights32(float (&v)[NV], const Scale& scale,
   }
   const float best = w.best < kInf ? w.best : 0.f;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    v[j] = __builtin_amdgcn_exp2f((best - v[j]) * scale.to_exponent);  // (0 of +inf)
-    w.total += v[j];
-  }
-  w.total = lanes_sum<S>(w.total);
+  for (int j = 0; j < NV; ++j) v[j] = __builtin_amdgcn_exp2f((best - v[j]) * scale.to_exponent);  // (0 of +inf)
+  w.total = lanes_sum<S>(tree_sum(v));
   return w;
 }
 
@@ -197,19 +224,22 @@ __device__ __forceinline__ Weights weights32(float (&v)[NV], const Scale& scale,
 // may be off, all relative to A and u = 2^-24:
 //   weights   3 roundings of an exponent x (3 u x w, and sum(x w) <= ln(n) sum(w): the entropy of n labels) and an ulp of the
 //             exponential: (2 + 3 ln 256) u < 19 u of their sum
-//   b A / B   those, of A and B as much and their own additions, (NV + S) u each, a quotient and a product: (59 + 2 (NV + S)) u
-//             over all labels
-//   a running sum of max(a - b A / B, 0): both of these, a rounding each, its own additions: (80 + 3 (NV + S)) u
+//   b A / B   those, of A and B as much and their own additions, H u each with H = NV / 4 + 4 + S, a quotient and a product:
+//             (59 + 2 H) u over all labels
+//   a running sum of max(a - b A / B, 0): both of these, a rounding each, the additions of what lies before the lane and of the
+//             lane's fours to it: (79 + 2 H + NV / 2 + 3 + S) u
 // and as much for a target, which is a product with such a sum.  Where a target is as close to a sum as both (kNear), 32 bits
-// do not tell, and verify_exactly() takes the pixel.  So it does where u0 q[d] is as close to p[d] as (3 x + 64 + 2 (NV + S)) u
-// of either, x being their exponents.
+// do not tell, and verify_exactly() takes the draft: with costs as a layer gives them one in 700 of 192 labels, one in 5000 of
+// 21.  So it does where u0 q[d] is as close to p[d] as (3 x + 64 + 2 H) u of either, x being their exponents.
 template <int NV, int S, bool COSTS, bool LAST>
 __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   using Tile = LaneTile<NV, S>;
-  constexpr float kU = 0x1p-24f, kNear = 2 * (81 + 3 * (NV + S)) * kU;
+  constexpr int kSteps = NV / 4 + 4 + S;
+  constexpr float kU = 0x1p-24f, kNear = 2 * (80 + 2 * kSteps + NV / 2 + 3 + S) * kU;
   constexpr float kLeast = 1e-30f;  // below it fp32 is not what the bounds say
   __shared__ __align__(16) float tile[kLanePixels * Tile::kStride];
-  __shared__ uint32_t left_over[2];  // pixels for verify_exactly()
+  __shared__ uint32_t left_over[2];           // pixels for verify_exactly(),
+  __shared__ uint32_t asked[kLanePixels];     // and their drafts
   const unsigned block = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.t.xcd_group), tiles = (unsigned)p.t.tiles;
   const int64_t item = block / tiles, p0 = (int64_t)(block - (unsigned)item * tiles) * kLanePixels;
   const int count = (int)min((int64_t)kLanePixels, p.t.pixels - p0), n = p.t.n;
@@ -217,6 +247,7 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   const int64_t first = item * n * p.t.pixels, at = item * p.t.pixels + p0 + of, drafts = p.items_pixels * p.n_drafts;
   const int64_t pixel = first + (LAST ? (p0 + of) * n : p0 + of), step = LAST ? 1 : p.t.pixels;
   if (tid < 2) left_over[tid] = 0;
+  if (s == 0) asked[px] = 0;
   // A draft to a lane: its label and uniform numbers, and the costs of that label.
   struct Drafted {
     int64_t place;
@@ -258,7 +289,8 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
               draft_scale = COSTS ? scale_of(p.draft_temperature, p.draft_temperature_all, image) : scale;
   const Weights wa = weights32<NV, S>(a, scale, s), wb = COSTS ? weights32<NV, S>(b, draft_scale, s) : wa;
   const bool empty = wa.best == kInf;
-  bool unsure = !(wa.best > -kInf) || scale.far || (COSTS && wb.best < kInf && (!(wb.best > -kInf) || draft_scale.far));
+  // (no draft of the pixel can be told)
+  const bool blind = !(wa.best > -kInf) || scale.far || (COSTS && wb.best < kInf && (!(wb.best > -kInf) || draft_scale.far));
   const float to_target = COSTS && wb.total > 0 ? wa.total / wb.total : 0.f;
   if (COSTS) {
     // what the draft leaves
@@ -273,19 +305,14 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   // more.
   float* const sums = &tile[px * Tile::kStride];
   const auto sum_up = [&](const float (&x)[NV]) {
-    float sum = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) sum += x[j];
-    sum = lanes_before<S>(sum, s);
+    float sum = lanes_before<S>(tree_sum(x), s);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int j = 0; j < NV; j += 4) {
-      float4 q;
-      q.x = sum += x[j];
-      q.y = sum += x[j + 1];
-      q.z = sum += x[j + 2];
-      q.w = sum += x[j + 3];
+      const float two = x[j] + x[j + 1], three = two + x[j + 2], four = two + (x[j + 2] + x[j + 3]);
+      const float4 q = {sum + x[j], sum + two, sum + three, sum + four};
       *reinterpret_cast<float4*>(sums + s * NV + j) = q;
+      sum = q.w;
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -310,6 +337,7 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
     near = !(least <= target - too_near && most > target + too_near) || label >= n;
     return label;
   };
+  bool unsure = false;
   bool ready = false;  // whether the sums in LDS are those that labels are drawn from
   float left = 0;
   for (int base = 0; base < p.n_drafts; base += S) {
@@ -327,12 +355,12 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
     const float p_d = has_p ? __builtin_amdgcn_exp2f(far_a) : 0.f;
     const float q_d = !has_q ? 0.f : COSTS ? __builtin_amdgcn_exp2f(far_b) * to_target : wa.total;
     const float u0 = positive(d.u0) ? (d.u0 < 1.f ? d.u0 : 1.f) : 0.f, u1 = positive(d.u1) ? (d.u1 < 2.f ? d.u1 : 2.f) : 0.f;
-    const float least = u0 * q_d, off = (64 + 2 * (NV + S) - 3 * (far_a < far_b ? far_a : far_b)) * kU;
+    const float least = u0 * q_d, off = (64 + 2 * kSteps - 3 * (far_a < far_b ? far_a : far_b)) * kU;
     const bool kept = has_q && least < p_d;
     bool near = has_q && (q_d < kLeast || fabsf(least - p_d) <= off * (least + p_d) + kLeast || (positive(d.u0) && d.u0 > 1.f));
     int label = d.label;
     // what the draft leaves, or all of p
-    const bool draws = mine && !empty && !kept && !near;
+    const bool draws = mine && !empty && !kept && !near && !blind;
     const bool draws_left = draws && (has_q || !COSTS), draws_all = draws && !has_q && COSTS;
     if (__builtin_amdgcn_ballot_w64(draws_left) != 0) {
       if (!ready) left = sum_up(COSTS ? b : a);
@@ -351,21 +379,25 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
       label = draws_all ? drawn : label;
       near |= draws_all && close;
     }
-    unsure |= near && mine;
-    if (mine && (empty || !unsure)) {
+    if (mine && !empty && (near || blind)) {
+      atomicOr(&asked[px], 1u << ((base + s) % 32));
+      unsure = true;
+    } else if (mine) {
       p.labels[d.place] = (uint8_t)(empty ? 0 : label);
       p.kept[d.place] = kept && !empty ? 1 : 0;
     }
   }
-  unsure = lanes_max<S>(unsure ? 1 : 0) != 0 && !empty && px < count;
+  unsure = lanes_max<S>(unsure ? 1 : 0) != 0;
   const auto exactly = [&](int of) {
     const int64_t from = first + (LAST ? (p0 + of) * n : p0 + of);
     verify_exactly<COSTS>(
-        p, image, item * p.t.pixels + p0 + of, [&](int l) { return p.cost[from + l * step]; },
+        p, image, item * p.t.pixels + p0 + of, (uint32_t)uniform_i((int)asked[of]), [&](int l) { return p.cost[from + l * step]; },
         [&](int l) { return p.draft_cost[from + l * step]; });
   };
   if (S == 1) {
     // (one wavefront)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     for (uint64_t rest = __builtin_amdgcn_ballot_w64(unsure); rest != 0; rest &= rest - 1) exactly(__builtin_ctzll(rest));
   } else {
     if (unsure && s == 0) atomicOr(&left_over[px >> 5], 1u << (px & 31));
