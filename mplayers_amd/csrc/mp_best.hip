@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
   {
     LaneLoads<NV, S, LAST, T> loads;
     loads.load((const T*)p.cost + item * p.t.n * p.t.pixels, p.t, p0, count, p.quads, tid);
-    loads.template to_tile<true>(tile, p.t, count, p.quads, tid);
+    loads.to_tile(tile, p.t, count, p.quads, tid);
   }
   __syncthreads();
   // quad g of this lane is at own[g * 4 * S]; nobody else reads or writes it from here on

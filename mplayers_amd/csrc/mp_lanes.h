@@ -191,13 +191,12 @@ struct LaneLoads {
           c[4 * i + j] = cost[(int64_t)min(4 * (wave + i * S) + j, n - 1) * t.pixels + p0 + of];
     }
   }
-  // CLEAN: what is no candidate as +inf, labels behind the last too.
-  template <bool CLEAN = false>
+  // What is no candidate goes there as +inf, and what lies behind the last label too.
   __device__ __forceinline__ void to_tile(float* tile, const LaneTiles& t, int count, bool quads, int tid) const {
     using Tile = LaneTile<NV, S>;
     constexpr int kJ = NV / 4, kThreads = kLanePixels * S;
-    const auto cost = [&](int k) { return CLEAN ? candidate((float)c[k]) : (float)c[k]; };
-    if (CLEAN && LAST) {
+    const auto cost = [&](int k) { return candidate((float)c[k]); };
+    if (LAST) {
       for (int l = t.n + tid % S; l < S * NV; l += S) tile[tid / S * Tile::kStride + Tile::place(l >> 2) + (l & 3)] = kInf;
     }
     if (LAST) {
@@ -224,7 +223,7 @@ struct LaneLoads {
       for (int i = 0; i < kJ; ++i) {
         const int l = 4 * (wave + i * S);
         float4* const to = reinterpret_cast<float4*>(&tile[tid % kLanePixels * Tile::kStride + Tile::place(wave + i * S)]);
-        if (!CLEAN || l + 3 < t.n) {
+        if (l + 3 < t.n) {
           *to = float4{cost(4 * i), cost(4 * i + 1), cost(4 * i + 2), cost(4 * i + 3)};
         } else {
           const auto of = [&](int j) { return l + j < t.n ? cost(4 * i + j) : kInf; };

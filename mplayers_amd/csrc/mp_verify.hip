@@ -274,12 +274,12 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
     target.load(p.cost + first, p.t, p0, count, p.quads, tid);
     if (COSTS) draft.load(p.draft_cost + first, p.t, p0, count, p.quads, tid);
     fetch_costs(d);
-    target.template to_tile<true>(tile, p.t, count, p.quads, tid);
+    target.to_tile(tile, p.t, count, p.quads, tid);
     __syncthreads();
     from_lane_tile<NV, S>(tile, px, s, a);
     if (COSTS) {
       __syncthreads();
-      draft.template to_tile<true>(tile, p.t, count, p.quads, tid);
+      draft.to_tile(tile, p.t, count, p.quads, tid);
       __syncthreads();
       from_lane_tile<NV, S>(tile, px, s, b);
     }
