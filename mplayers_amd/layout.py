@@ -110,5 +110,12 @@ def labels_last_norm(x, weight=None, bias=None, eps=1e-5, labels_first=True):
   An infinite cost or NaN makes its pixel's results NaN.  CPU tensors go through torch."""
   if x.is_cuda:
     return _lib.autograd().labels_last_norm(x, weight, bias, eps, labels_first)
+  if x.dim() != 5 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    raise RuntimeError("labels_last_norm: x must be a (batch, cv, labels, H, W) or (batch, cv, H, W, labels) float32, float16 or "
+                       "bfloat16 tensor, got %s of %d axes" % (x.dtype, x.dim()))
   x = (x.movedim(2, -1) if labels_first else x).float()
+  if not 1 <= x.size(-1) <= 256:
+    raise RuntimeError("labels_last_norm: 1 to 256 labels, got %d" % x.size(-1))
+  if not 0 <= eps < float("inf"):
+    raise RuntimeError("labels_last_norm: eps must be finite and not below 0, got %r" % eps)
   return torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps).contiguous()

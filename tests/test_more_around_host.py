@@ -85,6 +85,11 @@ def test_norm_of_cpu_tensors(dtype):
   assert torch.equal(labels_last_norm(x.movedim(2, -1), w, b, 1e-3, labels_first=False), y)
   dx, dw = torch.autograd.grad(y.sum(), (x, w))
   assert dx.shape == x.shape and dx.dtype == dtype and dw.shape == (6,)
+  for wrong in (dict(x=x[0]), dict(x=x.double()), dict(eps=-1.0), dict(eps=math.nan), dict(eps=math.inf), dict(weight=w[:5]),
+                dict(labels_first=False), dict(x=torch.zeros(1, 1, 257, 2, 2), weight=None, bias=None),
+                dict(x=torch.zeros(1, 1, 0, 2, 2), weight=None, bias=None)):
+    with pytest.raises(RuntimeError):
+      labels_last_norm(**{**dict(x=x, weight=w, bias=b), **wrong})
 
 
 @pytest.mark.parametrize("soft", [False, True])
