@@ -53,6 +53,12 @@ struct Mass {
 __device__ __forceinline__ float weight(float least, float c, float to_exponent) {
   return c == kInf ? 0.f : __builtin_amdgcn_exp2f((least - c) * to_exponent);
 }
+// The least of three numbers, of those that are numbers; one instruction (and comparisons that may meet NaN are two each).
+__device__ __forceinline__ float least_of(float a, float b, float c) {
+  float least;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(least) : "v"(a), "v"(b), "v"(c));
+  return least;
+}
 // Those of the W wavefronts of a tile.
 template <int W>
 __device__ __forceinline__ Mass join(Mass own, float2 (*part)[kTilePixels], int w, int lane, float to_exponent) {
@@ -73,8 +79,9 @@ __device__ __forceinline__ Mass join(Mass own, float2 (*part)[kTilePixels], int 
 
 constexpr float kFaint = 0x1p-60f;  // others that weigh less than this beside the best label: see distill_kernel
 
+// (Up to 24 labels to a wavefront in 128 registers, so that two workgroups of eight share a compute unit.)
 template <typename T, bool FIRST, bool GRAD, int W, int I, int G>
-__global__ void __launch_bounds__(64 * W * G) distill_kernel(Distill p) {
+__global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Distill p) {
   constexpr int kStride = tile_stride(W * I), kShift = W == 1 ? 0 : W == 2 ? 1 : W == 4 ? 2 : 3, kParts = W > 1 ? W : 1;
   __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
   __shared__ float2 part[2][kParts][kTilePixels];
@@ -126,14 +133,14 @@ __global__ void __launch_bounds__(64 * W * G) distill_kernel(Distill p) {
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      c[i][j] = 4 * (w + i * W) + j < n ? c[i][j] : kInf;
-      least = c[i][j] < least ? c[i][j] : least;
-    }
+    for (int j = 0; j < 4; ++j) c[i][j] = 4 * (w + i * W) + j < n ? c[i][j] : kInf;
+#pragma unroll
+  for (int i = 0; i < I; ++i) least = least_of(c[i][2], c[i][3], least_of(c[i][0], c[i][1], least));
+  const float beside_least = least == kInf ? 0.f : least;  // (+inf weighs nothing beside any number)
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum += a[i][j] = weight(least, c[i][j], p.to_exponent);
+    for (int j = 0; j < 4; ++j) sum += a[i][j] = __builtin_amdgcn_exp2f((beside_least - c[i][j]) * p.to_exponent);
   if (W > 1) {
     named_by[w][lane] = 0;
     if (tid == 0) twice = 0;
