@@ -7,7 +7,8 @@
 // The costs are read once, a pixel's labels over S lanes (mp_lanes.h), and stay in LDS; a lane has the least cost of each quad of
 // its labels in registers.  A place of the list is the least of those over the lanes: the first lane that has it looks its
 // quad up, takes the label out and finds the quad's next.  So a place costs the instructions of the quads and not of the
-// labels, and no sort is needed.
+// labels, and no sort is needed.  us: 96 labels 384x1248, lists of 8, 53 (3.9 TB/s; label by label 83), about 800
+// instructions to a wavefront of 16 pixels, 0.8 of the time; 21 labels 12x129x129, lists of 4, 8.8; 192 labels 377x501, lists of 32, 109, bound by the instructions.
 
 #include "mp_lanes.h"
 
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
       const float4 q = quad(g);
       const float c[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += c[j] < kInf ? __builtin_amdgcn_exp2f((m - c[j]) * p.to_exponent) : 0.f;
+      for (int j = 0; j < 4; ++j) sum += __builtin_amdgcn_exp2f((m - c[j]) * p.to_exponent);  // (0 of +inf beside a number)
     }
     sum = lanes_sum<S>(sum);
     if (s == 0 && px < count) p.rest[item * p.t.pixels + p0 + px] = m < kInf ? (m - best) - p.temperature * logf(sum) : kInf;

@@ -38,6 +38,12 @@ __device__ __forceinline__ double exp2_64(double y) {
   e = fma(e, x, 1.0);
   return ldexp(e, (int)whole);
 }
+// The same in two instructions (the library is compiled for code without NaNs, where a comparison cannot tell one).
+__device__ __forceinline__ float candidate_of(float c) {
+  float out;
+  asm("v_cmp_u_f32 vcc, %1, %1\n\tv_cndmask_b32 %0, %1, %2, vcc" : "=v"(out) : "v"(c), "v"(kInf) : "vcc");
+  return out;
+}
 // x > 0 and a number
 __device__ __forceinline__ bool positive(float x) {
   const int bits = __builtin_bit_cast(int, x);
@@ -195,7 +201,7 @@ struct LaneLoads {
   __device__ __forceinline__ void to_tile(float* tile, const LaneTiles& t, int count, bool quads, int tid) const {
     using Tile = LaneTile<NV, S>;
     constexpr int kJ = NV / 4, kThreads = kLanePixels * S;
-    const auto cost = [&](int k) { return candidate((float)c[k]); };
+    const auto cost = [&](int k) { return candidate_of((float)c[k]); };
     if (LAST) {
       for (int l = t.n + tid % S; l < S * NV; l += S) tile[tid / S * Tile::kStride + Tile::place(l >> 2) + (l & 3)] = kInf;
     }

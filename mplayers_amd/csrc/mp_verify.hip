@@ -5,6 +5,12 @@
 // what the draft leaves, max(p - q, 0): the first whose running sum, in label order, exceeds u1 * (sum of all).  A label drawn from
 // q then is one of p, and is the drafted one as often as any way of drawing it can have it.  Where q[d] is 0 or there is no
 // label d nothing was drafted, and one is drawn from p.
+//
+// Either volume is read once: a pixel's labels lie in the registers of one to eight lanes (mp_lanes.h), p and q are formed there, and
+// the running sums go to LDS only in wavefronts where a label is drawn anew.  Results are those of 64 bits, which 32 bits give but
+// for drafts next to a border (see verify_kernel).  Bound by HBM for one draft: us, 192 labels 1500x2000 1050 (4.4 TB/s; with 64 bits
+// throughout 15 300), 60 labels 1000x2000 184 (5.3 TB/s); 60 labels 375x450 in the operators' layout, 8 drafts, 37 by the
+// instructions (980 to a wavefront of 16 pixels) and the last wavefronts, which have the drafts that go to 64 bits: 31 without those.
 
 #include "mp_lanes.h"
 
@@ -229,8 +235,8 @@ __device__ __forceinline__ Weights weights32(float (&v)[NV], const Scale& scale,
 //   a running sum of max(a - b A / B, 0): both of these, a rounding each, the additions of what lies before the lane and of the
 //             lane's fours to it: (79 + 2 H + NV / 2 + 3 + S) u
 // and as much for a target, which is a product with such a sum.  Where a target is as close to a sum as both (kNear), 32 bits
-// do not tell, and verify_exactly() takes the draft: with costs as a layer gives them one in 700 of 192 labels, one in 5000 of
-// 21.  So it does where u0 q[d] is as close to p[d] as (3 x + 64 + 2 H) u of either, x being their exponents.
+// do not tell, and verify_exactly() takes the draft: with costs as a layer gives them and a draft of which a sixth is rejected one
+// draft in 490 of 192 labels, in 1300 of 60, in 3700 of 21.  So it does where u0 q[d] is as close to p[d] as (3 x + 64 + 2 H) u of either, x being their exponents.
 template <int NV, int S, bool COSTS, bool LAST>
 __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   using Tile = LaneTile<NV, S>;
@@ -408,6 +414,9 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   }
 }
 
+// Labels per lane and lanes per pixel.  us, one draft but where said, fewer lanes / this / more: 60 labels 375x450 26.2 / 23.1 / 29.5,
+// 8 drafts 41.9 / 32.6 / 39.0, 60 labels 1000x2000 185 / 184 / 288; 21 labels 129x1548 15.9 / 14.6 / 18.3, 600x2000 49 / 51 / 74; 96
+// labels 384x1248 101 / 79 / 90.
 template <bool COSTS, bool LAST>
 void launch(const Verify& p, unsigned blocks, hipStream_t st) {
   const int n = p.t.n;
