@@ -174,15 +174,16 @@ __device__ void verify_exactly(const Verify& p, int image, int64_t at, uint32_t 
 
 // A temperature as 32 bits use it.
 struct Scale {
-  float to_exponent;  // log2(e) / T
-  bool cold, far;     // T not above 0; beyond what fp32 exponents are sure of (an infinite one too)
+  float to_exponent;      // log2(e) / T
+  bool cold, flat, far;  // T not above 0; infinite; beyond what fp32 exponents are sure of
 };
 __device__ __forceinline__ Scale scale_of(const float* each, float all, int image) {
   const float t = each != nullptr ? each[image] : all;
   Scale s;
   s.cold = !positive(t);
-  s.far = !s.cold && !(t > 1e-30f && t < 1e30f);
-  s.to_exponent = s.cold ? 0.f : (float)(inverse(t) * 1.4426950408889634);
+  s.flat = t == kInf;
+  s.far = !s.cold && !s.flat && !(t > 1e-30f && t < 1e30f);
+  s.to_exponent = s.cold || s.flat ? 0.f : (float)(inverse(t) * 1.4426950408889634);
   return s;
 }
 
@@ -216,6 +217,12 @@ __device__ __forceinline__ Weights weights32(float (&v)[NV], const Scale& scale,
 #pragma unroll
     for (int j = 0; j < NV; ++j) v[j] = s * NV + j == w.first ? 1.f : 0.f;
     w.total = 1.f;
+    return w;
+  }
+  if (scale.flat) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = v[j] < kInf ? 1.f : 0.f;
+    w.total = lanes_sum<S>(tree_sum(v));
     return w;
   }
   const float best = w.best < kInf ? w.best : 0.f;
@@ -356,8 +363,8 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
     const float c = candidate(d.cost), dc = candidate(d.draft_cost);
     const bool has_p = exists && (scale.cold ? d.label == wa.first : c < kInf);
     const bool has_q = exists && (!COSTS || (draft_scale.cold ? d.label == wb.first : dc < kInf));
-    const float far_a = scale.cold || !has_p ? 0.f : (wa.best - c) * scale.to_exponent;
-    const float far_b = !COSTS || draft_scale.cold || !has_q ? 0.f : (wb.best - dc) * draft_scale.to_exponent;
+    const float far_a = scale.cold || scale.flat || !has_p ? 0.f : (wa.best - c) * scale.to_exponent;
+    const float far_b = !COSTS || draft_scale.cold || draft_scale.flat || !has_q ? 0.f : (wb.best - dc) * draft_scale.to_exponent;
     const float p_d = has_p ? __builtin_amdgcn_exp2f(far_a) : 0.f;
     const float q_d = !has_q ? 0.f : COSTS ? __builtin_amdgcn_exp2f(far_b) * to_target : wa.total;
     const float u0 = positive(d.u0) ? (d.u0 < 1.f ? d.u0 : 1.f) : 0.f, u1 = positive(d.u1) ? (d.u1 < 2.f ? d.u1 : 2.f) : 0.f;

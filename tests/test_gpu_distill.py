@@ -192,6 +192,19 @@ def test_lists(gpu, n, what):
                      torch.from_numpy(rest).float().cuda() if with_rest else None, 1.5, labels_first)
 
 
+@pytest.mark.parametrize("labels_first", [True, False])
+@pytest.mark.parametrize("n,k", [(1, 9), (5, 200), (21, 64), (40, 256), (100, 130), (200, 256)])
+def test_lists_that_are_longer_than_the_labels(gpu, n, k, labels_first):
+  """Labels named many times, and labels that there are none of between them."""
+  rng = np.random.default_rng(n + k)
+  cost, _, _, rest = _problem(n, 1, (1, 1, 2, 19), n)
+  labels = rng.integers(0, min(n + 3, 256), (1, 1, k, 2, 19)).astype(np.uint8)
+  costs = rng.random((1, 1, k, 2, 19)) * 5
+  for with_rest in (True, False):
+    _check_distill(_gpu(cost, labels_first), _gpu(labels, labels_first, torch.uint8), _gpu(costs, labels_first),
+                   torch.from_numpy(rest).float().cuda() if with_rest else None, 1.0, labels_first)
+
+
 @pytest.mark.parametrize("n", [3, 21, 50, 130])
 def test_costs_that_are_no_numbers(gpu, n):
   """NaN and infinities of either sign on either side; they stay in their pixel."""

@@ -209,6 +209,37 @@ def test_the_number_of_drafts_changes_nothing(gpu, n, labels_first):
     _same((labels, kept), oracle.verify_labels(cost, draft, u, costs))
 
 
+@pytest.mark.parametrize("with_costs", [True, False])
+@pytest.mark.parametrize("n,temperature", [(5, 1.0), (21, 1e-31), (40, 1e31), (130, 1.0), (21, INF)])
+def test_many_drafts(gpu, n, temperature, with_costs):
+  """More drafts than a wavefront has lanes, at temperatures that 32 bits leave to 64 as well; pixels at borders."""
+  rng = np.random.default_rng(n)
+  cost = np.round(rng.standard_normal((1, 1, n, 1, 9)) * 2).astype(np.float32) * np.float32(min(max(temperature, 1e-32), 1e32))
+  other = np.roll(cost, 1, 2)
+  draft = rng.integers(0, n + 1, (150, 1, 1, 1, 9)).astype(np.uint8)
+  u = (rng.integers(0, 16, (2,) + draft.shape) / 16).astype(np.float32)
+  costs = other if with_costs else None
+  temperatures = dict(temperature=temperature)
+  p = torch.softmax(-torch.from_numpy(cost).double().movedim(2, -1) / temperature, -1)
+  q = torch.softmax(-torch.from_numpy(other).double().movedim(2, -1) / temperature, -1) if with_costs else None
+  got, want = _verify(cost, draft, u, costs, **temperatures), oracle.verify_labels(cost, draft, u, costs, **temperatures)
+  # (uniform numbers of four bits: a target may be a sum exactly, where 64 bits go by the order of their additions)
+  told = np.ones(draft.shape, bool)
+  d = torch.from_numpy(draft).long()
+  p_d = p.expand(draft.shape + (n,)).gather(-1, d.clamp(max=n - 1)[..., None])[..., 0]
+  q_d = torch.ones_like(p_d) if q is None else q.expand(draft.shape + (n,)).gather(-1, d.clamp(max=n - 1)[..., None])[..., 0]
+  u0, u1 = torch.from_numpy(u[0]).double(), torch.from_numpy(u[1]).double()
+  told &= ((u0 * q_d - p_d).abs() > 1e-12).numpy()
+  left = (p - q).clamp(min=0).expand(draft.shape + (n,)) if with_costs else \
+      torch.where(torch.arange(n) == d[..., None], 0.0, p.expand(draft.shape + (n,)))
+  for weights in (left, p.expand(draft.shape + (n,))):
+    sums = weights.cumsum(-1)
+    told &= (((sums - u1[..., None] * sums[..., -1:]).abs().amin(-1) > 1e-12) | (sums[..., -1] == 0)).numpy()
+  assert told.mean() > 0.3
+  for g, w in zip(got, want):
+    assert np.array_equal(g[told], w[told])
+
+
 @pytest.mark.parametrize("n", [21, 24, 60, 192])
 def test_alignment(gpu, n):
   from mplayers_amd import verify_labels
