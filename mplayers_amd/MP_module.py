@@ -238,7 +238,8 @@ class MPModule(torch.nn.Module):
     self.args.enable_min_a_dir = enable_min_a_dir
     self.args.enable_sgm = args.mpnet_mrf_mode == 'SGM'
     self.args.enable_seg = True if (args.n_classes == 21) else False
-    if getattr(args, "mpnet_unary_norm", False):
+    self.unary_norm = bool(getattr(args, "mpnet_unary_norm", False))
+    if self.unary_norm:
       like = dict(device="cuda" if getattr(args, "enable_cuda", False) else "cpu")
       self.unary_norm_weight = torch.nn.Parameter(torch.ones(args.n_classes, **like))
       self.unary_norm_bias = torch.nn.Parameter(torch.zeros(args.n_classes, **like))
@@ -386,7 +387,7 @@ class MPModule(torch.nn.Module):
     """The unary costs in the kernels' layout, in training mode with the dropout that args asks for, and normalised if it
     asks for that."""
     rate = getattr(self.args, "mpnet_unary_dropout", None)
-    norm = getattr(self, "unary_norm_weight", None) is not None
+    norm = self.__dict__.get("unary_norm", False)  # (modules of files written before there was one have none)
     if rate and self.training:
       # (from torch's generator: it follows manual_seed, and a captured call has a new mask at every replay)
       state = torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), device=unary.device)

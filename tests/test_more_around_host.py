@@ -114,6 +114,17 @@ def test_a_module_that_normalises(soft):
   for off in (dict(), dict(mpnet_unary_norm=False), dict(mpnet_unary_norm=None)):
     plain = kind(_args(**fields, **off), enable_create_label_context=True)
     assert set(plain.state_dict()) == {"label_context"} and torch.equal(plain._labels_last(x), x.permute(0, 1, 3, 4, 2))
+  # copies, files, weights that are made of others, and modules of files from before
+  import copy
+  import pickle
+  for other in (copy.deepcopy(module), pickle.loads(pickle.dumps(module))):
+    assert torch.equal(other._labels_last(x), want)
+  double = copy.deepcopy(module)
+  torch.nn.utils.parametrize.register_parametrization(double, "unary_norm_weight", torch.nn.Softplus())
+  assert torch.equal(double._labels_last(x), labels_last_norm(x, torch.nn.functional.softplus(module.unary_norm_weight),
+                                                              module.unary_norm_bias, 1e-2))
+  del plain.__dict__["unary_norm"]
+  assert torch.equal(plain._labels_last(x), x.permute(0, 1, 3, 4, 2))
   # in evaluation a rate of dropout changes nothing
   dropped = kind(_args(mpnet_unary_norm=True, mpnet_unary_norm_eps=1e-2, mpnet_unary_dropout=0.5, **fields),
                  enable_create_label_context=True).eval()
