@@ -339,17 +339,18 @@ int mpl_dropout_labels_first(int dtype, int share, double rate, const int64_t* s
  * the reference.  src of `dtype` (MPL_F32, ...), (batch, n_disp, pixels) with labels_first, else (batch, pixels, n_disp)
  * -> dst (batch, pixels, n_disp) fp32 = (src - mean) * r * weight[label] + bias[label], r = 1 / sqrt(var + eps), mean and
  * var (of the n_disp values, not n_disp - 1) of the pixel's labels.  weight, bias: n_disp floats or NULL (1, 0); eps
- * finite and >= 0.  stats: NULL, or 2 floats per pixel for the gradient (mean, r).  Everything is formed in fp32.  A cost that
- * is infinite or NaN makes its pixel's results NaN; so does a pixel whose labels all have the same cost at an eps of 0.
- * mpl_norm_labels_last_grad: from ddst (as dst) and the src, weight and stats of that call
+ * finite and >= 0.  stats: NULL, or mpl_norm_stats(n_disp) floats per pixel that the gradient takes (where that is 0, NULL to
+ * both).  Everything is formed in fp32.  A cost that is infinite or NaN makes its pixel's results NaN; so does a pixel whose labels all have the same cost at an eps of 0.
+ * mpl_norm_labels_last_grad: from ddst (as dst) and the src, weight, eps and stats of that call
  *   dsrc = r * (g - mean(g) - xhat * mean(g * xhat)), g = ddst * weight, xhat = (src - mean) * r, in src's layout and type,
  *   dweight[label] = the sum over pixels of ddst * xhat, dbias[label] = the sum over pixels of ddst,
  * each NULL where it is not wanted.  dweight and dbias need a workspace of mpl_norm_workspace() floats (0 for nothing to
  * sum); they are summed in a fixed order, so the same call gives the same bits.  At most MPL_MAX_LABELS labels. */
 int mpl_norm_labels_last(int dtype, int labels_first, const void* src, const float* weight, const float* bias, float eps,
                          float* dst, float* stats, int batch, int n_disp, int64_t pixels, void* stream);
-int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, const float* weight, const float* stats,
-                              const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace, int batch,
+int mpl_norm_stats(int n_disp);
+int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, const float* weight, float eps,
+                              const float* stats, const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace, int batch,
                               int n_disp, int64_t pixels, void* stream);
 int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels);
 

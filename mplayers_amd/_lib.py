@@ -13,8 +13,8 @@ SYMBOLS = ("mpl_trwp_forward", "mpl_trwp_backward", "mpl_isgmr_forward", "mpl_is
            "mpl_trwp_soft_backward", "mpl_soft_weighted_message", "mpl_soft_weighted_message_back", "mpl_set_option",
            "mpl_stereo_data_cost", "mpl_gradient_cues", "mpl_mrf_energy", "mpl_transpose",
            "mpl_dropout_labels_last", "mpl_dropout_labels_first", "mpl_bucket_context", "mpl_bucket_sums",
-           "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace",
-           "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_verify_labels")
+           "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace", "mpl_norm_stats",
+           "mpl_norm_stats", "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_verify_labels")
 
 KERNEL_KINDS = ("fwd_sweep", "bwd_sweep", "belief", "aggregate", "label", "combine", "other",
                 "fwd_sweep_all", "bwd_sweep_all", "unary_all")
@@ -83,7 +83,8 @@ def load():
   lib.mpl_bucket_sums.argtypes = [vp, vp, ci, ci, ci, ci, vp, vp]
   lib.mpl_sample_labels.argtypes = [ci, vp, vp, ci, ci, ci, i64, ci, vp, cf, vp, ci, vp, cf, vp, cf, vp, vp]
   lib.mpl_norm_labels_last.argtypes = [ci, ci, vp, vp, vp, cf, vp, vp, ci, ci, i64, vp]
-  lib.mpl_norm_labels_last_grad.argtypes = [ci, ci] + [vp] * 8 + [ci, ci, i64, vp]
+  lib.mpl_norm_labels_last_grad.argtypes = [ci, ci, vp, vp, cf] + [vp] * 6 + [ci, ci, i64, vp]
+  lib.mpl_norm_stats.argtypes = [ci]
   lib.mpl_norm_workspace.argtypes = [ci, ci, i64]
   lib.mpl_best_labels.argtypes = [ci, ci, vp, ci, cf, ci, vp, vp, vp, ci, ci, i64, vp]
   lib.mpl_distill_costs.argtypes = [ci, ci, vp, ci, vp, vp, vp, cf, vp, ci, ci, ci, i64, vp]
@@ -177,7 +178,7 @@ def autograd():
     # (in the order of its EntryPoints)
     module.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
                  ("mpl_bucket_context", "mpl_bucket_sums", "mpl_dropout_labels_last", "mpl_dropout_labels_first",
-                  "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace",
+                  "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace", "mpl_norm_stats",
                   "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_verify_labels", "mpl_last_error")])
     _autograd = module
   return _autograd

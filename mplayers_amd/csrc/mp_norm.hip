@@ -7,8 +7,8 @@
 //   dbias[l] = sum over pixels of dy[l].
 //
 // The variance is that of the differences from the mean, in registers: each wavefront's own labels first, and those of
-// the W wavefronts of a tile joined as sum(M2_w + n_w * (mean_w - mean)^2).  mean and r are kept for the gradient, 8 bytes a
-// pixel.
+// the W wavefronts of a tile joined as sum(M2_w + n_w * (mean_w - mean)^2).  They are kept for the gradient, 8 bytes a pixel, from
+// 17 labels on; of fewer it forms them again from x, which it reads in any case.
 //
 // Bound by HBM: a pixel's labels are read once, and the change of layout is one that the layer makes anyway.  The sums over
 // pixels stay in registers while a workgroup goes from tile to tile: a fp32 sum for each lane and label, then over the 64
@@ -22,6 +22,10 @@ using namespace mpl;
 
 namespace {
 
+// Labels up to which the gradient forms mean and r again.  us for 64 M costs, forward / gradient, kept -> formed again: 2 labels 223 /
+// 213 -> 175 / 160, 8: 94 / 165 -> 87 / 152, 16: 91 / 167 -> 87 / 166, 40: 92 / 178 -> 88 / 188, 128: 90 / 171 -> 89 / 184 (their
+// registers and instructions); 192 labels 1500x2000 864 / 1405 -> 848 / 1507.
+constexpr int kFormedAgain = 16;
 constexpr unsigned kSumRows = 2048;  // workgroups of a gradient, at most
 
 struct Norm {
@@ -30,7 +34,7 @@ struct Norm {
   const float* weight;  // or nullptr: 1
   const float* bias;    // or nullptr: 0
   float* y;
-  float* stats;  // mean and r of each pixel
+  float* stats;  // mean and r of each pixel, or nullptr
   const float* dy;
   void* dx;      // or nullptr
   float* sums;   // of each workgroup: dweight, dbias
@@ -47,12 +51,52 @@ __device__ __forceinline__ int labels_of(int w, int n) {
   return count;
 }
 
+// Mean and squared differences from it of this wavefront's labels of a pixel,
+template <int W, int I>
+__device__ __forceinline__ float2 own_moments(const float (&x)[I][4], int w, int n) {
+  const auto is = [&](int i, int j) { return 4 * (w + i * W) + j < n; };
+  float sum = 0, m2 = 0;
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += is(i, j) ? x[i][j] : 0.f;
+  const int here = labels_of<W, I>(w, n);
+  const float mean = here > 0 ? sum / (float)here : 0.f;
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = is(i, j) ? x[i][j] - mean : 0.f;
+      m2 += d * d;
+    }
+  return float2{mean, m2};
+}
+// and the mean and r of the pixel from those of all W.
+template <int W, int I>
+__device__ __forceinline__ float2 join_moments(const float2 (*part)[kTilePixels], int lane, int n, float eps) {
+  const float labels = (float)n;
+  float2 of_wave[W];
+  float sum = 0, m2 = 0;
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    of_wave[k] = part[k][lane];
+    sum += of_wave[k].x * (float)labels_of<W, I>(k, n);
+  }
+  const float mean = W > 1 ? sum / labels : of_wave[0].x;
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    const float d = of_wave[k].x - mean;
+    m2 += W > 1 ? of_wave[k].y + (float)labels_of<W, I>(k, n) * d * d : of_wave[k].y;
+  }
+  return float2{mean, 1.f / sqrtf(m2 / labels + eps)};
+}
+
 template <typename T, bool FIRST, int W, int I, int G>
 __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
   constexpr int kStride = tile_stride(W * I);
   __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
   __shared__ __align__(16) float affine[2][4 * W * I];
-  __shared__ float2 part[W > 1 ? W : 1][kTilePixels];
+  __shared__ float2 part[W * G][kTilePixels];
   const int tid = (int)threadIdx.x % (64 * W), group = uniform_i((int)threadIdx.x / (64 * W));
   const int lane = tid % 64, w = uniform_i(tid / 64), n = p.t.labels;
   const unsigned at = (unsigned)xcd_block((int)blockIdx.x, (int)gridDim.x, p.t.xcd_group) * G + group;
@@ -82,49 +126,18 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
   __syncthreads();
   if (!work) return;
   if (!FIRST) from_tile<W, I>(mine, w, x);
-  const auto is = [&](int i, int j) { return 4 * (w + i * W) + j < n; };
-  const float labels = (float)n;
-  float sum = 0;
-#pragma unroll
-  for (int i = 0; i < I; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum += is(i, j) ? x[i][j] : 0.f;
-  const int here = labels_of<W, I>(w, n);
-  float mean = here > 0 ? sum / (float)here : 0.f, m2 = 0;
-#pragma unroll
-  for (int i = 0; i < I; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float d = is(i, j) ? x[i][j] - mean : 0.f;
-      m2 += d * d;
-    }
-  if (W > 1) {
-    part[w][lane] = float2{mean, m2};
-    tile_sync<W>();
-    float2 of_wave[W];
-    sum = 0;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      of_wave[k] = part[k][lane];
-      sum += of_wave[k].x * (float)labels_of<W, I>(k, n);
-    }
-    mean = sum / labels;
-    m2 = 0;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      const float d = of_wave[k].x - mean;
-      m2 += of_wave[k].y + (float)labels_of<W, I>(k, n) * d * d;
-    }
-  }
-  const float r = 1.f / sqrtf(m2 / labels + p.eps);
+  float2* const mine_of = &part[group + w][lane];
+  *mine_of = own_moments<W, I>(x, w, n);
+  if (W > 1) tile_sync<W>();
+  const float2 of_pixel = join_moments<W, I>(part + group, lane, n, p.eps);
   if (p.stats != nullptr && w == 0 && lane < count)
-    reinterpret_cast<float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + lane] = float2{mean, r};
+    reinterpret_cast<float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + lane] = of_pixel;
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int l = 4 * (w + i * W) + j;
-      x[i][j] = (x[i][j] - mean) * r * affine[0][l] + affine[1][l];
+      x[i][j] = (x[i][j] - of_pixel.x) * of_pixel.y * affine[0][l] + affine[1][l];
     }
   to_tile<W, I>(mine, w, x);
   tile_sync<W>();
@@ -137,7 +150,9 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
   constexpr int kStride = tile_stride(W * I);
   __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
   __shared__ __align__(16) float weight[4 * W * I];
-  __shared__ float2 part[W > 1 ? W : 1][kTilePixels];
+  __shared__ float2 part[W * G][kTilePixels];
+  constexpr bool kAgain = 4 * W * I <= kFormedAgain;
+  __shared__ float2 moments[kAgain ? W * G : 1][kTilePixels];
   const int tid = (int)threadIdx.x % (64 * W), group = uniform_i((int)threadIdx.x / (64 * W));
   const int lane = tid % 64, w = uniform_i(tid / 64), n = p.t.labels;
   float* const tile = tiles + group * kTilePixels * kStride;
@@ -158,7 +173,8 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
     float x[I][4], d[I][4];
     Run<I, float> dy;
     load_run<W, I>(p.dy + run, total, p.y_quads, tid, dy);
-    const float2 stats = reinterpret_cast<const float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + of];
+    float2 of_pixel;
+    if (!kAgain) of_pixel = reinterpret_cast<const float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + of];
     if (FIRST) {
       load_rows<W, I>((const T*)p.x + first + p0, p.t, w, of, x);
     } else {
@@ -169,9 +185,11 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
       from_tile<W, I>(mine, w, x);
       tile_sync<W>();
     }
+    if (kAgain) moments[group + w][lane] = own_moments<W, I>(x, w, n);
     run_to_tile<W, I>(dy, total, p.y_quads, tid, p.t, tile);
     tile_sync<W>();
     from_tile<W, I>(mine, w, d);
+    if (kAgain) of_pixel = join_moments<W, I>(moments + group, lane, n, p.eps);
     float s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < I; ++i)
@@ -181,7 +199,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
         // (behind the last label or pixel of a tile in LDS lies an earlier one's, or no number at all)
         const bool in = l < n && lane < count;
         d[i][j] = in ? d[i][j] : 0.f;
-        x[i][j] = in ? (x[i][j] - stats.x) * stats.y : 0.f;
+        x[i][j] = in ? (x[i][j] - of_pixel.x) * of_pixel.y : 0.f;
         if (SUMS) {
           dw[i][j] += d[i][j] * x[i][j];
           db[i][j] += d[i][j];
@@ -207,7 +225,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
 #pragma unroll
       for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = stats.y * (d[i][j] - s1 - x[i][j] * s2);
+        for (int j = 0; j < 4; ++j) x[i][j] = of_pixel.y * (d[i][j] - s1 - x[i][j] * s2);
       if (FIRST) {
         if (lane < count) store_rows<W, I>((T*)p.dx + first + p0, p.t, w, lane, x);
       } else {
@@ -341,9 +359,10 @@ void with_type(int dtype, bool labels_first, F f) {
     by_layout((__bf16)0);
 }
 
-int prepare(const char* what, Norm& p, int dtype, bool labels_first, int batch, int n_disp, int64_t pixels) {
+int prepare(const char* what, Norm& p, int dtype, bool labels_first, float eps, int batch, int n_disp, int64_t pixels) {
   if (dtype < 0 || dtype > MPL_BF16) return fail(MPL_EINVAL, "%s: unknown data type %d", what, dtype);
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
+  if (!(eps >= 0 && eps < __builtin_huge_valf())) return fail(MPL_EINVAL, "%s: eps must be finite and not below 0", what);
   if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
   if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels, labels_first, dtype == MPL_F32 ? 4 : 2)) return fail(MPL_EINVAL, "%s: too many pixels", what);
   return MPL_OK;
@@ -363,19 +382,20 @@ int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels) {
   return rows * 2 * n_disp;
 }
 
+int mpl_norm_stats(int n_disp) { return n_disp > kFormedAgain ? 2 : 0; }
+
 int mpl_norm_labels_last(int dtype, int labels_first, const void* src, const float* weight, const float* bias, float eps,
                          float* dst, float* stats, int batch, int n_disp, int64_t pixels, void* stream) {
   Norm p = {};
-  const int rc = prepare("norm_labels_last", p, dtype, labels_first != 0, batch, n_disp, pixels);
+  const int rc = prepare("norm_labels_last", p, dtype, labels_first != 0, eps, batch, n_disp, pixels);
   if (rc != MPL_OK) return rc;
-  if (!(eps >= 0 && eps < __builtin_huge_valf())) return fail(MPL_EINVAL, "norm_labels_last: eps must be finite and not below 0");
   if (batch == 0 || pixels == 0) return MPL_OK;
   if (src == nullptr || dst == nullptr) return fail(MPL_EINVAL, "norm_labels_last: null pointer");
   p.x = src;
   p.weight = weight;
   p.bias = bias;
   p.y = dst;
-  p.stats = stats;
+  p.stats = n_disp > kFormedAgain ? stats : nullptr;
   p.eps = eps;
   p.x_quads = whole_quads(src, n_disp, dtype);
   p.y_quads = whole_quads(dst, n_disp, MPL_F32);
@@ -383,11 +403,11 @@ int mpl_norm_labels_last(int dtype, int labels_first, const void* src, const flo
   return status("norm_labels_last");
 }
 
-int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, const float* weight, const float* stats,
-                              const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace, int batch, int n_disp,
+int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, const float* weight, float eps,
+                              const float* stats, const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace, int batch, int n_disp,
                               int64_t pixels, void* stream) {
   Norm p = {};
-  const int rc = prepare("norm_labels_last_grad", p, dtype, labels_first != 0, batch, n_disp, pixels);
+  const int rc = prepare("norm_labels_last_grad", p, dtype, labels_first != 0, eps, batch, n_disp, pixels);
   if (rc != MPL_OK) return rc;
   const bool sums = dweight != nullptr || dbias != nullptr;
   if (batch == 0 || pixels == 0) {
@@ -395,11 +415,12 @@ int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, cons
     if (sums) norm_sums_kernel<<<(2 * n_disp + 15) / 16, 1024, 0, (hipStream_t)stream>>>(nullptr, 0, n_disp, dweight, dbias);
     return sums ? status("norm_labels_last_grad") : MPL_OK;
   }
-  if (src == nullptr || stats == nullptr || ddst == nullptr || (sums && workspace == nullptr))
+  if (src == nullptr || ddst == nullptr || (stats == nullptr && n_disp > kFormedAgain) || (sums && workspace == nullptr))
     return fail(MPL_EINVAL, "norm_labels_last_grad: null pointer");
   if (dsrc == nullptr && !sums) return MPL_OK;
   p.x = src;
   p.weight = weight;
+  p.eps = eps;
   p.stats = const_cast<float*>(stats);
   p.dy = ddst;
   p.dx = dsrc;

@@ -243,7 +243,8 @@ __device__ __forceinline__ Weights weights32(float (&v)[NV], const Scale& scale,
 //             lane's fours to it: (79 + 2 H + NV / 2 + 3 + S) u
 // and as much for a target, which is a product with such a sum.  Where a target is as close to a sum as both (kNear), 32 bits
 // do not tell, and verify_exactly() takes the draft: with costs as a layer gives them and a draft of which a sixth is rejected one
-// draft in 490 of 192 labels, in 1300 of 60, in 3700 of 21.  So it does where u0 q[d] is as close to p[d] as (3 x + 64 + 2 H) u of either, x being their exponents.
+// draft in 490 of 192 labels, in 1300 of 60, in 3700 of 21.  So it does where u0 q[d] is as close to p[d] as (3 x + 64 + 2 H) u of
+// either, x being their exponents.
 template <int NV, int S, bool COSTS, bool LAST>
 __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   using Tile = LaneTile<NV, S>;

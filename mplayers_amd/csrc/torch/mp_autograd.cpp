@@ -31,6 +31,7 @@ struct EntryPoints {
   decltype(&mpl_norm_labels_last) norm_labels_last;
   decltype(&mpl_norm_labels_last_grad) norm_labels_last_grad;
   decltype(&mpl_norm_workspace) norm_workspace;
+  decltype(&mpl_norm_stats) norm_stats;
   decltype(&mpl_best_labels) best_labels;
   decltype(&mpl_distill_costs) distill_costs;
   decltype(&mpl_distill_costs_grad) distill_costs_grad;
@@ -52,6 +53,7 @@ void bind(const std::vector<uintptr_t>& at) {
   take(lib.norm_labels_last);
   take(lib.norm_labels_last_grad);
   take(lib.norm_workspace);
+  take(lib.norm_stats);
   take(lib.best_labels);
   take(lib.distill_costs);
   take(lib.distill_costs_grad);
@@ -240,13 +242,14 @@ T* or_null(const at::Tensor& t) {
 }
 void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// y, and the statistics that its gradient takes (undefined where they are not asked for)
+// y, and what its gradient takes (undefined where that is nothing, or not asked for)
 std::pair<at::Tensor, at::Tensor> norm_last(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double eps,
                                             bool labels_first, bool with_stats) {
   const Layout s(x, labels_first);
   const auto single = x.options().dtype(at::kFloat);
   at::Tensor y = at::empty({s.batch, s.cv, s.height, s.width, s.n}, single), stats;
-  if (with_stats) stats = at::empty({s.batch, s.cv, s.height, s.width, 2}, single);
+  const int kept = with_stats ? lib.norm_stats((int)s.n) : 0;
+  if (kept > 0) stats = at::empty({s.batch, s.cv, s.height, s.width, kept}, single);
   const c10::DeviceGuard guard(x.device());
   check(lib.norm_labels_last(mpl_type(x.scalar_type()), labels_first, x.data_ptr(), or_null<float>(weight), or_null<float>(bias),
                              (float)eps, y.data_ptr<float>(), or_null<float>(stats), small(s.batch * s.cv), (int)s.n, s.pixels(),
@@ -256,7 +259,7 @@ std::pair<at::Tensor, at::Tensor> norm_last(const at::Tensor& x, const at::Tenso
 }
 
 // dx, dweight, dbias, undefined where they are not asked for
-variable_list norm_grad(const at::Tensor& grad_in, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& stats,
+variable_list norm_grad(const at::Tensor& grad_in, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& stats, double eps,
                         bool labels_first, bool with_x, bool with_weight, bool with_bias) {
   const at::Tensor grad = grad_in.contiguous();
   const Layout s(x, labels_first);
@@ -267,9 +270,9 @@ variable_list norm_grad(const at::Tensor& grad_in, const at::Tensor& x, const at
   if (with_bias) dbias = at::empty({s.n}, grad.options());
   const int items = small(s.batch * s.cv);
   if (with_weight || with_bias) workspace = at::empty({lib.norm_workspace(items, (int)s.n, s.pixels())}, grad.options());
-  check(lib.norm_labels_last_grad(mpl_type(x.scalar_type()), labels_first, x.data_ptr(), or_null<float>(weight),
-                                  stats.data_ptr<float>(), grad.data_ptr<float>(), data_or_null(dx), or_null<float>(dweight),
-                                  or_null<float>(dbias), or_null<float>(workspace), items, (int)s.n, s.pixels(), stream_of(x)),
+  check(lib.norm_labels_last_grad(mpl_type(x.scalar_type()), labels_first, x.data_ptr(), or_null<float>(weight), (float)eps,
+                                  or_null<float>(stats), grad.data_ptr<float>(), data_or_null(dx), or_null<float>(dweight), or_null<float>(dbias),
+                                  or_null<float>(workspace), items, (int)s.n, s.pixels(), stream_of(x)),
         "labels_last_norm's gradient");
   return {dx, dweight, dbias};
 }
@@ -277,8 +280,10 @@ variable_list norm_grad(const at::Tensor& grad_in, const at::Tensor& x, const at
 // The gradient where it is recorded for another one, which there is none of: an error when that is asked for, not before.
 struct NormGrad : Function<NormGrad> {
   static variable_list forward(AutogradContext*, const at::Tensor& grad, const at::Tensor& x, const std::optional<at::Tensor>& weight,
-                               const at::Tensor& stats, bool labels_first, bool with_x, bool with_weight, bool with_bias) {
-    variable_list out = norm_grad(grad, x, weight.value_or(at::Tensor()), stats, labels_first, with_x, with_weight, with_bias);
+                               const std::optional<at::Tensor>& stats, double eps, bool labels_first, bool with_x, bool with_weight,
+                               bool with_bias) {
+    variable_list out = norm_grad(grad, x, weight.value_or(at::Tensor()), stats.value_or(at::Tensor()), eps, labels_first, with_x,
+                                  with_weight, with_bias);
     for (at::Tensor& t : out)
       if (!t.defined()) t = at::empty({0}, grad.options());
     return out;
@@ -297,23 +302,26 @@ struct NormLast : Function<NormLast> {
     ctx->saved_data["bias"] = bias_in.has_value();
     const auto [y, stats] = norm_last(x, weight, bias, eps, labels_first, true);
     ctx->save_for_backward({x, weight, stats});
+    ctx->saved_data["eps"] = eps;
     ctx->saved_data["labels_first"] = labels_first;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
+    const double eps = ctx->saved_data["eps"].toDouble();
     const bool labels_first = ctx->saved_data["labels_first"].toBool();
     const bool weighted = ctx->saved_data["weight"].toBool();
     const bool wanted[] = {ctx->needs_input_grad(0), weighted && ctx->needs_input_grad(1),
                            ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(weighted ? 2 : 1)};
     variable_list out;
     if (at::GradMode::is_enabled()) {
-      out = NormGrad::apply(grads[0], saved[0], weighted ? std::optional<at::Tensor>(saved[1]) : std::nullopt, saved[2],
-                            labels_first, wanted[0], wanted[1], wanted[2]);
+      out = NormGrad::apply(grads[0], saved[0], weighted ? std::optional<at::Tensor>(saved[1]) : std::nullopt,
+                            saved[2].defined() ? std::optional<at::Tensor>(saved[2]) : std::nullopt, eps, labels_first,
+                            wanted[0], wanted[1], wanted[2]);
       for (int k = 0; k < 3; ++k)
         if (!wanted[k]) out[k] = at::Tensor();
     } else {
-      out = norm_grad(grads[0], saved[0], saved[1], saved[2], labels_first, wanted[0], wanted[1], wanted[2]);
+      out = norm_grad(grads[0], saved[0], saved[1], saved[2], eps, labels_first, wanted[0], wanted[1], wanted[2]);
     }
     return {out[0], out[1], out[2], {}, {}};
   }

@@ -29,8 +29,8 @@ def test_norm_refusals(lib):
   def last(dtype=0, src=ONE, eps=1e-5, dst=ONE, batch=1, n=4, pixels=9):
     return lib.mpl_norm_labels_last(dtype, 1, src, None, None, eps, dst, None, batch, n, pixels, None)
 
-  def grad(dtype=0, src=ONE, stats=ONE, ddst=ONE, dsrc=ONE, dweight=None, workspace=None, batch=1, n=4, pixels=9):
-    return lib.mpl_norm_labels_last_grad(dtype, 1, src, None, stats, ddst, dsrc, dweight, None, workspace, batch, n, pixels, None)
+  def grad(dtype=0, src=ONE, eps=1e-5, stats=ONE, ddst=ONE, dsrc=ONE, dweight=None, workspace=None, batch=1, n=4, pixels=9):
+    return lib.mpl_norm_labels_last_grad(dtype, 1, src, None, eps, stats, ddst, dsrc, dweight, None, workspace, batch, n, pixels, None)
 
   for call in (last, grad):
     _refused(lib, call(src=None), b"null")
@@ -43,10 +43,12 @@ def test_norm_refusals(lib):
     _refused(lib, call(batch=1 << 20, pixels=1 << 30), b"too many")
     _refused(lib, call(pixels=1 << 32), b"too many")
     assert call(batch=0) == 0 and call(pixels=0) == 0
+    for eps in (-1e-9, math.nan, math.inf):
+      _refused(lib, call(eps=eps), b"eps")
   _refused(lib, last(dst=None), b"null")
-  for eps in (-1e-9, math.nan, math.inf):
-    _refused(lib, last(eps=eps), b"eps")
-  _refused(lib, grad(stats=None), b"null")
+  # what the forward call keeps for the gradient: nothing up to 16 labels
+  assert [lib.mpl_norm_stats(n) for n in (1, 16, 17, 256)] == [0, 0, 2, 2]
+  _refused(lib, grad(stats=None, n=17), b"null")
   _refused(lib, grad(ddst=None), b"null")
   _refused(lib, grad(dweight=ONE), b"null")  # no workspace
   assert grad(dsrc=None) == 0  # nothing wanted
