@@ -14,7 +14,7 @@ SYMBOLS = ("mpl_trwp_forward", "mpl_trwp_backward", "mpl_isgmr_forward", "mpl_is
            "mpl_stereo_data_cost", "mpl_gradient_cues", "mpl_mrf_energy", "mpl_transpose",
            "mpl_dropout_labels_last", "mpl_dropout_labels_first", "mpl_bucket_context", "mpl_bucket_sums",
            "mpl_sample_labels", "mpl_norm_labels_last", "mpl_norm_labels_last_grad", "mpl_norm_workspace", "mpl_norm_stats",
-           "mpl_norm_stats", "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_verify_labels")
+           "mpl_best_labels", "mpl_distill_costs", "mpl_distill_costs_grad", "mpl_verify_labels")
 
 KERNEL_KINDS = ("fwd_sweep", "bwd_sweep", "belief", "aggregate", "label", "combine", "other",
                 "fwd_sweep_all", "bwd_sweep_all", "unary_all")
