@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
 }
 
 // Labels per lane and lanes per pixel.  us for 48 M costs, lists of 8: 16 labels 74 (a lane) / 86 (two), 24: 82 / 87, 32: 70 / 73,
-// 48: 69 / 63, 64: 61 (two) / 61 (four), 96: 64 / 55, 128: 67 / 54, 192: 72 (four) / 67 (eight), 256: 68 / 60.
+// 48: 69 / 63, 64: 61 (two) / 61 (four), 96: 64 / 55, 128: 67 / 54, 192: 72 (four) / 67 (eight), 256: 68 / 60.  Where a quarter or a sixth of the lanes'
+// labels would be none: 72 labels 500x1000 52 -> 46, 150 93 -> 89, 220 134 -> 129 (104: 68 -> 69, not taken).
 template <typename T, bool LAST>
 void launch(const Best& p, unsigned blocks, hipStream_t st) {
   const int n = p.t.n;
@@ -150,12 +151,18 @@ void launch(const Best& p, unsigned blocks, hipStream_t st) {
     best_kernel<T, 24, 2, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
   else if (n <= 64)
     best_kernel<T, 16, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 80)
+    best_kernel<T, 20, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
   else if (n <= 96)
     best_kernel<T, 24, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
   else if (n <= 128)
     best_kernel<T, 32, 4, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 160)
+    best_kernel<T, 20, 8, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
   else if (n <= 192)
     best_kernel<T, 24, 8, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
+  else if (n <= 224)
+    best_kernel<T, 28, 8, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
   else
     best_kernel<T, 32, 8, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
 }

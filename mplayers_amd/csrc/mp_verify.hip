@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
 
 // Labels per lane and lanes per pixel.  us, one draft but where said, fewer lanes / this / more: 60 labels 375x450 26.2 / 23.1 / 29.5,
 // 8 drafts 41.9 / 32.6 / 39.0, 60 labels 1000x2000 185 / 184 / 288; 21 labels 129x1548 15.9 / 14.6 / 18.3, 600x2000 49 / 51 / 74; 96
-// labels 384x1248 101 / 79 / 90.
+// labels 384x1248 101 / 79 / 90.  Where a quarter or a sixth of the lanes' labels would be none: 72 labels 500x1000 78 -> 72, 104 98 ->
+// 91, 150 164 -> 151, 220 225 -> 200.
 template <bool COSTS, bool LAST>
 void launch(const Verify& p, unsigned blocks, hipStream_t st) {
   const int n = p.t.n;
@@ -442,12 +443,20 @@ void launch(const Verify& p, unsigned blocks, hipStream_t st) {
     verify_kernel<12, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
   else if (n <= 64)
     verify_kernel<16, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 80)
+    verify_kernel<20, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
   else if (n <= 96)
     verify_kernel<24, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 112)
+    verify_kernel<28, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
   else if (n <= 128)
     verify_kernel<32, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
+  else if (n <= 160)
+    verify_kernel<20, 8, COSTS, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
   else if (n <= 192)
     verify_kernel<24, 8, COSTS, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
+  else if (n <= 224)
+    verify_kernel<28, 8, COSTS, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
   else
     verify_kernel<32, 8, COSTS, LAST><<<blocks, kLanePixels * 8, 0, st>>>(p);
 }

@@ -13,7 +13,8 @@ from oracle import more_around_oracle as oracle
 pytestmark = pytest.mark.gpu
 
 INF, NAN = math.inf, math.nan
-COUNTS = [1, 2, 4, 5, 8, 11, 16, 17, 21, 24, 25, 32, 33, 48, 49, 64, 65, 96, 97, 128, 129, 192, 193, 255, 256]
+COUNTS = [1, 2, 4, 5, 8, 11, 16, 17, 21, 24, 25, 32, 33, 48, 49, 64, 65, 80, 81, 96, 97, 112, 113, 128, 129, 160, 161, 192, 193, 224,
+          225, 255, 256]
 
 
 def _verify(cost, draft, uniforms, draft_cost=None, labels_first=True, **temperatures):
