@@ -3,6 +3,7 @@
 #define MPLAYERS_AMD_MP_LANES_H_
 
 #include "mp_common.h"
+#include "mp_offsets.h"
 
 namespace mpl {
 
@@ -152,11 +153,6 @@ inline bool make_lane_tiles(LaneTiles& t, int64_t items, int n_disp, int64_t pix
   return true;
 }
 
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-  T x[4];
-};
-
 // In LDS the quads of a pixel lie in the order in which its lanes read them: quad q, of lane q / (NV / 4), at place
 // q % (NV / 4) * S + q / (NV / 4); pixels an odd number of quads apart.
 template <int NV, int S>
@@ -180,13 +176,14 @@ struct LaneLoads {
       if (quads) {
 #pragma unroll
         for (int k = 0; k < kJ; ++k) {
-          const Four<T> q = *reinterpret_cast<const Four<T>*>(from + min((unsigned)(tid + k * kThreads) * 4, total - 4));
+          T q[4];
+          load_quad(from, min((unsigned)(tid + k * kThreads), total / 4 - 1), q);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) c[4 * k + j] = q.x[j];
+          for (int j = 0; j < 4; ++j) c[4 * k + j] = q[j];
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) c[k] = from[min((unsigned)(tid + k * kThreads), total - 1)];
+        for (int k = 0; k < NV; ++k) c[k] = load_at(from, min((unsigned)(tid + k * kThreads), total - 1));
       }
     } else {
       const int of = min(tid % kLanePixels, count - 1), wave = uniform_i(tid / kLanePixels);

@@ -12,6 +12,7 @@
 #define MPLAYERS_AMD_MP_PIXELS_H_
 
 #include "mp_common.h"
+#include "mp_offsets.h"
 
 namespace mpl {
 
@@ -124,10 +125,6 @@ template <int I, typename T>
 struct Run {
   T x[4 * I];
 };
-template <typename T>
-struct alignas(4 * sizeof(T)) Quad {
-  T x[4];
-};
 
 // Entry i of a run in the tile.
 template <int STRIDE>
@@ -143,13 +140,14 @@ __device__ __forceinline__ void load_run(const T* from, unsigned total, bool qua
   if (quads) {
 #pragma unroll
     for (int k = 0; k < I; ++k) {
-      const Quad<T> q = *reinterpret_cast<const Quad<T>*>(from + min((unsigned)(tid + k * kThreads) * 4, total - 4));
+      T q[4];
+      load_quad(from, min((unsigned)(tid + k * kThreads), total / 4 - 1), q);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r.x[4 * k + j] = q.x[j];
+      for (int j = 0; j < 4; ++j) r.x[4 * k + j] = q[j];
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 4 * I; ++k) r.x[k] = from[min((unsigned)(tid + k * kThreads), total - 1)];
+    for (int k = 0; k < 4 * I; ++k) r.x[k] = load_at(from, min((unsigned)(tid + k * kThreads), total - 1));
   }
 }
 template <int W, int I, typename T>
@@ -172,10 +170,10 @@ __device__ __forceinline__ void store_run(T* to, unsigned total, bool quads, int
   if (quads) {
     for (unsigned i = (unsigned)tid * 4; i < total; i += kThreads * 4) {
       const float4 x = *reinterpret_cast<const float4*>(&tile[tile_place<kStride>(i, t)]);
-      *reinterpret_cast<Quad<T>*>(to + i) = Quad<T>{{(T)x.x, (T)x.y, (T)x.z, (T)x.w}};
+      store_quad(to, i / 4, (T)x.x, (T)x.y, (T)x.z, (T)x.w);
     }
   } else {
-    for (unsigned i = (unsigned)tid; i < total; i += kThreads) to[i] = (T)tile[tile_place<kStride>(i, t)];
+    for (unsigned i = (unsigned)tid; i < total; i += kThreads) store_at(to, i, (T)tile[tile_place<kStride>(i, t)]);
   }
 }
 
