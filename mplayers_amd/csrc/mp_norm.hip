@@ -6,9 +6,11 @@
 //   dx[l] = r * (g[l] - mean(g) - xhat[l] * mean(g * xhat)),   dweight[l] = sum over pixels of dy[l] * xhat[l],
 //   dbias[l] = sum over pixels of dy[l].
 //
-// The variance is that of the differences from the mean, in registers: each wavefront's own labels first, and those of
-// the W wavefronts of a tile joined as sum(M2_w + n_w * (mean_w - mean)^2).  They are kept for the gradient, 8 bytes a pixel, from
-// 17 labels on; of fewer it forms them again from x, which it reads in any case.
+// The mean is that of the differences from a first label, so that it is exact where the labels have one cost, and the variance that
+// of the differences from the mean, in registers: each wavefront's own labels first, and those of the W wavefronts of a tile
+// joined as sum(M2_w + n_w * (mean_w - mean)^2).  Where squares do not fit fp32 (costs 2^64 apart, a mask of the type's largest
+// number) the pixel's costs are taken 2^-70 as large, which leaves xhat as it is.  Mean and r are kept for the gradient, 8 bytes a
+// pixel, from 17 labels on; of fewer it forms them again from x, which it reads in any case.
 //
 // Bound by HBM: a pixel's labels are read once, and the change of layout is one that the layer makes anyway.  The sums over
 // pixels stay in registers while a workgroup goes from tile to tile: a fp32 sum for each lane and label, then over the 64
@@ -59,9 +61,9 @@ __device__ __forceinline__ float2 own_moments(const float (&x)[I][4], int w, int
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum += is(i, j) ? x[i][j] : 0.f;
+    for (int j = 0; j < 4; ++j) sum += is(i, j) ? x[i][j] - x[0][0] : 0.f;
   const int here = labels_of<W, I>(w, n);
-  const float mean = here > 0 ? sum / (float)here : 0.f;
+  const float mean = here > 0 ? x[0][0] + sum / (float)here : 0.f;
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -71,7 +73,7 @@ __device__ __forceinline__ float2 own_moments(const float (&x)[I][4], int w, int
     }
   return float2{mean, m2};
 }
-// and the mean and r of the pixel from those of all W.
+// and the mean and variance + eps of the pixel from those of all W.
 template <int W, int I>
 __device__ __forceinline__ float2 join_moments(const float2 (*part)[kTilePixels], int lane, int n, float eps) {
   const float labels = (float)n;
@@ -80,15 +82,40 @@ __device__ __forceinline__ float2 join_moments(const float2 (*part)[kTilePixels]
 #pragma unroll
   for (int k = 0; k < W; ++k) {
     of_wave[k] = part[k][lane];
-    sum += of_wave[k].x * (float)labels_of<W, I>(k, n);
+    sum += (of_wave[k].x - of_wave[0].x) * (float)labels_of<W, I>(k, n);
   }
-  const float mean = W > 1 ? sum / labels : of_wave[0].x;
+  const float mean = W > 1 ? of_wave[0].x + sum / labels : of_wave[0].x;
 #pragma unroll
   for (int k = 0; k < W; ++k) {
     const float d = of_wave[k].x - mean;
     m2 += W > 1 ? of_wave[k].y + (float)labels_of<W, I>(k, n) * d * d : of_wave[k].y;
   }
-  return float2{mean, 1.f / sqrtf(m2 / labels + eps)};
+  return float2{mean, m2 / labels + eps};
+}
+
+constexpr float kFar = 0x1p-70f;
+
+// Mean and r of the lane's pixel; r is that of costs kFar as large, and negative, and the costs and the mean are kFar as large,
+// where they are far apart.  All wavefronts of a tile come to the same.  part: of the W wavefronts that share the tile.
+template <int W, int I>
+__device__ __forceinline__ float2 moments(float (&x)[I][4], float2 (*part)[kTilePixels], int w, int lane, int n, float eps) {
+  part[w][lane] = own_moments<W, I>(x, w, n);
+  if (W > 1) tile_sync<W>();
+  float2 of = join_moments<W, I>(part, lane, n, eps);
+  const bool far = !(of.y < __builtin_huge_valf());
+  if (__builtin_amdgcn_ballot_w64(far) != 0) {
+    if (W > 1) tile_sync<W>();  // (the parts are read)
+    const float scale = far ? kFar : 1.f;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] *= scale;
+    part[w][lane] = own_moments<W, I>(x, w, n);
+    if (W > 1) tile_sync<W>();
+    of = join_moments<W, I>(part, lane, n, eps * scale * scale);
+  }
+  const float r = 1.f / sqrtf(of.y);
+  return float2{of.x, far ? -r : r};
 }
 
 template <typename T, bool FIRST, int W, int I, int G>
@@ -126,10 +153,8 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
   __syncthreads();
   if (!work) return;
   if (!FIRST) from_tile<W, I>(mine, w, x);
-  float2* const mine_of = &part[group + w][lane];
-  *mine_of = own_moments<W, I>(x, w, n);
-  if (W > 1) tile_sync<W>();
-  const float2 of_pixel = join_moments<W, I>(part + group, lane, n, p.eps);
+  const float2 of_pixel = moments<W, I>(x, part + group, w, lane, n, p.eps);
+  const float r = fabsf(of_pixel.y);
   if (p.stats != nullptr && w == 0 && lane < count)
     reinterpret_cast<float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + lane] = of_pixel;
 #pragma unroll
@@ -137,7 +162,7 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int l = 4 * (w + i * W) + j;
-      x[i][j] = (x[i][j] - of_pixel.x) * of_pixel.y * affine[0][l] + affine[1][l];
+      x[i][j] = (x[i][j] - of_pixel.x) * r * affine[0][l] + affine[1][l];
     }
   to_tile<W, I>(mine, w, x);
   tile_sync<W>();
@@ -152,7 +177,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
   __shared__ __align__(16) float weight[4 * W * I];
   __shared__ float2 part[W * G][kTilePixels];
   constexpr bool kAgain = 4 * W * I <= kFormedAgain;
-  __shared__ float2 moments[kAgain ? W * G : 1][kTilePixels];
+  __shared__ float2 part_again[kAgain ? W * G : 1][kTilePixels];
   const int tid = (int)threadIdx.x % (64 * W), group = uniform_i((int)threadIdx.x / (64 * W));
   const int lane = tid % 64, w = uniform_i(tid / 64), n = p.t.labels;
   float* const tile = tiles + group * kTilePixels * kStride;
@@ -185,11 +210,18 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
       from_tile<W, I>(mine, w, x);
       tile_sync<W>();
     }
-    if (kAgain) moments[group + w][lane] = own_moments<W, I>(x, w, n);
     run_to_tile<W, I>(dy, total, p.y_quads, tid, p.t, tile);
-    tile_sync<W>();
+    if (kAgain) {
+      of_pixel = moments<W, I>(x, part_again + group, w, lane, n, p.eps);
+    } else if (__builtin_amdgcn_ballot_w64(of_pixel.y < 0) != 0) {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] *= of_pixel.y < 0 ? kFar : 1.f;
+    }
+    const float r = fabsf(of_pixel.y), r_of_x = of_pixel.y < 0 ? r * kFar : r;
+    if (!kAgain || W == 1) tile_sync<W>();
     from_tile<W, I>(mine, w, d);
-    if (kAgain) of_pixel = join_moments<W, I>(moments + group, lane, n, p.eps);
     float s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < I; ++i)
@@ -199,7 +231,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
         // (behind the last label or pixel of a tile in LDS lies an earlier one's, or no number at all)
         const bool in = l < n && lane < count;
         d[i][j] = in ? d[i][j] : 0.f;
-        x[i][j] = in ? (x[i][j] - of_pixel.x) * of_pixel.y : 0.f;
+        x[i][j] = in ? (x[i][j] - of_pixel.x) * r : 0.f;
         if (SUMS) {
           dw[i][j] += d[i][j] * x[i][j];
           db[i][j] += d[i][j];
@@ -225,7 +257,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
 #pragma unroll
       for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = of_pixel.y * (d[i][j] - s1 - x[i][j] * s2);
+        for (int j = 0; j < 4; ++j) x[i][j] = r_of_x * (d[i][j] - s1 - x[i][j] * s2);
       if (FIRST) {
         if (lane < count) store_rows<W, I>((T*)p.dx + first + p0, p.t, w, lane, x);
       } else {

@@ -1,8 +1,9 @@
 """Layer norm in the layout change on the GPU against its plain form in 64 bits.
 
 Tolerances, with u = 2^-24 and, for each pixel, A = max |x|, r = 1 / sqrt(var + eps) and X = max |xhat|.  A mean is a sum of at
-most 32 labels of a wavefront and of 8 wavefronts: off by at most 45 u A.  So a difference from it is off by 46 u A, r by a part
-of 45 u A r, and xhat by e = 64 u (1 + |xhat|) (1 + A r), its own roundings in it.
+most 32 labels' differences, of up to 2 A, from a first one and of 8 wavefronts' such: 2 u A for the differences, the average
+partial sum of 33 A u, 3 u A for the division and what is added again, and so 2 + 2 + 9 + 3 over the wavefronts, 54 u A.  So a
+difference from it is off by 55 u A, r by a part of 54 u A r, and xhat by e = 64 u (1 + |xhat|) (1 + A r), its own roundings in it.
   y        e |weight| and two roundings more
   dx       with G = max |g|: r (46 u G + e G X + X (45 u G X + G e) + the part of r) <= 5 * 64 u r G (1 + A r) (1 + X)^2,
            and half a step of its type
@@ -136,6 +137,38 @@ def test_equal_costs(gpu, n):
   want[0] += 6  # r = 2
   # (a mean and a difference of it)
   assert torch.allclose(dx.cpu(), want.view(1, 1, n, 1, 1).expand_as(dx), rtol=0, atol=6 * 4 * U)
+
+
+@pytest.mark.parametrize("labels_first", [True, False])
+@pytest.mark.parametrize("n", [2, 3, 7, 13, 21, 47, 100, 133, 251])
+def test_equal_costs_of_any_size(gpu, n, labels_first):
+  """The mean of equal costs is that cost, whatever its bits: differences of 0, so the bias comes out."""
+  from mplayers_amd import labels_last_norm
+  g = torch.Generator().manual_seed(n)
+  x = (torch.randn(1, 2, 1, 5, 31, generator=g) * 10.0 ** torch.randint(-3, 30, (1, 2, 1, 5, 31), generator=g)).cuda()
+  x = x.expand(1, 2, n, 5, 31)
+  bias = torch.randn(n, generator=g).cuda()
+  y = labels_last_norm(x if labels_first else x.movedim(2, -1), None, bias, 1e-5, labels_first)
+  assert torch.equal(y, bias.expand_as(y))
+
+
+@pytest.mark.parametrize("labels_first", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 3, 8, 12, 16, 21, 32, 60, 130, 192, 256])
+def test_costs_far_apart(gpu, n, dtype, labels_first):
+  """The type's largest number as a mask, and costs whose squares are beyond fp32, in some of the pixels and not in others."""
+  x, weight, bias, dy = _inputs(2, 1, n, 3, 47, dtype, True)
+  largest = torch.finfo(dtype).max
+  with torch.no_grad():
+    x[0, 0, 0, :, ::3] = largest
+    x[0, 0, n - 1, :, 1::6] = -largest
+    x[1, 0, n // 2, 0] = min(1e22, largest)
+    x[1, 0, :, 1, ::2] *= min(1e20, largest / 1e3)
+    x[1, 0, :, 2, ::5] = largest
+  if not labels_first:
+    x = x.detach().movedim(2, -1).contiguous().requires_grad_(True)
+  _check(x, weight, bias, 1e-5, dy, labels_first)
+  _check(x, weight, bias, 1e38, dy, labels_first)
 
 
 @pytest.mark.parametrize("labels_first", [True, False])
