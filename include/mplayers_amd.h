@@ -340,7 +340,8 @@ int mpl_dropout_labels_first(int dtype, int share, double rate, const int64_t* s
  * -> dst (batch, pixels, n_disp) fp32 = (src - mean) * r * weight[label] + bias[label], r = 1 / sqrt(var + eps), mean and
  * var (of the n_disp values, not n_disp - 1) of the pixel's labels.  weight, bias: n_disp floats or NULL (1, 0); eps
  * finite and >= 0.  stats: NULL, or mpl_norm_stats(n_disp) floats per pixel that the gradient takes (where that is 0, NULL to
- * both).  Everything is formed in fp32.  A cost that is infinite or NaN makes its pixel's results NaN; so does a pixel whose labels all have the same cost at an eps of 0.
+ * both).  Everything is formed in fp32, costs that are further apart than squares go there included.  A cost that is infinite or
+ * NaN makes its pixel's results NaN; so does a pixel whose labels all have the same cost at an eps of 0.
  * mpl_norm_labels_last_grad: from ddst (as dst) and the src, weight, eps and stats of that call
  *   dsrc = r * (g - mean(g) - xhat * mean(g * xhat)), g = ddst * weight, xhat = (src - mean) * r, in src's layout and type,
  *   dweight[label] = the sum over pixels of ddst * xhat, dbias[label] = the sum over pixels of ddst,
@@ -360,7 +361,7 @@ int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels);
  * pixels) or (items, pixels, n_kept): the costs relative to the pixel's least one (a difference in fp32, rounded to the type).
  * A place whose difference is +inf or that no candidate is left for has label 0 and cost +inf.  rest: NULL, or (items, pixels)
  * fp32: -T log(sum of exp(-c / T)) over the other candidates' relative costs c, +inf where there are none.  The temperature T
- * is for it alone, finite and above 0.  1 <= n_kept <= n_disp <= MPL_MAX_LABELS.  No counterpart in the reference. */
+ * is for it alone, above 0, and log2(e) / T and T are finite in fp32.  1 <= n_kept <= n_disp <= MPL_MAX_LABELS.  No counterpart in the reference. */
 int mpl_best_labels(int dtype, int labels_first, const void* cost, int n_kept, float temperature, int kept_dtype,
                     uint8_t* kept_labels, void* kept_costs, float* rest, int items, int n_disp, int64_t pixels, void* stream);
 
@@ -376,8 +377,8 @@ int mpl_best_labels(int dtype, int labels_first, const void* cost, int n_kept, f
  * the list has twice counts with either entry's p.  NaN or -inf among a pixel's costs that take part makes its loss NaN, and
  * its gradient but for labels of cost +inf.
  * mpl_distill_costs_grad: dcost, in cost's layout and type, = dloss * (p - q) / T of the label, p being the entries' or, for
- * a label of the rest, p(rest) q / q(rest); 0 for a label of cost +inf.  Everything is formed in fp32.  T finite and above
- * 0. */
+ * a label of the rest, p(rest) q / q(rest); 0 for a label of cost +inf.  Everything is formed in fp32.  T as in
+ * mpl_best_labels. */
 int mpl_distill_costs(int dtype, int labels_first, const void* cost, int kept_dtype, const uint8_t* kept_labels,
                       const void* kept_costs, const float* rest, float temperature, float* loss, int items, int n_disp,
                       int n_kept, int64_t pixels, void* stream);

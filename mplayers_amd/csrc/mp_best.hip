@@ -177,8 +177,8 @@ extern "C" int mpl_best_labels(int dtype, int labels_first, const void* cost, in
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "best_labels: n_disp must be in [1, %d], got %d", kMaxL, n_disp);
   if (n_kept < 1 || n_kept > n_disp)
     return fail(MPL_EINVAL, "best_labels: the list must have 1 to n_disp = %d places, got %d", n_disp, n_kept);
-  if (!(temperature > 0 && temperature < kInf && 1.f / temperature < kInf))
-    return fail(MPL_EINVAL, "best_labels: the temperature must be finite and above 0");
+  if (!(temperature > 0 && temperature < kInf && (float)(1.4426950408889634 / (double)temperature) < kInf))
+    return fail(MPL_EINVAL, "best_labels: the temperature must be finite and above 0, and its inverse finite");
   if (items < 0 || pixels < 0) return fail(MPL_EINVAL, "best_labels: negative size");
   if (items == 0 || pixels == 0) return MPL_OK;
   if (cost == nullptr || kept_labels == nullptr || kept_costs == nullptr) return fail(MPL_EINVAL, "best_labels: null pointer");

@@ -296,8 +296,8 @@ int run(const char* what, int dtype, int labels_first, Distill& p, int kept_dtyp
   if (kept_dtype < 0 || kept_dtype > MPL_BF16) return fail(MPL_EINVAL, "%s: unknown data type %d of the list", what, kept_dtype);
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
   if (k < 1 || k > kMaxL) return fail(MPL_EINVAL, "%s: the list must have 1 to %d entries, got %d", what, kMaxL, k);
-  if (!(temperature > 0 && temperature < kInf && 1.f / temperature < kInf))
-    return fail(MPL_EINVAL, "%s: the temperature must be finite and above 0", what);
+  if (!(temperature > 0 && temperature < kInf && (float)(1.4426950408889634 / (double)temperature) < kInf))
+    return fail(MPL_EINVAL, "%s: the temperature must be finite and above 0, and its inverse finite", what);
   if (items < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
   if (items == 0 || pixels == 0) return MPL_OK;
   if (p.cost == nullptr || p.labels == nullptr || p.costs == nullptr ||

@@ -358,8 +358,9 @@ void check_costs(const char* what, const at::Tensor& cost, bool labels_first) {
 }
 void check_temperature(const char* what, double t) {
   const float single = (float)t;
-  TORCH_CHECK(single > 0 && single <= std::numeric_limits<float>::max() && 1.f / single <= std::numeric_limits<float>::max(), what,
-              ": temperature must be finite and above 0, got ", t);
+  const float most = std::numeric_limits<float>::max();
+  TORCH_CHECK(single > 0 && single <= most && (float)(1.4426950408889634 / (double)single) <= most, what,
+              ": temperature must be finite and above 0 (and its inverse finite), got ", t);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> best_labels(const at::Tensor& cost_in, int64_t k, double temperature,

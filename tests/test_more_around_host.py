@@ -180,6 +180,15 @@ def test_distill_refusals(lib):
   _refused(lib, grad(dloss=None), b"null")
 
 
+def test_temperatures_at_the_end_of_fp32(lib):
+  """log2(e) / T is what exponents are multiplied by: beside an infinite one a difference of 0 is no number."""
+  for t, taken in ((2.95e-39, False), (4.2e-39, False), (4.3e-39, True), (3e38, True)):
+    for rc in (lib.mpl_best_labels(0, 1, ONE, 1, t, 0, ONE, ONE, None, 0, 2, 1, None),
+               lib.mpl_distill_costs(0, 1, ONE, 0, ONE, ONE, None, t, ONE, 0, 2, 1, 1, None),
+               lib.mpl_distill_costs_grad(0, 1, ONE, 0, ONE, ONE, None, t, ONE, ONE, 0, 2, 1, 1, None)):
+      assert (rc == 0) == taken, t
+
+
 def test_best_labels_of_the_plain_form():
   inf, nan = math.inf, math.nan
   assert oracle.best_labels([3, 1, 1, nan, 2], 3, 1.0)[:2] == ([1, 2, 4], [0, 0, 1])
