@@ -351,8 +351,8 @@ int mpl_norm_labels_last(int dtype, int labels_first, const void* src, const flo
                          float* dst, float* stats, int batch, int n_disp, int64_t pixels, void* stream);
 int mpl_norm_stats(int n_disp);
 int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, const float* weight, float eps,
-                              const float* stats, const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace, int batch,
-                              int n_disp, int64_t pixels, void* stream);
+                              const float* stats, const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace,
+                              int batch, int n_disp, int64_t pixels, void* stream);
 int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels);
 
 /* What is kept of a teacher: the n_kept labels of least cost of every pixel, in order of cost, equal costs in order of label.
@@ -361,7 +361,8 @@ int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels);
  * pixels) or (items, pixels, n_kept): the costs relative to the pixel's least one (a difference in fp32, rounded to the type).
  * A place whose difference is +inf or that no candidate is left for has label 0 and cost +inf.  rest: NULL, or (items, pixels)
  * fp32: -T log(sum of exp(-c / T)) over the other candidates' relative costs c, +inf where there are none.  The temperature T
- * is for it alone, above 0, and log2(e) / T and T are finite in fp32.  1 <= n_kept <= n_disp <= MPL_MAX_LABELS.  No counterpart in the reference. */
+ * is for it alone, above 0, and log2(e) / T and T are finite in fp32.  1 <= n_kept <= n_disp <= MPL_MAX_LABELS.  No counterpart
+ * in the reference. */
 int mpl_best_labels(int dtype, int labels_first, const void* cost, int n_kept, float temperature, int kept_dtype,
                     uint8_t* kept_labels, void* kept_costs, float* rest, int items, int n_disp, int64_t pixels, void* stream);
 

@@ -7,8 +7,9 @@
 // The costs are read once, a pixel's labels over S lanes (mp_lanes.h), and stay in LDS; a lane has the least cost of each quad of
 // its labels in registers.  A place of the list is the least of those over the lanes: the first lane that has it looks its
 // quad up, takes the label out and finds the quad's next.  So a place costs the instructions of the quads and not of the
-// labels, and no sort is needed.  us: 96 labels 384x1248, lists of 8, 53 (3.9 TB/s; label by label 83), about 800
-// instructions to a wavefront of 16 pixels, 0.8 of the time; 21 labels 12x129x129, lists of 4, 8.8; 192 labels 377x501, lists of 32, 109, bound by the instructions.
+// labels, and no sort is needed.  us: 96 labels 384x1248, lists of 8, 53 (3.9 TB/s; label by label 83), 800 instructions to a
+// wavefront of 16 pixels, 0.8 of the time; 21 labels 12x129x129, lists of 4, 8.6; 192 labels 377x501, lists of 32, 109, bound by
+// the instructions.
 
 #include "mp_lanes.h"
 
@@ -134,8 +135,8 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
 }
 
 // Labels per lane and lanes per pixel.  us for 48 M costs, lists of 8: 16 labels 74 (a lane) / 86 (two), 24: 82 / 87, 32: 70 / 73,
-// 48: 69 / 63, 64: 61 (two) / 61 (four), 96: 64 / 55, 128: 67 / 54, 192: 72 (four) / 67 (eight), 256: 68 / 60.  Where a quarter or a sixth of the lanes'
-// labels would be none: 72 labels 500x1000 52 -> 46, 150 93 -> 89, 220 134 -> 129 (104: 68 -> 69, not taken).
+// 48: 69 / 63, 64: 61 (two) / 61 (four), 96: 64 / 55, 128: 67 / 54, 192: 72 (four) / 67 (eight), 256: 68 / 60.  Where a quarter or a
+// sixth of the lanes' labels would be none: 72 labels 500x1000 52 -> 46, 150 93 -> 89, 220 134 -> 129 (104: 68 -> 69, not taken).
 template <typename T, bool LAST>
 void launch(const Best& p, unsigned blocks, hipStream_t st) {
   const int n = p.t.n;
@@ -183,7 +184,8 @@ extern "C" int mpl_best_labels(int dtype, int labels_first, const void* cost, in
   if (items == 0 || pixels == 0) return MPL_OK;
   if (cost == nullptr || kept_labels == nullptr || kept_costs == nullptr) return fail(MPL_EINVAL, "best_labels: null pointer");
   Best p = {};
-  if (!make_lane_tiles(p.t, items, n_disp, pixels, labels_first != 0, dtype == MPL_F32 ? 4 : 2)) return fail(MPL_EINVAL, "best_labels: too many pixels");
+  if (!make_lane_tiles(p.t, items, n_disp, pixels, labels_first != 0, dtype == MPL_F32 ? 4 : 2))
+    return fail(MPL_EINVAL, "best_labels: too many pixels");
   p.cost = cost;
   p.labels = kept_labels;
   p.costs = kept_costs;

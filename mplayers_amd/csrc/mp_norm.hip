@@ -15,8 +15,8 @@
 // Bound by HBM: a pixel's labels are read once, and the change of layout is one that the layer makes anyway.  The sums over
 // pixels stay in registers while a workgroup goes from tile to tile: a fp32 sum for each lane and label, then over the 64
 // lanes, and the workgroups' sums in 64 bits and in their order by a second kernel, so that the same call gives the same bits.
-// us, forward / gradient with all sums: fp32, 192 labels 1500x2000 860 / 1412 (5.4 and 4.9 TB/s, where a large copy moves
-// 4.7); bf16, 21 labels 12x129x129 9.9 / 16.4; 97 labels 301x803 in the operators' layout 41 / 72.
+// us, forward / gradient with all sums: fp32, 192 labels 1500x2000 857 / 1364 (5.4 and 5.1 TB/s, where a large copy moves
+// 4.7); bf16, 21 labels 12x129x129 9.9 / 16.3; 97 labels 301x803 in the operators' layout 40 / 68.
 
 #include "mp_pixels.h"
 
@@ -24,8 +24,8 @@ using namespace mpl;
 
 namespace {
 
-// Labels up to which the gradient forms mean and r again.  us for 64 M costs, forward / gradient, kept -> formed again: 2 labels 223 /
-// 213 -> 175 / 160, 8: 94 / 165 -> 87 / 152, 16: 91 / 167 -> 87 / 166, 40: 92 / 178 -> 88 / 188, 128: 90 / 171 -> 89 / 184 (their
+// Labels up to which the gradient forms mean and r again.  us for 64 M costs, forward / gradient, kept -> formed again: 2
+// labels 223 / 213 -> 175 / 160, 8: 94 / 165 -> 87 / 152, 16: 91 / 167 -> 87 / 166, 40: 92 / 178 -> 88 / 188, 128: 90 / 171 -> 89 / 184 (their
 // registers and instructions); 192 labels 1500x2000 864 / 1405 -> 848 / 1507.
 constexpr int kFormedAgain = 16;
 constexpr unsigned kSumRows = 2048;  // workgroups of a gradient, at most
@@ -323,7 +323,7 @@ int status(const char* what) {
 // The gradient's shapes: fewer labels to a wavefront, whose sums over the pixels take two registers each.  us, with the shapes of
 // the forward pass -> these: bf16, 21 labels 12x129x129 19.5 -> 12.3, 16 labels 64x96 6.8 -> 4.1; images of 64 M costs the same
 // but for 21 labels (172 -> 179) and 8 (179 -> 165).  Up to 16 labels to a wavefront in 128 registers, so that two workgroups of
-// eight share a compute unit: 97 labels 301x803 in the operators' layout 101 -> 71.
+// eight share a compute unit: 97 labels 301x803 in the operators' layout 101 -> 71 when it was taken.
 template <typename F>
 void with_grad_shape(int n, F f) {
   if (n <= 4)
@@ -396,7 +396,8 @@ int prepare(const char* what, Norm& p, int dtype, bool labels_first, float eps, 
   if (n_disp < 1 || n_disp > kMaxL) return fail(MPL_EINVAL, "%s: n_disp must be in [1, %d], got %d", what, kMaxL, n_disp);
   if (!(eps >= 0 && eps < __builtin_huge_valf())) return fail(MPL_EINVAL, "%s: eps must be finite and not below 0", what);
   if (batch < 0 || pixels < 0) return fail(MPL_EINVAL, "%s: negative size", what);
-  if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels, labels_first, dtype == MPL_F32 ? 4 : 2)) return fail(MPL_EINVAL, "%s: too many pixels", what);
+  if (batch > 0 && !make_tiles(p.t, batch, n_disp, pixels, labels_first, dtype == MPL_F32 ? 4 : 2))
+    return fail(MPL_EINVAL, "%s: too many pixels", what);
   return MPL_OK;
 }
 int whole_quads(const void* at, int n_disp, int dtype) {
@@ -436,8 +437,8 @@ int mpl_norm_labels_last(int dtype, int labels_first, const void* src, const flo
 }
 
 int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, const float* weight, float eps,
-                              const float* stats, const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace, int batch, int n_disp,
-                              int64_t pixels, void* stream) {
+                              const float* stats, const float* ddst, void* dsrc, float* dweight, float* dbias, float* workspace,
+                              int batch, int n_disp, int64_t pixels, void* stream) {
   Norm p = {};
   const int rc = prepare("norm_labels_last_grad", p, dtype, labels_first != 0, eps, batch, n_disp, pixels);
   if (rc != MPL_OK) return rc;

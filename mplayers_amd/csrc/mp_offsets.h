@@ -1,9 +1,9 @@
 // Global memory at a base that the wavefront shares and an offset of 32 bits of each lane's own: one instruction, with the base in
 // scalar registers.  Left to itself the compiler adds the two before, with an addition of 64 bits and two vector registers to each
 // access in flight.  For runs of costs with the labels last, 500 x 1000 pixels, that was: the gradient of distillation over 256
-// labels 372 us, now 318; of layer norm over 32 labels 46, now 34; best of 96 labels 49, now 38;
-// verification over 256 labels 478, now 252.  With the labels first the bases
-// differ from row to row, and holding each in scalar registers is no gain (gradient over 192 labels 138 us as it was, 152 so).
+// labels 372 us, now 318; of layer norm over 32 labels 46, now 34; best of 96 labels 49, now 38; verification over 256 labels
+// 478, now 252.  With the labels first the bases differ from row to row, and holding each in scalar registers is no gain (gradient
+// over 192 labels 138 us as it was, 152 so).
 #ifndef MPLAYERS_AMD_MP_OFFSETS_H_
 #define MPLAYERS_AMD_MP_OFFSETS_H_
 

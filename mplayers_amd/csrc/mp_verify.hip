@@ -8,9 +8,10 @@
 //
 // Either volume is read once: a pixel's labels lie in the registers of one to eight lanes (mp_lanes.h), p and q are formed there, and
 // the running sums go to LDS only in wavefronts where a label is drawn anew.  Results are those of 64 bits, which 32 bits give but
-// for drafts next to a border (see verify_kernel).  Bound by HBM for one draft: us, 192 labels 1500x2000 1050 (4.4 TB/s; with 64 bits
-// throughout 15 300), 60 labels 1000x2000 184 (5.3 TB/s); 60 labels 375x450 in the operators' layout, 8 drafts, 37 by the
-// instructions (980 to a wavefront of 16 pixels) and the last wavefronts, which have the drafts that go to 64 bits: 31 without those.
+// for drafts next to a border (see verify_kernel).  Bound by HBM for one draft: us, 192 labels 1500x2000 1015 to 1035 (4.5 TB/s; with 64
+// bits throughout 15 300, without the drafts that do go there 945), 60 labels 1000x2000 184 (5.3 TB/s); 60 labels 375x450 in the
+// operators' layout, 8 drafts, 32 by the instructions (920 to a wavefront of 16 pixels) and the last wavefronts, which have the
+// drafts that go to 64 bits: 28 without those.
 
 #include "mp_lanes.h"
 
@@ -474,7 +475,8 @@ extern "C" int mpl_verify_labels(int labels_first, const float* cost, const uint
   if (cost == nullptr || draft == nullptr || uniforms == nullptr || labels == nullptr || kept == nullptr)
     return fail(MPL_EINVAL, "verify_labels: null pointer");
   Verify p;
-  if (!make_lane_tiles(p.t, (int64_t)batch * n_cv, n_disp, pixels, labels_first != 0, 4)) return fail(MPL_EINVAL, "verify_labels: too many pixels");
+  if (!make_lane_tiles(p.t, (int64_t)batch * n_cv, n_disp, pixels, labels_first != 0, 4))
+    return fail(MPL_EINVAL, "verify_labels: too many pixels");
   p.cost = cost;
   p.draft_cost = draft_cost;
   p.draft = draft;
