@@ -29,7 +29,7 @@ struct Best {
   float* rest;  // or nullptr
   int k, kept;  // places of the list, type of their costs
   float temperature, to_exponent;  // T, log2(e) / T
-  int quads;
+  int mode;  // of runs
 };
 
 template <typename T, int NV, int S, bool LAST>
@@ -45,8 +45,10 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
   constexpr int kJ = Tile::kJ;
   {
     LaneLoads<NV, S, LAST, T> loads;
-    loads.load((const T*)p.cost + item * p.t.n * p.t.pixels, p.t, p0, count, p.quads, tid);
-    loads.to_tile(tile, p.t, count, p.quads, tid);
+    const int64_t at = item * p.t.n * p.t.pixels;
+    const int mode = LAST ? run_mode_of(p.mode, at, (unsigned)(count * p.t.n)) : (int)kEach;
+    loads.load((const T*)p.cost + at, p.t, p0, count, mode, tid);
+    loads.to_tile(tile, p.t, count, mode, tid);
   }
   __syncthreads();
   // quad g of this lane is at own[g * 4 * S]; nobody else reads or writes it from here on
@@ -194,7 +196,7 @@ extern "C" int mpl_best_labels(int dtype, int labels_first, const void* cost, in
   p.kept = kept_dtype;
   p.temperature = temperature;
   p.to_exponent = (float)(1.4426950408889634 / (double)temperature);
-  p.quads = n_disp % 4 == 0 && ((uintptr_t)cost & (dtype == MPL_F32 ? 15 : 7)) == 0;
+  p.mode = run_mode(n_disp, ((uintptr_t)cost & (dtype == MPL_F32 ? 15 : 7)) == 0);
   const unsigned blocks = (unsigned)(p.t.tiles * items);
   const auto by_type = [&](auto type) {
     using T = decltype(type);

@@ -39,7 +39,7 @@ struct Distill {
   void* dcost;
   int k, kept;               // entries of a list, type of their costs
   float to_exponent, inv_t;  // log2(e) / T, 1 / T
-  int quads;                 // whole and aligned quads in the operators' layout
+  int mode;                  // of runs of both volumes
 };
 
 __device__ __forceinline__ float kept_cost(const Distill& p, int64_t base, unsigned of) {
@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
   const unsigned total = (unsigned)(count * n);
   const int of = min(lane, count - 1);
   const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n, pixel = (int64_t)item * p.t.pixels + p0 + of;
+  const int mode = FIRST ? (int)kEach : run_mode_of(p.mode, first, total);
   float* const tile = tiles + group * kTilePixels * kStride;
   float* const mine = tile + lane * kStride;
 
@@ -125,8 +126,8 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
     to_tile<W, I>(mine, w, c);
   } else {
     Run<I, T> r;
-    load_run<W, I>((const T*)p.cost + run, total, p.quads, tid, r);
-    run_to_tile<W, I>(r, total, p.quads, tid, p.t, tile);
+    load_run<W, I>((const T*)p.cost + run, total, mode, tid, r);
+    run_to_tile<W, I>(r, total, mode, tid, p.t, tile);
     tile_sync<W>();
     from_tile<W, I>(mine, w, c);
   }
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
     } else {
       to_tile<W, I>(mine, w, d);
       tile_sync<W>();
-      store_run<W, I>((T*)p.dcost + run, total, p.quads, tid, p.t, tile);
+      store_run<W, I>((T*)p.dcost + run, total, mode, tid, p.t, tile);
     }
   }
 }
@@ -310,7 +311,7 @@ int run(const char* what, int dtype, int labels_first, Distill& p, int kept_dtyp
   p.to_exponent = (float)(1.4426950408889634 / (double)temperature);
   p.inv_t = 1.f / temperature;
   const uintptr_t aligned = dtype == MPL_F32 ? 15 : 7;
-  p.quads = n_disp % 4 == 0 && (((uintptr_t)p.cost | (uintptr_t)p.dcost) & aligned) == 0;
+  p.mode = run_mode(n_disp, (((uintptr_t)p.cost | (uintptr_t)p.dcost) & aligned) == 0);
   const auto by_type = [&](auto type) {
     using T = decltype(type);
     labels_first != 0 ? launch<T, true, GRAD>(p, st) : launch<T, false, GRAD>(p, st);

@@ -158,7 +158,12 @@ inline bool make_lane_tiles(LaneTiles& t, int64_t items, int n_disp, int64_t pix
 template <int NV, int S>
 struct LaneTile {
   static constexpr int kQuads = S * NV / 4, kJ = NV / 4, kStride = 4 * (kQuads | 1);
-  static __device__ __forceinline__ int place(int q) { return (q % kJ * S + q / kJ) * 4; }
+  // (q is below 64, where these multiplications of 24 bits divide by kJ)
+  static __device__ __forceinline__ unsigned place(unsigned q) {
+    if (S == 1) return q * 4;
+    const unsigned lane = __umul24(q, (256 + kJ - 1) / kJ) >> 8;
+    return (__umul24(q - __umul24(lane, kJ), S) + lane) * 4;
+  }
 };
 
 // What a thread loads of a tile: the costs of the item begin at `cost`, the tile at pixel p0, `count` pixels of it are there.
@@ -167,13 +172,13 @@ template <int NV, int S, bool LAST, typename T>
 struct LaneLoads {
   T c[NV];
 
-  __device__ __forceinline__ void load(const T* cost, const LaneTiles& t, int64_t p0, int count, bool quads, int tid) {
+  __device__ __forceinline__ void load(const T* cost, const LaneTiles& t, int64_t p0, int count, int mode, int tid) {
     constexpr int kJ = NV / 4, kThreads = kLanePixels * S;
     const int n = t.n;
     if (LAST) {
       const unsigned total = (unsigned)(count * n);
       const T* from = cost + p0 * n;
-      if (quads) {
+      if (mode != kEach) {
 #pragma unroll
         for (int k = 0; k < kJ; ++k) {
           T q[4];
@@ -195,7 +200,7 @@ struct LaneLoads {
     }
   }
   // What is no candidate goes there as +inf, and what lies behind the last label too.
-  __device__ __forceinline__ void to_tile(float* tile, const LaneTiles& t, int count, bool quads, int tid) const {
+  __device__ __forceinline__ void to_tile(float* tile, const LaneTiles& t, int count, int mode, int tid) const {
     using Tile = LaneTile<NV, S>;
     constexpr int kJ = NV / 4, kThreads = kLanePixels * S;
     const auto cost = [&](int k) { return candidate_of((float)c[k]); };
@@ -204,20 +209,35 @@ struct LaneLoads {
     }
     if (LAST) {
       const unsigned n = (unsigned)t.n, total = (unsigned)count * n;
-      if (quads) {
+      if (mode == kQuads) {
 #pragma unroll
         for (int k = 0; k < kJ; ++k) {
           const unsigned i = min((unsigned)(tid + k * kThreads) * 4, total - 4);
           const unsigned of = __umulhi(i, t.reciprocal), l = i - of * n;
-          *reinterpret_cast<float4*>(&tile[of * Tile::kStride + Tile::place((int)(l >> 2))]) =
+          *reinterpret_cast<float4*>(&tile[of * Tile::kStride + Tile::place(l >> 2)]) =
               float4{cost(4 * k), cost(4 * k + 1), cost(4 * k + 2), cost(4 * k + 3)};
+        }
+      } else if (mode == kFours) {
+        // (which need not be of one pixel)
+#pragma unroll
+        for (int k = 0; k < kJ; ++k) {
+          const unsigned i = min((unsigned)(tid + k * kThreads) * 4, total - 4);
+          const unsigned of = n == 1 ? i : __umulhi(i, t.reciprocal);
+          unsigned l = i - of * n, row = of * Tile::kStride;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            tile[row + Tile::place(l >> 2) + (l & 3)] = cost(4 * k + j);
+            const bool last = l + 1 == n;
+            row += last ? Tile::kStride : 0;
+            l = last ? 0 : l + 1;
+          }
         }
       } else {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
           const unsigned i = min((unsigned)(tid + k * kThreads), total - 1);
           const unsigned of = n == 1 ? i : __umulhi(i, t.reciprocal), l = i - of * n;
-          tile[of * Tile::kStride + Tile::place((int)(l >> 2)) + (l & 3)] = cost(k);
+          tile[of * Tile::kStride + Tile::place(l >> 2) + (l & 3)] = cost(k);
         }
       }
     } else {

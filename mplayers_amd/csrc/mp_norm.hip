@@ -18,6 +18,8 @@
 // us, forward / gradient with all sums: fp32, 192 labels 1500x2000 857 / 1364 (5.4 and 5.1 TB/s, where a large copy moves
 // 4.7); bf16, 21 labels 12x129x129 9.9 / 16.3; 97 labels 301x803 in the operators' layout 40 / 68.
 
+#include <algorithm>
+
 #include "mp_pixels.h"
 
 using namespace mpl;
@@ -41,7 +43,7 @@ struct Norm {
   void* dx;      // or nullptr
   float* sums;   // of each workgroup: dweight, dbias
   float eps;
-  int x_quads, y_quads;  // whole and aligned quads in the operators' layout
+  int x_mode, y_mode;  // of runs in the operators' layout
 };
 
 // labels that wavefront w of W has
@@ -142,8 +144,9 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
       load_rows<W, I>((const T*)p.x + first + p0, p.t, w, of, x);
     } else {
       Run<I, T> r;
-      load_run<W, I>((const T*)p.x + run, total, p.x_quads, tid, r);
-      run_to_tile<W, I>(r, total, p.x_quads, tid, p.t, tile);
+      const int mode = run_mode_of(p.x_mode, first, total);
+      load_run<W, I>((const T*)p.x + run, total, mode, tid, r);
+      run_to_tile<W, I>(r, total, mode, tid, p.t, tile);
     }
   }
   for (int i = (int)threadIdx.x; i < 4 * W * I; i += 64 * W * G) {
@@ -166,7 +169,7 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
     }
   to_tile<W, I>(mine, w, x);
   tile_sync<W>();
-  store_run<W, I>(p.y + run, total, p.y_quads, tid, p.t, tile);
+  store_run<W, I>(p.y + run, total, run_mode_of(p.y_mode, first, total), tid, p.t, tile);
 }
 
 // SUMS: with the sums over pixels that dweight and dbias are made of.
@@ -197,20 +200,21 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
     const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n;
     float x[I][4], d[I][4];
     Run<I, float> dy;
-    load_run<W, I>(p.dy + run, total, p.y_quads, tid, dy);
+    const int x_mode = run_mode_of(p.x_mode, first, total), y_mode = run_mode_of(p.y_mode, first, total);
+    load_run<W, I>(p.dy + run, total, y_mode, tid, dy);
     float2 of_pixel;
     if (!kAgain) of_pixel = reinterpret_cast<const float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + of];
     if (FIRST) {
       load_rows<W, I>((const T*)p.x + first + p0, p.t, w, of, x);
     } else {
       Run<I, T> rx;
-      load_run<W, I>((const T*)p.x + run, total, p.x_quads, tid, rx);
-      run_to_tile<W, I>(rx, total, p.x_quads, tid, p.t, tile);
+      load_run<W, I>((const T*)p.x + run, total, x_mode, tid, rx);
+      run_to_tile<W, I>(rx, total, x_mode, tid, p.t, tile);
       tile_sync<W>();
       from_tile<W, I>(mine, w, x);
       tile_sync<W>();
     }
-    run_to_tile<W, I>(dy, total, p.y_quads, tid, p.t, tile);
+    run_to_tile<W, I>(dy, total, y_mode, tid, p.t, tile);
     if (kAgain) {
       of_pixel = moments<W, I>(x, part_again + group, w, lane, n, p.eps);
     } else if (__builtin_amdgcn_ballot_w64(of_pixel.y < 0) != 0) {
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
       } else {
         to_tile<W, I>(mine, w, x);
         tile_sync<W>();
-        store_run<W, I>((T*)p.dx + run, total, p.x_quads, tid, p.t, tile);
+        store_run<W, I>((T*)p.dx + run, total, x_mode, tid, p.t, tile);
       }
     }
     tile_sync<W>();  // (the next tile overwrites this one and its parts)
@@ -400,8 +404,10 @@ int prepare(const char* what, Norm& p, int dtype, bool labels_first, float eps, 
     return fail(MPL_EINVAL, "%s: too many pixels", what);
   return MPL_OK;
 }
-int whole_quads(const void* at, int n_disp, int dtype) {
-  return n_disp % 4 == 0 && ((uintptr_t)at & (dtype == MPL_F32 ? 15 : 7)) == 0;
+// (Fours of up to three labels are of two pixels or more.  us one by one -> four side by side, 40 M costs, forward and gradient: 2
+// labels 256 -> 278, 3 203 -> 218, 5 225 -> 209, 7 178 -> 172; labels last, 5 261 -> 241, 150 218 -> 195.)
+int mode_of(const void* at, int n_disp, int dtype) {
+  return n_disp < 4 ? (int)kEach : run_mode(n_disp, ((uintptr_t)at & (dtype == MPL_F32 ? 15 : 7)) == 0);
 }
 
 }  // namespace
@@ -430,8 +436,8 @@ int mpl_norm_labels_last(int dtype, int labels_first, const void* src, const flo
   p.y = dst;
   p.stats = n_disp > kFormedAgain ? stats : nullptr;
   p.eps = eps;
-  p.x_quads = whole_quads(src, n_disp, dtype);
-  p.y_quads = whole_quads(dst, n_disp, MPL_F32);
+  p.x_mode = mode_of(src, n_disp, dtype);
+  p.y_mode = mode_of(dst, n_disp, MPL_F32);
   with_type(dtype, labels_first != 0, [&](auto type, auto first) { launch<decltype(type), first.value>(p, (hipStream_t)stream); });
   return status("norm_labels_last");
 }
@@ -458,8 +464,8 @@ int mpl_norm_labels_last_grad(int dtype, int labels_first, const void* src, cons
   p.dy = ddst;
   p.dx = dsrc;
   p.sums = sums ? workspace : nullptr;
-  p.x_quads = whole_quads(src, n_disp, dtype) && whole_quads(dsrc, n_disp, dtype);
-  p.y_quads = whole_quads(ddst, n_disp, MPL_F32);
+  p.x_mode = std::min(mode_of(src, n_disp, dtype), mode_of(dsrc, n_disp, dtype));
+  p.y_mode = mode_of(ddst, n_disp, MPL_F32);
   with_type(dtype, labels_first != 0,
             [&](auto type, auto first) { launch_grad<decltype(type), first.value>(p, dweight, dbias, (hipStream_t)stream); });
   return status("norm_labels_last_grad");

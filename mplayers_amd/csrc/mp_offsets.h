@@ -47,6 +47,14 @@ __device__ __forceinline__ void store_quad(T* base, unsigned index, T a, T b, T 
   *at_offset(reinterpret_cast<QuadWords<T>*>(base), index) = words;
 }
 
+// How a run of costs with the labels last is moved: one by one, four side by side, or so in quads that are of one pixel.
+enum { kEach, kFours, kQuads };
+inline int run_mode(int n_disp, bool aligned) { return !aligned ? kEach : n_disp % 4 == 0 ? kQuads : kFours; }
+// first: of the run, counted from what is aligned; a tile's pixels are whole fours, and its last one's costs need not be.
+__device__ __forceinline__ int run_mode_of(int mode, int64_t first, unsigned total) {
+  return mode == kFours && (((unsigned)first | total) & 3) != 0 ? (int)kEach : mode;
+}
+
 }  // namespace mpl
 
 #endif  // MPLAYERS_AMD_MP_OFFSETS_H_

@@ -133,11 +133,25 @@ __device__ __forceinline__ unsigned tile_place(unsigned i, const Tiles& t) {
   return p * STRIDE + (i - p * (unsigned)t.labels);
 }
 
-// quads: the labels are whole quads and the run is aligned to them.  tid: of the 64 * W threads of the tile.
+// Calls f with the place in the tile of each of the four entries from i on, which need not be of one pixel.
+template <int STRIDE, typename F>
+__device__ __forceinline__ void four_places(unsigned i, const Tiles& t, F f) {
+  const unsigned n = (unsigned)t.labels, p = n == 1 ? i : __umulhi(i, t.reciprocal);
+  unsigned l = i - p * n, place = p * STRIDE + l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f(j, place);
+    const bool last = l + 1 == n;
+    place += last ? STRIDE + 1 - n : 1;
+    l = last ? 0 : l + 1;
+  }
+}
+
+// mode: of the run (run_mode_of).  tid: of the 64 * W threads of the tile.
 template <int W, int I, typename T>
-__device__ __forceinline__ void load_run(const T* from, unsigned total, bool quads, int tid, Run<I, T>& r) {
+__device__ __forceinline__ void load_run(const T* from, unsigned total, int mode, int tid, Run<I, T>& r) {
   constexpr int kThreads = 64 * W;
-  if (quads) {
+  if (mode != kEach) {
 #pragma unroll
     for (int k = 0; k < I; ++k) {
       T q[4];
@@ -151,13 +165,18 @@ __device__ __forceinline__ void load_run(const T* from, unsigned total, bool qua
   }
 }
 template <int W, int I, typename T>
-__device__ __forceinline__ void run_to_tile(const Run<I, T>& r, unsigned total, bool quads, int tid, const Tiles& t, float* tile) {
+__device__ __forceinline__ void run_to_tile(const Run<I, T>& r, unsigned total, int mode, int tid, const Tiles& t, float* tile) {
   constexpr int kThreads = 64 * W, kStride = tile_stride(W * I);
-  if (quads) {
+  if (mode == kQuads) {
 #pragma unroll
     for (int k = 0; k < I; ++k)
       *reinterpret_cast<float4*>(&tile[tile_place<kStride>(min((unsigned)(tid + k * kThreads) * 4, total - 4), t)]) =
           float4{(float)r.x[4 * k], (float)r.x[4 * k + 1], (float)r.x[4 * k + 2], (float)r.x[4 * k + 3]};
+  } else if (mode == kFours) {
+#pragma unroll
+    for (int k = 0; k < I; ++k)
+      four_places<kStride>(min((unsigned)(tid + k * kThreads) * 4, total - 4), t,
+                           [&](int j, unsigned place) { tile[place] = (float)r.x[4 * k + j]; });
   } else {
 #pragma unroll
     for (int k = 0; k < 4 * I; ++k)
@@ -165,12 +184,18 @@ __device__ __forceinline__ void run_to_tile(const Run<I, T>& r, unsigned total, 
   }
 }
 template <int W, int I, typename T>
-__device__ __forceinline__ void store_run(T* to, unsigned total, bool quads, int tid, const Tiles& t, const float* tile) {
+__device__ __forceinline__ void store_run(T* to, unsigned total, int mode, int tid, const Tiles& t, const float* tile) {
   constexpr int kThreads = 64 * W, kStride = tile_stride(W * I);
-  if (quads) {
+  if (mode == kQuads) {
     for (unsigned i = (unsigned)tid * 4; i < total; i += kThreads * 4) {
       const float4 x = *reinterpret_cast<const float4*>(&tile[tile_place<kStride>(i, t)]);
       store_quad(to, i / 4, (T)x.x, (T)x.y, (T)x.z, (T)x.w);
+    }
+  } else if (mode == kFours) {
+    for (unsigned i = (unsigned)tid * 4; i < total; i += kThreads * 4) {
+      float x[4];
+      four_places<kStride>(i, t, [&](int j, unsigned place) { x[j] = tile[place]; });
+      store_quad(to, i / 4, (T)x[0], (T)x[1], (T)x[2], (T)x[3]);
     }
   } else {
     for (unsigned i = (unsigned)tid; i < total; i += kThreads) store_at(to, i, (T)tile[tile_place<kStride>(i, t)]);

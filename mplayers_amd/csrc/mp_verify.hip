@@ -32,7 +32,7 @@ struct Verify {
   float temperature_all, draft_temperature_all;
   int64_t items_pixels;
   int n_cv, n_drafts;
-  int quads;  // both volumes in whole and aligned quads, labels last
+  int mode;  // of runs of both volumes
 };
 
 __device__ __forceinline__ double inverse(float temperature) { return positive(temperature) ? 1.0 / (double)temperature : 0.0; }
@@ -286,15 +286,16 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   float a[NV], b[NV];
   {
     LaneLoads<NV, S, LAST, float> target, draft;
-    target.load(p.cost + first, p.t, p0, count, p.quads, tid);
-    if (COSTS) draft.load(p.draft_cost + first, p.t, p0, count, p.quads, tid);
+    const int mode = LAST ? run_mode_of(p.mode, first, (unsigned)(count * n)) : (int)kEach;
+    target.load(p.cost + first, p.t, p0, count, mode, tid);
+    if (COSTS) draft.load(p.draft_cost + first, p.t, p0, count, mode, tid);
     fetch_costs(d);
-    target.to_tile(tile, p.t, count, p.quads, tid);
+    target.to_tile(tile, p.t, count, mode, tid);
     __syncthreads();
     from_lane_tile<NV, S>(tile, px, s, a);
     if (COSTS) {
       __syncthreads();
-      draft.to_tile(tile, p.t, count, p.quads, tid);
+      draft.to_tile(tile, p.t, count, mode, tid);
       __syncthreads();
       from_lane_tile<NV, S>(tile, px, s, b);
     }
@@ -490,7 +491,7 @@ extern "C" int mpl_verify_labels(int labels_first, const float* cost, const uint
   p.items_pixels = (int64_t)batch * n_cv * pixels;
   p.n_cv = n_cv;
   p.n_drafts = n_drafts;
-  p.quads = n_disp % 4 == 0 && (((uintptr_t)cost | (uintptr_t)draft_cost) & 15) == 0;
+  p.mode = run_mode(n_disp, (((uintptr_t)cost | (uintptr_t)draft_cost) & 15) == 0);
   const unsigned blocks = (unsigned)(p.t.tiles * batch * n_cv);
   const hipStream_t st = (hipStream_t)stream;
   if (draft_cost != nullptr)
