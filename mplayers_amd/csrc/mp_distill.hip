@@ -43,9 +43,9 @@ struct Distill {
 };
 
 __device__ __forceinline__ float kept_cost(const Distill& p, int64_t base, unsigned of) {
-  return p.kept == MPL_F32   ? ((const float*)p.costs + base)[of]
-         : p.kept == MPL_F16 ? (float)((const _Float16*)p.costs + base)[of]
-                             : (float)((const __bf16*)p.costs + base)[of];
+  return p.kept == MPL_F32   ? load_at((const float*)p.costs + base, of)
+         : p.kept == MPL_F16 ? (float)load_at((const _Float16*)p.costs + base, of)
+                             : (float)load_at((const __bf16*)p.costs + base, of);
 }
 
 // A cost not above any of some costs, and the sum of their weights relative to it; (+inf, 0) of none.
@@ -81,8 +81,9 @@ __device__ __forceinline__ Mass join(Mass own, float2 (*part)[kTilePixels], int 
 
 constexpr float kFaint = 0x1p-60f;  // others that weigh less than this beside the best label: see distill_kernel
 
+// HELD: entries of the list that a wavefront keeps in registers, the rest is fetched twice or three times.
 // (Up to 24 labels to a wavefront in 128 registers, so that two workgroups of eight share a compute unit.)
-template <typename T, bool FIRST, bool GRAD, int W, int I, int G>
+template <typename T, bool FIRST, bool GRAD, int W, int I, int G, int HELD>
 __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Distill p) {
   constexpr int kStride = tile_stride(W * I), kShift = W == 1 ? 0 : W == 2 ? 1 : W == 4 ? 2 : 3, kParts = W > 1 ? W : 1;
   __shared__ __align__(16) float tiles[G * kTilePixels * kStride];
@@ -99,12 +100,12 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
   const int count = (int)min((int64_t)kTilePixels, p.t.pixels - p0);
   const unsigned total = (unsigned)(count * n);
   const int of = min(lane, count - 1);
-  const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n, pixel = (int64_t)item * p.t.pixels + p0 + of;
+  const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n, pixel = (int64_t)item * p.t.pixels + p0;
   const int mode = FIRST ? (int)kEach : run_mode_of(p.mode, first, total);
   float* const tile = tiles + group * kTilePixels * kStride;
   float* const mine = tile + lane * kStride;
 
-  // Entry e of the lane's list.  This wavefront has the entries w, w + W, ..., of which the first stays in registers.
+  // Entry e of the lane's list.  This wavefront has the entries w, w + W, ..., of which the first ones stay in registers.
   struct Entry {
     int label;
     float cost;
@@ -112,12 +113,16 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
   const auto fetch = [&](int e) {
     const int64_t base = FIRST ? ((int64_t)item * p.k + e) * p.t.pixels + p0 : ((int64_t)item * p.t.pixels + p0) * p.k + e;
     const unsigned at = (unsigned)(FIRST ? of : of * p.k);
-    return Entry{p.labels[base + at], kept_cost(p, base, at)};
+    return Entry{load_at(p.labels + base, at), kept_cost(p, base, at)};
   };
-  const Entry front = fetch(min(w, p.k - 1));
+  Entry held[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) held[i] = i == 0 || w + i * W < p.k ? fetch(min(w + i * W, p.k - 1)) : Entry{0, kInf};
   const auto entries = [&](auto f) {
-    if (w < p.k) f(front);
-    for (int e = w + W; e < p.k; e += W) f(fetch(e));
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (w + i * W < p.k) f(held[i]);
+    for (int e = w + HELD * W; e < p.k; e += W) f(fetch(e));
   };
 
   float c[I][4];
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
   Mass others = {kInf, 0.f};
   float rest = kInf;
   if (p.rest != nullptr) {
-    rest = p.rest[pixel];
+    rest = load_at(p.rest + pixel, of);
     Mass own = {least, 0.f};
 #pragma unroll
     for (int i = 0; i < I; ++i)
@@ -228,15 +233,19 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
     far = list_scale > 0 ? list_scale * (far - list.sum * (list.least - top)) * p.inv_t : 0.f;
     if (rest_weight > 0) far += rest_weight * (((others.least - student.least) - (rest - top)) * p.inv_t - logf(others.sum));
     const float loss = far / mass + (logf(student.sum) - logf(mass));
-    if (w == 0 && lane < count) p.loss[pixel] = mass == 0.f ? 0.f : loss;
+    if (w == 0 && lane < count) store_at(p.loss + pixel, lane, mass == 0.f ? 0.f : loss);
   } else {
     // p of the list's labels, in LDS where the costs were
     const float per_mass = 1.f / mass;
     const float none[I][4] = {};
     to_tile<W, I>(mine, w, none);  // (the list's join: all entries have found their costs)
     tile_sync<W>();
-    const bool in_turn = W == 1 || twice != 0;
-    if (!in_turn) {
+    const bool in_turn = W > 1 && twice != 0;
+    if (W == 1) {
+      entries([&](const Entry& e) {
+        if (exists(e)) mine[e.label] += weight(top, e.cost, p.to_exponent) * per_mass;
+      });
+    } else if (!in_turn) {
       entries([&](const Entry& e) {
         if (exists(e)) mine[e.label] = weight(top, e.cost, p.to_exponent) * per_mass;
       });
@@ -250,17 +259,18 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
     tile_sync<W>();
     float d[I][4];
     from_tile<W, I>(mine, w, d);
-    const float scale = p.dloss[pixel] * p.inv_t, of_student = weight(student.least, least, p.to_exponent) / student.sum;
+    const float scale = load_at(p.dloss + pixel, of) * p.inv_t, of_student = 1.f / student.sum;
     const float share = rest_weight > 0 ? rest_weight * per_mass / others.sum : 0.f;
     const bool beside = others.least == student.least;  // (the others' weights are those of a)
-    const float of_rest = beside ? share * weight(student.least, least, p.to_exponent) : 0.f;
+    // (the difference first: where the rest is all there is, it is 0)
+    const float own = weight(student.least, least, p.to_exponent);
+    const float of_named = -own * of_student, of_others = own * ((beside ? share : 0.f) - of_student);
     const float nan = mass - mass;  // 0, or NaN where the teacher has one
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float r = is_named(i, j) ? 0.f : of_rest;
-        d[i][j] += a[i][j] * (r - of_student) + nan;
+        d[i][j] += a[i][j] * (is_named(i, j) ? of_named : of_others) + nan;
       }
     if (__builtin_amdgcn_ballot_w64(!beside && share > 0) != 0) {
 #pragma unroll
@@ -283,11 +293,26 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
   }
 }
 
+// Eight entries of a list are held by the wavefronts of a tile, and four where the list has no more and one wavefront has it.  us,
+// loss / gradient, 16 M costs, one / four / eight held: 4 labels, lists of 4 147 / 117 / 123 and 210 / 142 / 183; 8 labels, 4 entries 83 /
+// 70 / 71 and 132 / 95 / 108, 8 entries 127 / 118 / 100 and 201 / 175 / 148; 42 M costs, 21 labels, 8 entries 82 (four) / 70 and 132 /
+// 106; 40 labels on two wavefronts, 8 entries, two and four each 55 / 50 and 72 / 62; 60 labels on four, one and two each 63 / 59 and
+// 97 / 86.
 template <typename T, bool FIRST, bool GRAD>
 void launch(const Distill& p, hipStream_t st) {
   with_shape(p.t.labels, [&](auto s) {
     constexpr int W = s.kW, I = s.kI, G = s.kG;
-    distill_kernel<T, FIRST, GRAD, W, I, G><<<(p.t.total + G - 1) / G, 64 * W * G, 0, st>>>(p);
+    const auto go = [&](auto held) {
+      distill_kernel<T, FIRST, GRAD, W, I, G, held.value><<<(p.t.total + G - 1) / G, 64 * W * G, 0, st>>>(p);
+    };
+    if constexpr (W > 1)
+      go(std::integral_constant<int, 8 / W>());
+    else if constexpr (I == 1)
+      go(std::integral_constant<int, 4>());
+    else if (p.k <= 4)
+      go(std::integral_constant<int, 4>());
+    else
+      go(std::integral_constant<int, 8>());
   });
 }
 template <bool GRAD>

@@ -417,3 +417,35 @@ def test_refusals(gpu):
   assert [tuple(t.shape) for t in kept] == [(0, 1, 2, 5, 6), (0, 1, 2, 5, 6), (0, 1, 5, 6)]
   loss = distill_costs(empty, *kept)
   assert loss.shape == (0, 1, 5, 6) and torch.autograd.grad(loss.sum(), empty)[0].shape == empty.shape
+
+
+@pytest.mark.parametrize("labels_first", [True, False])
+@pytest.mark.parametrize("n", [3, 12, 21, 46, 60, 96, 130, 192, 256])
+def test_a_rest_alone_has_no_gradient(gpu, n, labels_first):
+  """The list names a masked label, so the teacher says nothing about the others: exactly none."""
+  from mplayers_amd import distill_costs
+  g = torch.Generator().manual_seed(n)
+  cost = 4 * torch.randn(1, 1, n, 3, 40, generator=g)
+  cost[:, :, n // 2] = INF
+  labels = torch.full((1, 1, 1, 3, 40), n // 2, dtype=torch.uint8)
+  rest = torch.randn(1, 1, 3, 40, generator=g).cuda()
+  costs = torch.zeros(1, 1, 1, 3, 40)
+  if not labels_first:
+    cost, labels, costs = (t.movedim(2, -1).contiguous() for t in (cost, labels, costs))
+  cost = cost.cuda().requires_grad_(True)
+  loss = distill_costs(cost, labels.cuda(), costs.cuda(), rest, 0.7, labels_first)
+  assert float(loss.detach().abs().max()) <= 12 * U  # (two logarithms of up to 256, half a step each)
+  (grad,) = torch.autograd.grad(loss.sum(), cost)
+  assert not bool(grad.any())
+
+
+@pytest.mark.parametrize("labels_first", [True, False])
+@pytest.mark.parametrize("n,k", [(3, 5), (4, 9), (8, 4), (8, 5), (12, 8), (21, 9), (32, 8), (40, 8), (40, 9), (60, 7), (60, 9), (130, 9)])
+def test_lists_as_long_as_what_is_held_and_longer(gpu, n, k, labels_first):
+  """Longer than the labels too: such a list names some twice."""
+  cost, _, _, rest = _problem(n, 1, (2, 1, 3, 47), n + k)
+  rng = np.random.default_rng(k)
+  labels, costs = rng.integers(0, n, (2, 1, k, 3, 47)).astype(np.uint8), rng.random((2, 1, k, 3, 47)) * 5
+  costs[rng.random(costs.shape) < 0.1] = INF
+  _check_distill(_gpu(cost, labels_first), _gpu(labels, labels_first, torch.uint8), _gpu(costs, labels_first, torch.float16),
+                 torch.from_numpy(rest).float().cuda(), 1.0, labels_first)
