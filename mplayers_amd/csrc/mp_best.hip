@@ -138,16 +138,24 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
 
 // Labels per lane and lanes per pixel.  us for 48 M costs, lists of 8: 16 labels 74 (a lane) / 86 (two), 24: 82 / 87, 32: 70 / 73,
 // 48: 69 / 63, 64: 61 (two) / 61 (four), 96: 64 / 55, 128: 67 / 54, 192: 72 (four) / 67 (eight), 256: 68 / 60.  Where a quarter or a
-// sixth of the lanes' labels would be none: 72 labels 500x1000 52 -> 46, 150 93 -> 89, 220 134 -> 129 (104: 68 -> 69, not taken).
+// sixth of the lanes' labels would be none: 40 M costs, lists of 4, 4 labels 106 -> 82, 10 56 -> 49, 18 45 -> 38, 26 44 -> 36; 72 labels 500x1000 52 -> 46, 150 93 -> 89, 220 134 -> 129 (104: 68 -> 69, not taken).
 template <typename T, bool LAST>
 void launch(const Best& p, unsigned blocks, hipStream_t st) {
   const int n = p.t.n;
-  if (n <= 8)
+  if (n <= 4)
+    best_kernel<T, 4, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 8)
     best_kernel<T, 8, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 12)
+    best_kernel<T, 12, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 16)
     best_kernel<T, 16, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 20)
+    best_kernel<T, 20, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 24)
     best_kernel<T, 24, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 28)
+    best_kernel<T, 28, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 32)
     best_kernel<T, 32, 1, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 48)

@@ -424,23 +424,42 @@ __global__ void __launch_bounds__(kLanePixels* S) verify_kernel(Verify p) {
   }
 }
 
-// Labels per lane and lanes per pixel.  us, one draft but where said, fewer lanes / this / more: 60 labels 375x450 26.2 / 23.1 / 29.5,
-// 8 drafts 41.9 / 32.6 / 39.0, 60 labels 1000x2000 185 / 184 / 288; 21 labels 129x1548 15.9 / 14.6 / 18.3, 600x2000 49 / 51 / 74; 96
-// labels 384x1248 101 / 79 / 90.  Where a quarter or a sixth of the lanes' labels would be none: 72 labels 500x1000 78 -> 72, 104 98 ->
-// 91, 150 164 -> 151, 220 225 -> 200.
+// Labels per lane and lanes per pixel.  us, one draft but where said, fewer lanes / this / more: 60 labels 375x450 26.2 / 23.1 /
+// 29.5, 8 drafts 41.9 / 32.6 / 39.0, 60 labels 1000x2000 185 / 184 / 288; 96 labels 384x1248 101 / 79 / 90.  Where a quarter or a
+// sixth of the lanes' labels would be none: 72 labels 500x1000 78 -> 72, 104 98 -> 91, 150 164 -> 151, 220 225 -> 200.
+// Up to 48 labels a single draft has a lane or two to a pixel, and several have as many more as go over them at a time.  us, more /
+// fewer lanes, 40 M costs, labels first and last: one draft, 10 labels 120 / 78 and 148 / 79, 14 labels 98 / 77 and 101 / 73, 18: 89 /
+// 73 and 107 / 70, 21: 79 / 74 and 93 / 75, 26: 73 / 71 and 91 / 69, 38 (four lanes or two) 83 / 72 and 100 / 80, 46: 74 / 71 and 68 /
+// 63; eight drafts, 14 labels 1000x2000 144 / 178, 21 labels 1000x1000 87 / 106, 46 labels 1000x800 110 / 121, two drafts 44 / 51 for
+// 21 labels and 70 / 68 for 46.
 template <bool COSTS, bool LAST>
 void launch(const Verify& p, unsigned blocks, hipStream_t st) {
   const int n = p.t.n;
+  const bool one = p.n_drafts == 1;
   if (n <= 4)
     verify_kernel<4, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 8)
     verify_kernel<8, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 12)
+    verify_kernel<12, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 16 && one)
+    verify_kernel<16, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 16)
     verify_kernel<8, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 20 && one)
+    verify_kernel<20, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
+  else if (n <= 24 && one)
+    verify_kernel<24, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 24)
     verify_kernel<12, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 28 && one)
+    verify_kernel<28, 1, COSTS, LAST><<<blocks, kLanePixels, 0, st>>>(p);
   else if (n <= 32)
     verify_kernel<16, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 40 && one)
+    verify_kernel<20, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
+  else if (n <= 48 && one)
+    verify_kernel<24, 2, COSTS, LAST><<<blocks, kLanePixels * 2, 0, st>>>(p);
   else if (n <= 48)
     verify_kernel<12, 4, COSTS, LAST><<<blocks, kLanePixels * 4, 0, st>>>(p);
   else if (n <= 64)

@@ -19,7 +19,8 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 U = 2.0 ** -24
-COUNTS = [1, 2, 4, 5, 8, 11, 16, 17, 21, 24, 25, 32, 33, 48, 49, 60, 64, 65, 96, 97, 128, 129, 192, 193, 255, 256]
+COUNTS = [1, 2, 4, 5, 8, 9, 11, 12, 13, 16, 17, 20, 21, 24, 25, 28, 29, 32, 33, 48, 49, 60, 64, 65, 96, 97, 128, 129, 192, 193,
+          255, 256]
 
 
 def _flat(t, labels_first):

@@ -13,8 +13,8 @@ from oracle import more_around_oracle as oracle
 pytestmark = pytest.mark.gpu
 
 INF, NAN = math.inf, math.nan
-COUNTS = [1, 2, 4, 5, 8, 11, 16, 17, 21, 24, 25, 32, 33, 48, 49, 64, 65, 80, 81, 96, 97, 112, 113, 128, 129, 160, 161, 192, 193, 224,
-          225, 255, 256]
+COUNTS = [1, 2, 3, 4, 5, 7, 8, 9, 11, 12, 13, 16, 17, 18, 20, 21, 24, 25, 28, 29, 32, 33, 40, 41, 47, 48, 49, 64, 65, 80, 81, 96,
+          97, 112, 113, 128, 129, 160, 161, 192, 193, 224, 225, 255, 256]
 
 
 def _verify(cost, draft, uniforms, draft_cost=None, labels_first=True, **temperatures):
