@@ -16,8 +16,8 @@
 // A tile of 64 pixels, a lane to each (mp_pixels.h).  The costs lie in LDS too, where the entries find the student's cost of
 // their label; the wavefronts of a tile share the list, and each has weights of its own labels that serve the student's sum, the
 // others' and the gradient, so there is one exponential to a label.  us, loss / gradient: 192 labels 1500x2000, lists of 8 in fp16
-// and a rest, 590-610 / 957 (3.9 and 5.0 TB/s; with each wavefront going through the whole list 1190 / 2390); 21 labels
-// 12x129x129, lists of 4, 9.9 / 14.6.  Bound by HBM, the loss by the instructions as well: 580 to a wavefront of 24 labels, 0.6 of
+// and a rest, 600 / 950 (4.0 and 5.0 TB/s; with each wavefront going through the whole list 1190 / 2390); 21 labels
+// 12x129x129, lists of 4, 9.1 / 12.4.  Bound by HBM, the loss by the instructions as well: 580 to a wavefront of 24 labels, 0.6 of
 // the time.
 
 #include "mp_pixels.h"

@@ -16,7 +16,7 @@
 // pixels stay in registers while a workgroup goes from tile to tile: a fp32 sum for each lane and label, then over the 64
 // lanes, and the workgroups' sums in 64 bits and in their order by a second kernel, so that the same call gives the same bits.
 // us, forward / gradient with all sums: fp32, 192 labels 1500x2000 857 / 1364 (5.4 and 5.1 TB/s, where a large copy moves
-// 4.7); bf16, 21 labels 12x129x129 9.9 / 16.3; 97 labels 301x803 in the operators' layout 40 / 68.
+// 4.7); bf16, 21 labels 12x129x129 9.9 / 16.3; 97 labels 301x803 in the operators' layout 40 / 63.
 
 #include <algorithm>
 
