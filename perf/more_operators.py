@@ -279,7 +279,7 @@ def _weights(c, temperature):
   """exp(-cost / T) relative to the best, in 64 bits."""
   c = torch.where(c.isnan(), math.inf, c)
   best = c.amin(-1, keepdim=True)
-  weight = torch.exp((best - c).double() / temperature)
+  weight = torch.exp((best.double() - c.double()) / temperature)  # (in 32 bits the difference would be rounded already)
   weight = torch.where(c == best, 1.0, torch.where(c == math.inf, 0.0, weight))
   return torch.where(best == math.inf, 0.0, weight)
 
