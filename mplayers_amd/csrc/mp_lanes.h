@@ -13,6 +13,14 @@ constexpr float kInf = __builtin_huge_valf();
 __device__ __forceinline__ float candidate(float c) {
   return (__builtin_bit_cast(int, c) & 0x7fffffff) > 0x7f800000 ? kInf : c;
 }
+// The same in two instructions.  A minimum of two is the other one beside a NaN, or, beside a signalling one, that NaN made quiet,
+// which the second is of.  (In asm: where there are no NaNs the compiler takes a minimum with +inf for the number itself.  And no
+// comparison: a select may read a lane mask only two issue slots after it was written, which nothing in asm waits for.)
+__device__ __forceinline__ float candidate_of(float c) {
+  float out;
+  asm("v_min_f32 %0, %2, %1\n\tv_min_f32 %0, %2, %0" : "=v"(out) : "v"(c), "s"(kInf));
+  return out;
+}
 
 // 2^y, y <= 0, to about 2^-51: the exponential series of the fraction, whose 14th term is below 2^-52 of the first.
 __device__ __forceinline__ double exp2_64(double y) {
@@ -38,12 +46,6 @@ __device__ __forceinline__ double exp2_64(double y) {
   e = fma(e, x, 1.0);
   e = fma(e, x, 1.0);
   return ldexp(e, (int)whole);
-}
-// The same in two instructions (the library is compiled for code without NaNs, where a comparison cannot tell one).
-__device__ __forceinline__ float candidate_of(float c) {
-  float out;
-  asm("v_cmp_u_f32 vcc, %1, %1\n\tv_cndmask_b32 %0, %1, %2, vcc" : "=v"(out) : "v"(c), "v"(kInf) : "vcc");
-  return out;
 }
 // x > 0 and a number
 __device__ __forceinline__ bool positive(float x) {
