@@ -107,15 +107,24 @@ def labels_last_norm(x, weight=None, bias=None, eps=1e-5, labels_first=True):
   -> (batch, cv, H, W, labels) fp32, (x - mean) / sqrt(var + eps) * weight + bias with the mean and the variance of each
      pixel's labels.  Gradients come in x's layout and type; those of weight and bias are the same bits in every call.
 
-  An infinite cost or NaN makes its pixel's results NaN.  CPU tensors go through torch."""
+  An infinite cost or NaN makes its pixel's results NaN.  CPU tensors go through torch, in 64 bits."""
   if x.is_cuda:
     return _lib.autograd().labels_last_norm(x, weight, bias, eps, labels_first)
   if x.dim() != 5 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
     raise RuntimeError("labels_last_norm: x must be a (batch, cv, labels, H, W) or (batch, cv, H, W, labels) float32, float16 or "
                        "bfloat16 tensor, got %s of %d axes" % (x.dtype, x.dim()))
-  x = (x.movedim(2, -1) if labels_first else x).float()
-  if not 1 <= x.size(-1) <= 256:
-    raise RuntimeError("labels_last_norm: 1 to 256 labels, got %d" % x.size(-1))
-  if not 0 <= eps < float("inf"):
+  x = (x.movedim(2, -1) if labels_first else x).contiguous()
+  n = x.size(-1)
+  if not 1 <= n <= 256:
+    raise RuntimeError("labels_last_norm: 1 to 256 labels, got %d" % n)
+  for name, t in (("weight", weight), ("bias", bias)):
+    if t is not None and (t.device != x.device or t.dtype != torch.float32 or t.shape != (n,)):
+      raise RuntimeError("labels_last_norm: %s must be %d float32 numbers on the device of x" % (name, n))
+  if not 0 <= eps <= torch.finfo(torch.float32).max:
     raise RuntimeError("labels_last_norm: eps must be finite and not below 0, got %r" % eps)
-  return torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps).contiguous()
+  # (in 64 bits, where the squares of any costs and the sum of equal ones are what they are)
+  x = x.double()
+  centred = x - x.mean(-1, keepdim=True)
+  y = centred * torch.rsqrt((centred * centred).mean(-1, keepdim=True) + eps)
+  y = y if weight is None else y * weight.double()
+  return (y if bias is None else y + bias.double()).float()
