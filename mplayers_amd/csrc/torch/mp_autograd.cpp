@@ -69,8 +69,11 @@ int small(int64_t size) {
   TORCH_CHECK(size <= std::numeric_limits<int>::max(), "a size of ", size, " is too large");
   return (int)size;
 }
-// whether a gradient is itself to be differentiated
-bool recorded(const at::Tensor& grad) { return at::GradMode::is_enabled() && grad.requires_grad(); }
+// whether a tensor carries a derivative of the forward mode, which the functions have none of: apply() refuses it, and what
+// goes past apply() would lose it without a word
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+// whether autograd is to know of what is made of a tensor
+bool recorded(const at::Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || has_tangent(t); }
 
 // ------------------------------------------------------------------------------------------------ bucketed tables
 at::Tensor expand(const at::Tensor& table_in, const at::Tensor& starts, int64_t n, int64_t square) {
@@ -314,7 +317,7 @@ struct NormLast : Function<NormLast> {
     const bool wanted[] = {ctx->needs_input_grad(0), weighted && ctx->needs_input_grad(1),
                            ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(weighted ? 2 : 1)};
     variable_list out;
-    if (at::GradMode::is_enabled()) {
+    if (at::GradMode::is_enabled() || has_tangent(grads[0])) {
       out = NormGrad::apply(grads[0], saved[0], weighted ? std::optional<at::Tensor>(saved[1]) : std::nullopt,
                             saved[2].defined() ? std::optional<at::Tensor>(saved[2]) : std::nullopt, eps, labels_first,
                             wanted[0], wanted[1], wanted[2]);
@@ -334,16 +337,16 @@ at::Tensor labels_last_norm(const at::Tensor& x, const std::optional<at::Tensor>
   TORCH_CHECK(mpl_type(x.scalar_type()) >= 0, "labels_last_norm: x must be float32, float16 or bfloat16, got ", x.scalar_type());
   const int64_t n = Layout(x, labels_first).n;
   TORCH_CHECK(n >= 1 && n <= MPL_MAX_LABELS, "labels_last_norm: 1 to 256 labels, got ", n);
-  bool recorded = at::GradMode::is_enabled() && x.requires_grad();
+  bool through_autograd = recorded(x);
   const std::pair<const char*, const std::optional<at::Tensor>*> given[] = {{"weight", &weight}, {"bias", &bias}};
   for (const auto& [name, t] : given) {
     if (!t->has_value()) continue;
     TORCH_CHECK((*t)->device() == x.device() && (*t)->scalar_type() == at::kFloat && (*t)->dim() == 1 && (*t)->size(0) == n,
                 "labels_last_norm: ", name, " must be ", n, " float32 numbers on the device of x");
-    recorded |= at::GradMode::is_enabled() && (*t)->requires_grad();
+    through_autograd |= recorded(**t);
   }
   TORCH_CHECK(eps >= 0 && eps <= std::numeric_limits<float>::max(), "labels_last_norm: eps must be finite and not below 0, got ", eps);
-  if (recorded) return NormLast::apply(x, weight, bias, eps, labels_first);
+  if (through_autograd) return NormLast::apply(x, weight, bias, eps, labels_first);
   return norm_last(x.contiguous(), weight ? weight->contiguous() : at::Tensor(), bias ? bias->contiguous() : at::Tensor(), eps,
                    labels_first, false).first;
 }
@@ -435,7 +438,7 @@ struct Distill : Function<Distill> {
     const variable_list s = ctx->get_saved_variables();
     const double temperature = ctx->saved_data["temperature"].toDouble();
     const bool labels_first = ctx->saved_data["labels_first"].toBool(), with_rest = ctx->saved_data["rest"].toBool();
-    return {at::GradMode::is_enabled()
+    return {at::GradMode::is_enabled() || has_tangent(grads[0])
                 ? DistillGrad::apply(grads[0], s[0], s[1], s[2], with_rest ? std::optional<at::Tensor>(s[3]) : std::nullopt,
                                      temperature, labels_first)
                 : distill_grad(grads[0], s[0], s[1], s[2], s[3], temperature, labels_first),
@@ -456,7 +459,7 @@ at::Tensor distill_costs(const at::Tensor& cost, const at::Tensor& labels, const
     TORCH_CHECK(l.batch == s.batch && l.cv == s.cv && l.height == s.height && l.width == s.width && l.n >= 1 && l.n <= MPL_MAX_LABELS,
                 "distill_costs: ", name, " must have 1 to 256 entries for each of ", s.batch, "x", s.cv, "x", s.height, "x", s.width,
                 " pixels");
-    TORCH_CHECK(!t->requires_grad() || !at::GradMode::is_enabled(), "distill_costs: the teacher's ", name, " have no gradient");
+    TORCH_CHECK(!recorded(*t), "distill_costs: the teacher's ", name, " have no gradient");
   }
   TORCH_CHECK(labels.scalar_type() == at::kByte, "distill_costs: labels must be uint8, got ", labels.scalar_type());
   TORCH_CHECK(mpl_type(costs.scalar_type()) >= 0, "distill_costs: costs must be float32, float16 or bfloat16, got ",
@@ -466,9 +469,9 @@ at::Tensor distill_costs(const at::Tensor& cost, const at::Tensor& labels, const
     TORCH_CHECK(rest->device() == cost.device() && rest->scalar_type() == at::kFloat && rest->dim() == 4 && rest->size(0) == s.batch &&
                     rest->size(1) == s.cv && rest->size(2) == s.height && rest->size(3) == s.width,
                 "distill_costs: rest must be a float32 (batch, cv, H, W) tensor on the device of cost");
-    TORCH_CHECK(!rest->requires_grad() || !at::GradMode::is_enabled(), "distill_costs: the teacher's rest has no gradient");
+    TORCH_CHECK(!recorded(*rest), "distill_costs: the teacher's rest has no gradient");
   }
-  if (at::GradMode::is_enabled() && cost.requires_grad()) return Distill::apply(cost, labels, costs, rest, temperature, labels_first);
+  if (recorded(cost)) return Distill::apply(cost, labels, costs, rest, temperature, labels_first);
   return distill_loss(cost.contiguous(), labels.contiguous(), costs.contiguous(), rest ? rest->contiguous() : at::Tensor(), temperature,
                       labels_first);
 }
