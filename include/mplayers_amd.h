@@ -340,7 +340,7 @@ int mpl_dropout_labels_first(int dtype, int share, double rate, const int64_t* s
  * -> dst (batch, pixels, n_disp) fp32 = (src - mean) * r * weight[label] + bias[label], r = 1 / sqrt(var + eps), mean and
  * var (of the n_disp values, not n_disp - 1) of the pixel's labels.  weight, bias: n_disp floats or NULL (1, 0); eps
  * finite and >= 0.  stats: NULL, or mpl_norm_stats(n_disp) floats per pixel that the gradient takes (where that is 0, NULL to
- * both).  Everything is formed in fp32, costs that are further apart than squares go there included.  A cost that is infinite or
+ * both).  Everything is formed in fp32, costs that are further apart or closer together than squares go there included.  A cost that is infinite or
  * NaN makes its pixel's results NaN; so does a pixel whose labels all have the same cost at an eps of 0.
  * mpl_norm_labels_last_grad: from ddst (as dst) and the src, weight, eps and stats of that call
  *   dsrc = r * (g - mean(g) - xhat * mean(g * xhat)), g = ddst * weight, xhat = (src - mean) * r, in src's layout and type,

@@ -9,7 +9,8 @@
 // The mean is that of the differences from a first label, so that it is exact where the labels have one cost, and the variance that
 // of the differences from the mean, in registers: each wavefront's own labels first, and those of the W wavefronts of a tile
 // joined as sum(M2_w + n_w * (mean_w - mean)^2).  Where squares do not fit fp32 (costs 2^64 apart, a mask of the type's largest
-// number) the pixel's costs are taken 2^-70 as large, which leaves xhat as it is.  Mean and r are kept for the gradient, 8 bytes a
+// number) the pixel's costs are taken 2^-70 as large, and 2^100 times where they and eps are too small for it (costs 2^-50 apart
+// without eps), which leaves xhat as it is.  Mean and r are kept for the gradient, 8 bytes a
 // pixel, from 17 labels on; of fewer it forms them again from x, which it reads in any case.
 //
 // Bound by HBM: a pixel's labels are read once, and the change of layout is one that the layer makes anyway.  The sums over
@@ -95,19 +96,29 @@ __device__ __forceinline__ float2 join_moments(const float2 (*part)[kTilePixels]
   return float2{mean, m2 / labels + eps};
 }
 
-constexpr float kFar = 0x1p-70f;
+constexpr float kFar = 0x1p-70f, kClose = 0x1p100f;
 
-// Mean and r of the lane's pixel; r is that of costs kFar as large, and negative, and the costs and the mean are kFar as large,
-// where they are far apart.  All wavefronts of a tile come to the same.  part: of the W wavefronts that share the tile.
+// r as it is kept: negative where the costs and the mean are kFar as large, and r is of those (2^-59 to 2^6 then: a variance beyond
+// 2^128 becomes one of 2^-12 to 2^118); below kCloseMark where they are kClose times as large (r is 2^-50 to 2^53, kept
+// 2^60 times as large).
+constexpr float kCloseMark = -0x1p8f;
+__device__ __forceinline__ bool is_close(float kept) { return kept < kCloseMark; }
+__device__ __forceinline__ float r_of(float kept) { return is_close(kept) ? kept * -0x1p-60f : fabsf(kept); }
+__device__ __forceinline__ float scale_of(float kept) { return is_close(kept) ? kClose : kept < 0 ? kFar : 1.f; }
+
+// Mean and r of the lane's pixel, r as it is kept, and the costs as large as it says.  All wavefronts of a tile come to the
+// same.  part: of the W wavefronts that share the tile.
 template <int W, int I>
 __device__ __forceinline__ float2 moments(float (&x)[I][4], float2 (*part)[kTilePixels], int w, int lane, int n, float eps) {
   part[w][lane] = own_moments<W, I>(x, w, n);
   if (W > 1) tile_sync<W>();
   float2 of = join_moments<W, I>(part, lane, n, eps);
   const bool far = !(of.y < __builtin_huge_valf());
-  if (__builtin_amdgcn_ballot_w64(far) != 0) {
+  // (costs of 2^-10 or more are further apart than that, or all the same)
+  const bool close = of.y < 0x1p-100f && fabsf(of.x) < 0x1p-10f;
+  if (__builtin_amdgcn_ballot_w64(far || close) != 0) {
     if (W > 1) tile_sync<W>();  // (the parts are read)
-    const float scale = far ? kFar : 1.f;
+    const float scale = far ? kFar : close ? kClose : 1.f;
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -117,7 +128,7 @@ __device__ __forceinline__ float2 moments(float (&x)[I][4], float2 (*part)[kTile
     of = join_moments<W, I>(part, lane, n, eps * scale * scale);
   }
   const float r = 1.f / sqrtf(of.y);
-  return float2{of.x, far ? -r : r};
+  return float2{of.x, far ? -r : close ? r * -0x1p60f : r};
 }
 
 template <typename T, bool FIRST, int W, int I, int G>
@@ -157,7 +168,7 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
   if (!work) return;
   if (!FIRST) from_tile<W, I>(mine, w, x);
   const float2 of_pixel = moments<W, I>(x, part + group, w, lane, n, p.eps);
-  const float r = fabsf(of_pixel.y);
+  const float r = r_of(of_pixel.y);
   if (p.stats != nullptr && w == 0 && lane < count)
     reinterpret_cast<float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + lane] = of_pixel;
 #pragma unroll
@@ -221,9 +232,11 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
 #pragma unroll
       for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] *= of_pixel.y < 0 ? kFar : 1.f;
+        for (int j = 0; j < 4; ++j) x[i][j] *= scale_of(of_pixel.y);
     }
-    const float r = fabsf(of_pixel.y), r_of_x = of_pixel.y < 0 ? r * kFar : r;
+    // (of close costs r * kClose may be beyond fp32 where the gradient is not: half of the scale before, half behind)
+    const bool close = is_close(of_pixel.y);
+    const float r = r_of(of_pixel.y), r_of_x = close ? r * 0x1p50f : of_pixel.y < 0 ? r * kFar : r;
     if (!kAgain || W == 1) tile_sync<W>();
     from_tile<W, I>(mine, w, d);
     float s1 = 0, s2 = 0;
@@ -262,6 +275,12 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
       for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i][j] = r_of_x * (d[i][j] - s1 - x[i][j] * s2);
+      if (__builtin_amdgcn_ballot_w64(close) != 0) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i][j] *= close ? 0x1p50f : 1.f;
+      }
       if (FIRST) {
         if (lane < count) store_rows<W, I>((T*)p.dx + first + p0, p.t, w, lane, x);
       } else {
