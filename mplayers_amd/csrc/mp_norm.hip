@@ -27,9 +27,9 @@ using namespace mpl;
 
 namespace {
 
-// Labels up to which the gradient forms mean and r again.  us for 64 M costs, forward / gradient, kept -> formed again: 2
-// labels 223 / 213 -> 175 / 160, 8: 94 / 165 -> 87 / 152, 16: 91 / 167 -> 87 / 166, 40: 92 / 178 -> 88 / 188, 128: 90 / 171 -> 89 / 184 (their
-// registers and instructions); 192 labels 1500x2000 864 / 1405 -> 848 / 1507.
+// Labels up to which the gradient forms mean and r again.  us for 40 M costs, forward / gradient, kept -> formed again: 2 labels
+// 129 / 123 -> 114 / 114, 4: 73 / 115 -> 66 / 99, 8: 68 / 105 -> 62 / 97, 16: 64 / 107 -> 60 / 102; 21: 66 / 117 -> 62 / 115, labels last
+// 67 / 107 -> 63 / 116, bf16 44 / 76 -> 43 / 84, 4.2 M bf16 costs 8.4 / 14.7 -> 8.3 / 17.6 (registers and instructions).
 constexpr int kFormedAgain = 16;
 constexpr unsigned kSumRows = 2048;  // workgroups of a gradient, at most
 
@@ -46,6 +46,14 @@ struct Norm {
   float eps;
   int x_mode, y_mode;  // of runs in the operators' layout
 };
+
+// Up to four labels no run is one of fours (mode_of).
+template <int W, int I>
+constexpr bool kFoursToo = W * I > 1;
+template <int W, int I>
+__device__ __forceinline__ int run_mode_here(int mode, int64_t first, unsigned total) {
+  return kFoursToo<W, I> ? run_mode_of(mode, first, total) : mode;
+}
 
 // labels that wavefront w of W has
 template <int W, int I>
@@ -113,12 +121,13 @@ __device__ __forceinline__ float2 moments(float (&x)[I][4], float2 (*part)[kTile
   part[w][lane] = own_moments<W, I>(x, w, n);
   if (W > 1) tile_sync<W>();
   float2 of = join_moments<W, I>(part, lane, n, eps);
-  const bool far = !(of.y < __builtin_huge_valf());
-  // (costs of 2^-10 or more are further apart than that, or all the same)
-  const bool close = of.y < 0x1p-100f && fabsf(of.x) < 0x1p-10f;
-  if (__builtin_amdgcn_ballot_w64(far || close) != 0) {
+  float mark = 1;
+  if (__builtin_amdgcn_ballot_w64(!(of.y >= 0x1p-100f && of.y < __builtin_huge_valf())) != 0) {
     if (W > 1) tile_sync<W>();  // (the parts are read)
+    // (costs of 2^-10 or more are further apart than 2^-50, or all the same)
+    const bool far = !(of.y < __builtin_huge_valf()), close = of.y < 0x1p-100f && fabsf(of.x) < 0x1p-10f;
     const float scale = far ? kFar : close ? kClose : 1.f;
+    mark = far ? -1.f : close ? -0x1p60f : 1.f;
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -127,8 +136,7 @@ __device__ __forceinline__ float2 moments(float (&x)[I][4], float2 (*part)[kTile
     if (W > 1) tile_sync<W>();
     of = join_moments<W, I>(part, lane, n, eps * scale * scale);
   }
-  const float r = 1.f / sqrtf(of.y);
-  return float2{of.x, far ? -r : close ? r * -0x1p60f : r};
+  return float2{of.x, 1.f / sqrtf(of.y) * mark};
 }
 
 template <typename T, bool FIRST, int W, int I, int G>
@@ -155,9 +163,9 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
       load_rows<W, I>((const T*)p.x + first + p0, p.t, w, of, x);
     } else {
       Run<I, T> r;
-      const int mode = run_mode_of(p.x_mode, first, total);
-      load_run<W, I>((const T*)p.x + run, total, mode, tid, r);
-      run_to_tile<W, I>(r, total, mode, tid, p.t, tile);
+      const int mode = run_mode_here<W, I>(p.x_mode, first, total);
+      load_run<W, I, kFoursToo<W, I>>((const T*)p.x + run, total, mode, tid, r);
+      run_to_tile<W, I, kFoursToo<W, I>>(r, total, mode, tid, p.t, tile);
     }
   }
   for (int i = (int)threadIdx.x; i < 4 * W * I; i += 64 * W * G) {
@@ -168,7 +176,8 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
   if (!work) return;
   if (!FIRST) from_tile<W, I>(mine, w, x);
   const float2 of_pixel = moments<W, I>(x, part + group, w, lane, n, p.eps);
-  const float r = r_of(of_pixel.y);
+  float r = of_pixel.y;
+  if (__builtin_amdgcn_ballot_w64(r < 0) != 0) r = r_of(r);
   if (p.stats != nullptr && w == 0 && lane < count)
     reinterpret_cast<float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + lane] = of_pixel;
 #pragma unroll
@@ -180,7 +189,7 @@ __global__ void __launch_bounds__(64 * W * G) norm_kernel(Norm p) {
     }
   to_tile<W, I>(mine, w, x);
   tile_sync<W>();
-  store_run<W, I>(p.y + run, total, run_mode_of(p.y_mode, first, total), tid, p.t, tile);
+  store_run<W, I, kFoursToo<W, I>>(p.y + run, total, run_mode_here<W, I>(p.y_mode, first, total), tid, p.t, tile);
 }
 
 // SUMS: with the sums over pixels that dweight and dbias are made of.
@@ -211,32 +220,35 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
     const int64_t first = (int64_t)item * n * p.t.pixels, run = first + p0 * n;
     float x[I][4], d[I][4];
     Run<I, float> dy;
-    const int x_mode = run_mode_of(p.x_mode, first, total), y_mode = run_mode_of(p.y_mode, first, total);
-    load_run<W, I>(p.dy + run, total, y_mode, tid, dy);
+    const int x_mode = run_mode_here<W, I>(p.x_mode, first, total), y_mode = run_mode_here<W, I>(p.y_mode, first, total);
+    load_run<W, I, kFoursToo<W, I>>(p.dy + run, total, y_mode, tid, dy);
     float2 of_pixel;
     if (!kAgain) of_pixel = reinterpret_cast<const float2*>(p.stats)[(int64_t)item * p.t.pixels + p0 + of];
     if (FIRST) {
       load_rows<W, I>((const T*)p.x + first + p0, p.t, w, of, x);
     } else {
       Run<I, T> rx;
-      load_run<W, I>((const T*)p.x + run, total, x_mode, tid, rx);
-      run_to_tile<W, I>(rx, total, x_mode, tid, p.t, tile);
+      load_run<W, I, kFoursToo<W, I>>((const T*)p.x + run, total, x_mode, tid, rx);
+      run_to_tile<W, I, kFoursToo<W, I>>(rx, total, x_mode, tid, p.t, tile);
       tile_sync<W>();
       from_tile<W, I>(mine, w, x);
       tile_sync<W>();
     }
-    run_to_tile<W, I>(dy, total, y_mode, tid, p.t, tile);
-    if (kAgain) {
-      of_pixel = moments<W, I>(x, part_again + group, w, lane, n, p.eps);
-    } else if (__builtin_amdgcn_ballot_w64(of_pixel.y < 0) != 0) {
+    run_to_tile<W, I, kFoursToo<W, I>>(dy, total, y_mode, tid, p.t, tile);
+    if (kAgain) of_pixel = moments<W, I>(x, part_again + group, w, lane, n, p.eps);
+    float r = of_pixel.y, r_of_x = r;
+    const bool scaled = __builtin_amdgcn_ballot_w64(of_pixel.y < 0) != 0;
+    if (scaled) {
+      if (!kAgain) {
 #pragma unroll
-      for (int i = 0; i < I; ++i)
+        for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] *= scale_of(of_pixel.y);
+          for (int j = 0; j < 4; ++j) x[i][j] *= scale_of(of_pixel.y);
+      }
+      // (of close costs r * kClose may be beyond fp32 where the gradient is not: half of the scale here, half behind)
+      r = r_of(of_pixel.y);
+      r_of_x = is_close(of_pixel.y) ? r * 0x1p50f : r * scale_of(of_pixel.y);
     }
-    // (of close costs r * kClose may be beyond fp32 where the gradient is not: half of the scale before, half behind)
-    const bool close = is_close(of_pixel.y);
-    const float r = r_of(of_pixel.y), r_of_x = close ? r * 0x1p50f : of_pixel.y < 0 ? r * kFar : r;
     if (!kAgain || W == 1) tile_sync<W>();
     from_tile<W, I>(mine, w, d);
     float s1 = 0, s2 = 0;
@@ -275,18 +287,18 @@ __global__ void __launch_bounds__(64 * W * G, I <= 4 ? 4 : 1) norm_grad_kernel(N
       for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i][j] = r_of_x * (d[i][j] - s1 - x[i][j] * s2);
-      if (__builtin_amdgcn_ballot_w64(close) != 0) {
+      if (scaled) {
 #pragma unroll
         for (int i = 0; i < I; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[i][j] *= close ? 0x1p50f : 1.f;
+          for (int j = 0; j < 4; ++j) x[i][j] *= is_close(of_pixel.y) ? 0x1p50f : 1.f;
       }
       if (FIRST) {
         if (lane < count) store_rows<W, I>((T*)p.dx + first + p0, p.t, w, lane, x);
       } else {
         to_tile<W, I>(mine, w, x);
         tile_sync<W>();
-        store_run<W, I>((T*)p.dx + run, total, x_mode, tid, p.t, tile);
+        store_run<W, I, kFoursToo<W, I>>((T*)p.dx + run, total, x_mode, tid, p.t, tile);
       }
     }
     tile_sync<W>();  // (the next tile overwrites this one and its parts)
@@ -374,9 +386,12 @@ void with_grad_shape(int n, F f) {
 }
 
 // Workgroups of a gradient, each with as many tiles as the others.  Those of eight wavefronts are a quarter as many: 192 labels
-// 1500x2000 as fast with 512 as with 2048, the sum of their rows 12 -> 6 us.
+// 1500x2000 as fast with 512 as with 2048, the sum of their rows 12 -> 6 us.  Of four wavefronts seven are resident to a compute unit
+// and not eight where they need more than 80 scalar registers (16 more are set aside for each), and what is left over
+// makes a second round.  us with 2048 -> 1792, 40 M costs: 2 labels 142 -> 115, 3 120 -> 98, 4 108 -> 99, 12 130 -> 109, 16 118 ->
+// 103; of two wavefronts 6 labels 112 -> 119, 8 97 -> 97, not taken.
 unsigned grad_blocks(unsigned tiles, int waves, int per_block) {
-  const unsigned most = waves >= 8 ? kSumRows / 4 : kSumRows, groups = (tiles + (unsigned)per_block - 1) / (unsigned)per_block;
+  const unsigned most = waves >= 8 ? kSumRows / 4 : waves == 4 ? kSumRows / 8 * 7 : kSumRows, groups = (tiles + (unsigned)per_block - 1) / (unsigned)per_block;
   const unsigned rounds = (groups + most - 1) / most;
   return (groups + rounds - 1) / rounds;
 }
@@ -423,8 +438,9 @@ int prepare(const char* what, Norm& p, int dtype, bool labels_first, float eps, 
     return fail(MPL_EINVAL, "%s: too many pixels", what);
   return MPL_OK;
 }
-// (Fours of up to three labels are of two pixels or more.  us one by one -> four side by side, 40 M costs, forward and gradient: 2
-// labels 256 -> 278, 3 203 -> 218, 5 225 -> 209, 7 178 -> 172; labels last, 5 261 -> 241, 150 218 -> 195.)
+// (Fours of up to three labels are of two pixels or more, and their kernels are without them.  us one by one -> four side by side, 40 M
+// costs, forward and gradient: 2 labels 228 -> 223, labels last 243 -> 248, 3 184 -> 196 and 192 -> 191; 5 225 -> 209, 7 178 -> 172;
+// labels last, 5 261 -> 241, 150 218 -> 195.)
 int mode_of(const void* at, int n_disp, int dtype) {
   return n_disp < 4 ? (int)kEach : run_mode(n_disp, ((uintptr_t)at & (dtype == MPL_F32 ? 15 : 7)) == 0);
 }

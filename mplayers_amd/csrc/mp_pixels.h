@@ -156,8 +156,8 @@ __device__ __forceinline__ void four_places(unsigned i, const Tiles& t, F f) {
   }
 }
 
-// mode: of the run (run_mode_of).  tid: of the 64 * W threads of the tile.
-template <int W, int I, typename T>
+// mode: of the run (run_mode_of), with FOURS any, else not kFours.  tid: of the 64 * W threads of the tile.
+template <int W, int I, bool FOURS = true, typename T>
 __device__ __forceinline__ void load_run(const T* from, unsigned total, int mode, int tid, Run<I, T>& r) {
   constexpr int kThreads = 64 * W;
   if (mode != kEach) {
@@ -173,15 +173,15 @@ __device__ __forceinline__ void load_run(const T* from, unsigned total, int mode
     for (int k = 0; k < 4 * I; ++k) r.x[k] = load_at(from, min((unsigned)(tid + k * kThreads), total - 1));
   }
 }
-template <int W, int I, typename T>
+template <int W, int I, bool FOURS = true, typename T>
 __device__ __forceinline__ void run_to_tile(const Run<I, T>& r, unsigned total, int mode, int tid, const Tiles& t, float* tile) {
   constexpr int kThreads = 64 * W, kStride = tile_stride(W * I);
-  if (mode == kQuads) {
+  if (FOURS ? mode == kQuads : mode != kEach) {
 #pragma unroll
     for (int k = 0; k < I; ++k)
       *reinterpret_cast<float4*>(&tile[tile_place<kStride>(min((unsigned)(tid + k * kThreads) * 4, total - 4), t)]) =
           float4{(float)r.x[4 * k], (float)r.x[4 * k + 1], (float)r.x[4 * k + 2], (float)r.x[4 * k + 3]};
-  } else if (mode == kFours) {
+  } else if (FOURS && mode == kFours) {
 #pragma unroll
     for (int k = 0; k < I; ++k)
       four_places<kStride>(min((unsigned)(tid + k * kThreads) * 4, total - 4), t,
@@ -192,15 +192,15 @@ __device__ __forceinline__ void run_to_tile(const Run<I, T>& r, unsigned total, 
       tile[tile_place<kStride>(min((unsigned)(tid + k * kThreads), total - 1), t)] = (float)r.x[k];
   }
 }
-template <int W, int I, typename T>
+template <int W, int I, bool FOURS = true, typename T>
 __device__ __forceinline__ void store_run(T* to, unsigned total, int mode, int tid, const Tiles& t, const float* tile) {
   constexpr int kThreads = 64 * W, kStride = tile_stride(W * I);
-  if (mode == kQuads) {
+  if (FOURS ? mode == kQuads : mode != kEach) {
     for (unsigned i = (unsigned)tid * 4; i < total; i += kThreads * 4) {
       const float4 x = *reinterpret_cast<const float4*>(&tile[tile_place<kStride>(i, t)]);
       store_quad(to, i / 4, (T)x.x, (T)x.y, (T)x.z, (T)x.w);
     }
-  } else if (mode == kFours) {
+  } else if (FOURS && mode == kFours) {
     for (unsigned i = (unsigned)tid * 4; i < total; i += kThreads * 4) {
       float x[4];
       four_places<kStride>(i, t, [&](int j, unsigned place) { x[j] = tile[place]; });
