@@ -359,8 +359,9 @@ int64_t mpl_norm_workspace(int batch, int n_disp, int64_t pixels);
  * cost of `dtype`, (items, n_disp, pixels) with labels_first, else (items, pixels, n_disp); +inf and NaN are no candidates,
  * beside a cost of -inf only others of -inf are -> kept_labels, uint8, and kept_costs of `kept_dtype`, (items, n_kept,
  * pixels) or (items, pixels, n_kept): the costs relative to the pixel's least one (a difference in fp32, rounded to the type).
- * A place whose difference is +inf or that no candidate is left for has label 0 and cost +inf.  rest: NULL, or (items, pixels)
- * fp32: -T log(sum of exp(-c / T)) over the other candidates' relative costs c, +inf where there are none.  The temperature T
+ * A place whose difference is +inf in kept_dtype or that no candidate is left for has label 0 and cost +inf.  rest: NULL, or
+ * (items, pixels) fp32: -T log(sum of exp(-c / T)) over the relative costs c in fp32 of the candidates that the list has not
+ * got (those that were too far for its type among them), +inf where there are none.  The temperature T
  * is for it alone, above 0, and log2(e) / T and T are finite in fp32.  1 <= n_kept <= n_disp <= MPL_MAX_LABELS.  No counterpart
  * in the reference. */
 int mpl_best_labels(int dtype, int labels_first, const void* cost, int n_kept, float temperature, int kept_dtype,

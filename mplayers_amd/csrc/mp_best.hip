@@ -3,6 +3,7 @@
 //
 // cost -> k labels by cost, equal ones by label, with their costs relative to the best one (what a softmax of them needs, and what
 // fits a narrow type), and rest = -T log(sum over the other candidates of exp(-(c - best) / T)).  +inf and NaN are no candidates.
+// A difference that the list's type has no number for is not in the list, so its label is one of the others.
 //
 // The costs are read once, a pixel's labels over S lanes (mp_lanes.h), and stay in LDS; a lane has the least cost of each quad of
 // its labels in registers.  A place of the list is the least of those over the lanes: the first lane that has it looks its
@@ -28,6 +29,7 @@ struct Best {
   void* costs;
   float* rest;  // or nullptr
   int k, kept;  // places of the list, type of their costs
+  float limit;  // from here on a difference is +inf in that type
   float temperature, to_exponent;  // T, log2(e) / T
   int mode;  // of runs
 };
@@ -90,17 +92,20 @@ __global__ void __launch_bounds__(kLanePixels* S) best_kernel(Best p) {
         float* const at = own + g * 4 * S;
         float4 q = *reinterpret_cast<const float4*>(at);
         const int j = q.x == all ? 0 : q.y == all ? 1 : q.z == all ? 2 : 3;
-        at[j] = kInf;
-        q.x = j == 0 ? kInf : q.x;
-        q.y = j == 1 ? kInf : q.y;
-        q.z = j == 2 ? kInf : q.z;
-        q.w = j == 3 ? kInf : q.w;
-        const float next = least_of(q);
-#pragma unroll
-        for (int i = 0; i < kJ; ++i) least[i] = i == g ? next : least[i];
         const float c = all < kInf ? all - best : kInf;
-        found_cost[k][px] = c;
-        found_label[k][px] = (uint8_t)(c < kInf ? s * NV + 4 * g + j : 0);
+        const bool fits = c < p.limit;
+        if (fits) {  // (else it stays, for the rest)
+          at[j] = kInf;
+          q.x = j == 0 ? kInf : q.x;
+          q.y = j == 1 ? kInf : q.y;
+          q.z = j == 2 ? kInf : q.z;
+          q.w = j == 3 ? kInf : q.w;
+          const float next = least_of(q);
+#pragma unroll
+          for (int i = 0; i < kJ; ++i) least[i] = i == g ? next : least[i];
+        }
+        found_cost[k][px] = fits ? c : kInf;
+        found_label[k][px] = (uint8_t)(fits ? s * NV + 4 * g + j : 0);
       }
     }
     __syncthreads();
@@ -202,6 +207,8 @@ extern "C" int mpl_best_labels(int dtype, int labels_first, const void* cost, in
   p.rest = rest;
   p.k = n_kept;
   p.kept = kept_dtype;
+  // (half a step above the type's largest number)
+  p.limit = kept_dtype == MPL_F16 ? 65520.f : kept_dtype == MPL_BF16 ? 0x1.ffp127f : kInf;
   p.temperature = temperature;
   p.to_exponent = (float)(1.4426950408889634 / (double)temperature);
   p.mode = run_mode(n_disp, ((uintptr_t)cost & (dtype == MPL_F32 ? 15 : 7)) == 0);

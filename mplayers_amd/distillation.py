@@ -16,8 +16,8 @@ def best_labels(cost, k, temperature=1.0, labels_first=True, dtype=torch.float32
          (batch, cv, H, W, labels) as the operators do.  +inf and NaN are no candidates.
   -> labels  uint8, (batch, cv, k, H, W) or (batch, cv, H, W, k)
      costs   of `dtype`, relative to the least cost of the pixel (so the first is 0); +inf, and label 0, where there is no
-             candidate left
-     rest    (batch, cv, H, W) fp32, what the other candidates weigh together, as a cost: -T log(sum of exp(-cost / T)) with
+             candidate left, or none near enough for `dtype` (65504 in fp16)
+     rest    (batch, cv, H, W) fp32, what the other candidates weigh together (all that the list has not got), as a cost: -T log(sum of exp(-cost / T)) with
              the temperature T, which is for this alone; +inf where there are none
 
   No gradients."""

@@ -35,8 +35,9 @@ def softmin(costs, temperature):
   return best - temperature * math.log(math.fsum(math.exp(-(c - best) / temperature) for c in costs))
 
 
-def best_labels(cost, k, temperature):
-  """One pixel: k labels, their costs relative to the best one, and the softmin of the other candidates'."""
+def best_labels(cost, k, temperature, limit=math.inf):
+  """One pixel: k labels, their costs relative to the best one, and the softmin of the other candidates'.  limit: from here on
+  a relative cost is +inf in the list's type, which then has not got it."""
   cost = [math.inf if c != c else float(c) for c in cost]
   order = sorted((c, l) for l, c in enumerate(cost) if c < math.inf)
   if order and order[0][0] == -math.inf:
@@ -45,7 +46,8 @@ def best_labels(cost, k, temperature):
     with np.errstate(over="ignore"):  # (the difference is one of fp32)
       order = [(float(np.float32(c) - np.float32(order[0][0])), l) for c, l in order]
     order = [(c, l) for c, l in order if c < math.inf]
-  kept, others = order[:k], order[k:]
+  kept = [(c, l) for c, l in order[:k] if c < limit]
+  others = order[len(kept):]
   labels = [l for _, l in kept] + [0] * (k - len(kept))
   return labels, [c for c, _ in kept] + [math.inf] * (k - len(kept)), softmin([c for c, _ in others], temperature)
 

@@ -49,3 +49,11 @@ def test_verified_labels_next_to_borders(n, t, draft_t, costs, last):
                               other.movedim(-1, 2).numpy() if costs else None, t, draft_t)
   assert np.array_equal(kept.numpy(), want[1]) and np.array_equal(labels.numpy(), want[0])
   assert 0.2 < want[1][0].mean() < 0.9 and want[1][1].mean() < 0.9  # (both answers occur at the border)
+
+
+def test_best_labels_beyond_the_lists_type():
+  """The plain form of lists whose type has no number for a cost."""
+  inf = float("inf")
+  assert oracle.best_labels([0, 7e4, 5], 3, 1.0, 65520.0) == ([0, 2, 0], [0, 5, inf], 7e4)
+  assert oracle.best_labels([0, 7e4, 5], 2, 1.0, 65520.0) == ([0, 2], [0, 5], 7e4)
+  assert oracle.best_labels([0, 65519, 65520], 3, 1.0, 65520.0) == ([0, 1, 0], [0, 65519, inf], 65520)
