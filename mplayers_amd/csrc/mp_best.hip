@@ -8,8 +8,8 @@
 // The costs are read once, a pixel's labels over S lanes (mp_lanes.h), and stay in LDS; a lane has the least cost of each quad of
 // its labels in registers.  A place of the list is the least of those over the lanes: the first lane that has it looks its
 // quad up, takes the label out and finds the quad's next.  So a place costs the instructions of the quads and not of the
-// labels, and no sort is needed.  us: 96 labels 384x1248, lists of 8, 53 (3.9 TB/s; label by label 83), 800 instructions to a
-// wavefront of 16 pixels, 0.8 of the time; 21 labels 12x129x129, lists of 4, 8.5; 192 labels 377x501, lists of 32, 109, bound by
+// labels, and no sort is needed.  us: 96 labels 384x1248, lists of 8, 53 (3.9 TB/s; label by label 83), 810 instructions to a
+// wavefront of 16 pixels, 0.8 of the time; 21 labels 12x129x129, lists of 4, 8.5; 192 labels 377x501, lists of 32, 106, bound by
 // the instructions.
 
 #include "mp_lanes.h"

@@ -16,8 +16,8 @@
 // A tile of 64 pixels, a lane to each (mp_pixels.h).  The costs lie in LDS too, where the entries find the student's cost of
 // their label; the wavefronts of a tile share the list, and each has weights of its own labels that serve the student's sum, the
 // others' and the gradient, so there is one exponential to a label.  us, loss / gradient: 192 labels 1500x2000, lists of 8 in fp16
-// and a rest, 600 / 950 (4.0 and 5.0 TB/s; with each wavefront going through the whole list 1190 / 2390); 21 labels
-// 12x129x129, lists of 4, 9.1 / 12.4.  Bound by HBM, the loss by the instructions as well: 580 to a wavefront of 24 labels, 0.6 of
+// and a rest, 596 / 945 (4.0 and 5.0 TB/s; with each wavefront going through the whole list 1190 / 2390); 21 labels
+// 12x129x129, lists of 4, 9.2 / 12.5.  Bound by HBM, the loss by the instructions as well: 570 to a wavefront of 24 labels, 0.6 of
 // the time.
 
 #include "mp_pixels.h"
@@ -294,10 +294,10 @@ __global__ void __launch_bounds__(64 * W * G, I <= 6 ? 4 : 1) distill_kernel(Dis
 }
 
 // Eight entries of a list are held by the wavefronts of a tile, and four where the list has no more and one wavefront has it.  us,
-// loss / gradient, 16 M costs, one / four / eight held: 4 labels, lists of 4 147 / 117 / 123 and 210 / 142 / 183; 8 labels, 4 entries 83 /
-// 70 / 71 and 132 / 95 / 108, 8 entries 127 / 118 / 100 and 201 / 175 / 148; 42 M costs, 21 labels, 8 entries 82 (four) / 70 and 132 /
-// 106; 40 labels on two wavefronts, 8 entries, two and four each 55 / 50 and 72 / 62; 60 labels on four, one and two each 63 / 59 and
-// 97 / 86.
+// loss and gradient, 40 M costs, one / four / eight held: 4 labels, lists of 4 142 / 114 / 119 and 201 / 155 / 182; 8 labels, 4 entries 67 /
+// 56 / 58 and 133 / 98 / 111, 8 entries 125 / 116 / 99 and 206 / 179 / 150; 21 labels, 4 entries 45 / 38 / 40 and 103 / 82 / 85, 8
+// entries 64 / 60 / 52 and 147 / 132 / 107; 40 labels on two wavefronts, 8 entries, two and four each 54 / 48 and 103 / 87; 60 labels on
+// four, one and two each 44 / 40 and 92 / 83.
 template <typename T, bool FIRST, bool GRAD>
 void launch(const Distill& p, hipStream_t st) {
   with_shape(p.t.labels, [&](auto s) {

@@ -19,8 +19,8 @@
 // (The first of these in 32 bits is a choice: they take two registers a label, as it is what the shapes of the gradient go by, and
 // a lane adds one term to its sum per tile.  Of N tiles to a workgroup a sum is off by at most (N + 16) 2^-24 of the sum of the
 // terms' sizes, and of 100 tiles, with terms of one sign, was by 4e-8.)
-// us, forward / gradient with all sums: fp32, 192 labels 1500x2000 857 / 1364 (5.4 and 5.1 TB/s, where a large copy moves
-// 4.7); bf16, 21 labels 12x129x129 9.9 / 16.3; 97 labels 301x803 in the operators' layout 40 / 63.
+// us, forward / gradient with all sums: fp32, 192 labels 1500x2000 858 / 1364 (5.4 and 5.1 TB/s, where a large copy moves
+// 4.7); bf16, 21 labels 12x129x129 10.4 / 16.2; 97 labels 301x803 in the operators' layout 40 / 64.
 
 #include <algorithm>
 

@@ -34,8 +34,9 @@ struct TileShape {
   static constexpr int kW = W, kI = I, kG = G;
 };
 // Shapes for every four labels up to 32, us for 40 M costs in place of those for the next eight: the divergence and its gradient
-// together, 10 labels 158 -> 154, labels last 165 -> 142, 18 labels 137 -> 117 and 132 -> 113, 26 labels 132 -> 115 and 124 -> 107;
-// layer norm with its gradient 203 -> 201, bf16 174 -> 168.
+// together, lists of 4, 10 labels 147 -> 141, labels last 160 -> 133, 18 labels 133 -> 114 and 130 -> 112, 26 labels 133 -> 116 and 125 ->
+// 109; layer norm's forward pass (its gradient has shapes of its own) 10 labels 65.5 -> 64.5, 18 labels 67.4 -> 64.3, bf16 47.4 ->
+// 45.9, 26 labels 64.8 -> 64.2 and 45.7 -> 43.7.
 template <typename F>
 inline void with_shape(int n, F f) {
   if (n <= 4)

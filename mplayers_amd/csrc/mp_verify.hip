@@ -9,9 +9,10 @@
 // Either volume is read once: a pixel's labels lie in the registers of one to eight lanes (mp_lanes.h), p and q are formed there, and
 // the running sums go to LDS only in wavefronts where a label is drawn anew.  Results are those of 64 bits, which 32 bits give but
 // for drafts next to a border (see verify_kernel).  Bound by HBM for one draft: us, 192 labels 1500x2000 1015 to 1075 (4.3 to 4.6 TB/s; with 64
-// bits throughout 15 300, without the drafts that do go there 945), 60 labels 1000x2000 184 (5.3 TB/s); 60 labels 375x450 in the
-// operators' layout, 8 drafts, 32 by the instructions (920 to a wavefront of 16 pixels) and the last wavefronts, which have the
-// drafts that go to 64 bits: 28 without those.
+// bits throughout 15 300, without the drafts that do go there 945), 60 labels 1000x2000 184 to 192 (5.3 TB/s); 60 labels 375x450 in the
+// operators' layout, 8 drafts, 32 by the instructions (910 to a wavefront of 16 pixels, half of the time) and the last wavefronts,
+// which have the drafts that go to 64 bits: 28 without those.  Without the draft's costs 192 labels 1500x2000 528 to 562 (4.1 to 4.4
+// TB/s), 60 labels 375x450, 8 drafts, 24.
 
 #include "mp_lanes.h"
 
